@@ -22,6 +22,11 @@ from .float8_linear_utils import sync_float8_amax_and_scale_history  # once per 
 from .float8_tensor import Float8Tensor, GemmInputRole, LinearMMConfig, ScaledMMConfig
 from .fsdp_utils import precompute_float8_dynamic_scale_for_fsdp  # all weight scales in one pass
 
+# beside the reference's names: linears with a scale for each block of 128, and the operators around them in a training step
+from .float8_blockwise import Float8BlockwiseInferenceLinear, Float8BlockwiseLinear, blockwise_linear
+from .norm import LayerNorm, convert_layer_norms, layer_norm
+from .grad_clip import clip_grad_norm_, clip_grads, grad_norm
+
 # checkpoints holding Float8Tensors load with torch.load(..., weights_only=True)
 _serialization.add_safe_globals([Float8Tensor, GemmInputRole, LinearMMConfig, ScaledMMConfig])
 

@@ -1,5 +1,5 @@
-"""Compiles csrc/*.hip into libf8mi.so for gfx950 with hipcc, and the host path over it (csrc/f8mi_torch.cpp) into a CPython
-module against torch's headers (no GPU needed)."""
+"""Compiles csrc/*.hip into libf8mi.so for gfx950 with hipcc, and the host path over it (csrc/f8mi_torch*.cpp) into CPython
+modules against torch's headers (no GPU needed)."""
 import glob
 import os
 import subprocess
@@ -15,6 +15,9 @@ PROBE_LIB = os.path.join(HERE, "libf8mi_probe.so")
 # the fused linear's host path: a CPython module on torch tensors, host code only
 EXT_SRC = os.path.join(CSRC, "f8mi_torch.cpp")
 EXT_LIB = os.path.join(HERE, "_f8mi_torch.so")
+# ... and that of the blockwise scaled linear, layer norm and gradient clipping
+OPS_SRC = os.path.join(CSRC, "f8mi_torch_ops.cpp")
+OPS_LIB = os.path.join(HERE, "_f8mi_torch_ops.so")
 OBJ_DIR = os.path.join(CSRC, "build")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -40,7 +43,7 @@ def _compile(src: str, obj_dir: str = OBJ_DIR, defines=()) -> str:
     return obj
 
 
-def build_extension() -> None:
+def build_extension(src: str = EXT_SRC, out: str = EXT_LIB) -> None:
     import sysconfig
 
     import torch
@@ -48,7 +51,7 @@ def build_extension() -> None:
     root, rocm = os.path.dirname(torch.__file__), os.path.dirname(os.path.dirname(HIPCC))
     subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include",
                     f"-I{rocm}/include", "-I" + sysconfig.get_paths()["include"], "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
-                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", EXT_SRC, "-o", EXT_LIB, f"-L{root}/lib",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", out, f"-L{root}/lib",
                     "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"], check=True)
 
 
@@ -59,9 +62,9 @@ def build(verbose: bool = True, out: str = LIB, defines=()) -> str:
     os.makedirs(obj_dir, exist_ok=True)
     srcs = sources()
     with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
-        ext = ex.submit(build_extension) if out == LIB else None
+        exts = [ex.submit(build_extension, *e) for e in ((EXT_SRC, EXT_LIB), (OPS_SRC, OPS_LIB))] if out == LIB else []
         objs = list(ex.map(lambda src: _compile(src, obj_dir, tuple(defines)), srcs))
-        if ext:
+        for ext in exts:
             ext.result()
     subprocess.run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, *objs], check=True)
     if out == LIB:

@@ -1,0 +1,163 @@
+"""The blockwise scaled linear and layer norm as ``torch.library`` custom ops, for ``torch.compile`` and whoever else has to see operators: opaque
+nodes with known shapes, one per direction, with the numbers of the eager path."""
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native
+from ._custom_ops import column_sum
+
+_e4m3 = torch.float8_e4m3fn
+_KB, _BLOCK = _native.KB, _native.BLOCK
+
+
+def _data_shape(rows: int, k: int):
+    return (_native.padded_k(k) // _KB, rows, _KB)
+
+
+def _scales_shape(rows: int, k: int):
+    return (_native.padded_k(k) // _BLOCK, -(-rows // _BLOCK) * _BLOCK)
+
+
+def _one_weight_copy(k: int, n: int) -> bool:
+    return k % _BLOCK == 0 and n % _BLOCK == 0
+
+
+@torch.library.custom_op("f8mi::blockwise_linear_fwd", mutates_args=())
+def blockwise_linear_fwd(x2: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], need_dx: bool, need_dw: bool) -> Tuple[
+        torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, x transposed: data, scales; weight for the gradient of x: data, scales); what backward will not need is empty."""
+    (m, k), n = x2.shape, weight.shape[0]
+    one = _one_weight_copy(k, n)
+    empty = lambda dt: torch.empty(0, dtype=dt, device=x2.device)
+    if m == 0:
+        return (x2.new_empty((0, n)), empty(_e4m3), empty(torch.uint8), empty(_e4m3), empty(torch.uint8))
+    with _native.transient_workspaces():
+        (x8, x8t), (w8, w8t) = _native.block_cast([(x2, False, True, need_dw), (weight, True, True, need_dx and ("scales" if one else True))])
+        y = _native.block_gemm(x8, w8, x2.dtype, None if bias is None else bias.to(x2.dtype).contiguous())
+    return (y, x8t.data if need_dw else empty(_e4m3), x8t.scales if need_dw else empty(torch.uint8),
+            (w8.data if one else w8t.data) if need_dx else empty(_e4m3), w8t.scales if need_dx else empty(torch.uint8))
+
+
+@blockwise_linear_fwd.register_fake
+def _(x2, weight, bias, need_dx, need_dw):
+    (m, k), n = x2.shape, weight.shape[0]
+    make = lambda shape, dt, wanted: torch.empty(shape if wanted else (0,), dtype=dt, device=x2.device)
+    w_shape = _data_shape(n, k) if _one_weight_copy(k, n) else _data_shape(k, n)
+    return (torch.empty((m, n), dtype=x2.dtype, device=x2.device), make(_data_shape(k, m), _e4m3, need_dw), make(_scales_shape(k, m), torch.uint8, need_dw),
+            make(w_shape, _e4m3, need_dx), make(_scales_shape(k, n), torch.uint8, need_dx))
+
+
+@torch.library.custom_op("f8mi::blockwise_linear_bwd", mutates_args=())
+def blockwise_linear_bwd(dy2: torch.Tensor, xt: torch.Tensor, xt_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, k: int, w_dtype: torch.dtype,
+                         need_dx: bool, need_dw: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dw); an unneeded gradient is empty."""
+    m, n = dy2.shape
+    empty = lambda dt: torch.empty(0, dtype=dt, device=dy2.device)
+    if m == 0:
+        return (dy2.new_empty((0, k)) if need_dx else empty(dy2.dtype), dy2.new_zeros((n, k), dtype=w_dtype) if need_dw else empty(w_dtype))
+    with _native.transient_workspaces():
+        ((g8, g8t),) = _native.block_cast([(dy2, False, need_dx, need_dw)])
+        dx, dw = empty(dy2.dtype), empty(w_dtype)
+        if need_dx:
+            one = _one_weight_copy(k, n)
+            dx = _native.block_gemm(g8, _native.Blocks(None if one else w, w_scales, k, n), dy2.dtype, transposed=_native.Blocks(w, None, n, k) if one else None)
+        if need_dw:
+            dw = _native.block_gemm(g8t, _native.Blocks(xt, xt_scales, k, m), w_dtype)
+    return dx, dw
+
+
+@blockwise_linear_bwd.register_fake
+def _(dy2, xt, xt_scales, w, w_scales, k, w_dtype, need_dx, need_dw):
+    m, n = dy2.shape
+    return (torch.empty((m, k) if need_dx else (0,), dtype=dy2.dtype, device=dy2.device), torch.empty((n, k) if need_dw else (0,), dtype=w_dtype, device=dy2.device))
+
+
+class _BlockwiseLinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2, weight, bias):
+        y, *saved = blockwise_linear_fwd(x2, weight, bias, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        ctx.k, ctx.w_dtype, ctx.b_dtype = x2.shape[1], weight.dtype, None if bias is None else bias.dtype
+        ctx.save_for_backward(*saved)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        need_dx, need_dw, need_db = ctx.needs_input_grad
+        dx = dw = None
+        if need_dx or need_dw:
+            dx, dw = blockwise_linear_bwd(gy, *ctx.saved_tensors, ctx.k, ctx.w_dtype, need_dx, need_dw)
+        return dx if need_dx else None, dw if need_dw else None, column_sum(gy, ctx.b_dtype) if need_db else None
+
+
+def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    y = _BlockwiseLinearFn.apply(x.reshape(-1, x.shape[-1]), weight, bias)
+    return y.reshape(*x.shape[:-1], weight.shape[0])
+
+
+@torch.library.custom_op("f8mi::blockwise_inference_linear", mutates_args=())
+def _blockwise_inference_linear(x2: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    n = data.shape[1]
+    if x2.shape[0] == 0:
+        return x2.new_empty((0, n))
+    y = _native.ops().blockwise_inference_linear(x2, data, scales, n, bias, torch._C._cuda_getDevice())
+    if y is None:
+        raise _native.Float8NativeError("blockwise_inference_linear: a weight of another shape or device than its scales")
+    return y
+
+
+@_blockwise_inference_linear.register_fake
+def _(x2, data, scales, bias):
+    return torch.empty((x2.shape[0], data.shape[1]), dtype=x2.dtype, device=x2.device)
+
+
+def blockwise_inference_linear(x: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    return _blockwise_inference_linear(x.reshape(-1, x.shape[-1]), data, scales, bias).reshape(*x.shape[:-1], data.shape[1])
+
+
+# ---- layer norm
+
+
+@torch.library.custom_op("f8mi::layer_norm_fwd", mutates_args=())
+def layer_norm_fwd(x2: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, (mean, rstd) of each row)"""
+    return _native.layer_norm(x2, weight, bias, eps)
+
+
+@layer_norm_fwd.register_fake
+def _(x2, weight, bias, eps):
+    return torch.empty(x2.shape, dtype=x2.dtype, device=x2.device), torch.empty((x2.shape[0], 2), dtype=torch.float32, device=x2.device)
+
+
+@torch.library.custom_op("f8mi::layer_norm_bwd", mutates_args=())
+def layer_norm_bwd(dy2: torch.Tensor, x2: torch.Tensor, weight: Optional[torch.Tensor], p_dtype: torch.dtype, stats: torch.Tensor) -> Tuple[
+        torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias)"""
+    return _native.layer_norm_backward(dy2, x2, weight, p_dtype, stats)
+
+
+@layer_norm_bwd.register_fake
+def _(dy2, x2, weight, p_dtype, stats):
+    p = lambda: torch.empty(x2.shape[1], dtype=p_dtype, device=x2.device)
+    return torch.empty(x2.shape, dtype=x2.dtype, device=x2.device), p(), p()
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2, weight, bias, eps):
+        y, stats = layer_norm_fwd(x2, weight, bias, eps)
+        ctx.p_dtype = next((p.dtype for p in (weight, bias) if p is not None), x2.dtype)
+        ctx.has_weight = weight is not None
+        ctx.save_for_backward(x2, stats, *([weight] if weight is not None else []))
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x2, stats, *weight = ctx.saved_tensors
+        dx, dw, db = layer_norm_bwd(gy, x2, weight[0] if ctx.has_weight else None, ctx.p_dtype, stats)
+        return tuple(g if need else None for g, need in zip((dx, dw, db), ctx.needs_input_grad)) + (None,)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], cols: int, eps: float) -> torch.Tensor:
+    flat = lambda p: None if p is None else p.reshape(-1)
+    return _LayerNormFn.apply(x.reshape(-1, cols), flat(weight), flat(bias), eps).reshape(x.shape)

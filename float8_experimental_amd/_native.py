@@ -10,7 +10,7 @@ import functools
 import importlib.util
 import os
 import threading
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.overrides import _get_current_function_mode_stack
@@ -66,6 +66,15 @@ EXPORTS = (
     "f8mi_sync",
     "f8mi_sync_host",
     "f8mi_delayed_init",
+    "f8mi_block_scale_bytes",
+    "f8mi_block_cast",
+    "f8mi_block_gemm",
+    "f8mi_block_gemm_workspace_bytes",
+    "f8mi_layer_norm",
+    "f8mi_layer_norm_backward",
+    "f8mi_layer_norm_workspace_bytes",
+    "f8mi_grad_clip",
+    "f8mi_grad_clip_workspace_bytes",
     "f8mi_prof_enable",
     "f8mi_prof_reset",
     "f8mi_prof_read",
@@ -73,6 +82,19 @@ EXPORTS = (
 
 _lib = None
 _lock = threading.Lock()
+
+
+class Grad(C.Structure):
+    """f8mi_grad of include/f8mi.h."""
+
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int), ("out_dtype", C.c_int)]
+
+
+class BlockCastJob(C.Structure):
+    """f8mi_block_cast_job of include/f8mi.h."""
+
+    _fields_ = [("x", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64), ("dtype", C.c_int), ("square", C.c_int),
+                ("out", C.c_void_p), ("out_scales", C.c_void_p), ("out_t", C.c_void_p), ("out_t_scales", C.c_void_p)]
 
 
 class Float8NativeError(RuntimeError):
@@ -165,6 +187,24 @@ def lib() -> C.CDLL:
         L.f8mi_sync_host.argtypes = [vp, i32, i32, i32, i32, vp]
         L.f8mi_delayed_init.restype = i32
         L.f8mi_delayed_init.argtypes = [fp, fp, fp, i32, i32, i32, vp]
+        L.f8mi_block_scale_bytes.restype = i64
+        L.f8mi_block_scale_bytes.argtypes = [i64, i64]
+        L.f8mi_block_cast.restype = i32
+        L.f8mi_block_cast.argtypes = [C.POINTER(BlockCastJob), i32, vp]
+        L.f8mi_block_gemm.restype = i32
+        L.f8mi_block_gemm.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, i32, i64, vp, vp, i64, vp]
+        L.f8mi_block_gemm_workspace_bytes.restype = i64
+        L.f8mi_block_gemm_workspace_bytes.argtypes = [i64, i64, i64]
+        L.f8mi_layer_norm.restype = i32
+        L.f8mi_layer_norm.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, C.c_float, vp, fp, vp]
+        L.f8mi_layer_norm_workspace_bytes.restype = i64
+        L.f8mi_layer_norm_workspace_bytes.argtypes = [i64, i64, i32]
+        L.f8mi_layer_norm_backward.restype = i32
+        L.f8mi_layer_norm_backward.argtypes = [vp, i64, vp, i64, i64, i64, i32, vp, i32, fp, vp, vp, vp, vp, i64, vp]
+        L.f8mi_grad_clip_workspace_bytes.restype = i64
+        L.f8mi_grad_clip_workspace_bytes.argtypes = [i64]
+        L.f8mi_grad_clip.restype = i32
+        L.f8mi_grad_clip.argtypes = [C.POINTER(Grad), i64, i32, C.c_float, i32, fp, vp, i64, vp]
         L.f8mi_prof_enable.restype = i32
         L.f8mi_prof_enable.argtypes = [i32]
         L.f8mi_prof_reset.restype = i32
@@ -181,7 +221,20 @@ def lib() -> C.CDLL:
 
 
 _EXT_PATH = os.path.join(_HERE, "_f8mi_torch.so")
+_OPS_PATH = os.path.join(_HERE, "_f8mi_torch_ops.so")
 _ext = None
+_ops = None
+
+
+def _load_extension(name: str, path: str):
+    if not os.path.exists(path):
+        raise Float8NativeError(f"{path} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+                                "(or `python float8_experimental_amd/_build.py`)")
+    spec = importlib.util.spec_from_file_location("float8_experimental_amd." + name, path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.load(LIB_PATH, Float8NativeError)
+    return module
 
 
 def ext():
@@ -191,15 +244,20 @@ def ext():
         lib()
         with _lock:
             if _ext is None:
-                if not os.path.exists(_EXT_PATH):
-                    raise Float8NativeError(f"{_EXT_PATH} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
-                                            "(or `python float8_experimental_amd/_build.py`)")
-                spec = importlib.util.spec_from_file_location("float8_experimental_amd._f8mi_torch", _EXT_PATH)
-                module = importlib.util.module_from_spec(spec)
-                spec.loader.exec_module(module)
-                module.load(LIB_PATH, Float8NativeError)
-                _ext = module
+                _ext = _load_extension("_f8mi_torch", _EXT_PATH)
     return _ext
+
+
+def ops():
+    """The CPython module with the host path of the blockwise scaled linear, layer norm and gradient clipping
+    (csrc/f8mi_torch_ops.cpp), on the loaded library."""
+    global _ops
+    if _ops is None:
+        lib()
+        with _lock:
+            if _ops is None:
+                _ops = _load_extension("_f8mi_torch_ops", _OPS_PATH)
+    return _ops
 
 
 def build_knobs() -> str:
@@ -853,6 +911,106 @@ def dequant(data: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torc
     rc = lib().f8mi_dequant(data.data_ptr(), _F8[data.dtype], data.numel(), scale.data_ptr(), _DT[dtype], out.data_ptr(), _stream(data))
     _check(rc, "f8mi_dequant")
     return out
+
+
+BLOCK = 128  # values that share a scale, along the contraction
+
+
+class Blocks(NamedTuple):
+    """An e4m3 operand with block scales, as f8mi_block_gemm reads it: ``data`` [padded_k(k)/64, rows, 64], ``scales`` (uint8, biased
+    exponents) [padded_k(k)/128, rows padded to 128] in the order of include/f8mi.h."""
+
+    data: Optional[torch.Tensor]
+    scales: torch.Tensor
+    rows: int
+    k: int
+
+    def dequant(self) -> torch.Tensor:
+        """[rows, k] in fp64: the values the operand stands for (composed of torch operations).  The largest of bf16 and fp32 are kept as 2^128."""
+        values = self.data.double().permute(1, 0, 2).reshape(self.rows, -1)
+        order = torch.arange(128, device=self.scales.device)
+        exponents = self.scales.view(self.scales.shape[0], -1, 128)[:, :, order % 16 * 8 + order // 16].reshape(self.scales.shape[0], -1)
+        powers = (exponents.t()[:self.rows].long() + 896 << 52).view(torch.float64)
+        return (values.view(self.rows, -1, BLOCK) * powers[:, :, None]).view(self.rows, -1)[:, :self.k]
+
+
+def _blocks_alloc(rows: int, k: int, device, data: bool = True) -> Blocks:
+    kp = padded_k(k)
+    return Blocks(torch.empty((kp // KB, rows, KB), dtype=torch.float8_e4m3fn, device=device) if data else None,
+                  torch.empty((kp // BLOCK, -(-rows // BLOCK) * BLOCK), dtype=torch.uint8, device=device), rows, k)
+
+
+def block_cast(jobs):
+    """[(copy contracting over the columns or None, copy contracting over the rows or None)] of one or two 2-D tensors, in one pass over
+    each.  A job is ``(x, square, want, want_t)``: ``square`` gives every 128 x 128 values one scale, otherwise blocks are 128
+    values along the contraction of each copy; ``want_t`` may be ``"scales"`` for a square tensor that another product reads transposed.
+    See f8mi_block_cast."""
+    structs, out = (BlockCastJob * len(jobs))(), []
+    held = []
+    for s, (x, square, want, want_t) in zip(structs, jobs):
+        _require_gpu(x, "x")
+        assert x.dim() == 2 and x.dtype in _DT and x.numel() > 0
+        xs, rows, cols, ld = _as_2d(x)
+        held.append(xs)
+        a = _blocks_alloc(rows, cols, x.device) if want else None
+        b = _blocks_alloc(cols, rows, x.device, data=want_t != "scales") if want_t else None
+        s.x, s.rows, s.cols, s.ld, s.dtype, s.square = xs.data_ptr(), rows, cols, ld, _DT[x.dtype], int(square)
+        if a is not None:
+            s.out, s.out_scales = a.data.data_ptr(), a.scales.data_ptr()
+        if b is not None:
+            s.out_t, s.out_t_scales = b.data.data_ptr() if b.data is not None else None, b.scales.data_ptr()
+        out.append((a, b))
+    _check_device(jobs[0][0].device)
+    _check(lib().f8mi_block_cast(structs, len(jobs), _stream(jobs[0][0])), "f8mi_block_cast")
+    return out
+
+
+def block_gemm(a: Blocks, b: Blocks, out_dtype: torch.dtype, bias: Optional[torch.Tensor] = None, transposed: Optional[Blocks] = None) -> torch.Tensor:
+    """a [m, k] times b [n, k] transposed, plus the bias, in ``out_dtype``.  ``transposed``: the copy of b's tensor that another product
+    contracts over n, read transposed (``b`` then holds scales only).  See f8mi_block_gemm."""
+    _require_gpu(a.data, "a")
+    assert a.k == b.k and (transposed is None or (transposed.rows == b.k and transposed.k == b.rows))
+    m, n, k = a.rows, b.rows, padded_k(a.k)
+    bias = _checked_bias(bias, n, out_dtype, a.data.device)
+    out = torch.empty((m, n), dtype=out_dtype, device=a.data.device)
+    _check_device(a.data.device)
+    ws_ptr, ws_bytes = gemm_workspace(a.data.device, m, k, n)
+    rc = lib().f8mi_block_gemm(a.data.data_ptr(), a.scales.data_ptr(), (transposed if transposed is not None else b).data.data_ptr(), b.scales.data_ptr(),
+                               int(transposed is not None), m, n, k, out.data_ptr(), _DT[out_dtype], n, bias.data_ptr() if bias is not None else None,
+                               ws_ptr, ws_bytes, _stream(a.data))
+    _check(rc, "f8mi_block_gemm")
+    return out
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float):
+    """(y, (mean, rstd) of each row [rows, 2]) of a matrix.  See f8mi_layer_norm."""
+    _require_gpu(x, "x")
+    xs, rows, cols, ld = _as_2d(x)
+    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
+    p_dtype = next((p.dtype for p in (weight, bias) if p is not None), x.dtype)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    _check_device(x.device)
+    rc = lib().f8mi_layer_norm(xs.data_ptr(), rows, cols, ld, _DT[x.dtype], weight.data_ptr() if weight is not None else None,
+                               bias.data_ptr() if bias is not None else None, _DT[p_dtype], eps, y.data_ptr(), stats.data_ptr(), _stream(x))
+    _check(rc, "f8mi_layer_norm")
+    return y, stats
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], p_dtype: torch.dtype, stats: torch.Tensor):
+    """(dx, dweight, dbias) of a matrix, the latter two in ``p_dtype``.  See f8mi_layer_norm_backward."""
+    _require_gpu(dy, "dy")
+    xs, rows, cols, ld = _as_2d(x)
+    gs, _, _, ld_dy = _as_2d(dy)
+    weight = None if weight is None else weight.contiguous()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw, db = (torch.empty(cols, dtype=p_dtype, device=x.device) for _ in range(2))
+    need = lib().f8mi_layer_norm_workspace_bytes(rows, cols, _DT[x.dtype])
+    ws = torch.empty(max(need // 4, 1), dtype=torch.float32, device=x.device)
+    rc = lib().f8mi_layer_norm_backward(gs.data_ptr(), ld_dy, xs.data_ptr(), ld, rows, cols, _DT[x.dtype], weight.data_ptr() if weight is not None else None,
+                                        _DT[p_dtype], stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), need, _stream(x))
+    _check(rc, "f8mi_layer_norm_backward")
+    return dx, dw, db
 
 
 def sync_table(entries, device: torch.device) -> torch.Tensor:

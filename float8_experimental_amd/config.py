@@ -9,9 +9,10 @@ class ScalingType(enum.Enum):
 
     DELAYED = "delayed"  # from the amax history of earlier iterations
     DYNAMIC = "dynamic"  # from the tensor itself, every time
+    BLOCKWISE = "blockwise"  # from each block of 128 of its values, every time (all three tensors of a linear or none)
 
     def short_str(self) -> str:
-        return {ScalingType.DELAYED: "del", ScalingType.DYNAMIC: "dyn"}[self]
+        return {ScalingType.DELAYED: "del", ScalingType.DYNAMIC: "dyn", ScalingType.BLOCKWISE: "blk"}[self]
 
 
 @dataclass(frozen=True)
@@ -72,6 +73,11 @@ class Float8LinearConfig:
     emulate: bool = False
 
     delayed_scaling_config: DelayedScalingConfig = DelayedScalingConfig()
+
+    def __post_init__(self):
+        kinds = {c.scaling_type for c in (self.cast_config_input, self.cast_config_weight, self.cast_config_grad_output)}
+        if ScalingType.BLOCKWISE in kinds and len(kinds) > 1:
+            raise ValueError("blockwise scaling is for all three tensors of a linear (input, weight, grad_output) or for none")
 
 
 # The reference can switch to the "fnuz" fp8 flavours of older AMD GPUs through this module

@@ -12,7 +12,7 @@ int launch_gemm_mid(int a_fmt, int b_fmt, int c_dtype, bool wide, hipStream_t st
     return launch_mid1<false, false>(a_fmt, b_fmt, c_dtype, wide, stream, A, lda, a_unit, Bt, ldb, b_unit, M, N, K, sa, sb, C, ldc, bias, c_vec_ok, 1);
 }
 
-// C = (partial[0] + partial[1] + ... in this order) / (sa * sb) + bias: four neighbouring columns per lane (N % 4 == 0)
+// C = (partial[0] + partial[1] + ... in this order) / (sa * sb) + bias (block scales: they are in the parts already, sa and sb null): four neighbouring columns per lane (N % 4 == 0)
 template <int C_DT>
 __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restrict__ partial, int k_splits, int M, int N,
                                                             const float* __restrict__ sa_dev, const float* __restrict__ sb_dev,
@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restr
     if (q >= (int64_t)M * quads) return;
     const int64_t row = q / quads;
     const int col = (int)(q % quads) * 4;
-    const float inv = __fdiv_rn(1.0f, *sa_dev) * __fdiv_rn(1.0f, *sb_dev);
+    const float inv = sa_dev ? __fdiv_rn(1.0f, *sa_dev) * __fdiv_rn(1.0f, *sb_dev) : 1.0f;
     const int64_t slab = (int64_t)M * N;
     float4 sum = *(const float4*)(partial + row * N + col);
     for (int s = 1; s < k_splits; s++) {
@@ -52,6 +52,16 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restr
     }
 }
 
+int launch_splitk_reduce(int c_dtype, int k_splits, const float* partial, hipStream_t stream, int M, int N, const float* sa, const float* sb, void* C,
+                         int64_t ldc, const void* bias, int c_vec_ok) {
+    const int64_t quads = (int64_t)M * (N / 4);
+    const dim3 grid((unsigned)((quads + 255) / 256));
+    if (c_dtype == F8MI_BF16) hipLaunchKernelGGL(splitk_reduce_kernel<F8MI_BF16>, grid, dim3(256), 0, stream, partial, k_splits, M, N, sa, sb, C, ldc, bias, c_vec_ok);
+    else if (c_dtype == F8MI_FP16) hipLaunchKernelGGL(splitk_reduce_kernel<F8MI_FP16>, grid, dim3(256), 0, stream, partial, k_splits, M, N, sa, sb, C, ldc, bias, c_vec_ok);
+    else hipLaunchKernelGGL(splitk_reduce_kernel<F8MI_FP32>, grid, dim3(256), 0, stream, partial, k_splits, M, N, sa, sb, C, ldc, bias, c_vec_ok);
+    return check_hip(hipGetLastError(), "gemm split-k reduction kernel launch");
+}
+
 // The contraction split k_splits ways over workgroups (outputs of few tiles and a long k: every CU gets a part).
 // `partial` holds k_splits x M x N floats (16-byte aligned); host side has checked K % (128 * k_splits) == 0, N % 4 == 0.
 int launch_gemm_mid_splitk(int a_fmt, int b_fmt, int c_dtype, bool wide, int k_splits, float* partial, hipStream_t stream, const uint8_t* A,
@@ -59,12 +69,7 @@ int launch_gemm_mid_splitk(int a_fmt, int b_fmt, int c_dtype, bool wide, int k_s
                            const float* sb, void* C, int64_t ldc, const void* bias, int c_vec_ok) {
     if (int rc = launch_mid1<false, false>(a_fmt, b_fmt, F8MI_FP32, wide, stream, A, lda, a_unit, Bt, ldb, b_unit, M, N, K, sa, sb, partial, N, nullptr, 1, k_splits))
         return rc;
-    const int64_t quads = (int64_t)M * (N / 4);
-    const dim3 grid((unsigned)((quads + 255) / 256));
-    if (c_dtype == F8MI_BF16) hipLaunchKernelGGL(splitk_reduce_kernel<F8MI_BF16>, grid, dim3(256), 0, stream, partial, k_splits, M, N, sa, sb, C, ldc, bias, c_vec_ok);
-    else if (c_dtype == F8MI_FP16) hipLaunchKernelGGL(splitk_reduce_kernel<F8MI_FP16>, grid, dim3(256), 0, stream, partial, k_splits, M, N, sa, sb, C, ldc, bias, c_vec_ok);
-    else hipLaunchKernelGGL(splitk_reduce_kernel<F8MI_FP32>, grid, dim3(256), 0, stream, partial, k_splits, M, N, sa, sb, C, ldc, bias, c_vec_ok);
-    return check_hip(hipGetLastError(), "gemm split-k reduction kernel launch");
+    return launch_splitk_reduce(c_dtype, k_splits, partial, stream, M, N, sa, sb, C, ldc, bias, c_vec_ok);
 }
 
 }  // namespace f8mi

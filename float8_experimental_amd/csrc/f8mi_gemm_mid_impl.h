@@ -36,20 +36,51 @@ constexpr int MID_A_UNIT = MID_TILE_M * 64;  // A, one 64-deep unit of a stage: 
 
 // TJ = 16-column tiles per wave: 4 -> 128 x 128 workgroup tiles, five stages of 32 KB;
 //                                8 -> 128 x 256, three stages of 48 KB.
-template <int TJ>
+// BLK: operands with block scales; a stage ends with 256 bytes of scales for each wave, and five stages of 128 x 128 tiles would be too many.
+template <int TJ, bool BLK = false>
 struct MidCfg {
     static constexpr int TILE_N = 32 * TJ;
     static constexpr int B_UNIT = TILE_N * 64;
-    static constexpr int STAGE = 2 * MID_A_UNIT + 2 * B_UNIT;
-    static constexpr int NSTAGE = TJ == 4 ? 5 : 3;
-    static constexpr int LDS = NSTAGE * STAGE;  // 160 KB / 144 KB
+    static constexpr int SCALES = 2 * MID_A_UNIT + 2 * B_UNIT;  // where a stage's scales start
+    static constexpr int STAGE = SCALES + (BLK ? 1024 : 0);
+    static constexpr int NSTAGE = TJ == 8 ? 3 : BLK ? 4 : 5;
+    static constexpr int LDS = NSTAGE * STAGE;  // 160 KB / 144 KB; BLK: 132 KB / 147 KB
     static constexpr int BI = TJ / 2;           // Bt row groups (16 rows) per wave and unit
-    static constexpr int NDMA = 4 + 2 * BI;     // DMAs per wave and step
+    static constexpr int NDMA = 4 + 2 * BI + (BLK ? 1 : 0);  // DMAs per wave and step
 };
 
 __device__ __forceinline__ void dma_mid(const uint8_t* base, uint32_t voff, uint32_t lds_addr) {
     // M0 carries the LDS address; one wait state between the scalar write of M0 and its use
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds_addr) : "memory");
+}
+
+// 4 bytes a lane to 256 consecutive bytes
+__device__ __forceinline__ void dma_scales(const uint8_t* p, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_addr) : "memory");
+}
+
+// acc + first * second^T, each of the 16 rows of both scaled by its byte of scale_first / scale_second: the SF-th, the SS-th.
+template <int F1, int F2, int SF, int SS>
+__device__ __forceinline__ v4f_m mfma_block(const v8i& first, const v8i& second, const v4f_m& acc, uint32_t scale_first, uint32_t scale_second) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(first, second, acc, F1, F2, SF, (int)scale_first, SS, (int)scale_second);
+}
+template <int F1, int F2, int SF>
+__device__ __forceinline__ v4f_m mfma_block_ss(int ss, const v8i& first, const v8i& second, const v4f_m& acc, uint32_t scale_first, uint32_t scale_second) {
+    switch (ss) {  // a constant once the caller's loop is unrolled
+        case 0: return mfma_block<F1, F2, SF, 0>(first, second, acc, scale_first, scale_second);
+        case 1: return mfma_block<F1, F2, SF, 1>(first, second, acc, scale_first, scale_second);
+        case 2: return mfma_block<F1, F2, SF, 2>(first, second, acc, scale_first, scale_second);
+        default: return mfma_block<F1, F2, SF, 3>(first, second, acc, scale_first, scale_second);
+    }
+}
+template <int F1, int F2>
+__device__ __forceinline__ v4f_m mfma_block_any(int sf, int ss, const v8i& first, const v8i& second, const v4f_m& acc, uint32_t scale_first, uint32_t scale_second) {
+    switch (sf) {
+        case 0: return mfma_block_ss<F1, F2, 0>(ss, first, second, acc, scale_first, scale_second);
+        case 1: return mfma_block_ss<F1, F2, 1>(ss, first, second, acc, scale_first, scale_second);
+        case 2: return mfma_block_ss<F1, F2, 2>(ss, first, second, acc, scale_first, scale_second);
+        default: return mfma_block_ss<F1, F2, 3>(ss, first, second, acc, scale_first, scale_second);
+    }
 }
 
 // A float through the scalar cache (the address is the same for every lane).
@@ -83,12 +114,14 @@ __device__ __forceinline__ uint32_t mid_tr_voff(int instr, int64_t ld, int64_t u
 
 // Workgroup `bid` of the `grid` that compute this product (or one part of its k).
 // ODD_ROWS: rows of C start at odd multiples of two bytes too (see ShiftedRows); a piece is then stored behind the next one.
-template <int AF, int BF, int C_DT, int TJ, bool A_TR, bool B_TR, bool ODD_ROWS, bool BIAS_AFTER = false>
+// BLK: block scales (f8mi_block.h) in sa_blk / sb_blk, whose rows for the next 128 of k are sa_ld / sb_ld bytes on; sa_dev and sb_dev are not read.
+template <int AF, int BF, int C_DT, int TJ, bool A_TR, bool B_TR, bool ODD_ROWS, bool BIAS_AFTER = false, bool BLK = false>
 __device__ __forceinline__ void gemm_mid_tile(
     const int bid, const int grid, const int split, const uint8_t* __restrict__ A, int64_t lda, int64_t a_unit, const uint8_t* __restrict__ Bt,
     int64_t ldb, int64_t b_unit, int M, int N, int K, const float* sa_dev, const float* sb_dev, void* __restrict__ C,
-    int64_t ldc, const void* __restrict__ bias, int tiles_m, int tiles_n, int c_vec_ok, int k_splits, int bias_fp32 = 0) {
-    using Cfg = MidCfg<TJ>;
+    int64_t ldc, const void* __restrict__ bias, int tiles_m, int tiles_n, int c_vec_ok, int k_splits, int bias_fp32 = 0,
+    const uint8_t* __restrict__ sa_blk = nullptr, int64_t sa_ld = 0, const uint8_t* __restrict__ sb_blk = nullptr, int64_t sb_ld = 0) {
+    using Cfg = MidCfg<TJ, BLK>;
     constexpr int NSTAGE = Cfg::NSTAGE, NDMA = Cfg::NDMA;
     extern __shared__ __align__(16) uint8_t smem[];
     // consecutive workgroup ids go to the 8 XCDs round-robin; re-deal them so that one XCD (one L2) gets a contiguous
@@ -127,9 +160,20 @@ __device__ __forceinline__ void gemm_mid_tile(
     const int64_t k0 = (int64_t)split * K_part;
     const uint8_t* a_ptr = A_TR ? A + (int64_t)(m0 / 64) * a_unit + k0 * lda : A + (int64_t)m0 * lda + k0 / 64 * a_unit;
     const uint8_t* b_ptr = B_TR ? Bt + (int64_t)(n0 / 64) * b_unit + k0 * ldb : Bt + (int64_t)n0 * ldb + k0 / 64 * b_unit;
-    // DMA d = 0..NDMA-1 of this wave's share of a step (4 of A, then Bt); the pointers move on after the last
+    // Block scales, 256 bytes a wave: lanes 0 - 31 bring those of A's 128 rows, the others those of the 128 rows of Bt that hold the wave's
+    const uint8_t* s_ptr = nullptr;
+    int64_t s_step = 0;
+    if constexpr (BLK) {
+        const int64_t group = min((int64_t)n0 + (TJ == 8 ? wn * 128 : 0), sb_ld - 128);  // past the edge: the last group again
+        s_step = lane < 32 ? sa_ld : sb_ld;
+        s_ptr = (lane < 32 ? sa_blk + m0 : sb_blk + group) + (lane & 31) * 4 + k0 / 128 * s_step;
+    }
+    // DMA d = 0..NDMA-1 of this wave's share of a step (4 of A, then Bt, then the scales); the pointers move on after the last
     auto issue1 = [&](uint32_t base, int d) __attribute__((always_inline)) {
-        if (d < 4) {
+        if (BLK && d == NDMA - 1) {
+            dma_scales(s_ptr, base + Cfg::SCALES + wave * 256);
+            s_ptr += s_step;
+        } else if (d < 4) {
             if constexpr (A_TR) dma_mid(a_ptr, a_voff[d], base + (wave * 4 + d) * 1024);
             else dma_mid(a_ptr + (d >> 1) * a_unit, a_voff[d & 1], base + (d >> 1) * MID_A_UNIT + (wave * 2 + (d & 1)) * 1024);
         } else {
@@ -157,6 +201,14 @@ __device__ __forceinline__ void gemm_mid_tile(
 #pragma unroll
         for (int ti = 0; ti < 4; ti++) acc[tj][ti] = (v4f_m){0.f, 0.f, 0.f, 0.f};
     v8i fa[2][4], fb[2][TJ];  // [parity of the step]: one step's fragments are multiplied while the next one's are read
+    uint32_t fsa[2], fsb[2][TJ / 4];  // and their scales: byte ti; byte tj % 4 of word tj / 4
+    auto frag_scales = [&](const uint8_t* st, auto parity) __attribute__((always_inline)) {
+        constexpr int P = decltype(parity)::value;
+        const uint8_t* p = st + Cfg::SCALES + wave * 256 + (lane & 15) * 8;
+        fsa[P] = *(const uint32_t*)(p + 4 * wm);
+#pragma unroll
+        for (int i = 0; i < TJ / 4; i++) fsb[P][i] = *(const uint32_t*)(p + 128 + (TJ == 8 ? 4 * i : 4 * wn));
+    };
     // transposed operand: lane j of a 16-lane group q addresses contraction row 32q + 8t + j/2 (t-th read), byte column
     // tile*16 + 8*(j%2), through the slot swizzle (the same for all four reads of a lane)
     const int tr_row = 32 * fq + (frow >> 1);
@@ -185,6 +237,7 @@ __device__ __forceinline__ void gemm_mid_tile(
         for (int t = 0; t < 4; t++) fa[P][t] = frag_a(smem, t);
 #pragma unroll
         for (int t = 0; t < TJ; t++) fb[P][t] = frag_b(smem, t);
+        if constexpr (BLK) frag_scales(smem, parity);
     };
     constexpr std::integral_constant<int, 0> c0{};
     constexpr std::integral_constant<int, 1> c1{};
@@ -203,14 +256,14 @@ __device__ __forceinline__ void gemm_mid_tile(
     // 1 / (sa * sb) for the epilogue, kept in a scalar register.  The scales are asked for behind the DMAs (the pointers
     // pass through the asm, which keeps the compiler from moving the loads up): asked for first, the DMAs waited a
     // round trip to memory for them
-    asm volatile("" : "+s"(sa_dev), "+s"(sb_dev)::"memory");
-    const float inv = k_splits > 1 ? 1.0f : __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(
+    if constexpr (!BLK) asm volatile("" : "+s"(sa_dev), "+s"(sb_dev)::"memory");
+    const float inv = BLK || k_splits > 1 ? 1.0f : __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(
         int, __fdiv_rn(1.0f, load_scalar(sa_dev)) * __fdiv_rn(1.0f, load_scalar(sb_dev)))));
     // step 0's data is there; what was asked for behind it, min(steps, NSTAGE) - 1 steps, may still be in flight (with fewer steps than
     // stages too: waiting for all of it cost 512-deep products of many columns a tenth, 17 rows, 28672 x 512: 7.8 / 7.25 us)
     if (steps >= NSTAGE) mid_wait_barrier<(NSTAGE - 1) * NDMA>();
     else if (NSTAGE == 5 && steps == 4) mid_wait_barrier<3 * NDMA>();
-    else if (NSTAGE == 5 && steps == 3) mid_wait_barrier<2 * NDMA>();
+    else if (NSTAGE >= 4 && steps == 3) mid_wait_barrier<2 * NDMA>();
     else if (steps == 2) mid_wait_barrier<NDMA>();
     else mid_wait_barrier<0>();
     if (steps & 1) fetch_all(c0);
@@ -298,12 +351,16 @@ __device__ __forceinline__ void gemm_mid_tile(
 #pragma unroll
             for (int tj = 0; tj < TJ; tj++) {
                 const int i = ti * TJ + tj;
-                acc[tj][ti] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[P][tj], fa[P][ti], acc[tj][ti], BF, AF, 0, 0, 0, 0);
+                if constexpr (BLK) acc[tj][ti] = mfma_block_any<BF, AF>(tj & 3, ti, fb[P][tj], fa[P][ti], acc[tj][ti], fsb[P][tj >> 2], fsa[P]);
+                else acc[tj][ti] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[P][tj], fa[P][ti], acc[tj][ti], BF, AF, 0, 0, 0, 0);
                 if constexpr (MODE < 2) {
                     F8MI_SCHED_FENCE();
                     if (MODE == 0 && (i & 1) && i / 2 < NDMA) issue1(refill, i / 2);
+                    if (BLK && MODE == 0 && i == 4 * TJ - 1 && NDMA > 2 * TJ) issue1(refill, NDMA - 1);  // one more than there are places
                     if ((i & 1) == 0) {
                         const int f = i / 2;
+                        if constexpr (BLK)
+                            if (f == 0) frag_scales(st, std::integral_constant<int, P ^ 1>{});
                         if (f == 0) fa[P ^ 1][0] = frag_a(st, 0);
                         else if (f <= TJ) fb[P ^ 1][f - 1] = frag_b(st, f - 1);
                         else if (f < TJ + 4) fa[P ^ 1][f - TJ] = frag_a(st, f - TJ);
@@ -319,13 +376,17 @@ __device__ __forceinline__ void gemm_mid_tile(
     };
     constexpr std::integral_constant<int, NSTAGE - 2> steady{};
     int n_steady = steps - NSTAGE;  // steps that fetch
-    if (n_steady > 0 && (n_steady & 1)) { step(c1, c0, steady); n_steady--; }
+    constexpr std::integral_constant<int, NSTAGE & 1> last_steady{};  // parity of the last of them, NSTAGE steps before the last step
+    constexpr std::integral_constant<int, (NSTAGE & 1) ^ 1> before{};
+    if (n_steady > 0 && (n_steady & 1)) { step(last_steady, c0, steady); n_steady--; }
     for (; n_steady > 0; n_steady -= 2) {
-        step(c0, c0, steady);
-        step(c1, c0, steady);
+        step(before, c0, steady);
+        step(last_steady, c0, steady);
     }
     if constexpr (NSTAGE == 5) {
         if (steps >= 5) step(c0, c1, c3);
+        if (steps >= 4) step(c1, c1, c2);
+    } else if constexpr (NSTAGE == 4) {
         if (steps >= 4) step(c1, c1, c2);
     }
     if (steps >= 3) step(c0, c1, c1);

@@ -1,0 +1,500 @@
+// Layer norm over the last dimension: y = (x - mean) * rstd * w + b with rstd = 1 / sqrt(var + eps), and its backward pass
+//   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),  g = dy * w,  xhat = (x - mean) * rstd,
+//   dw = sum over rows of dy * xhat,  db = sum over rows of dy.
+// HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx.  A row stays in the registers of T lanes between its
+// first read and its last use (mean first, then the squares of what is left of it: no cancellation); a workgroup takes every
+// (number of workgroups)-th row, so that w and b are read once and, backward, a lane sums the columns it owns over its rows in
+// registers.  Backward's workgroups write those sums, fp32, and a second launch adds them in a fixed order.  Statistics and sums are fp32.
+//
+// Rows that do not fit (more than 16384 values of 16 bits, 8192 of fp32) are read once for each statistic and once for the result, out of the
+// L2 after the first time, and the column sums have a kernel of their own.
+#include <algorithm>
+
+#include "f8mi_gemm_util.h"
+
+namespace f8mi {
+
+template <int DT>
+struct Ln {
+    static constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2, V = 16 / SIZE;  // values of a lane's 16 bytes
+};
+
+template <int DT>
+__device__ __forceinline__ void ln_unpack(uint4 q, float (&v)[Ln<DT>::V]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (DT == F8MI_FP32) v[i] = __uint_as_float(w[i]);
+        else unpack2<DT>(w[i], v[2 * i], v[2 * i + 1]);
+    }
+}
+// values col .. col + V - 1 of a row, zeros past the end
+template <int DT>
+__device__ __forceinline__ uint4 ln_load(const uint8_t* row, int64_t col, int64_t cols) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+    if (col + V <= cols) return load_nt16_any(row + col * SIZE);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (col + i < cols) {
+            if constexpr (DT == F8MI_FP32) w[i] = ((const uint32_t*)row)[col + i];
+            else w[i >> 1] |= (uint32_t)((const uint16_t*)row)[col + i] << (16 * (i & 1));
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int DT>
+__device__ __forceinline__ void ln_store(uint8_t* row, int64_t col, int64_t cols, const float (&v)[Ln<DT>::V]) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (DT == F8MI_FP32) w[i] = __float_as_uint(v[i]);
+        else w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+    }
+    if (col + V <= cols) {
+        store16_any(row + col * SIZE, make_uint4(w[0], w[1], w[2], w[3]));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (col + i < cols) {
+            if constexpr (DT == F8MI_FP32) ((uint32_t*)row)[col + i] = w[i];
+            else ((uint16_t*)row)[col + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        }
+}
+// V values of a parameter (`otherwise` without one)
+template <int PT, int V>
+__device__ __forceinline__ void ln_param(const void* p, int64_t col, int64_t cols, float otherwise, float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = p && col + i < cols ? load_bias<PT>(p, (int)(col + i)) : otherwise;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+// Two sums over the T lanes of a row, in every one of them.  `slots`: two floats for each wave of the workgroup, not in use elsewhere
+// until the next barrier but one.
+template <int T>
+__device__ __forceinline__ void row_sums(float& a, float& b, float2* slots) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (T > 64) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) slots[wave] = make_float2(a, b);
+        __syncthreads();
+        const int first = wave / (T / 64) * (T / 64);
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < T / 64; i++) {
+            const float2 s = slots[first + i];
+            a += s.x;
+            b += s.y;
+        }
+    }
+}
+
+constexpr int ln_threads(int t) { return t < 256 ? 256 : t; }
+
+// T lanes a row, VPT pieces of 16 bytes a lane
+template <int DT, int PT, int T, int VPT>
+__global__ __launch_bounds__(ln_threads(T)) void layer_norm_kernel(const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int64_t cols, const void* __restrict__ weight,
+                                                                   const void* __restrict__ bias, float eps, uint8_t* __restrict__ y, float2* __restrict__ stats) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_threads(T) / T;
+    __shared__ float2 slots[2][ln_threads(T) / 64];
+    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    const float inv_cols = 1.0f / (float)cols;
+    float w[VPT][V], b[VPT][V];
+#pragma unroll
+    for (int p = 0; p < VPT; p++) {
+        ln_param<PT, V>(weight, (int64_t)(p * T + t) * V, cols, 1.f, w[p]);
+        ln_param<PT, V>(bias, (int64_t)(p * T + t) * V, cols, 0.f, b[p]);
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += (int64_t)gridDim.x * GROUPS) {
+        const int64_t row = r0 + group;
+        const bool in = row < rows;
+        uint4 q[VPT];
+        float v[VPT][V];
+#pragma unroll
+        for (int p = 0; p < VPT; p++) q[p] = in ? ln_load<DT>(x + row * ld * SIZE, (int64_t)(p * T + t) * V, cols) : make_uint4(0u, 0u, 0u, 0u);
+        float s = 0.f, none = 0.f;
+#pragma unroll
+        for (int p = 0; p < VPT; p++) {
+            ln_unpack<DT>(q[p], v[p]);
+#pragma unroll
+            for (int i = 0; i < V; i++) s += v[p][i];
+        }
+        row_sums<T>(s, none, slots[0]);
+        const float mean = s * inv_cols;
+        s = 0.f;
+#pragma unroll
+        for (int p = 0; p < VPT; p++)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                v[p][i] -= mean;
+                if ((int64_t)(p * T + t) * V + i < cols) s = __builtin_fmaf(v[p][i], v[p][i], s);
+            }
+        row_sums<T>(s, none, slots[1]);
+        const float rstd = 1.0f / __builtin_sqrtf(s * inv_cols + eps);
+        if (!in) continue;
+#pragma unroll
+        for (int p = 0; p < VPT; p++) {
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] = __builtin_fmaf(v[p][i] * rstd, w[p][i], b[p][i]);
+            const int64_t col = (int64_t)(p * T + t) * V;
+            if (col < cols) ln_store<DT>(y + row * cols * SIZE, col, cols, o);
+        }
+        if (stats && t == 0) stats[row] = make_float2(mean, rstd);
+    }
+}
+
+template <int DT, int PT, int T, int VPT>
+__global__ __launch_bounds__(ln_threads(T)) void layer_norm_backward_kernel(const uint8_t* __restrict__ dy, int64_t ld_dy, const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                                            const void* __restrict__ weight, const float2* __restrict__ stats, uint8_t* __restrict__ dx,
+                                                                            float* __restrict__ partial) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_threads(T) / T;
+    __shared__ float2 slots[2][ln_threads(T) / 64];
+    __shared__ float sums[GROUPS > 1 ? (GROUPS - 1) * T * 2 * V : 1];
+    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    const float inv_cols = 1.0f / (float)cols;
+    float w[VPT][V], dw[VPT][V], db[VPT][V];
+#pragma unroll
+    for (int p = 0; p < VPT; p++) {
+        ln_param<PT, V>(weight, (int64_t)(p * T + t) * V, cols, 1.f, w[p]);
+#pragma unroll
+        for (int i = 0; i < V; i++) dw[p][i] = db[p][i] = 0.f;
+    }
+    int parity = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += (int64_t)gridDim.x * GROUPS, parity ^= 1) {
+        const int64_t row = r0 + group;
+        const bool in = row < rows;
+        uint4 qx[VPT], qg[VPT];
+#pragma unroll
+        for (int p = 0; p < VPT; p++) {
+            const int64_t col = (int64_t)(p * T + t) * V;
+            qx[p] = in ? ln_load<DT>(x + row * ld * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
+            qg[p] = in ? ln_load<DT>(dy + row * ld_dy * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        const float2 st = in ? stats[row] : make_float2(0.f, 0.f);
+        float xh[VPT][V], g[VPT][V], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int p = 0; p < VPT; p++) {
+            ln_unpack<DT>(qx[p], xh[p]);
+            ln_unpack<DT>(qg[p], g[p]);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                xh[p][i] = (xh[p][i] - st.x) * st.y;
+                dw[p][i] = __builtin_fmaf(g[p][i], xh[p][i], dw[p][i]);
+                db[p][i] += g[p][i];
+                g[p][i] *= w[p][i];  // (past the end dy, and so g, is zero)
+                s1 += g[p][i];
+                s2 = __builtin_fmaf(g[p][i], xh[p][i], s2);
+            }
+        }
+        if (!dx) continue;
+        row_sums<T>(s1, s2, slots[parity]);
+        s1 *= inv_cols;
+        s2 *= inv_cols;
+        if (!in) continue;
+#pragma unroll
+        for (int p = 0; p < VPT; p++) {
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] = st.y * (g[p][i] - s1 - xh[p][i] * s2);
+            const int64_t col = (int64_t)(p * T + t) * V;
+            if (col < cols) ln_store<DT>(dx + row * cols * SIZE, col, cols, o);
+        }
+    }
+    if (!partial) return;
+    // one row of sums a workgroup: dw, then db
+    float* out = partial + (int64_t)blockIdx.x * 2 * cols;
+#pragma unroll
+    for (int p = 0; p < VPT; p++) {
+        if constexpr (GROUPS > 1) {
+            __syncthreads();
+            if (group > 0)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    sums[(((group - 1) * 2 + 0) * V + i) * T + t] = dw[p][i];
+                    sums[(((group - 1) * 2 + 1) * V + i) * T + t] = db[p][i];
+                }
+            __syncthreads();
+            if (group > 0) continue;
+#pragma unroll
+            for (int k = 0; k < GROUPS - 1; k++)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    dw[p][i] += sums[((k * 2 + 0) * V + i) * T + t];
+                    db[p][i] += sums[((k * 2 + 1) * V + i) * T + t];
+                }
+        }
+        const int64_t col = (int64_t)(p * T + t) * V;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (col + i < cols) {
+                out[col + i] = dw[p][i];
+                out[cols + col + i] = db[p][i];
+            }
+    }
+}
+
+// ---- rows that do not fit in registers: a workgroup a row
+constexpr int LN_WIDE_THREADS = 1024;
+
+template <int DT, int PT>
+__global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_wide_kernel(const uint8_t* __restrict__ x, int64_t ld, int64_t cols, const void* __restrict__ weight,
+                                                                          const void* __restrict__ bias, float eps, uint8_t* __restrict__ y, float2* __restrict__ stats) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+    __shared__ float2 slots[2][LN_WIDE_THREADS / 64];
+    const uint8_t* row = x + blockIdx.x * ld * SIZE;
+    float v[V], s = 0.f, none = 0.f;
+    for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
+        ln_unpack<DT>(ln_load<DT>(row, col, cols), v);
+#pragma unroll
+        for (int i = 0; i < V; i++) s += v[i];
+    }
+    row_sums<LN_WIDE_THREADS>(s, none, slots[0]);
+    const float mean = s / (float)cols;
+    s = 0.f;
+    for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
+        ln_unpack<DT>(ln_load<DT>(row, col, cols), v);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (col + i < cols) s = __builtin_fmaf(v[i] - mean, v[i] - mean, s);
+    }
+    row_sums<LN_WIDE_THREADS>(s, none, slots[1]);
+    const float rstd = 1.0f / __builtin_sqrtf(s / (float)cols + eps);
+    for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
+        float w[V], b[V];
+        ln_unpack<DT>(ln_load<DT>(row, col, cols), v);
+        ln_param<PT, V>(weight, col, cols, 1.f, w);
+        ln_param<PT, V>(bias, col, cols, 0.f, b);
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = __builtin_fmaf((v[i] - mean) * rstd, w[i], b[i]);
+        ln_store<DT>(y + blockIdx.x * cols * SIZE, col, cols, v);
+    }
+    if (stats && threadIdx.x == 0) stats[blockIdx.x] = make_float2(mean, rstd);
+}
+
+template <int DT, int PT>
+__global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_backward_wide_kernel(const uint8_t* __restrict__ dy, int64_t ld_dy, const uint8_t* __restrict__ x, int64_t ld, int64_t cols,
+                                                                                   const void* __restrict__ weight, const float2* __restrict__ stats, uint8_t* __restrict__ dx) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+    __shared__ float2 slots[LN_WIDE_THREADS / 64];
+    const uint8_t *row = x + blockIdx.x * ld * SIZE, *grow = dy + blockIdx.x * ld_dy * SIZE;
+    const float2 st = stats[blockIdx.x];
+    float xv[V], g[V], w[V], s1 = 0.f, s2 = 0.f;
+    for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
+        ln_unpack<DT>(ln_load<DT>(row, col, cols), xv);
+        ln_unpack<DT>(ln_load<DT>(grow, col, cols), g);
+        ln_param<PT, V>(weight, col, cols, 1.f, w);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            g[i] *= w[i];
+            s1 += g[i];
+            s2 = __builtin_fmaf(g[i], (xv[i] - st.x) * st.y, s2);
+        }
+    }
+    row_sums<LN_WIDE_THREADS>(s1, s2, slots);
+    s1 /= (float)cols;
+    s2 /= (float)cols;
+    for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
+        ln_unpack<DT>(ln_load<DT>(row, col, cols), xv);
+        ln_unpack<DT>(ln_load<DT>(grow, col, cols), g);
+        ln_param<PT, V>(weight, col, cols, 1.f, w);
+#pragma unroll
+        for (int i = 0; i < V; i++) g[i] = st.y * (g[i] * w[i] - s1 - (xv[i] - st.x) * st.y * s2);
+        ln_store<DT>(dx + blockIdx.x * cols * SIZE, col, cols, g);
+    }
+}
+
+// column sums of dy * xhat and dy: 256 lanes' columns of `chunk` rows a workgroup
+template <int DT>
+__global__ __launch_bounds__(256) void layer_norm_columns_kernel(const uint8_t* __restrict__ dy, int64_t ld_dy, const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                                 const float2* __restrict__ stats, int64_t chunk, float* __restrict__ partial) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+    const int64_t col = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+    if (col >= cols) return;
+    float dw[V], db[V], xv[V], g[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) dw[i] = db[i] = 0.f;
+    const int64_t end = std::min<int64_t>(rows, (blockIdx.y + 1) * chunk);
+#pragma unroll 4
+    for (int64_t r = blockIdx.y * chunk; r < end; r++) {
+        const float2 st = stats[r];
+        ln_unpack<DT>(ln_load<DT>(x + r * ld * SIZE, col, cols), xv);
+        ln_unpack<DT>(ln_load<DT>(dy + r * ld_dy * SIZE, col, cols), g);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            dw[i] = __builtin_fmaf(g[i], (xv[i] - st.x) * st.y, dw[i]);
+            db[i] += g[i];
+        }
+    }
+    float* out = partial + (int64_t)blockIdx.y * 2 * cols;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (col + i < cols) {
+            out[col + i] = dw[i];
+            out[cols + col + i] = db[i];
+        }
+}
+
+// Adds the `parts` rows of sums: 64 of the 2 * cols columns a workgroup, a wave every 16th row of them
+constexpr int LN_FINISH_WAVES = 16;
+__global__ __launch_bounds__(64 * LN_FINISH_WAVES) void layer_norm_finish_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols, void* __restrict__ dw,
+                                                                                 void* __restrict__ db, int p_dtype) {
+    __shared__ float red[LN_FINISH_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (col < 2 * cols) {
+#pragma unroll 8
+        for (int64_t i = wave; i < parts; i += LN_FINISH_WAVES) s += partial[i * 2 * cols + col];
+    }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || col >= 2 * cols) return;
+    s = red[0][lane];
+#pragma unroll
+    for (int i = 1; i < LN_FINISH_WAVES; i++) s += red[i][lane];
+    void* out = col < cols ? dw : db;
+    const int64_t at = col < cols ? col : col - cols;
+    if (!out) return;
+    if (p_dtype == F8MI_FP32) ((float*)out)[at] = s;
+    else if (p_dtype == F8MI_BF16) ((uint16_t*)out)[at] = (uint16_t)pack2<F8MI_BF16>(s, 0.f);
+    else ((uint16_t*)out)[at] = (uint16_t)pack2<F8MI_FP16>(s, 0.f);
+}
+
+struct LnArgs {
+    const uint8_t *dy, *x;
+    int64_t ld_dy, ld, rows, cols;
+    const void *weight, *bias;
+    float eps;
+    uint8_t* out;  // y, dx
+    float2* stats;
+    float* partial;
+    int64_t parts;  // workgroups of the backward kernel
+    hipStream_t stream;
+};
+
+// Lanes of a row and pieces a lane, by the number of 16-byte pieces of a row; 0: does not fit.
+struct LnShape {
+    int t, vpt;
+};
+static LnShape ln_shape(int64_t cols, int dtype) {
+    const int64_t pieces = (cols + (dtype == F8MI_FP32 ? 3 : 7)) / (dtype == F8MI_FP32 ? 4 : 8);
+    if (pieces <= 64) return {64, 1};
+    if (pieces <= 128) return {64, 2};
+    if (pieces <= 256) return {256, 1};
+    if (pieces <= 512) return {256, 2};
+    if (pieces <= 1024) return {512, 2};
+    if (pieces <= 2048) return {1024, 2};
+    return {0, 0};
+}
+static int64_t ln_groups(LnShape s) { return s.t && s.t < 256 ? 256 / s.t : 1; }
+// workgroups that together hold every CU's lanes, no more than there are rows
+static int64_t ln_workgroups(LnShape s, int64_t rows, int lanes_per_cu) {
+    const int64_t wg = std::max(s.t, 256), most = (int64_t)cu_count() * std::max<int64_t>(1, lanes_per_cu / wg);
+    return std::min(most, (rows + ln_groups(s) - 1) / ln_groups(s));
+}
+// Rows of sums that backward writes: two workgroups of 256 lanes a CU, one of more
+constexpr int LN_BACKWARD_LANES = 1024, LN_FORWARD_LANES = 2048;
+static int64_t ln_chunk_rows(int64_t rows, int64_t cols, int dtype) {  // of the column kernel for wide rows: 1024 workgroups or so
+    const int64_t strips = (cols + (dtype == F8MI_FP32 ? 1023 : 2047)) / (dtype == F8MI_FP32 ? 1024 : 2048), want = std::max<int64_t>(1, 1024 / strips);
+    return std::max<int64_t>(8, (rows + want - 1) / want);
+}
+static int64_t ln_parts(int64_t rows, int64_t cols, int dtype) {
+    const LnShape s = ln_shape(cols, dtype);
+    if (s.t) return ln_workgroups(s, rows, LN_BACKWARD_LANES);
+    const int64_t chunk = ln_chunk_rows(rows, cols, dtype);
+    return (rows + chunk - 1) / chunk;
+}
+
+template <int DT, int PT, int T, int VPT>
+static int launch_ln(const LnArgs& a, bool backward) {
+    const LnShape s{T, VPT};
+    if (backward) {
+        hipLaunchKernelGGL((layer_norm_backward_kernel<DT, PT, T, VPT>), dim3((unsigned)a.parts), dim3(ln_threads(T)), 0, a.stream, a.dy, a.ld_dy, a.x, a.ld, a.rows, a.cols, a.weight,
+                           a.stats, a.out, a.partial);
+        return check_hip(hipGetLastError(), "layer norm backward kernel launch");
+    }
+    hipLaunchKernelGGL((layer_norm_kernel<DT, PT, T, VPT>), dim3((unsigned)ln_workgroups(s, a.rows, LN_FORWARD_LANES)), dim3(ln_threads(T)), 0, a.stream, a.x, a.ld, a.rows, a.cols,
+                       a.weight, a.bias, a.eps, a.out, a.stats);
+    return check_hip(hipGetLastError(), "layer norm kernel launch");
+}
+template <int DT, int PT>
+static int launch_ln_wide(const LnArgs& a, bool backward) {
+    if (!backward) {
+        hipLaunchKernelGGL((layer_norm_wide_kernel<DT, PT>), dim3((unsigned)a.rows), dim3(LN_WIDE_THREADS), 0, a.stream, a.x, a.ld, a.cols, a.weight, a.bias, a.eps, a.out, a.stats);
+        return check_hip(hipGetLastError(), "layer norm kernel launch");
+    }
+    if (a.out)
+        hipLaunchKernelGGL((layer_norm_backward_wide_kernel<DT, PT>), dim3((unsigned)a.rows), dim3(LN_WIDE_THREADS), 0, a.stream, a.dy, a.ld_dy, a.x, a.ld, a.cols, a.weight, a.stats, a.out);
+    if (a.partial) {
+        const unsigned strips = (unsigned)((a.cols + 256 * Ln<DT>::V - 1) / (256 * Ln<DT>::V));
+        hipLaunchKernelGGL(layer_norm_columns_kernel<DT>, dim3(strips, (unsigned)a.parts), dim3(256), 0, a.stream, a.dy, a.ld_dy, a.x, a.ld, a.rows, a.cols, a.stats,
+                           ln_chunk_rows(a.rows, a.cols, DT), a.partial);
+    }
+    return check_hip(hipGetLastError(), "layer norm backward kernel launch");
+}
+template <int DT, int PT>
+static int launch_ln_by_size(const LnArgs& a, bool backward) {
+    const LnShape s = ln_shape(a.cols, DT);
+    if (s.t == 64 && s.vpt == 1) return launch_ln<DT, PT, 64, 1>(a, backward);
+    if (s.t == 64) return launch_ln<DT, PT, 64, 2>(a, backward);
+    if (s.t == 256 && s.vpt == 1) return launch_ln<DT, PT, 256, 1>(a, backward);
+    if (s.t == 256) return launch_ln<DT, PT, 256, 2>(a, backward);
+    if (s.t == 512) return launch_ln<DT, PT, 512, 2>(a, backward);
+    if (s.t == 1024) return launch_ln<DT, PT, 1024, 2>(a, backward);
+    return launch_ln_wide<DT, PT>(a, backward);
+}
+static int launch_ln_by_type(int dtype, int p_dtype, const LnArgs& a, bool backward) {
+    if (dtype == F8MI_BF16) return p_dtype == F8MI_FP32 ? launch_ln_by_size<F8MI_BF16, F8MI_FP32>(a, backward) : launch_ln_by_size<F8MI_BF16, F8MI_BF16>(a, backward);
+    if (dtype == F8MI_FP16) return p_dtype == F8MI_FP32 ? launch_ln_by_size<F8MI_FP16, F8MI_FP32>(a, backward) : launch_ln_by_size<F8MI_FP16, F8MI_FP16>(a, backward);
+    return launch_ln_by_size<F8MI_FP32, F8MI_FP32>(a, backward);
+}
+
+static int ln_check(const char* what, int64_t rows, int64_t cols, int dtype, int p_dtype) {
+    if (dtype < 0 || dtype > 2 || (p_dtype != dtype && p_dtype != F8MI_FP32)) { set_error("%s: parameters have x's type or are fp32 (dtype codes %d, %d)", what, dtype, p_dtype); return F8MI_ERR_INVALID_ARG; }
+    if (rows < 0 || cols <= 0) { set_error("%s: bad shape rows=%lld cols=%lld", what, (long long)rows, (long long)cols); return F8MI_ERR_INVALID_ARG; }
+    if (rows > 0x7fffffff || cols > 0x7fffff00) { set_error("%s: dimension too large", what); return F8MI_ERR_UNSUPPORTED; }
+    return F8MI_OK;
+}
+
+}  // namespace f8mi
+
+using namespace f8mi;
+
+extern "C" int f8mi_layer_norm(const void* x, int64_t rows, int64_t cols, int64_t ld, int dtype, const void* weight, const void* bias, int p_dtype, float eps, void* y,
+                               float* stats, void* stream) {
+    if (int rc = ln_check("f8mi_layer_norm", rows, cols, dtype, p_dtype)) return rc;
+    if (rows == 0) return F8MI_OK;
+    if (!x || !y || ld < 0 || (ld < cols && ld != 0)) { set_error("f8mi_layer_norm: null pointer or ld=%lld < cols=%lld", (long long)ld, (long long)cols); return F8MI_ERR_INVALID_ARG; }
+    if ((uintptr_t)stats % 8 != 0) { set_error("f8mi_layer_norm: statistics are 8-byte aligned pairs"); return F8MI_ERR_INVALID_ARG; }
+    return launch_ln_by_type(dtype, p_dtype, {nullptr, (const uint8_t*)x, 0, ld, rows, cols, weight, bias, eps, (uint8_t*)y, (float2*)stats, nullptr, 0, (hipStream_t)stream}, false);
+}
+
+extern "C" int64_t f8mi_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
+    return rows <= 0 || cols <= 0 || dtype < 0 || dtype > 2 ? 0 : ln_parts(rows, cols, dtype) * 2 * cols * 4;
+}
+
+extern "C" int f8mi_layer_norm_backward(const void* dy, int64_t ld_dy, const void* x, int64_t ld, int64_t rows, int64_t cols, int dtype, const void* weight, int p_dtype,
+                                        const float* stats, void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    if (int rc = ln_check("f8mi_layer_norm_backward", rows, cols, dtype, p_dtype)) return rc;
+    if (!dx && !dweight && !dbias) return F8MI_OK;
+    const bool sums = dweight || dbias;
+    if (rows > 0 && (!dy || !x || !stats || ld < 0 || (ld < cols && ld != 0) || ld_dy < 0 || (ld_dy < cols && ld_dy != 0))) { set_error("f8mi_layer_norm_backward: null pointer or row stride"); return F8MI_ERR_INVALID_ARG; }
+    if ((uintptr_t)stats % 8 != 0) { set_error("f8mi_layer_norm_backward: statistics are 8-byte aligned pairs"); return F8MI_ERR_INVALID_ARG; }
+    const int64_t need = sums ? f8mi_layer_norm_workspace_bytes(rows, cols, dtype) : 0;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0)) { set_error("f8mi_layer_norm_backward: workspace of %lld bytes needed", (long long)need); return F8MI_ERR_INVALID_ARG; }
+    const int64_t parts = rows > 0 ? ln_parts(rows, cols, dtype) : 0;
+    if (rows > 0)
+        if (int rc = launch_ln_by_type(dtype, p_dtype, {(const uint8_t*)dy, (const uint8_t*)x, ld_dy, ld, rows, cols, weight, nullptr, 0.f, (uint8_t*)dx, (float2*)stats,
+                                                         sums ? (float*)workspace : nullptr, parts, stream}, true)) return rc;
+    if (sums)
+        hipLaunchKernelGGL(layer_norm_finish_kernel, dim3((unsigned)((2 * cols + 63) / 64)), dim3(64 * LN_FINISH_WAVES), 0, stream, (const float*)workspace, parts, cols, dweight, dbias, p_dtype);
+    return check_hip(hipGetLastError(), "layer norm column sum kernel launch");
+}

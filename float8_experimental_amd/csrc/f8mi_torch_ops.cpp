@@ -1,0 +1,454 @@
+// The host path of the blockwise scaled linear, layer norm and gradient clipping over libf8mi's C ABI, as a CPython module on torch
+// tensors: one call allocates what the kernels write and queues all launches, and the backward passes are nodes that run without the
+// interpreter.  Host code only.
+//
+// Every function returns None, without having queued or allocated anything, for tensors that it does not take (subclasses, other devices or
+// types): the caller then goes through the registered operators, or raises.  Workspaces are temporaries of torch's caching allocator, which
+// hands their memory out again in stream order: calls on any number of threads, streams and captures share nothing.
+#include <dlfcn.h>
+
+#include <optional>
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+#include "../../include/f8mi.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Lib {
+    decltype(&f8mi_block_scale_bytes) block_scale_bytes;
+    decltype(&f8mi_block_cast) block_cast;
+    decltype(&f8mi_block_gemm) block_gemm;
+    decltype(&f8mi_block_gemm_workspace_bytes) block_gemm_workspace_bytes;
+    decltype(&f8mi_column_sum) column_sum;
+    decltype(&f8mi_column_sum_workspace_bytes) column_sum_workspace_bytes;
+    decltype(&f8mi_layer_norm) layer_norm;
+    decltype(&f8mi_layer_norm_backward) layer_norm_backward;
+    decltype(&f8mi_layer_norm_workspace_bytes) layer_norm_workspace_bytes;
+    decltype(&f8mi_grad_clip) grad_clip;
+    decltype(&f8mi_grad_clip_workspace_bytes) grad_clip_workspace_bytes;
+    decltype(&f8mi_last_error) last_error;
+} L;
+PyObject* native_error = nullptr;  // float8_experimental_amd._native.Float8NativeError
+
+struct NativeFailure : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+void check(int rc, const char* what) {
+    if (rc != 0) throw NativeFailure(std::string(what) + " failed with code " + std::to_string(rc) + ": " + L.last_error());
+}
+
+int dtype_code(at::ScalarType t) {
+    return t == at::kBFloat16 ? F8MI_BF16 : t == at::kHalf ? F8MI_FP16 : t == at::kFloat ? F8MI_FP32 : -1;
+}
+void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// Undefined: not taken.  A plain tensor (or Parameter) of a type that the kernels read, on the current device, whose memory holds its values
+at::Tensor plain(PyObject* o, int device) {
+    if (!THPVariable_CheckExact(o) || c10::impl::TorchDispatchModeTLS::any_modes_set()) return {};
+    const at::Tensor& t = THPVariable_Unpack(o);
+    using K = c10::DispatchKey;
+    constexpr c10::DispatchKeySet others({K::Python, K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Batched, K::Functionalize, K::Negative, K::ZeroTensor});
+    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(others) && t.get_device() == device && dtype_code(t.scalar_type()) >= 0 ? t : at::Tensor();
+}
+
+// A matrix as the kernels read it: unit column stride, `ld` from row to row (0: the same row throughout); copied where its layout needs it.
+struct Rows {
+    at::Tensor t;
+    int64_t rows, cols, ld;
+    Rows(const at::Tensor& x, int64_t cols_) : cols(cols_) {
+        rows = cols ? x.numel() / cols : 0;
+        t = x.is_neg() ? x.resolve_neg() : x;
+        if (t.dim() == 2 && t.size(1) == cols && (t.stride(1) == 1 || cols == 1) && (t.stride(0) >= cols || rows == 1)) {
+            ld = rows == 1 ? cols : t.stride(0);
+            return;
+        }
+        if (t.dim() >= 2 && t.size(-1) == cols && t.stride(-1) == 1 && rows > 1) {
+            bool one = true;  // expanded over all leading dimensions: what autograd hands to backward after a sum
+            for (int64_t d = 0; d + 1 < t.dim(); d++) one &= t.stride(d) == 0 || t.size(d) == 1;
+            if (one) {
+                ld = 0;
+                return;
+            }
+        }
+        t = t.contiguous();
+        ld = cols;
+    }
+    int dtype() const { return dtype_code(t.scalar_type()); }
+};
+
+// ---- blockwise scaled linear
+
+struct Blocks {  // a copy and its scales
+    at::Tensor data, scales;
+    static Blocks make(const at::Tensor& like, int64_t rows, int64_t k, bool with_data = true) {
+        const int64_t kp = (k + 127) / 128 * 128;
+        Blocks b;
+        if (with_data) b.data = at::empty({kp / 64, rows, 64}, like.options().dtype(at::kFloat8_e4m3fn));
+        b.scales = at::empty({kp / 128, (rows + 127) / 128 * 128}, like.options().dtype(at::kByte));
+        return b;
+    }
+};
+f8mi_block_cast_job job_of(const Rows& x, bool square, const Blocks& a, const Blocks& t) {
+    return {x.t.data_ptr(), x.rows, x.cols, x.ld, x.dtype(), square, ptr(a.data), a.data.defined() ? ptr(a.scales) : nullptr, ptr(t.data), ptr(t.scales)};
+}
+// [m, n] = a [m, k] times b [n, k]; `of`: the copy that b's product reads, the other one of the tensor with transposed
+at::Tensor block_gemm(const Blocks& a, const at::Tensor& b_data, const at::Tensor& b_scales, bool transposed, int64_t m, int64_t n, int64_t k, at::ScalarType type,
+                      const at::Tensor& bias = {}) {
+    const int64_t kp = (k + 127) / 128 * 128;
+    at::Tensor c = at::empty({m, n}, a.data.options().dtype(type));
+    const int64_t bytes = transposed ? 0 : L.block_gemm_workspace_bytes(m, n, kp);
+    const at::Tensor ws = bytes ? at::empty({bytes / 4}, a.data.options().dtype(at::kFloat)) : at::Tensor();
+    check(L.block_gemm(a.data.data_ptr(), a.scales.data_ptr(), b_data.data_ptr(), b_scales.data_ptr(), transposed, m, n, kp, c.data_ptr(), dtype_code(type), n, ptr(bias),
+                       ptr(ws), bytes, stream_of(c)), "f8mi_block_gemm");
+    return c;
+}
+at::Tensor column_sum(const Rows& dy, at::ScalarType type) {
+    const int64_t bytes = L.column_sum_workspace_bytes(dy.rows, dy.cols, dy.dtype());
+    const at::Tensor out = at::empty({dy.cols}, dy.t.options().dtype(type)), ws = bytes ? at::empty({bytes / 4}, dy.t.options().dtype(at::kFloat)) : at::Tensor();
+    check(L.column_sum(dy.t.data_ptr(), dy.rows, dy.cols, dy.ld, dy.dtype(), out.data_ptr(), dtype_code(type), ptr(ws), bytes, stream_of(out)), "f8mi_column_sum");
+    return out;
+}
+
+// The weight needs one copy if the backward product can read it transposed
+bool one_weight_copy(int64_t k, int64_t n) { return k % 128 == 0 && n % 128 == 0; }
+
+// An argument that may be absent: autograd gives it an edge only where it is there.
+using MaybeTensor = std::optional<at::Tensor>;
+MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+
+struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& bias_, bool need_dx, bool need_dw) {
+        const at::Tensor bias = bias_.value_or(at::Tensor());
+        const c10::DeviceGuard guard(x.device());
+        const int64_t k = weight.size(1), n = weight.size(0);
+        const Rows xr(x, k), wr(weight, k);
+        const int64_t m = xr.rows;
+        std::vector<int64_t> y_shape(x.sizes().begin(), x.sizes().end());
+        y_shape.back() = n;
+        ctx->saved_data["x_shape"] = x.sizes().vec();
+        ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
+        ctx->saved_data["w_type"] = (int64_t)weight.scalar_type();
+        ctx->saved_data["b_type"] = bias.defined() ? (int64_t)bias.scalar_type() : -1;
+        ctx->saved_data["k"] = k;
+        ctx->saved_data["n"] = n;
+        if (m == 0) {
+            ctx->save_for_backward({});
+            return at::empty(y_shape, x.options());
+        }
+        const bool one = one_weight_copy(k, n);
+        const Blocks x8 = Blocks::make(x, m, k), x8t = need_dw ? Blocks::make(x, k, m) : Blocks();
+        const Blocks w8 = Blocks::make(x, n, k), w8t = need_dx ? Blocks::make(x, k, n, !one) : Blocks();
+        const f8mi_block_cast_job jobs[2] = {job_of(xr, false, x8, x8t), job_of(wr, true, w8, w8t)};
+        check(L.block_cast(jobs, 2, stream_of(x)), "f8mi_block_cast");
+        const at::Tensor b = bias.defined() ? bias.to(x.scalar_type()).contiguous() : at::Tensor();
+        at::Tensor y = block_gemm(x8, w8.data, w8.scales, false, m, n, k, x.scalar_type(), b);
+        ctx->save_for_backward({x8t.data, x8t.scales, one && need_dx ? w8.data : w8t.data, w8t.scales});
+        return x.dim() == 2 ? y : at::_unsafe_view(y, y_shape);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "blockwise_linear has no second derivative (create_graph=True)");
+        const auto saved = ctx->get_saved_variables();
+        const int64_t k = ctx->saved_data["k"].toInt(), n = ctx->saved_data["n"].toInt();
+        const at::ScalarType xt = (at::ScalarType)ctx->saved_data["x_type"].toInt(), wt = (at::ScalarType)ctx->saved_data["w_type"].toInt();
+        const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
+        const bool need_db = ctx->saved_data["b_type"].toInt() >= 0 && ctx->needs_input_grad(2);
+        at::Tensor dx, dw, db;
+        if (!grads[0].defined()) return {dx, dw, db, at::Tensor(), at::Tensor()};
+        const c10::DeviceGuard guard(grads[0].device());
+        const auto x_shape = ctx->saved_data["x_shape"].toIntVector();
+        const Rows dy(grads[0].scalar_type() == xt ? grads[0] : grads[0].to(xt), n);
+        const int64_t m = dy.rows;
+        if (m == 0) {
+            if (need_dx) dx = at::empty(x_shape, dy.t.options());
+            if (need_dw) dw = at::zeros({n, k}, dy.t.options().dtype(wt));
+            if (need_db) db = at::zeros({n}, dy.t.options().dtype((at::ScalarType)ctx->saved_data["b_type"].toInt()));
+            return {dx, dw, db, at::Tensor(), at::Tensor()};
+        }
+        if (need_dx || need_dw) {
+            TORCH_CHECK((!need_dx || saved[3].defined()) && (!need_dw || saved[0].defined()), "blockwise_linear: a gradient is asked for that the forward pass was not told of");
+            const Blocks g8 = need_dx ? Blocks::make(dy.t, m, n) : Blocks(), g8t = need_dw ? Blocks::make(dy.t, n, m) : Blocks();
+            const f8mi_block_cast_job job = job_of(dy, false, g8, g8t);
+            check(L.block_cast(&job, 1, stream_of(dy.t)), "f8mi_block_cast");
+            if (need_dx) {
+                dx = block_gemm(g8, saved[2], saved[3], one_weight_copy(k, n), m, k, n, xt);
+                if (x_shape.size() != 2) dx = dx.view(x_shape);
+            }
+            if (need_dw) dw = block_gemm(g8t, saved[0], saved[1], false, n, k, m, wt);
+        }
+        if (need_db) db = column_sum(dy.ld == 0 ? Rows(dy.t.contiguous(), n) : dy, (at::ScalarType)ctx->saved_data["b_type"].toInt());
+        return {dx, dw, db, at::Tensor(), at::Tensor()};
+    }
+};
+
+// ---- layer norm
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& weight_, const MaybeTensor& bias_, int64_t cols, double eps, bool need_grad) {
+        const at::Tensor weight = weight_.value_or(at::Tensor()), bias = bias_.value_or(at::Tensor());
+        const c10::DeviceGuard guard(x.device());
+        const Rows r(x, cols);
+        const int pt = weight.defined() ? dtype_code(weight.scalar_type()) : bias.defined() ? dtype_code(bias.scalar_type()) : r.dtype();
+        const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+        const at::Tensor y = at::empty(x.sizes(), x.options()), stats = need_grad ? at::empty({r.rows, 2}, x.options().dtype(at::kFloat)) : at::Tensor();
+        if (r.rows) check(L.layer_norm(r.t.data_ptr(), r.rows, cols, r.ld, r.dtype(), ptr(w), ptr(b), pt, (float)eps, y.data_ptr(), (float*)ptr(stats), stream_of(x)), "f8mi_layer_norm");
+        ctx->save_for_backward({x, weight, stats});
+        ctx->saved_data["cols"] = cols;
+        ctx->saved_data["has_weight"] = weight.defined();
+        ctx->saved_data["has_bias"] = bias.defined();
+        ctx->saved_data["w_shape"] = weight.defined() ? weight.sizes().vec() : std::vector<int64_t>();
+        ctx->saved_data["b_shape"] = bias.defined() ? bias.sizes().vec() : std::vector<int64_t>();
+        ctx->saved_data["p_type"] = (int64_t)(weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type());
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm has no second derivative (create_graph=True)");
+        const bool has_weight = ctx->saved_data["has_weight"].toBool(), has_bias = ctx->saved_data["has_bias"].toBool();
+        const bool need_dx = ctx->needs_input_grad(0), need_dw = has_weight && ctx->needs_input_grad(1), need_db = has_bias && ctx->needs_input_grad(has_weight ? 2 : 1);
+        at::Tensor dx, dw, db;
+        if (!grads[0].defined() || !(need_dx || need_dw || need_db)) return {dx, dw, db, at::Tensor(), at::Tensor(), at::Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &stats = saved[2];
+        const c10::DeviceGuard guard(x.device());
+        const int64_t cols = ctx->saved_data["cols"].toInt();
+        const at::ScalarType pt = (at::ScalarType)ctx->saved_data["p_type"].toInt();
+        const Rows r(x, cols), dy(grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type()), cols);
+        const at::Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
+        if (need_dx) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+        if (need_dw) dw = at::empty(ctx->saved_data["w_shape"].toIntVector(), x.options().dtype(pt));
+        if (need_db) db = at::empty(ctx->saved_data["b_shape"].toIntVector(), x.options().dtype(pt));
+        const int64_t bytes = need_dw || need_db ? L.layer_norm_workspace_bytes(r.rows, cols, r.dtype()) : 0;
+        const at::Tensor ws = bytes ? at::empty({bytes / 4}, x.options().dtype(at::kFloat)) : at::Tensor();
+        check(L.layer_norm_backward(ptr(dy.t), dy.ld, ptr(r.t), r.ld, r.rows, cols, r.dtype(), ptr(w), dtype_code(pt), (const float*)ptr(stats), ptr(dx), ptr(dw), ptr(db), ptr(ws),
+                                    bytes, stream_of(x)), "f8mi_layer_norm_backward");
+        return {dx, dw, db, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// ---- Python
+
+PyObject* wrap(const at::Tensor& t) {
+    if (!t.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(t);
+}
+struct WithoutGil {
+    PyThreadState* state = PyEval_SaveThread();
+    ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+template <typename F>
+PyObject* guarded(F body) {
+    HANDLE_TH_ERRORS
+    try {
+        return body();
+    } catch (const NativeFailure& f) {
+        PyErr_SetString(native_error, f.what());
+        return nullptr;
+    }
+    END_HANDLE_TH_ERRORS
+}
+bool expect(Py_ssize_t got, Py_ssize_t want, const char* name) {
+    if (!L.last_error) PyErr_SetString(PyExc_RuntimeError, "f8mi_torch_ops: load() has not been called");
+    else if (got != want) PyErr_Format(PyExc_TypeError, "%s takes %zd arguments, got %zd", name, want, got);
+    else return true;
+    return false;
+}
+// false: not taken; None leaves t undefined
+bool optional(PyObject* o, int device, at::Tensor& t) {
+    if (o == Py_None) return true;
+    t = plain(o, device);
+    return t.defined();
+}
+bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+
+// blockwise_linear(x [..., k], weight [n, k], bias or None, device) -> y, with its history, or None.  Shapes have been checked.
+PyObject* blockwise_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (!expect(n_args, 4, "blockwise_linear")) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int device = (int)PyLong_AsLong(a[3]);
+        const at::Tensor x = plain(a[0], device), w = plain(a[1], device);
+        at::Tensor bias;
+        if (!x.defined() || !w.defined() || !optional(a[2], device, bias)) Py_RETURN_NONE;
+        at::Tensor y;
+        {
+            const WithoutGil no_gil;
+            y = BlockwiseLinear::apply(x, w, maybe(bias), wants_grad(x), wants_grad(w));
+        }
+        return wrap(y);
+    });
+}
+
+// blockwise_inference_linear(x [m, k], data, scales of the weight, n, bias or None, device) -> y or None
+PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (!expect(n_args, 6, "blockwise_inference_linear")) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int device = (int)PyLong_AsLong(a[5]);
+        const int64_t n = PyLong_AsLongLong(a[3]);
+        const at::Tensor x = plain(a[0], device);
+        at::Tensor bias;
+        if (!x.defined() || x.dim() < 1 || !THPVariable_Check(a[1]) || !THPVariable_Check(a[2]) || !optional(a[4], device, bias)) Py_RETURN_NONE;
+        const at::Tensor data = THPVariable_Unpack(a[1]), scales = THPVariable_Unpack(a[2]);
+        const int64_t k = x.size(-1), kp = (k + 127) / 128 * 128;
+        if (!data.is_cuda() || data.get_device() != device || data.scalar_type() != at::kFloat8_e4m3fn || !data.is_contiguous() || data.numel() != kp * n || !scales.is_cuda() ||
+            scales.get_device() != device || scales.scalar_type() != at::kByte || !scales.is_contiguous() || scales.numel() != L.block_scale_bytes(n, k))
+            Py_RETURN_NONE;
+        at::Tensor y;
+        {
+            const WithoutGil no_gil;
+            const c10::DeviceGuard guard(x.device());
+            std::vector<int64_t> y_shape(x.sizes().begin(), x.sizes().end());
+            y_shape.back() = n;
+            const Rows xr(x, k);
+            const at::Tensor b = bias.defined() ? bias.to(x.scalar_type()).contiguous() : at::Tensor();
+            if (xr.rows == 0) {
+                y = at::empty(y_shape, x.options());
+            } else {
+                const Blocks x8 = Blocks::make(x, xr.rows, k);
+                const f8mi_block_cast_job job = job_of(xr, false, x8, Blocks());
+                check(L.block_cast(&job, 1, stream_of(x)), "f8mi_block_cast");
+                y = block_gemm(x8, data, scales, false, xr.rows, n, k, x.scalar_type(), b);
+                if (x.dim() != 2) y = y.view(y_shape);
+            }
+        }
+        return wrap(y);
+    });
+}
+
+// layer_norm(x, weight or None, bias or None, cols, eps, device) -> y, with its history, or None.  Shapes and types have been checked.
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (!expect(n_args, 6, "layer_norm")) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int device = (int)PyLong_AsLong(a[5]);
+        const at::Tensor x = plain(a[0], device);
+        at::Tensor w, b;
+        if (!x.defined() || !optional(a[1], device, w) || !optional(a[2], device, b)) Py_RETURN_NONE;
+        const int64_t cols = PyLong_AsLongLong(a[3]);
+        const double eps = PyFloat_AsDouble(a[4]);
+        at::Tensor y;
+        {
+            const WithoutGil no_gil;
+            y = LayerNorm::apply(x, maybe(w), maybe(b), cols, eps, wants_grad(x) || wants_grad(w) || wants_grad(b));
+        }
+        return wrap(y);
+    });
+}
+
+// grad_clip(list, what, kind, max_norm, device) -> (norm (fp32, 0-dim), list or None), or None: something in the list is not taken.
+// what: "norm" of the tensors; "grads": the gradients of the tensors are clipped in place; None: clipped into new tensors of the tensors' own
+// types; a dtype: of that type.
+PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    if (!expect(n_args, 5, "grad_clip")) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int kind = (int)PyLong_AsLong(a[2]), device = (int)PyLong_AsLong(a[4]);
+        const double max_norm = PyFloat_AsDouble(a[3]);
+        const bool of_params = PyUnicode_Check(a[1]) && PyUnicode_CompareWithASCIIString(a[1], "grads") == 0;
+        const bool to_new = !PyUnicode_Check(a[1]);
+        const bool typed = THPDtype_Check(a[1]);
+        if (!PyList_Check(a[0])) Py_RETURN_NONE;
+        std::vector<at::Tensor> xs, outs;
+        xs.reserve((size_t)PyList_GET_SIZE(a[0]));
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); i++) {
+            PyObject* o = PyList_GET_ITEM(a[0], i);
+            at::Tensor g;
+            if (of_params) {
+                if (!THPVariable_Check(o)) Py_RETURN_NONE;
+                const at::Tensor grad = THPVariable_Unpack(o).grad();
+                if (!grad.defined()) continue;
+                THPObjectPtr wrapped(THPVariable_Wrap(grad));  // a subclass shows in its Python type only
+                g = plain(wrapped.get(), device);
+            } else {
+                g = plain(o, device);
+            }
+            if (!g.defined() || !g.is_non_overlapping_and_dense()) Py_RETURN_NONE;
+            xs.push_back(g);
+        }
+        at::Tensor norm;
+        {
+            const WithoutGil no_gil;
+            const at::AutoDispatchBelowADInplaceOrView below;
+            const c10::DeviceGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
+            const auto options = at::TensorOptions().device(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
+            std::vector<f8mi_grad> grads(xs.size());
+            for (size_t i = 0; i < xs.size(); i++) {
+                if (to_new) outs.push_back(at::empty_strided(xs[i].sizes(), xs[i].strides(), typed ? xs[i].options().dtype(((THPDtype*)a[1])->scalar_type) : xs[i].options()));
+                const at::Tensor& out = to_new ? outs[i] : xs[i];
+                grads[i] = {xs[i].data_ptr(), out.data_ptr(), xs[i].numel(), dtype_code(xs[i].scalar_type()), dtype_code(out.scalar_type())};
+                if (of_params) torch::autograd::impl::bump_version(xs[i]);
+            }
+            norm = at::empty({}, options.dtype(at::kFloat));
+            const int64_t count = (int64_t)xs.size(), bytes = L.grad_clip_workspace_bytes(count);
+            const at::Tensor ws = at::empty({bytes / 8}, options.dtype(at::kDouble));
+            check(L.grad_clip(grads.data(), count, kind, (float)max_norm, to_new || of_params, (float*)norm.data_ptr(), ws.data_ptr(), bytes, stream_of(norm)), "f8mi_grad_clip");
+        }
+        THPObjectPtr list(Py_None);
+        Py_INCREF(Py_None);
+        if (to_new) {
+            list = THPObjectPtr(PyList_New((Py_ssize_t)outs.size()));
+            if (!list) return nullptr;
+            for (size_t i = 0; i < outs.size(); i++) PyList_SET_ITEM(list.get(), (Py_ssize_t)i, wrap(outs[i]));
+        }
+        THPObjectPtr n(wrap(norm));
+        return PyTuple_Pack(2, n.get(), list.get());
+    });
+}
+
+// load(path of libf8mi.so, error class): resolves the entry points
+PyObject* load(PyObject*, PyObject* args) {
+    const char* path;
+    PyObject* error;
+    if (!PyArg_ParseTuple(args, "sO", &path, &error)) return nullptr;
+    void* h = dlopen(path, RTLD_NOW | RTLD_LOCAL);
+    if (!h) return PyErr_Format(PyExc_ImportError, "%s", dlerror());
+    const char* missing = nullptr;
+    auto get = [&](auto& f, const char* name) {
+        f = reinterpret_cast<std::decay_t<decltype(f)>>(dlsym(h, name));
+        if (!f) missing = name;
+    };
+    get(L.block_scale_bytes, "f8mi_block_scale_bytes");
+    get(L.block_cast, "f8mi_block_cast");
+    get(L.block_gemm, "f8mi_block_gemm");
+    get(L.block_gemm_workspace_bytes, "f8mi_block_gemm_workspace_bytes");
+    get(L.column_sum, "f8mi_column_sum");
+    get(L.column_sum_workspace_bytes, "f8mi_column_sum_workspace_bytes");
+    get(L.layer_norm, "f8mi_layer_norm");
+    get(L.layer_norm_backward, "f8mi_layer_norm_backward");
+    get(L.layer_norm_workspace_bytes, "f8mi_layer_norm_workspace_bytes");
+    get(L.grad_clip, "f8mi_grad_clip");
+    get(L.grad_clip_workspace_bytes, "f8mi_grad_clip_workspace_bytes");
+    get(L.last_error, "f8mi_last_error");
+    if (missing) {
+        L.last_error = nullptr;
+        return PyErr_Format(PyExc_ImportError, "%s does not export %s", path, missing);
+    }
+    Py_INCREF(error);
+    native_error = error;
+    Py_RETURN_NONE;
+}
+
+template <typename F>
+PyCFunction fast(F f) { return (PyCFunction)(void (*)(void))f; }
+PyMethodDef methods[] = {
+    {"load", load, METH_VARARGS, nullptr},
+    {"blockwise_linear", fast(blockwise_linear), METH_FASTCALL, nullptr},
+    {"blockwise_inference_linear", fast(blockwise_inference_linear), METH_FASTCALL, nullptr},
+    {"layer_norm", fast(layer_norm), METH_FASTCALL, nullptr},
+    {"grad_clip", fast(grad_clip), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr},
+};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_f8mi_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__f8mi_torch_ops(void) { return PyModule_Create(&module); }

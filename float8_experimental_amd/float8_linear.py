@@ -239,6 +239,8 @@ class Float8Linear(torch.nn.Linear):
         self.scaling_type_input = config.cast_config_input.scaling_type
         self.scaling_type_weight = config.cast_config_weight.scaling_type
         self.scaling_type_grad_output = config.cast_config_grad_output.scaling_type
+        if self.scaling_type_input is ScalingType.BLOCKWISE:
+            raise ValueError("a Float8Linear has one scale for a tensor; blockwise scaling is Float8BlockwiseLinear's (convert_to_float8_training picks it)")
         self.has_any_delayed_scaling = ScalingType.DELAYED in (
             self.scaling_type_input, self.scaling_type_weight, self.scaling_type_grad_output)
 

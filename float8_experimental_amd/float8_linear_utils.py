@@ -8,6 +8,7 @@ import torch.nn as nn
 
 from . import _native
 from .config import Float8LinearConfig, ScalingType
+from .float8_blockwise import Float8BlockwiseLinear
 from .float8_linear import Float8Linear
 from .float8_utils import e4m3_dtype, e5m2_dtype
 
@@ -59,11 +60,12 @@ def swap_linear_layers(module: nn.Module, from_float_func: Callable[[nn.Linear],
 
 def convert_to_float8_training(module: nn.Module, *, module_filter_fn: Optional[Callable[[nn.Module, str], bool]] = None,
                                config: Float8LinearConfig = None) -> nn.Module:
-    """Swaps ``nn.Linear`` modules for ``Float8Linear`` (reference :125-154)."""
+    """Swaps ``nn.Linear`` modules for ``Float8Linear`` (reference :125-154), for ``Float8BlockwiseLinear`` under a config with
+    ``ScalingType.BLOCKWISE``."""
     if config is None:
         config = Float8LinearConfig()
-    return swap_linear_layers(module, lambda m: Float8Linear.from_float(m, config=config),
-                              module_filter_fn=module_filter_fn)
+    layer = Float8BlockwiseLinear if config.cast_config_input.scaling_type is ScalingType.BLOCKWISE else Float8Linear
+    return swap_linear_layers(module, lambda m: layer.from_float(m, config=config), module_filter_fn=module_filter_fn)
 
 
 def get_float8_layers(model: torch.nn.Module) -> List[Float8Linear]:

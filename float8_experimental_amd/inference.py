@@ -18,6 +18,7 @@ import torch.nn as nn
 
 from . import _custom_ops  # noqa: F401  (registers torch.ops.f8mi.*)
 from . import _native
+from .float8_blockwise import Float8BlockwiseInferenceLinear
 from .float8_linear_utils import swap_linear_layers
 from .float8_tensor import (
     Float8Tensor,
@@ -37,11 +38,13 @@ class ActivationCasting(Enum):
     WEIGHT_ONLY: nothing; the fp8 weight is dequantised in the forward pass and the matmul runs in high precision
     DYNAMIC: cast per call with a scale computed from the activation
     STATIC: cast per call with the scale given at conversion time
+    BLOCKWISE: cast per call with a scale for each block of 128 values; the weight has one for each 128 x 128
     """
 
     WEIGHT_ONLY = auto()
     DYNAMIC = auto()
     STATIC = auto()
+    BLOCKWISE = auto()
 
 
 @dataclass(frozen=True)
@@ -174,6 +177,8 @@ class Float8InferenceLinear(torch.nn.Linear):
                  bias: bool = True, device: Optional[torch.device] = None, dtype: Optional[torch.dtype] = None) -> None:
         super().__init__(in_features, out_features, bias, device, dtype)
         self.linear_mm_config = linear_mm_config
+        if quant_config.activation_casting is ActivationCasting.BLOCKWISE:
+            raise ValueError("blockwise scaling is Float8BlockwiseInferenceLinear's (quantize_to_float8 picks it)")
         self.activation_casting = quant_config.activation_casting
         if self.activation_casting == ActivationCasting.STATIC:
             self.register_buffer("static_quantization_scale", quant_config.static_quantization_scale)
@@ -250,8 +255,11 @@ def cast_to_float8_e4m3_inference(inpt_tensor: torch.Tensor, linear_mm_config: L
 def quantize_to_float8(module: nn.Module, quant_config: QuantConfig, *,
                        module_filter_fn: Optional[Callable[[nn.Module, str], bool]] = None,
                        use_fast_accum: bool = True) -> nn.Module:
-    """Swaps every (filtered) ``nn.Linear`` of ``module`` for a ``Float8InferenceLinear`` (``inference.py:211-244``).
+    """Swaps every (filtered) ``nn.Linear`` of ``module`` for a ``Float8InferenceLinear`` (``inference.py:211-244``), with
+    ``ActivationCasting.BLOCKWISE`` for a ``Float8BlockwiseInferenceLinear``.
 
     A root-level ``nn.Linear`` is not modified in place but returned converted; one with children raises."""
+    if quant_config.activation_casting is ActivationCasting.BLOCKWISE:
+        return swap_linear_layers(module, Float8BlockwiseInferenceLinear.from_float, module_filter_fn=module_filter_fn)
     return swap_linear_layers(module, lambda m: Float8InferenceLinear.from_float(m, quant_config, use_fast_accum),
                               module_filter_fn=module_filter_fn)

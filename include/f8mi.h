@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define F8MI_VERSION 130
+#define F8MI_VERSION 140
 
 #define F8MI_OK 0
 #define F8MI_ERR_INVALID_ARG (-1) /* null pointer, negative size, unknown enum            */
@@ -450,6 +450,69 @@ int f8mi_delayed_init(const float* amax_dev, float* history_dev, float* scale_de
 int f8mi_prof_enable(int on);
 int f8mi_prof_reset(void);
 int f8mi_prof_read(int kernel, uint64_t* launches, double* total_ms, double* total_work);
+
+/* ---- block scales: e4m3 operands with one power of two for each 128 values of the contraction -----------------------------------
+ * A block of values v is kept as e4m3 of v / 2^S, rounded to nearest even, with the smallest S >= -126 for which max|v| <= 448 * 2^S;
+ * a block that holds an infinity or a NaN stands for NaN.  Blocks lie along the contraction: 1 x 128 values of a row, or 128 x 128 values
+ * (`square`) that share one S; the last may be shorter (zeros fill it up).
+ * A copy of `rows` rows contracting over k is [f8mi_padded_k(k)/64][rows][64] bytes, its scales are f8mi_block_scale_bytes(rows, k) bytes,
+ * [f8mi_padded_k(k)/128][rows padded to 128]: S + 127 of row r of a group of 128 rows at (r % 16) * 8 + r / 16.  Both 16-byte aligned.
+ */
+int64_t f8mi_block_scale_bytes(int64_t rows, int64_t k);
+
+typedef struct f8mi_block_cast_job {
+    const void* x;           /* [rows][cols], unit column stride */
+    int64_t rows, cols, ld;  /* ld: elements from row to row, >= cols, or 0: the same row throughout */
+    int dtype;               /* F8MI_BF16 / _FP16 / _FP32 */
+    int square;              /* one scale for each 128 x 128 instead of for each 1 x 128 (out) and 128 x 1 (out_t) */
+    void* out;               /* copy of `rows` rows contracting over the columns, or NULL */
+    void* out_scales;
+    void* out_t;             /* copy of `cols` rows contracting over the rows, or NULL; square: its scales alone may be asked for, for a */
+    void* out_t_scales;      /* product that reads `out` transposed */
+} f8mi_block_cast_job;
+
+/* One or two tensors in one pass over each; one launch where they have the same dtype. */
+int f8mi_block_cast(const f8mi_block_cast_job* jobs, int count, void* stream);
+
+/* c [m][n] = a bt^T + bias, added in fp32 and rounded once.  a: copy of m rows, bt: copy of n rows, both contracting over k (padded: a
+ * multiple of 128).  b_transposed: bt is the copy of another product instead, of k rows contracting over n (n a multiple of 128), read transposed;
+ * b_scales are those of n rows contracting over k all the same.  bias: n values of c_dtype or NULL.  workspace (16-byte aligned, may be
+ * NULL): with F8MI_GEMM_WORKSPACE_BYTES of it a long contraction of few tiles is split over workgroups, the parts added in a fixed order. */
+int f8mi_block_gemm(const void* a, const void* a_scales, const void* bt, const void* b_scales, int b_transposed, int64_t m, int64_t n, int64_t k,
+                    void* c, int c_dtype, int64_t ldc, const void* bias_dev, void* workspace, int64_t workspace_bytes, void* stream);
+/* Bytes of workspace that this product makes use of (0: none).  Needs no GPU. */
+int64_t f8mi_block_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
+
+/* ---- layer norm over the last dimension ---------------------------------------------------------------------------------------------
+ * y [rows][cols] = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps); var without Bessel's correction, statistics in fp32.
+ * weight, bias: cols values of p_dtype (x's dtype or F8MI_FP32), or NULL (1, 0).  ld: elements from row to row of x, or 0: one row throughout;
+ * y is dense.  stats: [rows] pairs (mean, rstd) for the backward pass, or NULL. */
+int f8mi_layer_norm(const void* x, int64_t rows, int64_t cols, int64_t ld, int dtype, const void* weight, const void* bias, int p_dtype, float eps, void* y,
+                    float* stats, void* stream);
+/* dx (dense, x's dtype), dweight, dbias (p_dtype): any of them may be NULL.  workspace: f8mi_layer_norm_workspace_bytes() for the sums of the rows, 16-byte
+ * aligned, contents arbitrary; only needed for dweight and dbias, whose sums are added in a fixed order. */
+int64_t f8mi_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype);
+int f8mi_layer_norm_backward(const void* dy, int64_t ld_dy, const void* x, int64_t ld, int64_t rows, int64_t cols, int dtype, const void* weight, int p_dtype,
+                             const float* stats, void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- norm of a list of gradients, and clipping ------------------------------------------------------------------------------------------ */
+#define F8MI_NORM_2 2
+#define F8MI_NORM_1 1
+#define F8MI_NORM_INF 0
+
+typedef struct f8mi_grad {
+    const void* x;  /* n values, dense, aligned to their size */
+    void* out;      /* n values of out_dtype: x itself (in place) or memory that does not overlap it */
+    int64_t n;
+    int dtype, out_dtype;
+} f8mi_grad;
+
+/* *norm_dev (fp32) = the norm of all values of all tensors; with `scale` out = x * min(1, max_norm / (norm + 1e-6)), the product in fp32 and
+ * rounded once.  Sums in fp64, in a fixed order.  The table is read before the call returns.  workspace: f8mi_grad_clip_workspace_bytes(count), 8-byte aligned,
+ * contents arbitrary. */
+int64_t f8mi_grad_clip_workspace_bytes(int64_t count);
+int f8mi_grad_clip(const f8mi_grad* grads, int64_t count, int norm_kind, float max_norm, int scale, float* norm_dev, void* workspace, int64_t workspace_bytes,
+                   void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,360 @@
+"""Linears with a power-of-two scale for each block of 128 values: casts to the bit, products within the matrix cores' tolerance of the exact product
+of what is kept, gradients against the formula and against differences."""
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+EPS = {BF16: 2.0**-8, FP16: 2.0**-11, FP32: 2.0**-23}
+
+
+@pytest.fixture(scope="module")
+def nat():
+    from float8_experimental_amd import _native
+
+    return _native
+
+
+@pytest.fixture(scope="module")
+def f8():
+    import float8_experimental_amd
+
+    return float8_experimental_amd
+
+
+def kept(t, rows, cols):
+    """What blocks of rows x cols of t [m, k] stand for, in 64 bits: numpy's frexp, ldexp and rint are exact."""
+    v = t.detach().double().cpu().numpy()
+    m, k = v.shape
+    v = np.pad(v, ((0, -m % rows), (0, -k % cols))).reshape(-(-m // rows), rows, -(-k // cols), cols)
+    amax = np.abs(v).max((1, 3), keepdims=True)
+    fraction, exponent = np.frexp(amax)
+    s = np.maximum(exponent - 9 + (fraction > 0.875), -126)
+    q = np.ldexp(v, -s)
+    step = np.maximum(np.frexp(q)[1], -5) - 4
+    q = np.ldexp(np.rint(np.ldexp(q, -step)), step)
+    assert not np.isfinite(q).any() or np.abs(q[np.isfinite(q)]).max() <= 448
+    q = np.where(np.isfinite(amax), np.ldexp(q, s), np.nan)
+    return torch.from_numpy(q.reshape(v.shape[0] * rows, -1)[:m, :k].copy())
+
+
+def values(shape, dtype, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * torch.randn(shape[-1], generator=g).exp() * std).to(dtype)
+
+
+def product_close(got, a, b, bias=None):
+    """One rounding to the output's type, the matrix instruction's, and fp32 additions.  The instruction adds groups of 8 neighbouring products, each cut to
+    multiples of 2^-13 of the power of two below the group's largest (which keeps all of its bits): at most 7 * 2^-13 of the largest
+    product for each group.  The groups are added in fp32, a tree or chain of k / 8 additions."""
+    exact, size = a @ b.t(), a.abs() @ b.abs().t()
+    groups = lambda t: torch.nn.functional.pad(t.abs(), (0, -t.shape[1] % 8)).view(t.shape[0], -1, 8).amax(2)
+    cut = 7 * 2.0**-13 * (groups(a) @ groups(b).t()) + (a.shape[1] / 8 + 8) * 2.0**-24 * size
+    if bias is not None:
+        exact = exact + bias.double().cpu()
+        cut = cut + 2.0**-24 * bias.double().cpu().abs()
+    tol = EPS[got.dtype] * exact.abs() + cut + 1e-30
+    if got.dtype is FP16:
+        tol = tol + 2.0**-25  # half a step of the subnormals
+    worst = ((got.detach().double().cpu() - exact).abs() / tol).max().item() if exact.numel() else 0.0
+    assert worst <= 1.0, worst
+
+
+SHAPES = [(1, 1), (1, 4096), (5, 130), (128, 128), (127, 129), (300, 257), (256, 384), (1000, 136)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_casts_are_exact(nat, m, k, dtype):
+    x = values((m, k), dtype, m + k).cuda()
+    ((a, b),) = nat.block_cast([(x, False, True, True)])
+    assert torch.equal(a.dequant().double().cpu(), kept(x, 1, 128)) and torch.equal(b.dequant().double().cpu(), kept(x, 128, 1).t())
+    ((a, b),) = nat.block_cast([(x, True, True, True)])
+    want = kept(x, 128, 128)
+    assert torch.equal(a.dequant().double().cpu(), want) and torch.equal(b.dequant().double().cpu(), want.t())
+    ((c, d),) = nat.block_cast([(x, True, True, "scales")])  # the transposed copy's scales alone
+    assert torch.equal(c.data.view(torch.uint8), a.data.view(torch.uint8)) and torch.equal(d.scales, b.scales) and d.data is None
+
+
+def test_two_tensors_in_one_call_are_cast_as_each_alone(nat):
+    for dx, dw in ((BF16, BF16), (BF16, FP32), (FP16, BF16)):
+        x, w = values((130, 300), dx).cuda(), values((500, 300), dw, 1).cuda()
+        both = nat.block_cast([(x, False, True, True), (w, True, True, True)])
+        alone = nat.block_cast([(x, False, True, True)]) + nat.block_cast([(w, True, True, True)])
+        for p, q in zip([c for pair in both for c in pair], [c for pair in alone for c in pair]):
+            assert torch.equal(p.data.view(torch.uint8), q.data.view(torch.uint8)) and torch.equal(p.scales, q.scales)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_casts_of_rows_with_any_stride(nat, dtype):
+    base = values((140, 400), dtype).cuda()
+    for view in (base[:, 3:260], base[1:, :129], base[::2, 5:6], base[:1, 1:].expand(140, 399), base.t()[:150, :139]):
+        ((a, b),) = nat.block_cast([(view, False, True, True)])
+        assert torch.equal(a.dequant().double().cpu(), kept(view, 1, 128)) and torch.equal(b.dequant().double().cpu(), kept(view, 128, 1).t())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_casts_at_the_ends_of_the_range(nat, dtype):
+    """Zeros, subnormals, the largest values, and every significand next to where the exponent steps."""
+    info = torch.finfo(dtype)
+    rows = [torch.zeros(256), torch.full((256,), info.tiny), torch.full((256,), info.smallest_normal / 4), torch.full((256,), info.max),
+            torch.linspace(0, info.max, 256), -torch.linspace(0, info.smallest_normal, 256)]
+    for e in range(-10, 11):
+        for m in (1.0, 1.7421875, 1.75, 1.7578125, 1.9921875):
+            rows.append(torch.cat([torch.full((1,), m * 2.0**e), torch.linspace(-m, m, 255) * 2.0**e]))
+    x = torch.stack(rows).to(dtype).cuda()
+    for square in (False, True):
+        ((a, b),) = nat.block_cast([(x, square, True, True)])
+        n = 128 if square else 1
+        assert torch.equal(a.dequant().double().cpu(), kept(x, n, 128)) and torch.equal(b.dequant().double().cpu(), kept(x, 128, n).t())
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_a_block_with_something_that_is_not_finite_is_nan(nat, f8, dtype, bad):
+    x, w = values((150, 300), dtype).cuda(), values((200, 300), dtype, 1).cuda()
+    x[3, 140] = bad
+    ((a, b),) = nat.block_cast([(x, False, True, True)])
+    got = a.dequant().isnan()
+    assert got[3, 128:256].all() and got.sum() == 128
+    got = b.dequant().isnan()
+    assert got[140, :128].all() and got.sum() == 128
+    y = f8.blockwise_linear(x, w)
+    assert y[3].isnan().all() and y.isnan().sum() == 200
+    x[3, 140] = 0
+    w[130, 10] = bad
+    y = f8.blockwise_linear(x, w)
+    assert y[:, 128:].isnan().all() and not y[:, :128].isnan().any()
+
+
+# (m, n, k): one block, edges inside tiles, tiles of 128 x 128 with 1 - 9 steps, 128 x 256, 256 x 256, split over k, few rows
+PRODUCTS = ([(1, 1, 1), (128, 128, 128), (128, 256, 256), (130, 127, 129), (200, 300, 500), (100, 4096, 16384), (512, 1024, 8192), (1000, 1001, 640), (2048, 4096, 1024),
+             (4099, 1031, 384), (4100, 2300, 520), (4352, 4096, 512), (3000, 8200, 900), (1, 8192, 2048), (7, 1000, 1100), (16, 4096, 4096), (17, 300, 512), (33, 8200, 700),
+             (64, 1024, 2048), (150, 520, 1400), (256, 512, 2100)] + [(200, 200, 128 * s) for s in range(3, 10)] + [(2300, 4100, 128 * s) for s in (1, 2, 3, 4, 5, 8)])
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_products(nat, m, n, k):
+    for dtype in (BF16, FP16, FP32) if m * n <= 1 << 20 else (BF16,):
+        x, w, bias = values((m, k), dtype, m + k).cuda(), values((n, k), dtype, n + k, k**-0.5).cuda(), values((n,), dtype, 7).cuda()
+        (a, _), (b, _) = nat.block_cast([(x, False, True, False), (w, True, True, False)])
+        ka, kb = a.dequant().double(), b.dequant().double()
+        product_close(nat.block_gemm(a, b, dtype), ka.cpu(), kb.cpu())
+        product_close(nat.block_gemm(a, b, dtype, bias), ka.cpu(), kb.cpu(), bias)
+
+
+@pytest.mark.parametrize("m,n,k", [(128, 128, 128), (200, 512, 1024), (1000, 2048, 640), (2048, 4096, 1024), (4099, 4096, 384), (3000, 8192, 896)])
+def test_products_that_read_the_weight_transposed(nat, m, n, k):
+    """m x k gradients from m x n ones: contracts the rows of the one copy of the weight, with the bits of a transposed copy."""
+    g, w = values((m, n), BF16, m).cuda(), values((n, k), BF16, n).cuda()
+    ((a, _),) = nat.block_cast([(g, False, True, False)])
+    ((b, bt),) = nat.block_cast([(w, True, True, True)])
+    one = nat.block_gemm(a, nat.Blocks(None, bt.scales, k, n), BF16, transposed=b)
+    product_close(one, a.dequant().double().cpu(), bt.dequant().double().cpu())
+    if nat.lib().f8mi_block_gemm_workspace_bytes(m, k, n) == 0:
+        assert torch.equal(one, nat.block_gemm(a, bt, BF16))
+
+
+def test_scales_of_both_operands_reach_every_row_and_block(nat):
+    """Every row and column has blocks of very different sizes: a scale that goes to the wrong row, column or block shows."""
+    m, n, k = 400, 700, 1100
+    g = torch.Generator().manual_seed(3)
+    spread = lambda rows: torch.ldexp(torch.randn(rows, k, generator=g), torch.randint(-20, 20, (rows, -(-k // 128)), generator=g).repeat_interleave(128, 1)[:, :k])
+    x, w = spread(m).to(BF16).cuda(), spread(n).to(BF16).cuda()
+    for jobs in ([(x, False, True, False), (w, False, True, False)], [(x, False, True, False), (w, True, True, False)]):
+        (a, _), (b, _) = nat.block_cast(jobs)
+        product_close(nat.block_gemm(a, b, FP32), kept(x, 1, 128), kept(w, 128 if jobs[1][1] else 1, 128))
+
+
+def formulas(x, w, bias, dy):
+    x2, g2 = x.detach().reshape(-1, x.shape[-1]), dy.reshape(-1, dy.shape[-1])
+    kw = kept(w, 128, 128)
+    return {"y": (kept(x2, 1, 128), kw, bias), "dx": (kept(g2, 1, 128), kw.t().contiguous(), None), "dw": (kept(g2, 128, 1).t(), kept(x2, 128, 1).t(), None)}
+
+
+@pytest.mark.parametrize("m,k,n,dtype,w_dtype,bias", [(1, 1, 1, BF16, BF16, True), (130, 200, 448, BF16, BF16, False), (512, 1024, 1024, BF16, BF16, False),
+                                                      (257, 300, 129, FP16, FP16, True), (300, 384, 256, BF16, FP32, True), (64, 500, 130, FP32, FP32, True),
+                                                      (4099, 520, 1031, BF16, BF16, True), (2100, 1152, 2304, FP16, FP16, False)])
+def test_linear_forward_and_backward(f8, m, k, n, dtype, w_dtype, bias):
+    x, w, dy = values((m, k), dtype).cuda().requires_grad_(), values((n, k), w_dtype, 1, k**-0.5).cuda().requires_grad_(), values((m, n), dtype, 2, 1e-2).cuda()
+    b = values((n,), w_dtype, 3).cuda().requires_grad_() if bias else None
+    y = f8.blockwise_linear(x, w, b)
+    y.backward(dy)
+    want = formulas(x, w, None if b is None else b.detach().to(dtype), dy)
+    for got, name in ((y, "y"), (x.grad, "dx"), (w.grad, "dw")):
+        product_close(got, *want[name])
+    assert y.dtype == x.grad.dtype == dtype and w.grad.dtype == w_dtype
+    if bias:  # fp32 sums, rounded to dy's type, in the type of the bias
+        exact = dy.double().sum(0)
+        tol = (EPS[dtype] + EPS[w_dtype]) * exact.abs() + m * 2.0**-24 * dy.double().abs().sum(0)
+        assert b.grad.dtype == w_dtype and ((b.grad.double() - exact).abs() <= tol).all()
+
+
+def test_linear_takes_inputs_of_any_layout_and_number_of_dimensions(f8):
+    w = values((200, 96), BF16, 1).cuda().requires_grad_()
+    for x in (values((96,), BF16).cuda(), values((3, 5, 96), BF16).cuda(), values((96, 40), BF16).cuda().t(), values((4, 7, 200), BF16).cuda()[:, :, 50:146],
+              values((1, 96), BF16).cuda().expand(50, 96)):
+        x = x.detach().requires_grad_()
+        y = f8.blockwise_linear(x, w)
+        assert y.shape == (*x.shape[:-1], 200)
+        w.grad = None
+        (y.float().sum() * 0.25).backward()  # a gradient that is one number expanded
+        want = formulas(x, w, None, torch.full(y.shape, 0.25, dtype=BF16))
+        for got, name in ((y.reshape(-1, 200), "y"), (x.grad.reshape(-1, 96), "dx"), (w.grad, "dw")):
+            product_close(got, *want[name])
+
+
+def test_gradients_against_differences(f8):
+    """On values that blocks keep as they are (small whole numbers) the layer is the exact product: its gradients are differences of the loss."""
+    g = torch.Generator().manual_seed(0)
+    whole = lambda *s: torch.randint(-4, 5, s, generator=g).to(FP32).cuda()
+    x, w, b, dy = whole(40, 130).requires_grad_(), whole(60, 130).requires_grad_(), whole(60).requires_grad_(), whole(40, 60)
+    loss = lambda: (f8.blockwise_linear(x, w, b).double() * dy.double()).sum()
+    loss().backward()
+    for t in (x, w, b):
+        for _ in range(5):
+            at = tuple(int(torch.randint(0, s, (1,), generator=g)) for s in t.shape)
+            with torch.no_grad():
+                t[at] += 1
+                up = loss()
+                t[at] -= 2
+                down = loss()
+                t[at] += 1
+            assert (up - down).item() == 2 * t.grad[at].item()
+
+
+def test_only_the_gradients_that_are_asked_for(f8):
+    x, w, b = values((64, 256), BF16).cuda(), values((128, 256), BF16, 1).cuda(), values((128,), BF16, 2).cuda()
+    dy = values((64, 128), BF16, 3).cuda()
+    full = {}
+    for which in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (0, 0, 0)):
+        ts = [t.clone().requires_grad_(bool(r)) for t, r in zip((x, w, b), which)]
+        y = f8.blockwise_linear(*ts)
+        assert y.requires_grad == any(which)
+        if any(which):
+            y.backward(dy)
+        for i, (t, r) in enumerate(zip(ts, which)):
+            assert (t.grad is not None) == bool(r)
+            if r:
+                full.setdefault(i, t.grad)
+                assert torch.equal(t.grad, full[i])
+    with torch.no_grad():
+        assert not f8.blockwise_linear(x.requires_grad_(), w, b).requires_grad
+
+
+def test_no_tokens(f8):
+    x, w, b = torch.zeros((0, 5, 64), dtype=BF16, device="cuda", requires_grad=True), values((32, 64), BF16).cuda().requires_grad_(), values((32,), BF16).cuda().requires_grad_()
+    y = f8.blockwise_linear(x, w, b)
+    y.sum().backward()
+    assert y.shape == (0, 5, 32) and x.grad.shape == x.shape and (w.grad == 0).all() and (b.grad == 0).all()
+
+
+def test_autocast(f8):
+    x, w = values((40, 130), FP32).cuda(), values((50, 130), FP32, 1).cuda().requires_grad_()
+    with torch.autocast("cuda", dtype=BF16):
+        y = f8.blockwise_linear(x, w)
+    y.backward(torch.ones_like(y))
+    assert y.dtype == BF16 and w.grad.dtype == FP32
+    product_close(y, kept(x.to(BF16), 1, 128), kept(w, 128, 128))
+
+
+def test_modules(f8):
+    from float8_experimental_amd.inference import ActivationCasting, QuantConfig, quantize_to_float8
+
+    blk = f8.CastConfig(scaling_type=f8.ScalingType.BLOCKWISE)
+    config = f8.Float8LinearConfig(cast_config_input=blk, cast_config_weight=blk, cast_config_grad_output=blk)
+    model = nn.Sequential(nn.Linear(96, 200), nn.ReLU(), nn.Linear(200, 64, bias=False)).to("cuda", BF16)
+    weights = list(model.parameters())
+    x = values((50, 96), BF16).cuda()
+    f8.convert_to_float8_training(model, config=config)
+    assert all(type(m) is f8.Float8BlockwiseLinear for m in (model[0], model[2])) and all(p is q for p, q in zip(weights, model.parameters()))
+    assert not f8.linear_requires_sync(config) and "blk" in repr(model[0])
+    y = model(x)
+    y.sum().backward()
+    assert all(p.grad is not None for p in weights)
+    served = quantize_to_float8(model, QuantConfig(ActivationCasting.BLOCKWISE))
+    assert all(type(m) is f8.Float8BlockwiseInferenceLinear for m in (served[0], served[2]))
+    with torch.no_grad():
+        product_close(served[0](x), kept(x, 1, 128), kept(weights[0], 128, 128), weights[1])
+        assert torch.equal(served[0].dequantized_weight().double().cpu(), kept(weights[0], 128, 128))
+        assert served[0](x[:0]).shape == (0, 200) and served[0](x[0]).shape == (200,)
+        again = f8.Float8BlockwiseInferenceLinear(96, 200, torch.zeros(200, dtype=BF16, device="cuda"), device="cuda")
+        again.load_state_dict(served[0].state_dict())
+        assert torch.equal(again(x), served[0](x))
+    root = quantize_to_float8(nn.Linear(96, 200).to("cuda", FP32), QuantConfig(ActivationCasting.BLOCKWISE))
+    with pytest.raises(RuntimeError, match="no backward"):
+        root(x.float().requires_grad_())
+
+
+@pytest.mark.parametrize("m", [1, 2, 9, 16, 17, 40, 100, 300])
+@pytest.mark.parametrize("k,n", [(128, 128), (1000, 700), (4096, 512), (2048, 8300)])
+def test_inference_from_one_token_to_a_prompt(f8, nat, m, k, n):
+    for dtype in (BF16, FP16, FP32):
+        layer = nn.Linear(k, n, device="cuda", dtype=dtype)
+        served = f8.Float8BlockwiseInferenceLinear.from_float(layer)
+        x = values((m, k), dtype, m).cuda()
+        with torch.no_grad():
+            product_close(served(x), kept(x, 1, 128), served.dequantized_weight().double().cpu(), layer.bias)
+
+
+def test_compiled(f8):
+    x, w, b = values((40, 256), BF16).cuda(), values((128, 256), BF16, 1).cuda(), values((128,), BF16, 2).cuda()
+    runs = []
+    for fn in (f8.blockwise_linear, torch.compile(f8.blockwise_linear, fullgraph=True)):
+        ts = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = fn(*ts)
+        y.backward(torch.ones_like(y))
+        runs.append([y] + [t.grad for t in ts])
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
+    served = f8.Float8BlockwiseInferenceLinear.from_float(nn.Linear(256, 128, device="cuda", dtype=BF16))
+    with torch.no_grad():
+        assert torch.equal(torch.compile(served, fullgraph=True)(x), served(x))
+
+
+def test_on_another_stream_and_captured(f8):
+    x, w = values((300, 256), BF16).cuda().requires_grad_(), values((384, 256), BF16, 1).cuda().requires_grad_()
+    dy = values((300, 384), BF16, 2).cuda()
+
+    def step():  # autograd.grad: nothing is left behind that accumulates gradients on the stream it first ran on
+        y = f8.blockwise_linear(x, w)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w), dy)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(values((300, 256), BF16, 10 + i).cuda())
+        graph.replay()
+        torch.cuda.synchronize()
+        recorded = [t.clone() for t in got]
+        assert all(torch.equal(p, q) for p, q in zip(recorded, step()))
+
+
+def test_refusals(f8, nat):
+    x, w = values((4, 64), BF16).cuda(), values((32, 64), BF16).cuda()
+    for bad in (lambda: f8.blockwise_linear(x[:, :60], w), lambda: f8.blockwise_linear(x, w[0]), lambda: f8.blockwise_linear(x, w, x[0]),
+                lambda: f8.blockwise_linear(x[:, :0], w[:, :0]), lambda: f8.blockwise_linear(x, w[:0])):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: f8.blockwise_linear(x.double(), w), lambda: f8.blockwise_linear(x, w.double()),
+                lambda: f8.Float8BlockwiseInferenceLinear.from_float(nn.Linear(4, 4, device="cuda", dtype=torch.float64))):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(nat.Float8NativeError):
+        f8.blockwise_linear(x, w.cpu())
+    y = f8.blockwise_linear(x.requires_grad_(), w)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
