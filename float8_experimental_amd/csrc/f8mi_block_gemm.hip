@@ -72,9 +72,16 @@ extern "C" int f8mi_block_gemm(const void* a, const void* a_scales, const void* 
         if ((uintptr_t)p % 16 != 0) { set_error("f8mi_block_gemm: operands, scales and workspace are 16-byte aligned"); return F8MI_ERR_INVALID_ARG; }
     if (m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff || ((m + 127) / 128) * ((n + 127) / 128) > 0x7fffffff) { set_error("f8mi_block_gemm: dimension too large"); return F8MI_ERR_UNSUPPORTED; }
     const BlockGemm g{(const uint8_t*)a, (const uint8_t*)a_scales, (const uint8_t*)bt, (const uint8_t*)b_scales, (int)m, (int)n, (int)k, c, ldc, bias_dev, c_dtype,
-                      b_transposed != 0, (uintptr_t)c % (c_dtype == F8MI_FP32 ? 4 : 2) == 0, (hipStream_t)stream_};
+                      b_transposed != 0, (uintptr_t)c % (c_dtype == F8MI_FP32 ? 4 : 2) == 0, (hipStream_t)stream_, (int)m};
     ProfScope prof(F8MI_K_GEMM, 2.0 * (double)m * (double)n * (double)k, g.stream);
     const int splits = workspace && !b_transposed ? pick_k_splits(m, n, k, workspace_bytes) : 0;
-    const int mid = use_mid_tiles(m, n, k);
-    return launch_block_mid(g, mid != 1, splits > 1 ? splits : 1, (float*)workspace);
+    if (splits > 1) return launch_block_mid(g, use_mid_tiles(m, n, k) == 2, splits, (float*)workspace);
+    if (const int mid = use_mid_tiles(m, n, k)) return launch_block_mid(g, mid == 2, 1, nullptr);
+    if (k < 384) return launch_block_mid(g, true, 1, nullptr);
+    // the tile rows that fill whole rounds of 256 x 256 tiles, and the rest on 128-row tiles where that is faster
+    const int64_t tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN;
+    const RowSplit split = split_last_round(tiles_m, tiles_n, k);
+    if (!split.rows_large) return launch_block_large(g, (int)tiles_m, (int)tiles_n);
+    if (int rc = launch_block_large(g, (int)split.rows_large, (int)tiles_n)) return rc;
+    return launch_block_mid(g.rows_from((int)split.rows_large * BM), split.mid == 2, 1, nullptr);
 }

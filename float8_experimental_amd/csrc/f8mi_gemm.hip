@@ -277,24 +277,6 @@ static int launch_gemm1(bool aligned, int c_dtype, dim3 g, hipStream_t stream, c
 
 using namespace f8mi;
 
-// An output whose last round of 256 x 256 tiles would leave most CUs idle (at most 128 tiles in it) is split by
-// rows: the tile rows that fill whole rounds go to the large-tile kernel, the rest to a 128-row-tile kernel that
-// spreads them over all CUs (same accumulation order, so no output bit depends on the split).  Returns the number
-// of tile rows for the large tiles (0: no split) and which 128-row tile takes the rest.
-struct RowSplit { int64_t rows_large; int mid; };
-static RowSplit split_last_round(int64_t tiles_m, int64_t tiles_n, int64_t k) {
-    const int64_t tiles = tiles_m * tiles_n, per_round = 256;
-    if (tiles <= per_round || tiles % per_round == 0) return {0, 0};
-    const int64_t rows_large = (tiles / per_round) * per_round / tiles_n;
-    if (rows_large < 1 || rows_large >= tiles_m) return {0, 0};
-    const int mid = use_mid_tiles((tiles_m - rows_large) * BM, tiles_n * BN, k);
-    if (!mid) return {0, 0};
-    // in rounds of the large-tile kernel (50 us at k = 4096): a round of 128 x 128 tiles takes about 0.4 (19 us), one of 128 x 256 tiles 0.65 (30 us)
-    const double cost = (double)((rows_large * tiles_n + per_round - 1) / per_round) + (mid == 1 ? 0.4 : 0.65);
-    if (cost > (double)((tiles + per_round - 1) / per_round) - 0.1) return {0, 0};
-    return {rows_large, mid};
-}
-
 // 256 x 224 tiles instead of 256 x 256: where they fill their rounds so much better that less is paid for.  A round of them takes 0.9
 // of one of those.  us, 256 / 224 columns: 2048 x 14336 over 1024: 38.6 / 36.5, over 4096: 98.5 / 90.1, over 8192: 176.7 / 162.1 (448 tiles, 1.75
 // rounds, against 512); 2048 x 28672 over 4096: 188.6 / 174.2; 4096 x 6144 over 4096 (384, 448): 92.4 / 87.0; 5120 x 5120 over 5120: 110.0 /

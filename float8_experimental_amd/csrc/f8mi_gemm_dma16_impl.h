@@ -43,6 +43,22 @@ __device__ __forceinline__ void mfma16_first(v4f& acc, const v8i& first, const v
     asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, 0 cbsz:%3 blgp:%4" : "=a"(acc) : "v"(first), "v"(second), "n"(F1), "n"(F2));
 }
 
+// The same with block scales: bytes TJ of scale_first's and TI of scale_second's words (OP: TJ % 4 + 4 * (TI % 4), the two op_sel bits of each).
+template <int F1, int F2, int OP>
+__device__ __forceinline__ void mfma16_block(v4f& acc, const v8i& first, const v8i& second, uint32_t scale_first, uint32_t scale_second, bool from_zero) {
+    if (from_zero)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:%9 blgp:%10"
+                     : "=a"(acc) : "v"(first), "v"(second), "v"(scale_first), "v"(scale_second), "n"(OP & 1), "n"((OP >> 2) & 1), "n"((OP >> 1) & 1), "n"((OP >> 3) & 1), "n"(F1), "n"(F2));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:%9 blgp:%10"
+                     : "+a"(acc) : "v"(first), "v"(second), "v"(scale_first), "v"(scale_second), "n"(OP & 1), "n"((OP >> 2) & 1), "n"((OP >> 1) & 1), "n"((OP >> 3) & 1), "n"(F1), "n"(F2));
+}
+template <int F1, int F2, int OP = 0>
+__device__ __forceinline__ void mfma16_block_any(int op, v4f& acc, const v8i& first, const v8i& second, uint32_t scale_first, uint32_t scale_second, bool from_zero) {
+    if (op == OP) mfma16_block<F1, F2, OP>(acc, first, second, scale_first, scale_second, from_zero);  // constants once the caller's loops are unrolled
+    else if constexpr (OP < 15) mfma16_block_any<F1, F2, OP + 1>(op, acc, first, second, scale_first, scale_second, from_zero);
+}
+
 // One accumulator register into a vector register, as an instruction of its own: it stays where it is written
 // relative to the MFMAs (also volatile asm).  Left to the compiler, which takes the MFMAs for ordinary
 // instructions, the copy may be placed right behind the MFMA that produces the value, where it reads the old one.
@@ -201,12 +217,24 @@ struct Epilogue16 {
 // are built with ds_read_b64_tr_b8.  For such an operand lda / ldb is the byte distance between contraction
 // rows (64 when k-blocked over `rows`, the row stride when row-major) and a_unit / b_unit the distance between
 // blocks of 64 rows (contraction length * 64 when k-blocked, 64 when row-major).
+// BLK: block scales (f8mi_block.h) in sa_blk / sb_blk, whose rows for the next 128 of k are sa_ld / sb_ld bytes on; sa_dev and sb_dev are not
+// read.  Each wave brings the 256 bytes it needs for a step (128 rows of A, 128 of Bt) with one DMA more.  They need LDS where the
+// five slabs fill it: three slabs of A hold three steps, of which the third is needed for what step t + 2 brings while step t is read.  But group 0 of
+// step t (the 16 + 16 rows of the first fragments) has been read by everybody before step t begins, so its place is free as well: A lies in a
+// ring of 23 groups of 4 KB, group g of step t in the ((8 t + g) mod 23)-th, and the 4 KB saved hold the scales of four steps.
 // Workgroup `lid` of the `npid` that compute this product.
-template <int AF, int BF, int C_DT, bool ODD, bool A_TR, bool B_TR, bool ODD_ROWS, int TJ, bool BIAS_AFTER = false>
+constexpr int RING_GROUPS = 23, GROUP_BYTES = 4096, BLK_SCALE_BYTES = 4 * 1024;
+__device__ __forceinline__ int ring_at(int i) { return i >= RING_GROUPS ? i - RING_GROUPS : i; }
+static_assert(RING_GROUPS * GROUP_BYTES + BLK_SCALE_BYTES == NSLAB_A * SLAB_BYTES, "the same LDS");
+template <int AF, int BF, int C_DT, bool ODD, bool A_TR, bool B_TR, bool ODD_ROWS, int TJ, bool BIAS_AFTER = false, bool BLK = false>
 __device__ __forceinline__ void gemm_dma16_tile(
     int lid, const int npid, const uint8_t* __restrict__ A, int64_t lda, int64_t a_unit, const uint8_t* __restrict__ Bt, int64_t ldb, int64_t b_unit,
     int M, int N, int K, const float* __restrict__ sa_dev, const float* __restrict__ sb_dev, void* __restrict__ C,
-    int64_t ldc, const void* __restrict__ bias, int tiles_m, int tiles_n, int c_vec_ok, int bias_fp32 = 0) {
+    int64_t ldc, const void* __restrict__ bias, int tiles_m, int tiles_n, int c_vec_ok, int bias_fp32 = 0,
+    const uint8_t* __restrict__ sa_blk = nullptr, int64_t sa_ld = 0, const uint8_t* __restrict__ sb_blk = nullptr, int64_t sb_ld = 0) {
+    static_assert(!BLK || (!A_TR && TJ == 8), "block scales: A as it is, 256 x 256 tiles");
+    constexpr int B_BASE = BLK ? RING_GROUPS * GROUP_BYTES : NSLAB_A * SLAB_BYTES;  // LDS: A, Bt, scales
+    constexpr int SCALE_BASE = B_BASE + NSLAB_B * LargeCfg<TJ>::B_SLAB;
     static_assert(TJ == 8 || (TJ == 7 && !A_TR && !B_TR && !ODD_ROWS), "narrower tiles: operands as they are");
     using Cfg = LargeCfg<TJ>;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -249,7 +277,8 @@ __device__ __forceinline__ void gemm_dma16_tile(
     const int m0 = tm * BM, n0 = tn * Cfg::TILE_N;
     // 1 / (sa * sb) for the epilogue, fetched now and kept in a scalar register: loaded after the main loop, the two
     // scales were a memory round trip with nothing to hide it
-    const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(
+    float inv = 1.0f;
+    if constexpr (!BLK) inv = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(
         int, __fdiv_rn(1.0f, *sa_dev) * __fdiv_rn(1.0f, *sb_dev))));
 
     const int t = threadIdx.x;
@@ -268,7 +297,7 @@ __device__ __forceinline__ void gemm_dma16_tile(
     // Transposed operand: instruction j = wave*8 + d covers contraction rows 4j .. 4j+3 of the slab, 256 bytes
     // (16 slots) each; lane l fetches row 4j + l/16, the slot that belongs at position l%16: (l%16) ^ f(row).
     const uint32_t lds_u32 = (uint32_t)(uintptr_t)smem;
-    uint32_t a_voff[A_TR ? 8 : 4], b_voff[B_TR ? 8 : TJ == 8 ? 4 : TJ];
+    uint32_t a_voff[A_TR || BLK ? 8 : 4], b_voff[B_TR ? 8 : TJ == 8 ? 4 : TJ];
     const uint8_t* a_ptr;  // first byte of the next step to be fetched
     const uint8_t* b_ptr;
     int64_t a_step, b_step;  // bytes from one step's data to the next
@@ -282,6 +311,15 @@ __device__ __forceinline__ void gemm_dma16_tile(
         }
         a_ptr = A + (int64_t)(m0 / 64) * a_unit;
         a_step = 128 * lda;
+    } else if constexpr (BLK) {
+        // DMA d of wave w brings a quarter of group d: unit w / 2 of the 16 rows 128 (w % 2) + 16 d ..
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            const int r = (wave & 1) * 128 + d * 16 + (lane >> 2);
+            a_voff[d] = (uint32_t)(min(r, M - 1 - m0) * lda) + (((lane & 3) ^ (lane >> 5)) << 4);
+        }
+        a_ptr = A + (int64_t)m0 * lda + (wave >> 1) * a_unit;
+        a_step = 2 * a_unit;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -312,9 +350,22 @@ __device__ __forceinline__ void gemm_dma16_tile(
         b_step = 2 * b_unit;
     }
     uint32_t a_dst = 0, b_dst = 0;  // LDS address of the slabs being refilled
+    int a_fill = 0, s_fill = 0;     // BLK: place in the ring of the first group being filled; which of the four steps' scales
+    const uint8_t* s_ptr = nullptr;
+    int64_t s_step = 0;
+    if constexpr (BLK) {  // lanes 0 - 31: the scales of the wave's rows of A, the others those of Bt; groups past the edge: the last one again
+        const int64_t row = lane < 32 ? min((int64_t)m0 + wm * 128, sa_ld - 128) : min((int64_t)n0 + wn * 128, sb_ld - 128);
+        s_ptr = (lane < 32 ? sa_blk : sb_blk) + row + (lane & 31) * 4;
+        s_step = lane < 32 ? sa_ld : sb_ld;
+    }
+    auto issue_scales = [&]() __attribute__((always_inline)) {
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(s_ptr), "s"(lds_u32 + SCALE_BASE + s_fill * 1024 + wave * 256) : "memory");
+        s_ptr += s_step;
+    };
     // DMA d = 0..7 of this wave's share of a slab
     auto issue_a = [&](int d) __attribute__((always_inline)) {
         if constexpr (A_TR) dma16b(a_ptr, a_voff[d], a_dst + (wave * 8 + d) * 1024);
+        else if constexpr (BLK) dma16b(a_ptr, a_voff[d], lds_u32 + ring_at(a_fill + d) * GROUP_BYTES + wave * 1024);
         else dma16b(d < 4 ? a_ptr : a_ptr + a_unit, a_voff[d & 3], a_dst + wave * 4096 + (d >> 2) * HALF_BYTES + (d & 3) * 1024);
         if (d == 7) a_ptr += a_step;
     };
@@ -347,9 +398,14 @@ __device__ __forceinline__ void gemm_dma16_tile(
     }
     const int a_frag_base = (wm * 128) * 64;
     const int b_frag_base = (wn * (16 * TJ)) * 64 + (fq >> 1) * (Cfg::B_HALF - HALF_BYTES);
-    auto frag_a = [&](const uint8_t* slab, int ti) __attribute__((always_inline)) {
+    const int g_off0 = (fq >> 1) * 2048 + wm * 1024 + frow * 64 + ((((fq & 1) * 2 + 0) ^ fsw) << 4);  // BLK: inside a group
+    const int g_off1 = (fq >> 1) * 2048 + wm * 1024 + frow * 64 + ((((fq & 1) * 2 + 1) ^ fsw) << 4);
+    auto frag_a = [&](const uint8_t* slab, int ti, int at = 0) __attribute__((always_inline)) {  // BLK: group ti from the place `at`
         if constexpr (A_TR) {
             return read_frag_tr(slab + a_tr_off[ti]);
+        } else if constexpr (BLK) {
+            const uint8_t* p = smem + ring_at(at + ti) * GROUP_BYTES;
+            return read_frag(p + g_off0, p + g_off1);
         } else {
             const uint8_t* p = slab + a_frag_base + ti * 16 * 64;
             return read_frag(p + f_off0, p + f_off1);
@@ -368,29 +424,41 @@ __device__ __forceinline__ void gemm_dma16_tile(
 
     v8i fb[2][TJ];  // [step parity][n tile]
     v8i fa[2];     // rolling: group ti multiplies fa[ti & 1] while fa[(ti + 1) & 1] is being fetched
+    uint2 fsa[2], fsb[2];  // [step parity]: byte ti / tj
+    auto frag_scales = [&](int step, bool of_b) __attribute__((always_inline)) {
+        return *(const uint2*)(smem + SCALE_BASE + (step & 3) * 1024 + wave * 256 + (of_b ? 128 : 0) + frow * 8);
+    };
 
     // ---- prologue: steps 0 and 1 (A into slabs 0, 1; Bt into slabs 3, 4), wait for step 0,
     // first fragments; a second barrier before step 0 refills the Bt slab just read.
 #pragma unroll
     for (int s = 0; s < 2; s++) {
         a_dst = lds_u32 + s * SLAB_BYTES;
-        b_dst = lds_u32 + NSLAB_A * SLAB_BYTES + s * Cfg::B_SLAB;
+        a_fill = s * 8;
+        s_fill = s;
+        b_dst = lds_u32 + B_BASE + s * Cfg::B_SLAB;
 #pragma unroll
         for (int d = 0; d < 8; d++) issue_a(d);
 #pragma unroll
         for (int d = 0; d < TJ; d++) issue_b(d);
+        if constexpr (BLK) issue_scales();
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(8 + TJ) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(8 + TJ + (BLK ? 1 : 0)) : "memory");
     lds_barrier();
 #pragma unroll
-    for (int x = 0; x < TJ; x++) fb[0][x] = frag_b(smem + NSLAB_A * SLAB_BYTES, x);
+    for (int x = 0; x < TJ; x++) fb[0][x] = frag_b(smem + B_BASE, x);
     fa[0] = frag_a(smem, 0);
+    if constexpr (BLK) {
+        fsa[0] = frag_scales(0, false);
+        fsb[0] = frag_scales(0, true);
+    }
     lds_barrier();
 
     // One step t.  P: parity of t.  MODE 0: steps t+1 and t+2 exist (refills the slabs freed at this
     // step's start with step t+2); 1: last but one (nothing left to fetch); 2: last step; 3: step 0 (as 0,
     // and the accumulators start from zero).
     int a_slab = 0;  // slab of A of this step; step t+2 goes to the slab before it in the rotation
+    int a_at = 0, s_at = 0;  // BLK: place in the ring of this step's first group; the step
     Epilogue16<C_DT, ODD_ROWS, TJ, BIAS_AFTER> epi(m0, n0, M, N, inv, C, ldc, bias, bias_fp32, c_vec_ok);
     auto step = [&](auto parity, auto mode) __attribute__((always_inline)) {
         constexpr int P = decltype(parity)::value;
@@ -400,10 +468,13 @@ __device__ __forceinline__ void gemm_dma16_tile(
         const int a_free = a_next + 1 == NSLAB_A ? 0 : a_next + 1;  // held step t-1
         const uint8_t* a_cur = smem + a_slab * SLAB_BYTES;
         const uint8_t* a_nxt = smem + a_next * SLAB_BYTES;
-        const uint8_t* b_nxt = smem + NSLAB_A * SLAB_BYTES + (P ^ 1) * Cfg::B_SLAB;
+        const uint8_t* b_nxt = smem + B_BASE + (P ^ 1) * Cfg::B_SLAB;
+        const int a_at_next = ring_at(a_at + 8);
         if (MODE == 0) {
             a_dst = lds_u32 + a_free * SLAB_BYTES;
-            b_dst = lds_u32 + NSLAB_A * SLAB_BYTES + P * Cfg::B_SLAB;  // Bt of this step: already in registers
+            a_fill = ring_at(a_at_next + 8);
+            s_fill = (s_at + 2) & 3;
+            b_dst = lds_u32 + B_BASE + P * Cfg::B_SLAB;  // Bt of this step: already in registers
         }
         // Everything that is not an MFMA sits in a fixed slot between two MFMAs (each keeps the matrix
         // core busy for 32 cycles): one fragment (two 16-byte LDS reads) or one DMA at a time.
@@ -420,15 +491,21 @@ __device__ __forceinline__ void gemm_dma16_tile(
             }
 #pragma unroll
             for (int tj = 0; tj < TJ; tj++) {
-                if (tj == 0 && ti < 7) fa[(ti + 1) & 1] = frag_a(a_cur, ti + 1);
-                if (tj == 0 && ti == 7 && MODE < 2) fa[0] = frag_a(a_nxt, 0);
+                if (tj == 0 && ti < 7) fa[(ti + 1) & 1] = frag_a(a_cur, ti + 1, a_at);
+                if (tj == 0 && ti == 7 && MODE < 2) fa[0] = frag_a(a_nxt, 0, a_at_next);
+                if constexpr (BLK) {
+                    if (MODE < 2 && ti == 6 && tj == 2) fsa[P ^ 1] = frag_scales(s_at + 1, false);
+                    if (MODE < 2 && ti == 6 && tj == 6) fsb[P ^ 1] = frag_scales(s_at + 1, true);
+                }
                 if constexpr (TJ == 8) {
                     if (MODE < 2 && ti >= 6 && (tj & 1) == 1) fb[P ^ 1][(ti - 6) * 4 + (tj >> 1)] = frag_b(b_nxt, (ti - 6) * 4 + (tj >> 1));
                 } else {  // four of the seven in the last but one row, three in the last
                     if (MODE < 2 && ti == 6 && (tj == 1 || tj == 3 || tj >= 5)) fb[P ^ 1][tj == 6 ? 3 : tj >> 1] = frag_b(b_nxt, tj == 6 ? 3 : tj >> 1);
                     if (MODE < 2 && ti == 7 && (tj & 1) == 1) fb[P ^ 1][4 + (tj >> 1)] = frag_b(b_nxt, 4 + (tj >> 1));
                 }
-                if (FIRST) mfma16_first<BF, AF>(acc[tj][ti], fb[P][tj], fa[ti & 1]);
+                if constexpr (BLK)
+                    mfma16_block_any<BF, AF>((tj & 3) | (ti & 3) << 2, acc[tj][ti], fb[P][tj], fa[ti & 1], tj < 4 ? fsb[P].x : fsb[P].y, ti < 4 ? fsa[P].x : fsa[P].y, FIRST);
+                else if (FIRST) mfma16_first<BF, AF>(acc[tj][ti], fb[P][tj], fa[ti & 1]);
                 else mfma16<BF, AF>(acc[tj][ti], fb[P][tj], fa[ti & 1]);
                 F8MI_SCHED_FENCE();
                 // (seven tiles: a place later, and the last one in the row after, for the same distance from the MFMA that wrote it)
@@ -450,10 +527,18 @@ __device__ __forceinline__ void gemm_dma16_tile(
                     else if (d - 8 < TJ) issue_b(d - 8);
                     F8MI_SCHED_FENCE();
                 }
+                if constexpr (BLK) {
+                    if (MODE == 0 && ti == 7 && tj == 6) {
+                        issue_scales();
+                        F8MI_SCHED_FENCE();
+                    }
+                }
             }
         }
         if (MODE < 2) lds_barrier();  // step boundary: everybody is done with A of step t and has Bt of step t+1 in registers
         a_slab = a_next;
+        a_at = a_at_next;
+        s_at++;
     };
 
     constexpr std::integral_constant<int, 0> c0{};

@@ -364,6 +364,23 @@ inline int use_mid_tiles(int64_t m, int64_t n, int64_t k) {
     if (row_tiles * ((n + 255) / 256) <= 256) return 2;
     return 0;
 }
+// An output whose last round of 256 x 256 tiles would leave most CUs idle (at most 128 tiles in it) is split by
+// rows: the tile rows that fill whole rounds go to the large-tile kernel, the rest to a 128-row-tile kernel that
+// spreads them over all CUs (same accumulation order, so no output bit depends on the split).  Returns the number
+// of tile rows for the large tiles (0: no split) and which 128-row tile takes the rest.
+struct RowSplit { int64_t rows_large; int mid; };
+inline RowSplit split_last_round(int64_t tiles_m, int64_t tiles_n, int64_t k) {
+    const int64_t tiles = tiles_m * tiles_n, per_round = 256;
+    if (tiles <= per_round || tiles % per_round == 0) return {0, 0};
+    const int64_t rows_large = (tiles / per_round) * per_round / tiles_n;
+    if (rows_large < 1 || rows_large >= tiles_m) return {0, 0};
+    const int mid = use_mid_tiles((tiles_m - rows_large) * BM, tiles_n * BN, k);
+    if (!mid) return {0, 0};
+    // in rounds of the large-tile kernel (50 us at k = 4096): a round of 128 x 128 tiles takes about 0.4 (19 us), one of 128 x 256 tiles 0.65 (30 us)
+    const double cost = (double)((rows_large * tiles_n + per_round - 1) / per_round) + (mid == 1 ? 0.4 : 0.65);
+    if (cost > (double)((tiles + per_round - 1) / per_round) - 0.1) return {0, 0};
+    return {rows_large, mid};
+}
 // few-row kernel (f8mi_gemm_skinny.hip): m <= SKINNY_MAX_M, K % 128 == 0, aligned operands.
 constexpr int SKINNY_MAX_M = 256;
 // Time estimates in us behind the choice between the few-row kernel, a round of 128-row tiles, and the same tiles
