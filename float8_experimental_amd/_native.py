@@ -70,6 +70,7 @@ EXPORTS = (
     "f8mi_block_cast",
     "f8mi_block_gemm",
     "f8mi_block_gemm_workspace_bytes",
+    "f8mi_block_linear_few_rows",
     "f8mi_layer_norm",
     "f8mi_layer_norm_backward",
     "f8mi_layer_norm_workspace_bytes",
@@ -193,6 +194,8 @@ def lib() -> C.CDLL:
         L.f8mi_block_cast.argtypes = [C.POINTER(BlockCastJob), i32, vp]
         L.f8mi_block_gemm.restype = i32
         L.f8mi_block_gemm.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, vp, i32, i64, vp, vp, i64, vp]
+        L.f8mi_block_linear_few_rows.restype = i32
+        L.f8mi_block_linear_few_rows.argtypes = [vp, i64, i32, vp, vp, i64, i64, i64, vp, i64, vp, vp]
         L.f8mi_block_gemm_workspace_bytes.restype = i64
         L.f8mi_block_gemm_workspace_bytes.argtypes = [i64, i64, i64]
         L.f8mi_layer_norm.restype = i32

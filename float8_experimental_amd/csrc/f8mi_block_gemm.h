@@ -32,6 +32,8 @@ struct BlockGemm {
 };
 
 int launch_block_mid(const BlockGemm& g, bool wide, int k_splits, float* partial);
+// M <= SKINNY_MAX_M, operands as they are
+int launch_block_few(const BlockGemm& g);
 // tiles_m tile rows of 256 from the first; K >= 384.  The second is taken by the first for such rows of C, the third for b_tr.
 int launch_block_large(const BlockGemm& g, int tiles_m, int tiles_n);
 int launch_block_large_odd(const BlockGemm& g, int tiles_m, int tiles_n);

@@ -1,5 +1,5 @@
 // Products of operands with block scales (f8mi_block.h) on 128-row tiles, and the choice of kernel.  Main loop, LDS layout and epilogue are
-// those of f8mi_gemm_mid_impl.h; a stage brings 256 bytes of scales more for each wave, and the matrix instruction applies them.
+// those of f8mi_gemm_mid_impl.h, the choice that of f8mi_gemm.hip; a stage brings 256 bytes of scales more for each wave, and the matrix instruction applies them.
 #include "f8mi_block_gemm.h"
 #include "f8mi_gemm_mid_impl.h"
 
@@ -76,6 +76,7 @@ extern "C" int f8mi_block_gemm(const void* a, const void* a_scales, const void* 
     ProfScope prof(F8MI_K_GEMM, 2.0 * (double)m * (double)n * (double)k, g.stream);
     const int splits = workspace && !b_transposed ? pick_k_splits(m, n, k, workspace_bytes) : 0;
     if (splits > 1) return launch_block_mid(g, use_mid_tiles(m, n, k) == 2, splits, (float*)workspace);
+    if (!b_transposed && use_skinny(m, n, k)) return launch_block_few(g);
     if (const int mid = use_mid_tiles(m, n, k)) return launch_block_mid(g, mid == 2, 1, nullptr);
     if (k < 384) return launch_block_mid(g, true, 1, nullptr);
     // the tile rows that fill whole rounds of 256 x 256 tiles, and the rest on 128-row tiles where that is faster

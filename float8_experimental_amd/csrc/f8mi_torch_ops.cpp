@@ -32,6 +32,7 @@ struct Lib {
     decltype(&f8mi_block_cast) block_cast;
     decltype(&f8mi_block_gemm) block_gemm;
     decltype(&f8mi_block_gemm_workspace_bytes) block_gemm_workspace_bytes;
+    decltype(&f8mi_block_linear_few_rows) block_linear_few_rows;
     decltype(&f8mi_column_sum) column_sum;
     decltype(&f8mi_column_sum_workspace_bytes) column_sum_workspace_bytes;
     decltype(&f8mi_layer_norm) layer_norm;
@@ -290,6 +291,13 @@ PyObject* blockwise_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
+// Cast and product of a few rows in one kernel: every workgroup converts all of the activations for itself, which costs more than the launch it saves
+// once there are many of them and many rows (the lines of the linears with one scale).
+bool one_kernel_pays(int64_t m, int64_t n, int64_t kp, int dt) {
+    if (m > 16 || m * kp > F8MI_FEW_ROWS_ELEMS) return false;
+    return dt == F8MI_FP32 ? n <= 16384 || m * n <= 65536 : m * n <= 262144;
+}
+
 // blockwise_inference_linear(x [m, k], data, scales of the weight, n, bias or None, device) -> y or None
 PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!expect(n_args, 6, "blockwise_inference_linear")) return nullptr;
@@ -314,6 +322,10 @@ PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n
             const at::Tensor b = bias.defined() ? bias.to(x.scalar_type()).contiguous() : at::Tensor();
             if (xr.rows == 0) {
                 y = at::empty(y_shape, x.options());
+            } else if (one_kernel_pays(xr.rows, n, kp, xr.dtype())) {
+                y = at::empty(y_shape, x.options());
+                check(L.block_linear_few_rows(xr.t.data_ptr(), xr.ld, xr.dtype(), data.data_ptr(), scales.data_ptr(), xr.rows, n, k, y.data_ptr(), n, ptr(b), stream_of(x)),
+                      "f8mi_block_linear_few_rows");
             } else {
                 const Blocks x8 = Blocks::make(x, xr.rows, k);
                 const f8mi_block_cast_job job = job_of(xr, false, x8, Blocks());
@@ -420,6 +432,7 @@ PyObject* load(PyObject*, PyObject* args) {
     get(L.block_cast, "f8mi_block_cast");
     get(L.block_gemm, "f8mi_block_gemm");
     get(L.block_gemm_workspace_bytes, "f8mi_block_gemm_workspace_bytes");
+    get(L.block_linear_few_rows, "f8mi_block_linear_few_rows");
     get(L.column_sum, "f8mi_column_sum");
     get(L.column_sum_workspace_bytes, "f8mi_column_sum_workspace_bytes");
     get(L.layer_norm, "f8mi_layer_norm");

@@ -480,6 +480,12 @@ int f8mi_block_cast(const f8mi_block_cast_job* jobs, int count, void* stream);
  * NULL): with F8MI_GEMM_WORKSPACE_BYTES of it a long contraction of few tiles is split over workgroups, the parts added in a fixed order. */
 int f8mi_block_gemm(const void* a, const void* a_scales, const void* bt, const void* b_scales, int b_transposed, int64_t m, int64_t n, int64_t k,
                     void* c, int c_dtype, int64_t ldc, const void* bias_dev, void* workspace, int64_t workspace_bytes, void* stream);
+/* A whole linear of at most 16 rows and F8MI_FEW_ROWS_ELEMS activations (k rounded up to a multiple of 128) in one kernel: the values of
+ * f8mi_block_cast of x and f8mi_block_gemm.  x [m][k] of `dtype`, also that of c and the bias, ldx 0: one row throughout; w, w_scales: copy of n rows contracting over k.
+ * F8MI_ERR_UNSUPPORTED for more rows or activations. */
+int f8mi_block_linear_few_rows(const void* x, int64_t ldx, int dtype, const void* w, const void* w_scales, int64_t m, int64_t n, int64_t k, void* c, int64_t ldc,
+                               const void* bias_dev, void* stream);
+
 /* Bytes of workspace that this product makes use of (0: none).  Needs no GPU. */
 int64_t f8mi_block_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
 

@@ -281,6 +281,7 @@ def test_modules(f8):
         product_close(served[0](x), kept(x, 1, 128), kept(weights[0], 128, 128), weights[1])
         assert torch.equal(served[0].dequantized_weight().double().cpu(), kept(weights[0], 128, 128))
         assert served[0](x[:0]).shape == (0, 200) and served[0](x[0]).shape == (200,)
+        assert torch.equal(served[0](x[:1].expand(9, 96)), served[0](x[:1].repeat(9, 1)))
         again = f8.Float8BlockwiseInferenceLinear(96, 200, torch.zeros(200, dtype=BF16, device="cuda"), device="cuda")
         again.load_state_dict(served[0].state_dict())
         assert torch.equal(again(x), served[0](x))
@@ -358,3 +359,19 @@ def test_refusals(f8, nat):
     y = f8.blockwise_linear(x.requires_grad_(), w)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 8192, 4096), (2, 300, 130), (4, 8192, 700), (16, 2048, 8300), (16, 100, 512), (3, 4097, 5000), (1, 32768, 64)])
+def test_one_kernel_linears_have_the_values_of_cast_and_product(nat, m, k, n):
+    for dtype in (BF16, FP16, FP32):
+        base, w, bias = values((m, k + 3), dtype, m + k).cuda(), values((n, k), dtype, 1, k**-0.5).cuda(), values((n,), dtype, 2).cuda()
+        x = base[:, 3:]  # rows at any alignment
+        (a, _), (b, _) = nat.block_cast([(x, False, True, False), (w, True, True, False)])
+        want = nat.block_gemm(a, b, dtype, bias)
+        got = torch.empty_like(want)
+        rc = nat.lib().f8mi_block_linear_few_rows(x.data_ptr(), x.stride(0), nat._DT[dtype], b.data.data_ptr(), b.scales.data_ptr(), m, n, k, got.data_ptr(), n, bias.data_ptr(),
+                                                  torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        product_close(got, a.dequant().cpu(), b.dequant().cpu(), bias)
+        if nat.lib().f8mi_block_gemm_workspace_bytes(m, n, nat.padded_k(k)) == 0:  # both few-row kernels split k the same way
+            assert torch.equal(got, want)
