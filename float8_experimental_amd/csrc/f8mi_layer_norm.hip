@@ -28,22 +28,33 @@ __device__ __forceinline__ void ln_unpack(uint4 q, float (&v)[Ln<DT>::V]) {
         else unpack2<DT>(w[i], v[2 * i], v[2 * i + 1]);
     }
 }
-// values col .. col + V - 1 of a row, zeros past the end
-template <int DT>
-__device__ __forceinline__ uint4 ln_load(const uint8_t* row, int64_t col, int64_t cols) {
+// Values col .. col + V - 1 of a row, zeros past its end: there the last V values of the row are read and shifted (element by element that
+// part held 30 registers more, in every lane).  I: int, or int64_t where columns may need it.
+template <int DT, typename I>
+__device__ __forceinline__ uint4 ln_load(const uint8_t* row, I col, I cols) {
     constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
     if (col + V <= cols) return load_nt16_any(row + col * SIZE);
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < V; i++)
-        if (col + i < cols) {
-            if constexpr (DT == F8MI_FP32) w[i] = ((const uint32_t*)row)[col + i];
-            else w[i >> 1] |= (uint32_t)((const uint16_t*)row)[col + i] << (16 * (i & 1));
+    uint64_t lo = 0, hi = 0;
+    if (col < cols && cols >= V) {
+        const uint4 q = load_nt16_any(row + (cols - V) * SIZE);
+        const int shift = (int)(col + V - cols) * SIZE * 8;  // 0 < shift < 128
+        lo = q.x | (uint64_t)q.y << 32;
+        hi = q.z | (uint64_t)q.w << 32;
+        lo = shift >= 64 ? hi >> (shift - 64) : (lo >> shift) | (hi << (64 - shift));
+        hi = shift >= 64 ? 0 : hi >> shift;
+    } else {
+#pragma unroll 1
+        for (I i = col; i < cols; i++) {  // a row of less than V values
+            const uint64_t e = DT == F8MI_FP32 ? ((const uint32_t*)row)[i] : ((const uint16_t*)row)[i];
+            const int at = (int)(i - col) * SIZE * 8;
+            if (at < 64) lo |= e << at;
+            else hi |= e << (at - 64);
         }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
-template <int DT>
-__device__ __forceinline__ void ln_store(uint8_t* row, int64_t col, int64_t cols, const float (&v)[Ln<DT>::V]) {
+template <int DT, typename I>
+__device__ __forceinline__ void ln_store(uint8_t* row, I col, I cols, const float (&v)[Ln<DT>::V]) {
     constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
     uint32_t w[4];
 #pragma unroll
@@ -55,24 +66,49 @@ __device__ __forceinline__ void ln_store(uint8_t* row, int64_t col, int64_t cols
         store16_any(row + col * SIZE, make_uint4(w[0], w[1], w[2], w[3]));
         return;
     }
-#pragma unroll
-    for (int i = 0; i < V; i++)
-        if (col + i < cols) {
-            if constexpr (DT == F8MI_FP32) ((uint32_t*)row)[col + i] = w[i];
-            else ((uint16_t*)row)[col + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-        }
+    uint64_t lo = w[0] | (uint64_t)w[1] << 32, hi = w[2] | (uint64_t)w[3] << 32;
+#pragma unroll 1
+    for (; col < cols; col++) {
+        if constexpr (DT == F8MI_FP32) ((uint32_t*)row)[col] = (uint32_t)lo;
+        else ((uint16_t*)row)[col] = (uint16_t)lo;
+        lo = lo >> (SIZE * 8) | hi << (64 - SIZE * 8);
+        hi >>= SIZE * 8;
+    }
+}
+// What is unpacked after this is not kept from before: 16-bit rows stay packed while their sums are waited for.
+template <int DT>
+__device__ __forceinline__ void set_apart(uint4& q) {
+    if constexpr (DT != F8MI_FP32) asm("" : "+v"(q.x), "+v"(q.y), "+v"(q.z), "+v"(q.w));
 }
 // V values of a parameter (`otherwise` without one)
-template <int PT, int V>
-__device__ __forceinline__ void ln_param(const void* p, int64_t col, int64_t cols, float otherwise, float (&v)[V]) {
+template <int PT, int V, typename I>
+__device__ __forceinline__ void ln_param(const void* p, I col, I cols, float otherwise, float (&v)[V]) {
+    constexpr int PV = Ln<PT>::V;
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i] = p && col + i < cols ? load_bias<PT>(p, (int)(col + i)) : otherwise;
+    for (int i = 0; i < V; i += PV) {
+        float f[PV];
+        if (p) {
+            ln_unpack<PT>(ln_load<PT, I>((const uint8_t*)p, col + i, cols), f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PV; j++) f[j] = otherwise;
+        }
+#pragma unroll
+        for (int j = 0; j < PV; j++) v[i + j] = f[j];
+    }
 }
 
+// The sum over a wave, in every lane: rotations inside the rows of 16 lanes, then exchanges of rows and halves
+template <int CTRL>
+__device__ __forceinline__ float plus_rotated(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    v = plus_rotated<0x128>(plus_rotated<0x124>(plus_rotated<0x122>(plus_rotated<0x121>(v))));  // row_ror 1, 2, 4, 8
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 // Two sums over the T lanes of a row, in every one of them.  `slots`: two floats for each wave of the workgroup, not in use elsewhere
 // until the next barrier but one.
@@ -86,7 +122,7 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float2* slots) {
         __syncthreads();
         const int first = wave / (T / 64) * (T / 64);
         a = b = 0.f;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < T / 64; i++) {
             const float2 s = slots[first + i];
             a += s.x;
@@ -95,102 +131,171 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float2* slots) {
     }
 }
 
+// Mean and sum of squares about it, of the T lanes of a row that hold VPT pieces each.  A wave finds its own (in two passes over its
+// registers, so nothing cancels), and those of the waves are put together: the squares about the common mean are a wave's own plus count * (mean of
+// the wave - mean)^2.  One barrier a row.
+template <int T, int VPT, int V>
+__device__ __forceinline__ int wave_count(int wave, int cols) {  // values of the row in this wave of it
+    int n = 0;
+#pragma unroll
+    for (int p = 0; p < VPT; p++) n += min(max(cols - (p * T + wave * 64) * V, 0), 64 * V);
+    return n;
+}
+template <int T, int VPT, int V>
+__device__ __forceinline__ void row_moments(float& mean, float& m2, int cols, float inv_cols, float2* slots) {
+    if constexpr (T > 64) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) slots[wave] = make_float2(mean, m2);
+        __syncthreads();
+        const int first = wave / (T / 64) * (T / 64);
+        float total = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < T / 64; i++) total = __builtin_fmaf(slots[first + i].x, (float)wave_count<T, VPT, V>(i, cols), total);
+        mean = total * inv_cols;
+        m2 = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < T / 64; i++) {
+            const float2 w = slots[first + i];
+            const float d = w.x - mean;
+            m2 += __builtin_fmaf(d * d, (float)wave_count<T, VPT, V>(i, cols), w.y);
+        }
+    }
+}
+
 constexpr int ln_threads(int t) { return t < 256 ? 256 : t; }
+// One piece of 16 bytes a lane: 64 registers do, and a CU holds 2048 lanes; more pieces, or 16 waves that wait for each other: 1024 lanes.
+constexpr int ln_lanes(int t, int vpt) { return vpt == 1 && t < 1024 ? 2048 : 1024; }
+// Whether a row is asked for while the one before is waited for; the others have no registers for it.
+constexpr bool ln_ahead(int vpt) { return vpt == 1; }
+// Of a workgroup of the backward kernel, which writes a row of sums: one a CU, or two whose waits overlap where a row takes many pieces a lane.
+constexpr int ln_backward_threads(int vpt) { return vpt > 2 ? 512 : 1024; }
 
 // T lanes a row, VPT pieces of 16 bytes a lane
 template <int DT, int PT, int T, int VPT>
-__global__ __launch_bounds__(ln_threads(T)) void layer_norm_kernel(const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int64_t cols, const void* __restrict__ weight,
+__global__ __launch_bounds__(ln_threads(T), ln_lanes(T, VPT) / 256) void layer_norm_kernel(const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int cols, const void* __restrict__ weight,
                                                                    const void* __restrict__ bias, float eps, uint8_t* __restrict__ y, float2* __restrict__ stats) {
     constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_threads(T) / T;
     __shared__ float2 slots[2][ln_threads(T) / 64];
-    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    const int t = threadIdx.x % T, group = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
     const float inv_cols = 1.0f / (float)cols;
     float w[VPT][V], b[VPT][V];
 #pragma unroll
     for (int p = 0; p < VPT; p++) {
-        ln_param<PT, V>(weight, (int64_t)(p * T + t) * V, cols, 1.f, w[p]);
-        ln_param<PT, V>(bias, (int64_t)(p * T + t) * V, cols, 0.f, b[p]);
+        ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[p]);
+        ln_param<PT, V, int>(bias, (p * T + t) * V, cols, 0.f, b[p]);
     }
-    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += (int64_t)gridDim.x * GROUPS) {
-        const int64_t row = r0 + group;
-        const bool in = row < rows;
-        uint4 q[VPT];
-        float v[VPT][V];
+    const float inv_count = 1.0f / (float)max(wave_count<T, VPT, V>(t >> 6, cols), 1);
+    int parity = 0;
+    const int64_t stride = (int64_t)gridDim.x * GROUPS;
+    uint4 next[VPT];  // of the row after this one: asked for before this one's sums have to wait for each other
+    auto fetch = [&](int64_t row) __attribute__((always_inline)) {
 #pragma unroll
-        for (int p = 0; p < VPT; p++) q[p] = in ? ln_load<DT>(x + row * ld * SIZE, (int64_t)(p * T + t) * V, cols) : make_uint4(0u, 0u, 0u, 0u);
-        float s = 0.f, none = 0.f;
+        for (int p = 0; p < VPT; p++) next[p] = row < rows ? ln_load<DT, int>(x + row * ld * SIZE, (p * T + t) * V, cols) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    if (ln_ahead(VPT)) fetch((int64_t)blockIdx.x * GROUPS + group);
+    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += stride) {
+        const int64_t row = r0 + group;
+        if (!ln_ahead(VPT)) fetch(row);
+        const bool in = row < rows;
+        uint4 q[VPT];  // the row as it came: unpacking it again costs less than registers that keep waves from running
+#pragma unroll
+        for (int p = 0; p < VPT; p++) q[p] = next[p];
+        if (ln_ahead(VPT) && r0 + stride < rows) fetch(row + stride);
+        float s = 0.f, v[V];
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
-            ln_unpack<DT>(q[p], v[p]);
+            ln_unpack<DT>(q[p], v);
 #pragma unroll
-            for (int i = 0; i < V; i++) s += v[p][i];
+            for (int i = 0; i < V; i++) s += v[i];
         }
-        row_sums<T>(s, none, slots[0]);
-        const float mean = s * inv_cols;
+        float mean = wave_sum(s) * inv_count;
         s = 0.f;
 #pragma unroll
-        for (int p = 0; p < VPT; p++)
+        for (int p = 0; p < VPT; p++) {
+            set_apart<DT>(q[p]);
+            ln_unpack<DT>(q[p], v);
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                v[p][i] -= mean;
-                if ((int64_t)(p * T + t) * V + i < cols) s = __builtin_fmaf(v[p][i], v[p][i], s);
+                v[i] -= mean;
+                if ((p * T + t) * V + i < cols) s = __builtin_fmaf(v[i], v[i], s);
             }
-        row_sums<T>(s, none, slots[1]);
+        }
+        s = wave_sum(s);
+        row_moments<T, VPT, V>(mean, s, cols, inv_cols, slots[parity]);
+        parity ^= 1;
         const float rstd = 1.0f / __builtin_sqrtf(s * inv_cols + eps);
         if (!in) continue;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
-            float o[V];
+            set_apart<DT>(q[p]);
+            ln_unpack<DT>(q[p], v);
 #pragma unroll
-            for (int i = 0; i < V; i++) o[i] = __builtin_fmaf(v[p][i] * rstd, w[p][i], b[p][i]);
-            const int64_t col = (int64_t)(p * T + t) * V;
-            if (col < cols) ln_store<DT>(y + row * cols * SIZE, col, cols, o);
+            for (int i = 0; i < V; i++) v[i] = __builtin_fmaf((v[i] - mean) * rstd, w[p][i], b[p][i]);
+            const int col = (p * T + t) * V;
+            if (col < cols) ln_store<DT, int>(y + row * cols * SIZE, col, cols, v);
         }
         if (stats && t == 0) stats[row] = make_float2(mean, rstd);
     }
 }
 
 template <int DT, int PT, int T, int VPT>
-__global__ __launch_bounds__(ln_threads(T)) void layer_norm_backward_kernel(const uint8_t* __restrict__ dy, int64_t ld_dy, const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+__global__ __launch_bounds__(ln_backward_threads(VPT), 4) void layer_norm_backward_kernel(const uint8_t* __restrict__ dy, int64_t ld_dy, const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int cols,
                                                                             const void* __restrict__ weight, const float2* __restrict__ stats, uint8_t* __restrict__ dx,
                                                                             float* __restrict__ partial) {
-    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_threads(T) / T;
-    __shared__ float2 slots[2][ln_threads(T) / 64];
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_backward_threads(VPT) / T;
+    __shared__ float2 slots[2][ln_backward_threads(VPT) / 64];
     __shared__ float sums[GROUPS > 1 ? (GROUPS - 1) * T * 2 * V : 1];
-    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    const int t = threadIdx.x % T, group = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
     const float inv_cols = 1.0f / (float)cols;
-    float w[VPT][V], dw[VPT][V], db[VPT][V];
+    constexpr bool KEEP_W = VPT == 1 || DT == F8MI_FP32;  // else it is read again for each row, out of the L2: there are no registers for it
+    float w[KEEP_W ? VPT : 1][V], dw[VPT][V], db[VPT][V];
 #pragma unroll
     for (int p = 0; p < VPT; p++) {
-        ln_param<PT, V>(weight, (int64_t)(p * T + t) * V, cols, 1.f, w[p]);
+        if constexpr (KEEP_W) ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[p]);
 #pragma unroll
         for (int i = 0; i < V; i++) dw[p][i] = db[p][i] = 0.f;
     }
     int parity = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += (int64_t)gridDim.x * GROUPS, parity ^= 1) {
+    const int64_t stride = (int64_t)gridDim.x * GROUPS;
+    uint4 nx[VPT], ng[VPT];  // of the row after this one: asked for before this one's sums have to wait for each other
+    float2 ns;
+    auto fetch = [&](int64_t row) __attribute__((always_inline)) {
+        const bool in = row < rows;
+#pragma unroll
+        for (int p = 0; p < VPT; p++) {
+            const int col = (p * T + t) * V;
+            nx[p] = in ? ln_load<DT, int>(x + row * ld * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
+            ng[p] = in ? ln_load<DT, int>(dy + row * ld_dy * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        ns = in ? stats[row] : make_float2(0.f, 0.f);
+    };
+    if (ln_ahead(VPT)) fetch((int64_t)blockIdx.x * GROUPS + group);
+    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += stride, parity ^= 1) {
         const int64_t row = r0 + group;
+        if (!ln_ahead(VPT)) fetch(row);
         const bool in = row < rows;
         uint4 qx[VPT], qg[VPT];
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
-            const int64_t col = (int64_t)(p * T + t) * V;
-            qx[p] = in ? ln_load<DT>(x + row * ld * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
-            qg[p] = in ? ln_load<DT>(dy + row * ld_dy * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
+            qx[p] = nx[p];
+            qg[p] = ng[p];
         }
-        const float2 st = in ? stats[row] : make_float2(0.f, 0.f);
-        float xh[VPT][V], g[VPT][V], s1 = 0.f, s2 = 0.f;
+        const float2 st = ns;
+        if (ln_ahead(VPT) && r0 + stride < rows) fetch(row + stride);
+        float xh[V], g[V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
-            ln_unpack<DT>(qx[p], xh[p]);
-            ln_unpack<DT>(qg[p], g[p]);
+            ln_unpack<DT>(qx[p], xh);
+            ln_unpack<DT>(qg[p], g);
+            if constexpr (!KEEP_W) ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[0]);
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                xh[p][i] = (xh[p][i] - st.x) * st.y;
-                dw[p][i] = __builtin_fmaf(g[p][i], xh[p][i], dw[p][i]);
-                db[p][i] += g[p][i];
-                g[p][i] *= w[p][i];  // (past the end dy, and so g, is zero)
-                s1 += g[p][i];
-                s2 = __builtin_fmaf(g[p][i], xh[p][i], s2);
+                xh[i] = (xh[i] - st.x) * st.y;
+                dw[p][i] = __builtin_fmaf(g[i], xh[i], dw[p][i]);
+                db[p][i] += g[i];
+                g[i] *= w[KEEP_W ? p : 0][i];  // (past the end dy, and so g, is zero)
+                s1 += g[i];
+                s2 = __builtin_fmaf(g[i], xh[i], s2);
             }
         }
         if (!dx) continue;
@@ -200,11 +305,15 @@ __global__ __launch_bounds__(ln_threads(T)) void layer_norm_backward_kernel(cons
         if (!in) continue;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
-            float o[V];
+            set_apart<DT>(qx[p]);
+            set_apart<DT>(qg[p]);
+            ln_unpack<DT>(qx[p], xh);
+            ln_unpack<DT>(qg[p], g);
+            if constexpr (!KEEP_W) ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[0]);
 #pragma unroll
-            for (int i = 0; i < V; i++) o[i] = st.y * (g[p][i] - s1 - xh[p][i] * s2);
-            const int64_t col = (int64_t)(p * T + t) * V;
-            if (col < cols) ln_store<DT>(dx + row * cols * SIZE, col, cols, o);
+            for (int i = 0; i < V; i++) g[i] = st.y * (g[i] * w[KEEP_W ? p : 0][i] - s1 - (xh[i] - st.x) * st.y * s2);
+            const int col = (p * T + t) * V;
+            if (col < cols) ln_store<DT, int>(dx + row * cols * SIZE, col, cols, g);
         }
     }
     if (!partial) return;
@@ -222,7 +331,7 @@ __global__ __launch_bounds__(ln_threads(T)) void layer_norm_backward_kernel(cons
                 }
             __syncthreads();
             if (group > 0) continue;
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < GROUPS - 1; k++)
 #pragma unroll
                 for (int i = 0; i < V; i++) {
@@ -230,7 +339,7 @@ __global__ __launch_bounds__(ln_threads(T)) void layer_norm_backward_kernel(cons
                     db[p][i] += sums[((k * 2 + 1) * V + i) * T + t];
                 }
         }
-        const int64_t col = (int64_t)(p * T + t) * V;
+        const int col = (p * T + t) * V;
 #pragma unroll
         for (int i = 0; i < V; i++)
             if (col + i < cols) {
@@ -251,7 +360,7 @@ __global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_wide_kernel(const 
     const uint8_t* row = x + blockIdx.x * ld * SIZE;
     float v[V], s = 0.f, none = 0.f;
     for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
-        ln_unpack<DT>(ln_load<DT>(row, col, cols), v);
+        ln_unpack<DT>(ln_load<DT, int64_t>(row, col, cols), v);
 #pragma unroll
         for (int i = 0; i < V; i++) s += v[i];
     }
@@ -259,7 +368,7 @@ __global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_wide_kernel(const 
     const float mean = s / (float)cols;
     s = 0.f;
     for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
-        ln_unpack<DT>(ln_load<DT>(row, col, cols), v);
+        ln_unpack<DT>(ln_load<DT, int64_t>(row, col, cols), v);
 #pragma unroll
         for (int i = 0; i < V; i++)
             if (col + i < cols) s = __builtin_fmaf(v[i] - mean, v[i] - mean, s);
@@ -268,12 +377,12 @@ __global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_wide_kernel(const 
     const float rstd = 1.0f / __builtin_sqrtf(s / (float)cols + eps);
     for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
         float w[V], b[V];
-        ln_unpack<DT>(ln_load<DT>(row, col, cols), v);
-        ln_param<PT, V>(weight, col, cols, 1.f, w);
-        ln_param<PT, V>(bias, col, cols, 0.f, b);
+        ln_unpack<DT>(ln_load<DT, int64_t>(row, col, cols), v);
+        ln_param<PT, V, int64_t>(weight, col, cols, 1.f, w);
+        ln_param<PT, V, int64_t>(bias, col, cols, 0.f, b);
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] = __builtin_fmaf((v[i] - mean) * rstd, w[i], b[i]);
-        ln_store<DT>(y + blockIdx.x * cols * SIZE, col, cols, v);
+        ln_store<DT, int64_t>(y + blockIdx.x * cols * SIZE, col, cols, v);
     }
     if (stats && threadIdx.x == 0) stats[blockIdx.x] = make_float2(mean, rstd);
 }
@@ -287,9 +396,9 @@ __global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_backward_wide_kern
     const float2 st = stats[blockIdx.x];
     float xv[V], g[V], w[V], s1 = 0.f, s2 = 0.f;
     for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
-        ln_unpack<DT>(ln_load<DT>(row, col, cols), xv);
-        ln_unpack<DT>(ln_load<DT>(grow, col, cols), g);
-        ln_param<PT, V>(weight, col, cols, 1.f, w);
+        ln_unpack<DT>(ln_load<DT, int64_t>(row, col, cols), xv);
+        ln_unpack<DT>(ln_load<DT, int64_t>(grow, col, cols), g);
+        ln_param<PT, V, int64_t>(weight, col, cols, 1.f, w);
 #pragma unroll
         for (int i = 0; i < V; i++) {
             g[i] *= w[i];
@@ -301,12 +410,12 @@ __global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_backward_wide_kern
     s1 /= (float)cols;
     s2 /= (float)cols;
     for (int64_t col = threadIdx.x * V; col < cols; col += LN_WIDE_THREADS * V) {
-        ln_unpack<DT>(ln_load<DT>(row, col, cols), xv);
-        ln_unpack<DT>(ln_load<DT>(grow, col, cols), g);
-        ln_param<PT, V>(weight, col, cols, 1.f, w);
+        ln_unpack<DT>(ln_load<DT, int64_t>(row, col, cols), xv);
+        ln_unpack<DT>(ln_load<DT, int64_t>(grow, col, cols), g);
+        ln_param<PT, V, int64_t>(weight, col, cols, 1.f, w);
 #pragma unroll
         for (int i = 0; i < V; i++) g[i] = st.y * (g[i] * w[i] - s1 - (xv[i] - st.x) * st.y * s2);
-        ln_store<DT>(dx + blockIdx.x * cols * SIZE, col, cols, g);
+        ln_store<DT, int64_t>(dx + blockIdx.x * cols * SIZE, col, cols, g);
     }
 }
 
@@ -324,8 +433,8 @@ __global__ __launch_bounds__(256) void layer_norm_columns_kernel(const uint8_t* 
 #pragma unroll 4
     for (int64_t r = blockIdx.y * chunk; r < end; r++) {
         const float2 st = stats[r];
-        ln_unpack<DT>(ln_load<DT>(x + r * ld * SIZE, col, cols), xv);
-        ln_unpack<DT>(ln_load<DT>(dy + r * ld_dy * SIZE, col, cols), g);
+        ln_unpack<DT>(ln_load<DT, int64_t>(x + r * ld * SIZE, col, cols), xv);
+        ln_unpack<DT>(ln_load<DT, int64_t>(dy + r * ld_dy * SIZE, col, cols), g);
 #pragma unroll
         for (int i = 0; i < V; i++) {
             dw[i] = __builtin_fmaf(g[i], (xv[i] - st.x) * st.y, dw[i]);
@@ -383,31 +492,26 @@ struct LnArgs {
 struct LnShape {
     int t, vpt;
 };
-static LnShape ln_shape(int64_t cols, int dtype) {
+static LnShape ln_shape(int64_t cols, int dtype, bool backward) {
     const int64_t pieces = (cols + (dtype == F8MI_FP32 ? 3 : 7)) / (dtype == F8MI_FP32 ? 4 : 8);
-    if (pieces <= 64) return {64, 1};
-    if (pieces <= 128) return {64, 2};
-    if (pieces <= 256) return {256, 1};
-    if (pieces <= 512) return {256, 2};
-    if (pieces <= 1024) return {512, 2};
-    if (pieces <= 2048) return {1024, 2};
-    return {0, 0};
+    for (int t = 64; t <= 1024; t *= 2)
+        if (pieces <= t) return {t, 1};
+    if (pieces > 2048) return {0, 0};
+    if (backward && dtype != F8MI_FP32) return {1024, 2};
+    return {512, pieces <= 1536 ? 3 : 4};
 }
-static int64_t ln_groups(LnShape s) { return s.t && s.t < 256 ? 256 / s.t : 1; }
-// workgroups that together hold every CU's lanes, no more than there are rows
-static int64_t ln_workgroups(LnShape s, int64_t rows, int lanes_per_cu) {
-    const int64_t wg = std::max(s.t, 256), most = (int64_t)cu_count() * std::max<int64_t>(1, lanes_per_cu / wg);
-    return std::min(most, (rows + ln_groups(s) - 1) / ln_groups(s));
+// Workgroups of `threads` lanes, `per_cu` of them on every CU, no more than the rows need
+static int64_t ln_workgroups(LnShape s, int64_t rows, int threads, int per_cu) {
+    const int64_t groups = threads / s.t;
+    return std::min<int64_t>((int64_t)cu_count() * per_cu, (rows + groups - 1) / groups);
 }
-// Rows of sums that backward writes: two workgroups of 256 lanes a CU, one of more
-constexpr int LN_BACKWARD_LANES = 1024, LN_FORWARD_LANES = 2048;
 static int64_t ln_chunk_rows(int64_t rows, int64_t cols, int dtype) {  // of the column kernel for wide rows: 1024 workgroups or so
     const int64_t strips = (cols + (dtype == F8MI_FP32 ? 1023 : 2047)) / (dtype == F8MI_FP32 ? 1024 : 2048), want = std::max<int64_t>(1, 1024 / strips);
     return std::max<int64_t>(8, (rows + want - 1) / want);
 }
 static int64_t ln_parts(int64_t rows, int64_t cols, int dtype) {
-    const LnShape s = ln_shape(cols, dtype);
-    if (s.t) return ln_workgroups(s, rows, LN_BACKWARD_LANES);
+    const LnShape s = ln_shape(cols, dtype, true);
+    if (s.t) return ln_workgroups(s, rows, ln_backward_threads(s.vpt), 1024 / ln_backward_threads(s.vpt));
     const int64_t chunk = ln_chunk_rows(rows, cols, dtype);
     return (rows + chunk - 1) / chunk;
 }
@@ -415,12 +519,15 @@ static int64_t ln_parts(int64_t rows, int64_t cols, int dtype) {
 template <int DT, int PT, int T, int VPT>
 static int launch_ln(const LnArgs& a, bool backward) {
     const LnShape s{T, VPT};
+    constexpr bool HAS_BACKWARD = VPT == 1 || (VPT > 2) == (DT == F8MI_FP32), HAS_FORWARD = VPT != 2;  // (ln_shape)
+    if constexpr (HAS_BACKWARD)
     if (backward) {
-        hipLaunchKernelGGL((layer_norm_backward_kernel<DT, PT, T, VPT>), dim3((unsigned)a.parts), dim3(ln_threads(T)), 0, a.stream, a.dy, a.ld_dy, a.x, a.ld, a.rows, a.cols, a.weight,
+        hipLaunchKernelGGL((layer_norm_backward_kernel<DT, PT, T, VPT>), dim3((unsigned)a.parts), dim3(ln_backward_threads(VPT)), 0, a.stream, a.dy, a.ld_dy, a.x, a.ld, a.rows, (int)a.cols, a.weight,
                            a.stats, a.out, a.partial);
         return check_hip(hipGetLastError(), "layer norm backward kernel launch");
     }
-    hipLaunchKernelGGL((layer_norm_kernel<DT, PT, T, VPT>), dim3((unsigned)ln_workgroups(s, a.rows, LN_FORWARD_LANES)), dim3(ln_threads(T)), 0, a.stream, a.x, a.ld, a.rows, a.cols,
+    if constexpr (HAS_FORWARD)
+    hipLaunchKernelGGL((layer_norm_kernel<DT, PT, T, VPT>), dim3((unsigned)ln_workgroups(s, a.rows, ln_threads(T), ln_lanes(T, VPT) / ln_threads(T))), dim3(ln_threads(T)), 0, a.stream, a.x, a.ld, a.rows, (int)a.cols,
                        a.weight, a.bias, a.eps, a.out, a.stats);
     return check_hip(hipGetLastError(), "layer norm kernel launch");
 }
@@ -441,13 +548,13 @@ static int launch_ln_wide(const LnArgs& a, bool backward) {
 }
 template <int DT, int PT>
 static int launch_ln_by_size(const LnArgs& a, bool backward) {
-    const LnShape s = ln_shape(a.cols, DT);
-    if (s.t == 64 && s.vpt == 1) return launch_ln<DT, PT, 64, 1>(a, backward);
-    if (s.t == 64) return launch_ln<DT, PT, 64, 2>(a, backward);
-    if (s.t == 256 && s.vpt == 1) return launch_ln<DT, PT, 256, 1>(a, backward);
-    if (s.t == 256) return launch_ln<DT, PT, 256, 2>(a, backward);
-    if (s.t == 512) return launch_ln<DT, PT, 512, 2>(a, backward);
-    if (s.t == 1024) return launch_ln<DT, PT, 1024, 2>(a, backward);
+    const LnShape s = ln_shape(a.cols, DT, backward);
+    if (s.t == 64) return launch_ln<DT, PT, 64, 1>(a, backward);
+    if (s.t == 128) return launch_ln<DT, PT, 128, 1>(a, backward);
+    if (s.t == 256) return launch_ln<DT, PT, 256, 1>(a, backward);
+    if (s.t == 512 && s.vpt == 1) return launch_ln<DT, PT, 512, 1>(a, backward);
+    if (s.t == 512) return s.vpt == 3 ? launch_ln<DT, PT, 512, 3>(a, backward) : launch_ln<DT, PT, 512, 4>(a, backward);
+    if (s.t == 1024) return s.vpt == 1 ? launch_ln<DT, PT, 1024, 1>(a, backward) : launch_ln<DT, PT, 1024, 2>(a, backward);
     return launch_ln_wide<DT, PT>(a, backward);
 }
 static int launch_ln_by_type(int dtype, int p_dtype, const LnArgs& a, bool backward) {
