@@ -100,7 +100,7 @@ def _blockwise_inference_linear(x2: torch.Tensor, data: torch.Tensor, scales: to
     n = data.shape[1]
     if x2.shape[0] == 0:
         return x2.new_empty((0, n))
-    y = _native.ops().blockwise_inference_linear(x2, data, scales, n, bias, torch._C._cuda_getDevice())
+    y = _native.ops().blockwise_inference_linear(x2.detach(), data, scales, n, x2.shape[1], bias)
     if y is None:
         raise _native.Float8NativeError("blockwise_inference_linear: a weight of another shape or device than its scales")
     return y

@@ -259,7 +259,10 @@ def ops():
         lib()
         with _lock:
             if _ops is None:
-                _ops = _load_extension("_f8mi_torch_ops", _OPS_PATH)
+                module = _load_extension("_f8mi_torch_ops", _OPS_PATH)
+                if torch.cuda.is_available():  # (without a GPU nothing is taken, and the callers say so)
+                    _check_device(torch.device("cuda", torch.cuda.current_device()))
+                _ops = module
     return _ops
 
 

@@ -12,6 +12,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -132,24 +133,16 @@ using MaybeTensor = std::optional<at::Tensor>;
 MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
-    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& bias_, bool need_dx, bool need_dw) {
-        const at::Tensor bias = bias_.value_or(at::Tensor());
+    // `saved`: what backward needs (x's transposed copy and scales, the weight's), or null
+    static at::Tensor compute(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, bool need_dx, bool need_dw, variable_list* saved) {
         const c10::DeviceGuard guard(x.device());
+        const at::AutoDispatchBelowADInplaceOrView below;
         const int64_t k = weight.size(1), n = weight.size(0);
         const Rows xr(x, k), wr(weight, k);
         const int64_t m = xr.rows;
         std::vector<int64_t> y_shape(x.sizes().begin(), x.sizes().end());
         y_shape.back() = n;
-        ctx->saved_data["x_shape"] = x.sizes().vec();
-        ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
-        ctx->saved_data["w_type"] = (int64_t)weight.scalar_type();
-        ctx->saved_data["b_type"] = bias.defined() ? (int64_t)bias.scalar_type() : -1;
-        ctx->saved_data["k"] = k;
-        ctx->saved_data["n"] = n;
-        if (m == 0) {
-            ctx->save_for_backward({});
-            return at::empty(y_shape, x.options());
-        }
+        if (m == 0) return at::empty(y_shape, x.options());
         const bool one = one_weight_copy(k, n);
         const Blocks x8 = Blocks::make(x, m, k), x8t = need_dw ? Blocks::make(x, k, m) : Blocks();
         const Blocks w8 = Blocks::make(x, n, k), w8t = need_dx ? Blocks::make(x, k, n, !one) : Blocks();
@@ -157,26 +150,37 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
         check(L.block_cast(jobs, 2, stream_of(x)), "f8mi_block_cast");
         const at::Tensor b = bias.defined() ? bias.to(x.scalar_type()).contiguous() : at::Tensor();
         at::Tensor y = block_gemm(x8, w8.data, w8.scales, false, m, n, k, x.scalar_type(), b);
-        ctx->save_for_backward({x8t.data, x8t.scales, one && need_dx ? w8.data : w8t.data, w8t.scales});
+        if (saved) *saved = {x8t.data, x8t.scales, one && need_dx ? w8.data : w8t.data, w8t.scales};
         return x.dim() == 2 ? y : at::_unsafe_view(y, y_shape);
+    }
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& bias_, bool need_dx, bool need_dw) {
+        const at::Tensor bias = bias_.value_or(at::Tensor());
+        variable_list saved;
+        at::Tensor y = compute(x, weight, bias, need_dx, need_dw, &saved);
+        ctx->saved_data["x_shape"] = x.sizes().vec();
+        ctx->saved_data["types"] = (int64_t)x.scalar_type() | (int64_t)weight.scalar_type() << 8 | (bias.defined() ? (int64_t)bias.scalar_type() + 1 : 0) << 16;
+        ctx->saved_data["n"] = weight.size(0);
+        ctx->save_for_backward(std::move(saved));
+        return y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "blockwise_linear has no second derivative (create_graph=True)");
         const auto saved = ctx->get_saved_variables();
-        const int64_t k = ctx->saved_data["k"].toInt(), n = ctx->saved_data["n"].toInt();
-        const at::ScalarType xt = (at::ScalarType)ctx->saved_data["x_type"].toInt(), wt = (at::ScalarType)ctx->saved_data["w_type"].toInt();
+        const auto x_shape = ctx->saved_data["x_shape"].toIntVector();
+        const int64_t k = x_shape.back(), n = ctx->saved_data["n"].toInt(), types = ctx->saved_data["types"].toInt();
+        const at::ScalarType xt = (at::ScalarType)(types & 255), wt = (at::ScalarType)(types >> 8 & 255), bt = (at::ScalarType)((types >> 16) - 1);
         const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
-        const bool need_db = ctx->saved_data["b_type"].toInt() >= 0 && ctx->needs_input_grad(2);
+        const bool need_db = types >> 16 && ctx->needs_input_grad(2);
         at::Tensor dx, dw, db;
         if (!grads[0].defined()) return {dx, dw, db, at::Tensor(), at::Tensor()};
         const c10::DeviceGuard guard(grads[0].device());
-        const auto x_shape = ctx->saved_data["x_shape"].toIntVector();
+        const at::AutoDispatchBelowADInplaceOrView below;
         const Rows dy(grads[0].scalar_type() == xt ? grads[0] : grads[0].to(xt), n);
         const int64_t m = dy.rows;
         if (m == 0) {
             if (need_dx) dx = at::empty(x_shape, dy.t.options());
             if (need_dw) dw = at::zeros({n, k}, dy.t.options().dtype(wt));
-            if (need_db) db = at::zeros({n}, dy.t.options().dtype((at::ScalarType)ctx->saved_data["b_type"].toInt()));
+            if (need_db) db = at::zeros({n}, dy.t.options().dtype(bt));
             return {dx, dw, db, at::Tensor(), at::Tensor()};
         }
         if (need_dx || need_dw) {
@@ -190,7 +194,7 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
             }
             if (need_dw) dw = block_gemm(g8t, saved[0], saved[1], false, n, k, m, wt);
         }
-        if (need_db) db = column_sum(dy.ld == 0 ? Rows(dy.t.contiguous(), n) : dy, (at::ScalarType)ctx->saved_data["b_type"].toInt());
+        if (need_db) db = column_sum(dy.ld == 0 ? Rows(dy.t.contiguous(), n) : dy, bt);
         return {dx, dw, db, at::Tensor(), at::Tensor()};
     }
 };
@@ -198,14 +202,21 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
 // ---- layer norm
 
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
-    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& weight_, const MaybeTensor& bias_, int64_t cols, double eps, bool need_grad) {
-        const at::Tensor weight = weight_.value_or(at::Tensor()), bias = bias_.value_or(at::Tensor());
+    static at::Tensor compute(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, int64_t cols, double eps, at::Tensor* stats_out) {
         const c10::DeviceGuard guard(x.device());
+        const at::AutoDispatchBelowADInplaceOrView below;
         const Rows r(x, cols);
         const int pt = weight.defined() ? dtype_code(weight.scalar_type()) : bias.defined() ? dtype_code(bias.scalar_type()) : r.dtype();
         const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
-        const at::Tensor y = at::empty(x.sizes(), x.options()), stats = need_grad ? at::empty({r.rows, 2}, x.options().dtype(at::kFloat)) : at::Tensor();
+        const at::Tensor y = at::empty(x.sizes(), x.options()), stats = stats_out ? at::empty({r.rows, 2}, x.options().dtype(at::kFloat)) : at::Tensor();
         if (r.rows) check(L.layer_norm(r.t.data_ptr(), r.rows, cols, r.ld, r.dtype(), ptr(w), ptr(b), pt, (float)eps, y.data_ptr(), (float*)ptr(stats), stream_of(x)), "f8mi_layer_norm");
+        if (stats_out) *stats_out = stats;
+        return y;
+    }
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& weight_, const MaybeTensor& bias_, int64_t cols, double eps) {
+        const at::Tensor weight = weight_.value_or(at::Tensor()), bias = bias_.value_or(at::Tensor());
+        at::Tensor stats;
+        at::Tensor y = compute(x, weight, bias, cols, eps, &stats);
         ctx->save_for_backward({x, weight, stats});
         ctx->saved_data["cols"] = cols;
         ctx->saved_data["has_weight"] = weight.defined();
@@ -220,10 +231,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const bool has_weight = ctx->saved_data["has_weight"].toBool(), has_bias = ctx->saved_data["has_bias"].toBool();
         const bool need_dx = ctx->needs_input_grad(0), need_dw = has_weight && ctx->needs_input_grad(1), need_db = has_bias && ctx->needs_input_grad(has_weight ? 2 : 1);
         at::Tensor dx, dw, db;
-        if (!grads[0].defined() || !(need_dx || need_dw || need_db)) return {dx, dw, db, at::Tensor(), at::Tensor(), at::Tensor()};
+        if (!grads[0].defined() || !(need_dx || need_dw || need_db)) return {dx, dw, db, at::Tensor(), at::Tensor()};
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &stats = saved[2];
         const c10::DeviceGuard guard(x.device());
+        const at::AutoDispatchBelowADInplaceOrView below;
         const int64_t cols = ctx->saved_data["cols"].toInt();
         const at::ScalarType pt = (at::ScalarType)ctx->saved_data["p_type"].toInt();
         const Rows r(x, cols), dy(grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type()), cols);
@@ -235,7 +247,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const at::Tensor ws = bytes ? at::empty({bytes / 4}, x.options().dtype(at::kFloat)) : at::Tensor();
         check(L.layer_norm_backward(ptr(dy.t), dy.ld, ptr(r.t), r.ld, r.rows, cols, r.dtype(), ptr(w), dtype_code(pt), (const float*)ptr(stats), ptr(dx), ptr(dw), ptr(db), ptr(ws),
                                     bytes, stream_of(x)), "f8mi_layer_norm_backward");
-        return {dx, dw, db, at::Tensor(), at::Tensor(), at::Tensor()};
+        return {dx, dw, db, at::Tensor(), at::Tensor()};
     }
 };
 
@@ -274,18 +286,28 @@ bool optional(PyObject* o, int device, at::Tensor& t) {
 }
 bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
-// blockwise_linear(x [..., k], weight [n, k], bias or None, device) -> y, with its history, or None.  Shapes have been checked.
+// The current device as torch has it for this thread, without a call into Python.
+int current_device() {
+    static const bool any = c10::hip::device_count() > 0;
+    return any ? (int)c10::hip::current_device() : -1;
+}
+
+// blockwise_linear(x [..., k], weight [n, k], bias or None) -> y, with its history, or None (also for shapes that do not fit: the caller says what is
+// wrong with them).
 PyObject* blockwise_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    if (!expect(n_args, 4, "blockwise_linear")) return nullptr;
+    if (!expect(n_args, 3, "blockwise_linear")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int device = (int)PyLong_AsLong(a[3]);
+        const int device = current_device();
         const at::Tensor x = plain(a[0], device), w = plain(a[1], device);
         at::Tensor bias;
         if (!x.defined() || !w.defined() || !optional(a[2], device, bias)) Py_RETURN_NONE;
+        if (w.dim() != 2 || w.size(0) == 0 || w.size(1) == 0 || x.dim() == 0 || x.size(-1) != w.size(1) || (bias.defined() && (bias.dim() != 1 || bias.size(0) != w.size(0)))) Py_RETURN_NONE;
         at::Tensor y;
         {
             const WithoutGil no_gil;
-            y = BlockwiseLinear::apply(x, w, maybe(bias), wants_grad(x), wants_grad(w));
+            const bool gx = wants_grad(x), gw = wants_grad(w);
+            if (gx || gw || wants_grad(bias)) y = BlockwiseLinear::apply(x, w, maybe(bias), gx, gw);
+            else y = BlockwiseLinear::compute(x, w, bias, false, false, nullptr);
         }
         return wrap(y);
     });
@@ -298,17 +320,18 @@ bool one_kernel_pays(int64_t m, int64_t n, int64_t kp, int dt) {
     return dt == F8MI_FP32 ? n <= 16384 || m * n <= 65536 : m * n <= 262144;
 }
 
-// blockwise_inference_linear(x [m, k], data, scales of the weight, n, bias or None, device) -> y or None
+// blockwise_inference_linear(x [..., k], data, scales of the weight, n, k, bias or None) -> y or None
 PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!expect(n_args, 6, "blockwise_inference_linear")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int device = (int)PyLong_AsLong(a[5]);
-        const int64_t n = PyLong_AsLongLong(a[3]);
+        const int device = current_device();
+        const int64_t n = PyLong_AsLongLong(a[3]), k = PyLong_AsLongLong(a[4]);
         const at::Tensor x = plain(a[0], device);
         at::Tensor bias;
-        if (!x.defined() || x.dim() < 1 || !THPVariable_Check(a[1]) || !THPVariable_Check(a[2]) || !optional(a[4], device, bias)) Py_RETURN_NONE;
+        if (!x.defined() || x.dim() < 1 || x.size(-1) != k || k <= 0 || wants_grad(x) || !THPVariable_Check(a[1]) || !THPVariable_Check(a[2]) || !optional(a[5], device, bias)) Py_RETURN_NONE;
+        if (bias.defined() && (bias.dim() != 1 || bias.size(0) != n)) Py_RETURN_NONE;
         const at::Tensor data = THPVariable_Unpack(a[1]), scales = THPVariable_Unpack(a[2]);
-        const int64_t k = x.size(-1), kp = (k + 127) / 128 * 128;
+        const int64_t kp = (k + 127) / 128 * 128;
         if (!data.is_cuda() || data.get_device() != device || data.scalar_type() != at::kFloat8_e4m3fn || !data.is_contiguous() || data.numel() != kp * n || !scales.is_cuda() ||
             scales.get_device() != device || scales.scalar_type() != at::kByte || !scales.is_contiguous() || scales.numel() != L.block_scale_bytes(n, k))
             Py_RETURN_NONE;
@@ -316,6 +339,7 @@ PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n
         {
             const WithoutGil no_gil;
             const c10::DeviceGuard guard(x.device());
+            const at::AutoDispatchBelowADInplaceOrView below;
             std::vector<int64_t> y_shape(x.sizes().begin(), x.sizes().end());
             y_shape.back() = n;
             const Rows xr(x, k);
@@ -338,37 +362,52 @@ PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n
     });
 }
 
-// layer_norm(x, weight or None, bias or None, cols, eps, device) -> y, with its history, or None.  Shapes and types have been checked.
+// layer_norm(x, normalized_shape (an int or a tuple), weight or None, bias or None, eps) -> y, with its history, or None (also for shapes and types that
+// do not fit: the caller says what is wrong with them, or converts them).
 PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    if (!expect(n_args, 6, "layer_norm")) return nullptr;
+    if (!expect(n_args, 5, "layer_norm")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int device = (int)PyLong_AsLong(a[5]);
+        const int device = current_device();
         const at::Tensor x = plain(a[0], device);
         at::Tensor w, b;
-        if (!x.defined() || !optional(a[1], device, w) || !optional(a[2], device, b)) Py_RETURN_NONE;
-        const int64_t cols = PyLong_AsLongLong(a[3]);
+        if (!x.defined() || !optional(a[2], device, w) || !optional(a[3], device, b)) Py_RETURN_NONE;
+        std::vector<int64_t> shape;
+        if (PyLong_Check(a[1])) shape.push_back(PyLong_AsLongLong(a[1]));
+        else if (PyTuple_Check(a[1]))  // (torch.Size is one)
+            for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[1]); i++) {
+                if (!PyLong_Check(PyTuple_GET_ITEM(a[1], i))) Py_RETURN_NONE;
+                shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(a[1], i)));
+            }
+        int64_t cols = 1;
+        for (const int64_t s : shape) cols *= s;
+        const int64_t d = (int64_t)shape.size();
+        if (d == 0 || cols <= 0 || x.dim() < d || x.sizes().slice(x.dim() - d) != at::IntArrayRef(shape)) Py_RETURN_NONE;
+        for (const at::Tensor* p : {&w, &b})
+            if (p->defined() && (p->sizes() != at::IntArrayRef(shape) || (p->scalar_type() != x.scalar_type() && p->scalar_type() != at::kFloat))) Py_RETURN_NONE;
+        if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()) Py_RETURN_NONE;
         const double eps = PyFloat_AsDouble(a[4]);
         at::Tensor y;
         {
             const WithoutGil no_gil;
-            y = LayerNorm::apply(x, maybe(w), maybe(b), cols, eps, wants_grad(x) || wants_grad(w) || wants_grad(b));
+            if (wants_grad(x) || wants_grad(w) || wants_grad(b)) y = LayerNorm::apply(x, maybe(w), maybe(b), cols, eps);
+            else y = LayerNorm::compute(x, w, b, cols, eps, nullptr);
         }
         return wrap(y);
     });
 }
 
-// grad_clip(list, what, kind, max_norm, device) -> (norm (fp32, 0-dim), list or None), or None: something in the list is not taken.
+// grad_clip(list, what, kind, max_norm) -> (norm (fp32, 0-dim), list or None), or None: something in the list is not taken.
 // what: "norm" of the tensors; "grads": the gradients of the tensors are clipped in place; None: clipped into new tensors of the tensors' own
 // types; a dtype: of that type.
 PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    if (!expect(n_args, 5, "grad_clip")) return nullptr;
+    if (!expect(n_args, 4, "grad_clip")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int kind = (int)PyLong_AsLong(a[2]), device = (int)PyLong_AsLong(a[4]);
+        const int kind = (int)PyLong_AsLong(a[2]), device = current_device();
         const double max_norm = PyFloat_AsDouble(a[3]);
         const bool of_params = PyUnicode_Check(a[1]) && PyUnicode_CompareWithASCIIString(a[1], "grads") == 0;
         const bool to_new = !PyUnicode_Check(a[1]);
         const bool typed = THPDtype_Check(a[1]);
-        if (!PyList_Check(a[0])) Py_RETURN_NONE;
+        if (!PyList_Check(a[0]) || device < 0) Py_RETURN_NONE;
         std::vector<at::Tensor> xs, outs;
         xs.reserve((size_t)PyList_GET_SIZE(a[0]));
         for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); i++) {

@@ -46,6 +46,10 @@ def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     the gradient of x have x's type, those of weight and bias the parameters' own.  Under autocast x takes the autocast type first."""
     if torch.is_autocast_enabled():
         x = x.to(torch.get_autocast_dtype("cuda"))
+    if not torch.compiler.is_compiling():
+        y = _native.ops().blockwise_linear(x, weight, bias)
+        if y is not None:
+            return y
     if weight.dim() != 2:
         raise ValueError(f"blockwise_linear: weight of shape {tuple(weight.shape)} is no matrix")
     n, k = weight.shape
@@ -53,11 +57,6 @@ def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     _native._require_gpu(weight, "weight")
     if weight.dtype not in _HP_DTYPES:
         raise TypeError(f"blockwise_linear: weight is {weight.dtype}; bfloat16, float16 or float32 is needed")
-    if not torch.compiler.is_compiling():
-        _native._check_device(x.device)
-        y = _native.ops().blockwise_linear(x, weight, bias, torch._C._cuda_getDevice())
-        if y is not None:
-            return y
     return _compiled.blockwise_linear(x, weight, bias)
 
 
@@ -102,14 +101,13 @@ class Float8BlockwiseInferenceLinear(nn.Module):
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         if torch.is_autocast_enabled():
             input = input.to(torch.get_autocast_dtype("cuda"))
+        if not torch.compiler.is_compiling():
+            y = _native.ops().blockwise_inference_linear(input, self.weight_data, self.weight_scales, self.out_features, self.in_features, self.bias)
+            if y is not None:
+                return y
         _checked(input, self.out_features, self.in_features, self.bias, "Float8BlockwiseInferenceLinear")
         if torch.is_grad_enabled() and input.requires_grad:
             raise RuntimeError("Float8BlockwiseInferenceLinear has no backward pass: call it under torch.no_grad() or torch.inference_mode()")
-        if not torch.compiler.is_compiling():
-            _native._check_device(input.device)
-            y = _native.ops().blockwise_inference_linear(input, self.weight_data, self.weight_scales, self.out_features, self.bias, torch._C._cuda_getDevice())
-            if y is not None:
-                return y
         return _compiled.blockwise_inference_linear(input, self.weight_data, self.weight_scales, self.bias)
 
     def dequantized_weight(self) -> torch.Tensor:

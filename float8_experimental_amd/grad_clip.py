@@ -32,13 +32,15 @@ def _readable(tensors: Iterable[torch.Tensor]) -> List[torch.Tensor]:
 
 
 @torch._dynamo.disable
+def _call_outside_graph(tensors, what, kind, max_norm):
+    return _native.ops().grad_clip(tensors, what, kind, max_norm)
+
+
 def _call(tensors: List[torch.Tensor], what, kind: int, max_norm: float):
     """(norm, new tensors or None), or None: something has to be looked at one by one."""
-    if not torch.cuda.is_available():
-        raise _native.Float8NativeError("gradients are clipped on MI355X device tensors only (no CPU fallback)")
-    device = torch._C._cuda_getDevice()
-    _native._check_device(torch.device("cuda", device))
-    return _native.ops().grad_clip(tensors, what, kind, max_norm, device)
+    if torch.compiler.is_compiling():
+        return _call_outside_graph(tensors, what, kind, max_norm)
+    return _native.ops().grad_clip(tensors, what, kind, max_norm)
 
 
 def _must(result):
@@ -69,7 +71,6 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
     return _call(grads, out_dtype, kind, float(max_norm)) or _must(_call(_readable(grads), out_dtype, kind, float(max_norm)))
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_``: scales the gradients of ``parameters`` in place so that their norm as one vector is at most
@@ -82,6 +83,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     if done is None:
         grads = [p.grad for p in parameters if p.grad is not None]
         done = _must(_call(_readable(grads), None, kind, float(max_norm)))
-        for g, clipped in zip(grads, done[1]):
-            g.copy_(clipped)
+        with torch.no_grad():
+            for g, clipped in zip(grads, done[1]):
+                g.copy_(clipped)
     return done[0]

@@ -17,6 +17,10 @@ def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], wei
 
     ``x`` in bfloat16, float16 or float32, the result in its type (also under autocast); weight and bias in that type or in float32, their
     gradients in their own.  Statistics and sums are fp32; the sums of the parameters' gradients have a fixed order."""
+    if not torch.compiler.is_compiling():
+        y = _native.ops().layer_norm(x, normalized_shape, weight, bias, eps)
+        if y is not None:
+            return y
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     _native._require_gpu(x, "x")
     if x.dtype not in _HP_DTYPES:
@@ -34,8 +38,7 @@ def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], wei
             weight is not None and bias is not None and weight.dtype != bias.dtype):
         weight, bias = (None if p is None else p.float() for p in (weight, bias))
     if not torch.compiler.is_compiling():
-        _native._check_device(x.device)
-        y = _native.ops().layer_norm(x, weight, bias, math.prod(shape), float(eps), torch._C._cuda_getDevice())
+        y = _native.ops().layer_norm(x, shape, weight, bias, float(eps))  # with parameters of the types it takes
         if y is not None:
             return y
     return _compiled.layer_norm(x, weight, bias, math.prod(shape), float(eps))
