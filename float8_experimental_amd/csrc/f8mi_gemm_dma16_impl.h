@@ -224,7 +224,6 @@ struct Epilogue16 {
 // ring of 23 groups of 4 KB, group g of step t in the ((8 t + g) mod 23)-th, and the 4 KB saved hold the scales of four steps.
 // Workgroup `lid` of the `npid` that compute this product.
 constexpr int RING_GROUPS = 23, GROUP_BYTES = 4096, BLK_SCALE_BYTES = 4 * 1024;
-__device__ __forceinline__ int ring_at(int i) { return i >= RING_GROUPS ? i - RING_GROUPS : i; }
 static_assert(RING_GROUPS * GROUP_BYTES + BLK_SCALE_BYTES == NSLAB_A * SLAB_BYTES, "the same LDS");
 template <int AF, int BF, int C_DT, bool ODD, bool A_TR, bool B_TR, bool ODD_ROWS, int TJ, bool BIAS_AFTER = false, bool BLK = false>
 __device__ __forceinline__ void gemm_dma16_tile(
@@ -350,7 +349,7 @@ __device__ __forceinline__ void gemm_dma16_tile(
         b_step = 2 * b_unit;
     }
     uint32_t a_dst = 0, b_dst = 0;  // LDS address of the slabs being refilled
-    int a_fill = 0, s_fill = 0;     // BLK: place in the ring of the first group being filled; which of the four steps' scales
+    uint32_t a_fill = lds_u32 + wave * 1024, s_fill = lds_u32 + SCALE_BASE + wave * 256;  // BLK: where this wave's next group and scales go
     const uint8_t* s_ptr = nullptr;
     int64_t s_step = 0;
     if constexpr (BLK) {  // lanes 0 - 31: the scales of the wave's rows of A, the others those of Bt; groups past the edge: the last one again
@@ -359,13 +358,18 @@ __device__ __forceinline__ void gemm_dma16_tile(
         s_step = lane < 32 ? sa_ld : sb_ld;
     }
     auto issue_scales = [&]() __attribute__((always_inline)) {
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(s_ptr), "s"(lds_u32 + SCALE_BASE + s_fill * 1024 + wave * 256) : "memory");
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(s_ptr), "s"(s_fill) : "memory");
         s_ptr += s_step;
+        s_fill = lds_u32 + SCALE_BASE + wave * 256 + ((s_fill - (lds_u32 + SCALE_BASE) + 1024) & 4095 & ~1023);
     };
     // DMA d = 0..7 of this wave's share of a slab
     auto issue_a = [&](int d) __attribute__((always_inline)) {
         if constexpr (A_TR) dma16b(a_ptr, a_voff[d], a_dst + (wave * 8 + d) * 1024);
-        else if constexpr (BLK) dma16b(a_ptr, a_voff[d], lds_u32 + ring_at(a_fill + d) * GROUP_BYTES + wave * 1024);
+        else if constexpr (BLK) {
+            dma16b(a_ptr, a_voff[d], a_fill);
+            a_fill += GROUP_BYTES;
+            if (a_fill >= lds_u32 + RING_GROUPS * GROUP_BYTES) a_fill -= RING_GROUPS * GROUP_BYTES;
+        }
         else dma16b(d < 4 ? a_ptr : a_ptr + a_unit, a_voff[d & 3], a_dst + wave * 4096 + (d >> 2) * HALF_BYTES + (d & 3) * 1024);
         if (d == 7) a_ptr += a_step;
     };
@@ -400,12 +404,20 @@ __device__ __forceinline__ void gemm_dma16_tile(
     const int b_frag_base = (wn * (16 * TJ)) * 64 + (fq >> 1) * (Cfg::B_HALF - HALF_BYTES);
     const int g_off0 = (fq >> 1) * 2048 + wm * 1024 + frow * 64 + ((((fq & 1) * 2 + 0) ^ fsw) << 4);  // BLK: inside a group
     const int g_off1 = (fq >> 1) * 2048 + wm * 1024 + frow * 64 + ((((fq & 1) * 2 + 1) ^ fsw) << 4);
-    auto frag_a = [&](const uint8_t* slab, int ti, int at = 0) __attribute__((always_inline)) {  // BLK: group ti from the place `at`
+    // BLK: where the next fragment of A lies.  Moved on between two MFMAs that have nothing else between them: with the additions beside the reads
+    // and a DMA, steps took 5 % longer.
+    const uint8_t *g0 = smem + g_off0, *g1 = smem + g_off1;
+    int g_at = 0;  // place in the ring
+    auto next_group = [&]() __attribute__((always_inline)) {
+        g_at = g_at + 1 == RING_GROUPS ? 0 : g_at + 1;
+        g0 = smem + g_off0 + g_at * GROUP_BYTES;
+        g1 = smem + g_off1 + g_at * GROUP_BYTES;
+    };
+    auto frag_a = [&](const uint8_t* slab, int ti) __attribute__((always_inline)) {  // BLK: the next one
         if constexpr (A_TR) {
             return read_frag_tr(slab + a_tr_off[ti]);
         } else if constexpr (BLK) {
-            const uint8_t* p = smem + ring_at(at + ti) * GROUP_BYTES;
-            return read_frag(p + g_off0, p + g_off1);
+            return read_frag(g0, g1);
         } else {
             const uint8_t* p = slab + a_frag_base + ti * 16 * 64;
             return read_frag(p + f_off0, p + f_off1);
@@ -425,23 +437,20 @@ __device__ __forceinline__ void gemm_dma16_tile(
     v8i fb[2][TJ];  // [step parity][n tile]
     v8i fa[2];     // rolling: group ti multiplies fa[ti & 1] while fa[(ti + 1) & 1] is being fetched
     uint2 fsa[2], fsb[2];  // [step parity]: byte ti / tj
-    auto frag_scales = [&](int step, bool of_b) __attribute__((always_inline)) {
-        return *(const uint2*)(smem + SCALE_BASE + (step & 3) * 1024 + wave * 256 + (of_b ? 128 : 0) + frow * 8);
-    };
+    const uint8_t* const s_lane = smem + SCALE_BASE + wave * 256 + frow * 8;
+    auto frag_scales = [&](int step, bool of_b) __attribute__((always_inline)) { return *(const uint2*)(s_lane + (step & 3) * 1024 + (of_b ? 128 : 0)); };
 
     // ---- prologue: steps 0 and 1 (A into slabs 0, 1; Bt into slabs 3, 4), wait for step 0,
     // first fragments; a second barrier before step 0 refills the Bt slab just read.
 #pragma unroll
     for (int s = 0; s < 2; s++) {
         a_dst = lds_u32 + s * SLAB_BYTES;
-        a_fill = s * 8;
-        s_fill = s;
         b_dst = lds_u32 + B_BASE + s * Cfg::B_SLAB;
+        if constexpr (BLK) issue_scales();
 #pragma unroll
         for (int d = 0; d < 8; d++) issue_a(d);
 #pragma unroll
         for (int d = 0; d < TJ; d++) issue_b(d);
-        if constexpr (BLK) issue_scales();
     }
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(8 + TJ + (BLK ? 1 : 0)) : "memory");
     lds_barrier();
@@ -449,6 +458,7 @@ __device__ __forceinline__ void gemm_dma16_tile(
     for (int x = 0; x < TJ; x++) fb[0][x] = frag_b(smem + B_BASE, x);
     fa[0] = frag_a(smem, 0);
     if constexpr (BLK) {
+        next_group();
         fsa[0] = frag_scales(0, false);
         fsb[0] = frag_scales(0, true);
     }
@@ -458,7 +468,7 @@ __device__ __forceinline__ void gemm_dma16_tile(
     // step's start with step t+2); 1: last but one (nothing left to fetch); 2: last step; 3: step 0 (as 0,
     // and the accumulators start from zero).
     int a_slab = 0;  // slab of A of this step; step t+2 goes to the slab before it in the rotation
-    int a_at = 0, s_at = 0;  // BLK: place in the ring of this step's first group; the step
+    int s_at = 0;    // BLK: the step
     Epilogue16<C_DT, ODD_ROWS, TJ, BIAS_AFTER> epi(m0, n0, M, N, inv, C, ldc, bias, bias_fp32, c_vec_ok);
     auto step = [&](auto parity, auto mode) __attribute__((always_inline)) {
         constexpr int P = decltype(parity)::value;
@@ -469,11 +479,8 @@ __device__ __forceinline__ void gemm_dma16_tile(
         const uint8_t* a_cur = smem + a_slab * SLAB_BYTES;
         const uint8_t* a_nxt = smem + a_next * SLAB_BYTES;
         const uint8_t* b_nxt = smem + B_BASE + (P ^ 1) * Cfg::B_SLAB;
-        const int a_at_next = ring_at(a_at + 8);
         if (MODE == 0) {
             a_dst = lds_u32 + a_free * SLAB_BYTES;
-            a_fill = ring_at(a_at_next + 8);
-            s_fill = (s_at + 2) & 3;
             b_dst = lds_u32 + B_BASE + P * Cfg::B_SLAB;  // Bt of this step: already in registers
         }
         // Everything that is not an MFMA sits in a fixed slot between two MFMAs (each keeps the matrix
@@ -484,18 +491,20 @@ __device__ __forceinline__ void gemm_dma16_tile(
 #pragma unroll
         for (int ti = 0; ti < 8; ti++) {
             if (ti == 6 && MODE < 2) {
-                // this wave's DMAs of step t+1 have landed (the 12 of step t+2 issued so far may be in flight) ...
-                if (MODE == 0) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+                // this wave's DMAs of step t+1 have landed (the 12 of step t+2 issued so far, with scales 13, may be in flight) ...
+                if (MODE == 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BLK ? 13 : 12) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 asm volatile("s_barrier" ::: "memory");  // ... and so have everybody's; no LDS hazard here, so no wait on LDS reads
             }
 #pragma unroll
             for (int tj = 0; tj < TJ; tj++) {
-                if (tj == 0 && ti < 7) fa[(ti + 1) & 1] = frag_a(a_cur, ti + 1, a_at);
-                if (tj == 0 && ti == 7 && MODE < 2) fa[0] = frag_a(a_nxt, 0, a_at_next);
+                if (tj == 0 && ti < 7) fa[(ti + 1) & 1] = frag_a(a_cur, ti + 1);
+                if (tj == 0 && ti == 7 && MODE < 2) fa[0] = frag_a(a_nxt, 0);
                 if constexpr (BLK) {
-                    if (MODE < 2 && ti == 6 && tj == 2) fsa[P ^ 1] = frag_scales(s_at + 1, false);
-                    if (MODE < 2 && ti == 6 && tj == 6) fsb[P ^ 1] = frag_scales(s_at + 1, true);
+                    if (MODE < 2 && ti == 7 && tj == 6) {
+                        fsa[P ^ 1] = frag_scales(s_at + 1, false);
+                        fsb[P ^ 1] = frag_scales(s_at + 1, true);
+                    }
                 }
                 if constexpr (TJ == 8) {
                     if (MODE < 2 && ti >= 6 && (tj & 1) == 1) fb[P ^ 1][(ti - 6) * 4 + (tj >> 1)] = frag_b(b_nxt, (ti - 6) * 4 + (tj >> 1));
@@ -519,7 +528,7 @@ __device__ __forceinline__ void gemm_dma16_tile(
                         F8MI_SCHED_FENCE();
                     }
                 }
-                if (MODE == 0 && (tj & 3) == 0) {
+                if (MODE == 0 && (BLK ? tj == 2 || tj == 4 : (tj & 3) == 0)) {
                     // 16 DMAs over the 64 MFMAs, one after every fourth: A slab first, then Bt.  (Packed into
                     // the first half of the step they cost 3 % more time: the four waves share one load unit.)
                     const int d = ti * 2 + (tj >> 2);
@@ -528,8 +537,12 @@ __device__ __forceinline__ void gemm_dma16_tile(
                     F8MI_SCHED_FENCE();
                 }
                 if constexpr (BLK) {
-                    if (MODE == 0 && ti == 7 && tj == 6) {
+                    if (MODE == 0 && ti == 0 && tj == 3) {  // early: at the end of the step they were what the next one waited for
                         issue_scales();
+                        F8MI_SCHED_FENCE();
+                    }
+                    if (tj == 6 && (ti < 6 || MODE < 2)) {
+                        next_group();
                         F8MI_SCHED_FENCE();
                     }
                 }
@@ -537,7 +550,6 @@ __device__ __forceinline__ void gemm_dma16_tile(
         }
         if (MODE < 2) lds_barrier();  // step boundary: everybody is done with A of step t and has Bt of step t+1 in registers
         a_slab = a_next;
-        a_at = a_at_next;
         s_at++;
     };
 

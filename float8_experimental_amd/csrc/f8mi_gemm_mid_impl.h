@@ -168,9 +168,10 @@ __device__ __forceinline__ void gemm_mid_tile(
         s_step = lane < 32 ? sa_ld : sb_ld;
         s_ptr = (lane < 32 ? sa_blk + m0 : sb_blk + group) + (lane & 31) * 4 + k0 / 128 * s_step;
     }
-    // DMA d = 0..NDMA-1 of this wave's share of a step (4 of A, then Bt, then the scales); the pointers move on after the last
-    auto issue1 = [&](uint32_t base, int d) __attribute__((always_inline)) {
-        if (BLK && d == NDMA - 1) {
+    // DMA n = 0..NDMA-1 of this wave's share of a step (block scales first, 4 of A, then Bt); the pointers move on after the last
+    auto issue1 = [&](uint32_t base, int n) __attribute__((always_inline)) {
+        const int d = BLK ? n - 1 : n;
+        if (BLK && n == 0) {
             dma_scales(s_ptr, base + Cfg::SCALES + wave * 256);
             s_ptr += s_step;
         } else if (d < 4) {
@@ -181,7 +182,7 @@ __device__ __forceinline__ void gemm_mid_tile(
             if constexpr (B_TR) dma_mid(b_ptr, b_voff[d - 4], base + 2 * MID_A_UNIT + (wave * 2 * Cfg::BI + d - 4) * 1024);
             else dma_mid(b_ptr + h * b_unit, b_voff[i], base + 2 * MID_A_UNIT + h * Cfg::B_UNIT + (wave * Cfg::BI + i) * 1024);
         }
-        if (d == NDMA - 1) {
+        if (n == NDMA - 1) {
             a_ptr += A_TR ? 128 * lda : 2 * a_unit;
             b_ptr += B_TR ? 128 * ldb : 2 * b_unit;
         }
