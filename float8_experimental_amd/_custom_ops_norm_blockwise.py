@@ -5,7 +5,6 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native
-from ._custom_ops import column_sum
 
 _e4m3 = torch.float8_e4m3fn
 _KB, _BLOCK = _native.KB, _native.BLOCK
@@ -50,27 +49,29 @@ def _(x2, weight, bias, need_dx, need_dw):
 
 @torch.library.custom_op("f8mi::blockwise_linear_bwd", mutates_args=())
 def blockwise_linear_bwd(dy2: torch.Tensor, xt: torch.Tensor, xt_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, k: int, w_dtype: torch.dtype,
-                         need_dx: bool, need_dw: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(dx, dw); an unneeded gradient is empty."""
+                         b_dtype: Optional[torch.dtype], need_dx: bool, need_dw: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dw, dbias); an unneeded gradient (``b_dtype`` None: of the bias) is empty."""
     m, n = dy2.shape
     empty = lambda dt: torch.empty(0, dtype=dt, device=dy2.device)
     if m == 0:
-        return (dy2.new_empty((0, k)) if need_dx else empty(dy2.dtype), dy2.new_zeros((n, k), dtype=w_dtype) if need_dw else empty(w_dtype))
+        return (dy2.new_empty((0, k)) if need_dx else empty(dy2.dtype), dy2.new_zeros((n, k), dtype=w_dtype) if need_dw else empty(w_dtype),
+                dy2.new_zeros(n, dtype=b_dtype) if b_dtype is not None else empty(dy2.dtype))
     with _native.transient_workspaces():
-        ((g8, g8t),) = _native.block_cast([(dy2, False, need_dx, need_dw)])
+        ((g8, g8t, *db),) = _native.block_cast([(dy2, False, need_dx, need_dw, *([b_dtype] if b_dtype is not None else []))])
         dx, dw = empty(dy2.dtype), empty(w_dtype)
         if need_dx:
             one = _one_weight_copy(k, n)
             dx = _native.block_gemm(g8, _native.Blocks(None if one else w, w_scales, k, n), dy2.dtype, transposed=_native.Blocks(w, None, n, k) if one else None)
         if need_dw:
             dw = _native.block_gemm(g8t, _native.Blocks(xt, xt_scales, k, m), w_dtype)
-    return dx, dw
+    return dx, dw, db[0] if db else empty(dy2.dtype)
 
 
 @blockwise_linear_bwd.register_fake
-def _(dy2, xt, xt_scales, w, w_scales, k, w_dtype, need_dx, need_dw):
+def _(dy2, xt, xt_scales, w, w_scales, k, w_dtype, b_dtype, need_dx, need_dw):
     m, n = dy2.shape
-    return (torch.empty((m, k) if need_dx else (0,), dtype=dy2.dtype, device=dy2.device), torch.empty((n, k) if need_dw else (0,), dtype=w_dtype, device=dy2.device))
+    return (torch.empty((m, k) if need_dx else (0,), dtype=dy2.dtype, device=dy2.device), torch.empty((n, k) if need_dw else (0,), dtype=w_dtype, device=dy2.device),
+            torch.empty(0 if b_dtype is None else n, dtype=b_dtype or dy2.dtype, device=dy2.device))
 
 
 class _BlockwiseLinearFn(torch.autograd.Function):
@@ -84,10 +85,8 @@ class _BlockwiseLinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gy):
         need_dx, need_dw, need_db = ctx.needs_input_grad
-        dx = dw = None
-        if need_dx or need_dw:
-            dx, dw = blockwise_linear_bwd(gy, *ctx.saved_tensors, ctx.k, ctx.w_dtype, need_dx, need_dw)
-        return dx if need_dx else None, dw if need_dw else None, column_sum(gy, ctx.b_dtype) if need_db else None
+        dx, dw, db = blockwise_linear_bwd(gy, *ctx.saved_tensors, ctx.k, ctx.w_dtype, ctx.b_dtype if need_db else None, need_dx, need_dw)
+        return dx if need_dx else None, dw if need_dw else None, db if need_db else None
 
 
 def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:

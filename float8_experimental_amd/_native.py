@@ -62,6 +62,7 @@ EXPORTS = (
     "f8mi_gemm_kb_bias",
     "f8mi_column_sum",
     "f8mi_column_sum_workspace_bytes",
+    "f8mi_column_sum_finish",
     "f8mi_gemm_ex",
     "f8mi_sync",
     "f8mi_sync_host",
@@ -95,7 +96,8 @@ class BlockCastJob(C.Structure):
     """f8mi_block_cast_job of include/f8mi.h."""
 
     _fields_ = [("x", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64), ("dtype", C.c_int), ("square", C.c_int),
-                ("out", C.c_void_p), ("out_scales", C.c_void_p), ("out_t", C.c_void_p), ("out_t_scales", C.c_void_p)]
+                ("out", C.c_void_p), ("out_scales", C.c_void_p), ("out_t", C.c_void_p), ("out_t_scales", C.c_void_p),
+                ("col_sums", C.c_void_p)]
 
 
 class Float8NativeError(RuntimeError):
@@ -164,6 +166,8 @@ def lib() -> C.CDLL:
         L.f8mi_gemm_kb_bias.argtypes = [vp, vp, i64, i64, i64, fp, fp, vp, i32, i64, vp, i32, i64, vp]
         L.f8mi_column_sum.restype = i32
         L.f8mi_column_sum.argtypes = [vp, i64, i64, i64, i32, vp, i32, vp, i64, vp]
+        L.f8mi_column_sum_finish.restype = i32
+        L.f8mi_column_sum_finish.argtypes = [vp, i64, i64, i32, vp, i32, vp]
         L.f8mi_column_sum_workspace_bytes.restype = i64
         L.f8mi_column_sum_workspace_bytes.argtypes = [i64, i64, i32]
         L.f8mi_gemm_ex.restype = i32
@@ -949,11 +953,11 @@ def _blocks_alloc(rows: int, k: int, device, data: bool = True) -> Blocks:
 def block_cast(jobs):
     """[(copy contracting over the columns or None, copy contracting over the rows or None)] of one or two 2-D tensors, in one pass over
     each.  A job is ``(x, square, want, want_t)``: ``square`` gives every 128 x 128 values one scale, otherwise blocks are 128
-    values along the contraction of each copy; ``want_t`` may be ``"scales"`` for a square tensor that another product reads transposed.
-    See f8mi_block_cast."""
+    values along the contraction of each copy; ``want_t`` may be ``"scales"`` for a square tensor that another product reads transposed.  A fifth entry of
+    a job, a dtype, asks for the columns summed up in that type (see ``column_sum``) as the third of its results.  See f8mi_block_cast."""
     structs, out = (BlockCastJob * len(jobs))(), []
     held = []
-    for s, (x, square, want, want_t) in zip(structs, jobs):
+    for s, (x, square, want, want_t, *sum_dtype) in zip(structs, jobs):
         _require_gpu(x, "x")
         assert x.dim() == 2 and x.dtype in _DT and x.numel() > 0
         xs, rows, cols, ld = _as_2d(x)
@@ -965,9 +969,18 @@ def block_cast(jobs):
             s.out, s.out_scales = a.data.data_ptr(), a.scales.data_ptr()
         if b is not None:
             s.out_t, s.out_t_scales = b.data.data_ptr() if b.data is not None else None, b.scales.data_ptr()
-        out.append((a, b))
+        sums = torch.empty((-(-rows // BLOCK), cols), dtype=torch.float32, device=x.device) if sum_dtype else None
+        s.col_sums = sums.data_ptr() if sum_dtype else None
+        out.append((a, b, sums) if sum_dtype else (a, b))
     _check_device(jobs[0][0].device)
-    _check(lib().f8mi_block_cast(structs, len(jobs), _stream(jobs[0][0])), "f8mi_block_cast")
+    stream = _stream(jobs[0][0])
+    _check(lib().f8mi_block_cast(structs, len(jobs), stream), "f8mi_block_cast")
+    for i, (x, _, _, _, *sum_dtype) in enumerate(jobs):
+        if sum_dtype:
+            a, b, sums = out[i]
+            total = torch.empty(sums.shape[1], dtype=sum_dtype[0], device=x.device)
+            _check(lib().f8mi_column_sum_finish(sums.data_ptr(), *sums.shape, _DT[x.dtype], total.data_ptr(), _DT[total.dtype], stream), "f8mi_column_sum_finish")
+            out[i] = (a, b, total)
     return out
 
 

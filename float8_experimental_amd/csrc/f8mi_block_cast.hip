@@ -18,6 +18,7 @@ struct BlockCastItem {
     const uint8_t* x;
     int64_t rows, cols, ld;  // ld in elements
     uint8_t *out, *out_scales, *out_t, *out_t_scales;
+    float* sums;  // [rows / 128][cols]: the columns of each tile added up (the first half of a bias's gradient), or null
     int square;  // one scale for each 128 x 128
     int tiles_c;
 };
@@ -86,6 +87,14 @@ __device__ __forceinline__ void transpose4x4(const uint32_t (&r)[4], uint32_t (&
     c[3] = __builtin_amdgcn_perm(e, b, 0x07060302u);
 }
 
+// v and that of the lanes 16 and 32 further on and back: over the four rows of 16 lanes, in all of them
+__device__ __forceinline__ float sum_of_rows(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+
 template <int DT>
 __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastItem first, const BlockCastItem second, int tiles_first) {
     constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2;
@@ -93,6 +102,7 @@ __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastI
     __shared__ __align__(16) uint8_t turned[BLOCK * BLOCK];
     __shared__ __align__(16) uint32_t col_max[4][16 * CW];
     __shared__ __align__(16) uint8_t row_bytes[BLOCK], col_bytes[BLOCK];
+    __shared__ __align__(16) float col_sum[4][BLOCK];
     const bool in_first = (int)blockIdx.x < tiles_first;
     const BlockCastItem it = in_first ? first : second;
     const int tile = (int)blockIdx.x - (in_first ? 0 : tiles_first);
@@ -140,6 +150,20 @@ __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastI
         else return widen_bits<DT>((rmax[i >> 1] >> (16 * (i & 1))) & 0xffffu);
     };
 
+    if (it.sums) {  // the same for the whole workgroup, as all of `it`
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            float s[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                s[c] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[c] += value(v[i], j + c);
+                s[c] = sum_of_rows(s[c]);
+            }
+            if (lane < 16) *(float4*)&col_sum[wave][8 * tx + j] = make_float4(s[0], s[1], s[2], s[3]);
+        }
+    }
     const bool by_cols = it.out_t_scales || it.square;  // the same for the whole workgroup
     uint32_t cmax[CW];
     if (by_cols) {
@@ -209,6 +233,7 @@ __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastI
             }
     }
     __syncthreads();
+    if (it.sums && t < BLOCK && c0 + t < it.cols) it.sums[tr * it.cols + c0 + t] = (col_sum[0][t] + col_sum[1][t]) + (col_sum[2][t] + col_sum[3][t]);
     if (it.out_t) {
         const int64_t rows_kept = it.cols;  // of the transposed copy
 #pragma unroll
@@ -244,14 +269,15 @@ extern "C" int f8mi_block_cast(const f8mi_block_cast_job* jobs, int count, void*
         const f8mi_block_cast_job& j = jobs[i];
         if (j.rows <= 0 || j.cols <= 0 || (j.ld < j.cols && j.ld != 0)) { set_error("f8mi_block_cast: bad shape rows=%lld cols=%lld ld=%lld", (long long)j.rows, (long long)j.cols, (long long)j.ld); return F8MI_ERR_INVALID_ARG; }
         if (j.dtype < 0 || j.dtype > 2) { set_error("f8mi_block_cast: unknown dtype code %d", j.dtype); return F8MI_ERR_INVALID_ARG; }
-        if (!j.x || (!j.out && !j.out_t) || !j.out != !j.out_scales || (j.out_t && !j.out_t_scales) || (j.out_t_scales && !j.out_t && !(j.square && j.out))) { set_error("f8mi_block_cast: null pointer, or a copy without its scales"); return F8MI_ERR_INVALID_ARG; }
+        if (!j.x || (!j.out && !j.out_t && !j.col_sums) || !j.out != !j.out_scales || (j.out_t && !j.out_t_scales) || (j.out_t_scales && !j.out_t && !(j.square && j.out))) { set_error("f8mi_block_cast: null pointer, or a copy without its scales"); return F8MI_ERR_INVALID_ARG; }
         for (const void* p : {(const void*)j.out, (const void*)j.out_scales, (const void*)j.out_t, (const void*)j.out_t_scales})
             if ((uintptr_t)p % 16 != 0) { set_error("f8mi_block_cast: copies and scales are 16-byte aligned"); return F8MI_ERR_INVALID_ARG; }
+        if ((uintptr_t)j.col_sums % 4 != 0) { set_error("f8mi_block_cast: column sums not aligned to a float"); return F8MI_ERR_INVALID_ARG; }
         if ((uintptr_t)j.x % (j.dtype == F8MI_FP32 ? 4 : 2) != 0) { set_error("f8mi_block_cast: input not aligned to its elements"); return F8MI_ERR_INVALID_ARG; }
         const int64_t tiles_c = (j.cols + BLOCK - 1) / BLOCK;
         tiles[i] = tiles_c * ((j.rows + BLOCK - 1) / BLOCK);
         if (tiles_c > 0x3fffffff || tiles[i] > 0x3fffffff) { set_error("f8mi_block_cast: more than 2^30 tiles of 128 x 128"); return F8MI_ERR_UNSUPPORTED; }
-        items[i] = {(const uint8_t*)j.x, j.rows, j.cols, j.ld, (uint8_t*)j.out, (uint8_t*)j.out_scales, (uint8_t*)j.out_t, (uint8_t*)j.out_t_scales, j.square != 0, (int)tiles_c};
+        items[i] = {(const uint8_t*)j.x, j.rows, j.cols, j.ld, (uint8_t*)j.out, (uint8_t*)j.out_scales, (uint8_t*)j.out_t, (uint8_t*)j.out_t_scales, j.col_sums, j.square != 0, (int)tiles_c};
     }
     hipStream_t s = (hipStream_t)stream;
     if (count == 2 && jobs[0].dtype != jobs[1].dtype) {

@@ -149,3 +149,15 @@ extern "C" int f8mi_column_sum(const void* x, int64_t rows, int64_t cols, int64_
     if (dtype == F8MI_FP16) return launch_colsum<F8MI_FP16>(x, rows, cols, ld, out, out_dtype, (float*)workspace, (hipStream_t)stream);
     return launch_colsum<F8MI_FP32>(x, rows, cols, ld, out, out_dtype, (float*)workspace, (hipStream_t)stream);
 }
+
+extern "C" int f8mi_column_sum_finish(const float* col_sums, int64_t parts, int64_t cols, int dtype, void* out, int out_dtype, void* stream_) {
+    if (parts <= 0 || cols <= 0 || cols > 0x7fffffff) { set_error("f8mi_column_sum_finish: bad shape parts=%lld cols=%lld", (long long)parts, (long long)cols); return F8MI_ERR_INVALID_ARG; }
+    if (dtype < 0 || dtype > 2 || out_dtype < 0 || out_dtype > 2) { set_error("f8mi_column_sum_finish: unknown dtype code"); return F8MI_ERR_INVALID_ARG; }
+    if (!col_sums || !out) { set_error("f8mi_column_sum_finish: null pointer"); return F8MI_ERR_INVALID_ARG; }
+    const dim3 grid((unsigned)((cols + 63) / 64)), threads(64 * FINISH_WAVES);
+    hipStream_t stream = (hipStream_t)stream_;
+    if (dtype == F8MI_BF16) hipLaunchKernelGGL(colsum_finish_kernel<F8MI_BF16>, grid, threads, 0, stream, col_sums, parts, cols, out, out_dtype);
+    else if (dtype == F8MI_FP16) hipLaunchKernelGGL(colsum_finish_kernel<F8MI_FP16>, grid, threads, 0, stream, col_sums, parts, cols, out, out_dtype);
+    else hipLaunchKernelGGL(colsum_finish_kernel<F8MI_FP32>, grid, threads, 0, stream, col_sums, parts, cols, out, out_dtype);
+    return check_hip(hipGetLastError(), "column sum kernel launch");
+}

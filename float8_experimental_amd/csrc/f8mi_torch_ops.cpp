@@ -34,8 +34,7 @@ struct Lib {
     decltype(&f8mi_block_gemm) block_gemm;
     decltype(&f8mi_block_gemm_workspace_bytes) block_gemm_workspace_bytes;
     decltype(&f8mi_block_linear_few_rows) block_linear_few_rows;
-    decltype(&f8mi_column_sum) column_sum;
-    decltype(&f8mi_column_sum_workspace_bytes) column_sum_workspace_bytes;
+    decltype(&f8mi_column_sum_finish) column_sum_finish;
     decltype(&f8mi_layer_norm) layer_norm;
     decltype(&f8mi_layer_norm_backward) layer_norm_backward;
     decltype(&f8mi_layer_norm_workspace_bytes) layer_norm_workspace_bytes;
@@ -104,8 +103,8 @@ struct Blocks {  // a copy and its scales
         return b;
     }
 };
-f8mi_block_cast_job job_of(const Rows& x, bool square, const Blocks& a, const Blocks& t) {
-    return {x.t.data_ptr(), x.rows, x.cols, x.ld, x.dtype(), square, ptr(a.data), a.data.defined() ? ptr(a.scales) : nullptr, ptr(t.data), ptr(t.scales)};
+f8mi_block_cast_job job_of(const Rows& x, bool square, const Blocks& a, const Blocks& t, const at::Tensor& sums = {}) {
+    return {x.t.data_ptr(), x.rows, x.cols, x.ld, x.dtype(), square, ptr(a.data), a.data.defined() ? ptr(a.scales) : nullptr, ptr(t.data), ptr(t.scales), (float*)ptr(sums)};
 }
 // [m, n] = a [m, k] times b [n, k]; `of`: the copy that b's product reads, the other one of the tensor with transposed
 at::Tensor block_gemm(const Blocks& a, const at::Tensor& b_data, const at::Tensor& b_scales, bool transposed, int64_t m, int64_t n, int64_t k, at::ScalarType type,
@@ -118,13 +117,6 @@ at::Tensor block_gemm(const Blocks& a, const at::Tensor& b_data, const at::Tenso
                        ptr(ws), bytes, stream_of(c)), "f8mi_block_gemm");
     return c;
 }
-at::Tensor column_sum(const Rows& dy, at::ScalarType type) {
-    const int64_t bytes = L.column_sum_workspace_bytes(dy.rows, dy.cols, dy.dtype());
-    const at::Tensor out = at::empty({dy.cols}, dy.t.options().dtype(type)), ws = bytes ? at::empty({bytes / 4}, dy.t.options().dtype(at::kFloat)) : at::Tensor();
-    check(L.column_sum(dy.t.data_ptr(), dy.rows, dy.cols, dy.ld, dy.dtype(), out.data_ptr(), dtype_code(type), ptr(ws), bytes, stream_of(out)), "f8mi_column_sum");
-    return out;
-}
-
 // The weight needs one copy if the backward product can read it transposed
 bool one_weight_copy(int64_t k, int64_t n) { return k % 128 == 0 && n % 128 == 0; }
 
@@ -183,18 +175,21 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
             if (need_db) db = at::zeros({n}, dy.t.options().dtype(bt));
             return {dx, dw, db, at::Tensor(), at::Tensor()};
         }
-        if (need_dx || need_dw) {
-            TORCH_CHECK((!need_dx || saved[3].defined()) && (!need_dw || saved[0].defined()), "blockwise_linear: a gradient is asked for that the forward pass was not told of");
-            const Blocks g8 = need_dx ? Blocks::make(dy.t, m, n) : Blocks(), g8t = need_dw ? Blocks::make(dy.t, n, m) : Blocks();
-            const f8mi_block_cast_job job = job_of(dy, false, g8, g8t);
-            check(L.block_cast(&job, 1, stream_of(dy.t)), "f8mi_block_cast");
-            if (need_dx) {
-                dx = block_gemm(g8, saved[2], saved[3], one_weight_copy(k, n), m, k, n, xt);
-                if (x_shape.size() != 2) dx = dx.view(x_shape);
-            }
-            if (need_dw) dw = block_gemm(g8t, saved[0], saved[1], false, n, k, m, wt);
+        if (!(need_dx || need_dw || need_db)) return {dx, dw, db, at::Tensor(), at::Tensor()};
+        TORCH_CHECK((!need_dx || saved[3].defined()) && (!need_dw || saved[0].defined()), "blockwise_linear: a gradient is asked for that the forward pass was not told of");
+        const Blocks g8 = need_dx ? Blocks::make(dy.t, m, n) : Blocks(), g8t = need_dw ? Blocks::make(dy.t, n, m) : Blocks();
+        const at::Tensor sums = need_db ? at::empty({(m + 127) / 128, n}, dy.t.options().dtype(at::kFloat)) : at::Tensor();
+        const f8mi_block_cast_job job = job_of(dy, false, g8, g8t, sums);
+        check(L.block_cast(&job, 1, stream_of(dy.t)), "f8mi_block_cast");
+        if (need_dx) {
+            dx = block_gemm(g8, saved[2], saved[3], one_weight_copy(k, n), m, k, n, xt);
+            if (x_shape.size() != 2) dx = dx.view(x_shape);
         }
-        if (need_db) db = column_sum(dy.ld == 0 ? Rows(dy.t.contiguous(), n) : dy, bt);
+        if (need_dw) dw = block_gemm(g8t, saved[0], saved[1], false, n, k, m, wt);
+        if (need_db) {
+            db = at::empty({n}, dy.t.options().dtype(bt));
+            check(L.column_sum_finish((const float*)sums.data_ptr(), sums.size(0), n, dy.dtype(), db.data_ptr(), dtype_code(bt), stream_of(dy.t)), "f8mi_column_sum_finish");
+        }
         return {dx, dw, db, at::Tensor(), at::Tensor()};
     }
 };
@@ -472,8 +467,7 @@ PyObject* load(PyObject*, PyObject* args) {
     get(L.block_gemm, "f8mi_block_gemm");
     get(L.block_gemm_workspace_bytes, "f8mi_block_gemm_workspace_bytes");
     get(L.block_linear_few_rows, "f8mi_block_linear_few_rows");
-    get(L.column_sum, "f8mi_column_sum");
-    get(L.column_sum_workspace_bytes, "f8mi_column_sum_workspace_bytes");
+    get(L.column_sum_finish, "f8mi_column_sum_finish");
     get(L.layer_norm, "f8mi_layer_norm");
     get(L.layer_norm_backward, "f8mi_layer_norm_backward");
     get(L.layer_norm_workspace_bytes, "f8mi_layer_norm_workspace_bytes");

@@ -469,7 +469,11 @@ typedef struct f8mi_block_cast_job {
     void* out_scales;
     void* out_t;             /* copy of `cols` rows contracting over the rows, or NULL; square: its scales alone may be asked for, for a */
     void* out_t_scales;      /* product that reads `out` transposed */
+    float* col_sums;         /* [rows / 128, rounded up][cols]: the columns of every 128 rows added up in fp32, or NULL */
 } f8mi_block_cast_job;
+
+/* out [cols] (out_dtype) = the `parts` rows of col_sums added up in a fixed order, rounded to `dtype` first: the gradient of a bias. */
+int f8mi_column_sum_finish(const float* col_sums, int64_t parts, int64_t cols, int dtype, void* out, int out_dtype, void* stream);
 
 /* One or two tensors in one pass over each; one launch where they have the same dtype. */
 int f8mi_block_cast(const f8mi_block_cast_job* jobs, int count, void* stream);
