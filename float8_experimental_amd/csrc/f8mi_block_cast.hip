@@ -9,6 +9,7 @@
 // transposed one each lane turns its 4 x 8 blocks (v_perm), parks them in a swizzled LDS tile and the tile leaves as 16-byte stores that
 // are contiguous over 4 KB.
 #include "f8mi_block.h"
+#include "f8mi_gemm_util.h"
 
 namespace f8mi {
 
@@ -36,29 +37,39 @@ __device__ __forceinline__ float value(const Eight<DT>& r, int i) {
     else return fp16_bits_to_float(h);
 }
 
-// elements col .. + 7 of a row; zeros past `cols`
-template <int DT>
-__device__ __forceinline__ Eight<DT> load_eight(const uint8_t* row, int64_t col, int64_t cols) {
-    constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2;
+// Elements col .. + 7 of a row, zeros past `cols`.  Rows that start at multiples of 16 bytes are streamed.  Others (not ALIGNED) share a line of the
+// cache wherever two tiles meet in a row: neighbouring tiles go to the same XCD and the lines are left in its L2 (11007 x 4097 bf16: 34.6 -> 29.0 us; the
+// same tile with aligned rows: 27.2).
+template <int DT, bool ALIGNED>
+__device__ __forceinline__ Eight<DT> load_eight(const uint8_t* row, int64_t col, int64_t cols, bool in) {
+    constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2, W = SIZE * 2;  // words of eight elements
     Eight<DT> r;
-    const uint8_t* p = row + col * SIZE;
-    if (col + 8 <= cols) {
 #pragma unroll
-        for (int i = 0; i < SIZE / 2; i++) {
-            const uint4 v = load_nt16_any(p + 16 * i);
-            r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+    for (uint32_t& w : r.w) w = 0u;
+    if (in && col + 8 <= cols) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const uint8_t* p = row + col * SIZE + 4 * i;
+            const u32x4 v = ALIGNED ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4_any*)p;
+            r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
         }
-    } else {
+    } else if (in && col < cols) {
+#pragma unroll 1
+        for (int64_t c = cols - 1; c >= col; c--) {  // from the last one: each moves those behind it up by one place
 #pragma unroll
-        for (uint32_t& w : r.w) w = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (col + i < cols) {
-                if constexpr (DT == F8MI_FP32) r.w[i] = ((const uint32_t*)p)[i];
-                else r.w[i >> 1] |= (uint32_t)((const uint16_t*)p)[i] << (16 * (i & 1));
-            }
+            for (int i = W - 1; i > 0; i--) r.w[i] = DT == F8MI_FP32 ? r.w[i - 1] : r.w[i] << 16 | r.w[i - 1] >> 16;
+            if constexpr (DT == F8MI_FP32) r.w[0] = ((const uint32_t*)row)[c];
+            else r.w[0] = r.w[0] << 16 | ((const uint16_t*)row)[c];
+        }
     }
     return r;
+}
+// What is unpacked after this is not kept from before.
+template <int DT>
+__device__ __forceinline__ void set_apart(Eight<DT>& r) {
+    if constexpr (DT != F8MI_FP32)
+#pragma unroll
+        for (uint32_t& w : r.w) asm("" : "+v"(w));
 }
 
 // maximum over the 16 lanes that hold a row; two 16-bit maxima side by side, or one of 32 bits
@@ -95,7 +106,7 @@ __device__ __forceinline__ float sum_of_rows(float v) {
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-template <int DT>
+template <int DT, bool ALIGNED>
 __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastItem first, const BlockCastItem second, int tiles_first) {
     constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2;
     constexpr int CW = DT == F8MI_FP32 ? 8 : 4;  // words of a lane's column maxima
@@ -103,9 +114,15 @@ __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastI
     __shared__ __align__(16) uint32_t col_max[4][16 * CW];
     __shared__ __align__(16) uint8_t row_bytes[BLOCK], col_bytes[BLOCK];
     __shared__ __align__(16) float col_sum[4][BLOCK];
-    const bool in_first = (int)blockIdx.x < tiles_first;
-    const BlockCastItem it = in_first ? first : second;
-    const int tile = (int)blockIdx.x - (in_first ? 0 : tiles_first);
+    const int bid = ALIGNED ? (int)blockIdx.x : xcd_contiguous_id(blockIdx.x, gridDim.x);
+    const bool in_first = bid < tiles_first;
+    BlockCastItem it = first;  // (field by field: a choice of the whole went through memory)
+    if (!in_first) {
+        it.x = second.x; it.rows = second.rows; it.cols = second.cols; it.ld = second.ld;
+        it.out = second.out; it.out_scales = second.out_scales; it.out_t = second.out_t; it.out_t_scales = second.out_t_scales;
+        it.sums = second.sums; it.square = second.square; it.tiles_c = second.tiles_c;
+    }
+    const int tile = bid - (in_first ? 0 : tiles_first);
     const int tr = tile / it.tiles_c, tc = tile % it.tiles_c;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, tx = t & 15, ty = t >> 4;
     const int64_t r0 = (int64_t)tr * BLOCK, c0 = (int64_t)tc * BLOCK, col = c0 + 8 * tx;
@@ -114,10 +131,7 @@ __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastI
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int64_t row = r0 + 64 * (i >> 2) + 4 * ty + (i & 3);
-        if (row < it.rows) v[i] = load_eight<DT>(it.x + row * it.ld * SIZE, col, it.cols);
-        else
-#pragma unroll
-            for (uint32_t& w : v[i].w) w = 0u;
+        v[i] = load_eight<DT, ALIGNED>(it.x + row * it.ld * SIZE, col, it.cols, row < it.rows);
     }
 
     // maxima of the rows, in every lane of a row: row i in half i % 2 of word i / 2 (fp32: a word each)
@@ -206,6 +220,8 @@ __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastI
             if (row < it.rows) *(uint2*)(it.out + ((col >> 6) * it.rows + row) * 64 + (col & 63)) = make_uint2(lo, hi);
         }
     }
+#pragma unroll
+    for (int i = 0; i < 8; i++) set_apart<DT>(v[i]);
     if (it.out_t_scales) {
         float f[8];
 #pragma unroll
@@ -250,8 +266,9 @@ __global__ __launch_bounds__(BC_THREADS) void block_cast_kernel(const BlockCastI
 }
 
 template <int DT>
-static int launch_block_cast(const BlockCastItem& a, const BlockCastItem& b, int tiles_a, int tiles, hipStream_t stream) {
-    hipLaunchKernelGGL(block_cast_kernel<DT>, dim3((unsigned)tiles), dim3(BC_THREADS), 0, stream, a, b, tiles_a);
+static int launch_block_cast(const BlockCastItem& a, const BlockCastItem& b, int tiles_a, int tiles, bool aligned, hipStream_t stream) {
+    if (aligned) hipLaunchKernelGGL((block_cast_kernel<DT, true>), dim3((unsigned)tiles), dim3(BC_THREADS), 0, stream, a, b, tiles_a);
+    else hipLaunchKernelGGL((block_cast_kernel<DT, false>), dim3((unsigned)tiles), dim3(BC_THREADS), 0, stream, a, b, tiles_a);
     return check_hip(hipGetLastError(), "block cast kernel launch");
 }
 
@@ -289,7 +306,9 @@ extern "C" int f8mi_block_cast(const f8mi_block_cast_job* jobs, int count, void*
     ProfScope prof(F8MI_K_CAST, elements * (jobs[0].dtype == F8MI_FP32 ? 4 : 2), s);
     const int total = (int)(tiles[0] + tiles[1]);
     if (count == 1) items[1] = items[0];
-    if (jobs[0].dtype == F8MI_BF16) return launch_block_cast<F8MI_BF16>(items[0], items[1], (int)tiles[0], total, s);
-    if (jobs[0].dtype == F8MI_FP16) return launch_block_cast<F8MI_FP16>(items[0], items[1], (int)tiles[0], total, s);
-    return launch_block_cast<F8MI_FP32>(items[0], items[1], (int)tiles[0], total, s);
+    bool aligned = true;
+    for (const BlockCastItem& it : items) aligned &= (uintptr_t)it.x % 16 == 0 && it.ld * (jobs[0].dtype == F8MI_FP32 ? 4 : 2) % 16 == 0;
+    if (jobs[0].dtype == F8MI_BF16) return launch_block_cast<F8MI_BF16>(items[0], items[1], (int)tiles[0], total, aligned, s);
+    if (jobs[0].dtype == F8MI_FP16) return launch_block_cast<F8MI_FP16>(items[0], items[1], (int)tiles[0], total, aligned, s);
+    return launch_block_cast<F8MI_FP32>(items[0], items[1], (int)tiles[0], total, aligned, s);
 }
