@@ -16,6 +16,9 @@ constexpr int GRADS = 96;             // tensors a launch
 constexpr int GRAD_THREADS = 256, GRAD_UNROLL = 8;
 constexpr int GRAD_PIECE = GRAD_THREADS * GRAD_UNROLL * 16;  // bytes of input
 constexpr int GRAD_PARTS = 1024;      // workgroups of all launches for the norm, or as many as there are launches if that is more
+// Workgroups of a launch that scales: one for each piece where it copies (4.4e8 bf16 values to fp32, us with 4096 / 8192 / 65536 of them: 640 / 625 /
+// 595).  In place few, which are over sooner where there is nothing to clip.
+constexpr int64_t GRAD_COPY_WGS = 65536, GRAD_IN_PLACE_WGS = 4096;
 
 struct GradTable {
     const uint8_t* x[GRADS];
@@ -164,22 +167,41 @@ __device__ __forceinline__ float scaled(float v, float factor) {
     return p;
 }
 
+__device__ __forceinline__ void stream16(uint8_t* dst, float a, float b, float c, float d) {
+    __builtin_nontemporal_store((u32x4){__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d)}, (u32x4_any*)dst);
+}
+
 template <int DT, int OT>
 __device__ __forceinline__ void grad_scale_piece(const uint8_t* x, uint8_t* out, int64_t first, int64_t n, float factor) {
     constexpr int V = GradVec<DT>::V, SIZE = GradVec<DT>::SIZE, OSIZE = OT == F8MI_FP32 ? 4 : 2;
     auto store = [&](uint8_t* dst, const float (&v)[V]) __attribute__((always_inline)) {
         if constexpr (OT == F8MI_FP32) {
 #pragma unroll
-            for (int i = 0; i < V; i += 4)
-                store16_any(dst + i * 4, make_uint4(__float_as_uint(v[i] * factor), __float_as_uint(v[i + 1] * factor), __float_as_uint(v[i + 2] * factor), __float_as_uint(v[i + 3] * factor)));
+            for (int i = 0; i < V; i += 4) stream16(dst + i * 4, v[i] * factor, v[i + 1] * factor, v[i + 2] * factor, v[i + 3] * factor);
         } else {
             uint32_t w[V / 2];
 #pragma unroll
             for (int i = 0; i < V / 2; i++) w[i] = pack2<OT>(scaled<OT>(v[2 * i], factor), scaled<OT>(v[2 * i + 1], factor));
-            if constexpr (V == 8) store16_any(dst, make_uint4(w[0], w[1], w[2], w[3]));
-            else store8_any(dst, w[0], w[1]);
+            if constexpr (V == 8) __builtin_nontemporal_store((u32x4){w[0], w[1], w[2], w[3]}, (u32x4_any*)dst);
+            else __builtin_nontemporal_store((u32x2){w[0], w[1]}, (u32x2_any*)dst);
         }
     };
+    if (DT != F8MI_FP32 && OT == F8MI_FP32 && first + grad_piece(DT) <= n) {
+        // four values a lane, 8 bytes in and 16 out: a lane's eight would leave as two stores of every other 16 bytes, which streamed
+        // (not through the caches, which the gradients would push out of) took 1.5 times as long
+        u32x2 q[2 * GRAD_UNROLL];
+        const int64_t at = first + threadIdx.x * 4;
+#pragma unroll
+        for (int u = 0; u < 2 * GRAD_UNROLL; u++) q[u] = __builtin_nontemporal_load((const u32x2_any*)(x + (at + u * GRAD_THREADS * 4) * SIZE));
+#pragma unroll
+        for (int u = 0; u < 2 * GRAD_UNROLL; u++) {
+            float v[4];
+            unpack2<DT == F8MI_FP32 ? F8MI_BF16 : DT>(q[u].x, v[0], v[1]);
+            unpack2<DT == F8MI_FP32 ? F8MI_BF16 : DT>(q[u].y, v[2], v[3]);
+            stream16(out + (at + u * GRAD_THREADS * 4) * OSIZE, v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor);
+        }
+        return;
+    }
     if (first + grad_piece(DT) <= n) {
         uint4 q[GRAD_UNROLL];
         const int64_t at = first + threadIdx.x * V;
@@ -272,7 +294,7 @@ static int launch_grads(const f8mi_grad* g, int64_t count, float max_norm, bool 
                 hipLaunchKernelGGL(grad_norm_kernel<KIND>, dim3((unsigned)wgs), dim3(GRAD_THREADS), 0, stream, t, parts + n_parts);
                 n_parts += wgs;
             } else {
-                const unsigned wgs = (unsigned)std::min<int64_t>(pieces, 4 * GRAD_PARTS);
+                const unsigned wgs = (unsigned)std::min<int64_t>(pieces, in_place ? GRAD_IN_PLACE_WGS : GRAD_COPY_WGS);
                 hipLaunchKernelGGL(grad_scale_kernel<KIND>, dim3(wgs), dim3(GRAD_THREADS), 0, stream, t, parts, n_parts, max_norm, in_place, first_launch ? norm_out : nullptr);
             }
             first_launch = false;
