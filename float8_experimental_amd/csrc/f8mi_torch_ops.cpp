@@ -93,40 +93,71 @@ struct Rows {
 
 // ---- blockwise scaled linear
 
-struct Blocks {  // a copy and its scales
-    at::Tensor data, scales;
-    static Blocks make(const at::Tensor& like, int64_t rows, int64_t k, bool with_data = true) {
-        const int64_t kp = (k + 127) / 128 * 128;
-        Blocks b;
-        if (with_data) b.data = at::empty({kp / 64, rows, 64}, like.options().dtype(at::kFloat8_e4m3fn));
-        b.scales = at::empty({kp / 128, (rows + 127) / 128 * 128}, like.options().dtype(at::kByte));
-        return b;
+struct Blocks {  // where a copy and its scales lie
+    uint8_t *data = nullptr, *scales = nullptr;
+};
+// Parts of one allocation: a layer allocates what it keeps for backward and what it does not with one call each, not eight.
+struct Parts {
+    int64_t bytes = 0;
+    int64_t take(int64_t n) {
+        const int64_t at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
     }
 };
-f8mi_block_cast_job job_of(const Rows& x, bool square, const Blocks& a, const Blocks& t, const at::Tensor& sums = {}) {
-    return {x.t.data_ptr(), x.rows, x.cols, x.ld, x.dtype(), square, ptr(a.data), a.data.defined() ? ptr(a.scales) : nullptr, ptr(t.data), ptr(t.scales), (float*)ptr(sums)};
+struct BlocksAt {  // offsets in such an allocation; -1: not there
+    int64_t data = -1, scales = -1;
+    BlocksAt() = default;
+    BlocksAt(Parts& p, int64_t rows, int64_t k, bool with_data = true, bool with_scales = true) {
+        const int64_t kp = (k + 127) / 128 * 128;
+        if (with_data) data = p.take(kp * rows);
+        if (with_scales) scales = p.take(kp / 128 * ((rows + 127) / 128 * 128));
+    }
+    Blocks in(const at::Tensor& t) const {
+        uint8_t* base = (uint8_t*)t.data_ptr();
+        return {data < 0 ? nullptr : base + data, scales < 0 ? nullptr : base + scales};
+    }
+};
+at::Tensor bytes_on(const at::Tensor& like, const Parts& p) { return at::empty({p.bytes}, like.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous)); }
+
+f8mi_block_cast_job job_of(const Rows& x, bool square, const Blocks& a, const Blocks& t, float* sums = nullptr) {
+    return {x.t.data_ptr(), x.rows, x.cols, x.ld, x.dtype(), square, a.data, a.data ? a.scales : nullptr, t.data, t.scales, sums};
 }
-// [m, n] = a [m, k] times b [n, k]; `of`: the copy that b's product reads, the other one of the tensor with transposed
-at::Tensor block_gemm(const Blocks& a, const at::Tensor& b_data, const at::Tensor& b_scales, bool transposed, int64_t m, int64_t n, int64_t k, at::ScalarType type,
-                      const at::Tensor& bias = {}) {
+// [m, n] = a [m, k] times b [n, k]; transposed: b's data is the other copy of its tensor
+at::Tensor block_gemm(const at::Tensor& like, const Blocks& a, const Blocks& b, bool transposed, int64_t m, int64_t n, int64_t k, at::ScalarType type, const at::Tensor& bias = {}) {
     const int64_t kp = (k + 127) / 128 * 128;
-    at::Tensor c = at::empty({m, n}, a.data.options().dtype(type));
+    at::Tensor c = at::empty({m, n}, like.options().dtype(type).memory_format(at::MemoryFormat::Contiguous));
     const int64_t bytes = transposed ? 0 : L.block_gemm_workspace_bytes(m, n, kp);
-    const at::Tensor ws = bytes ? at::empty({bytes / 4}, a.data.options().dtype(at::kFloat)) : at::Tensor();
-    check(L.block_gemm(a.data.data_ptr(), a.scales.data_ptr(), b_data.data_ptr(), b_scales.data_ptr(), transposed, m, n, kp, c.data_ptr(), dtype_code(type), n, ptr(bias),
-                       ptr(ws), bytes, stream_of(c)), "f8mi_block_gemm");
+    const at::Tensor ws = bytes ? at::empty({bytes / 4}, like.options().dtype(at::kFloat)) : at::Tensor();
+    check(L.block_gemm(a.data, a.scales, b.data, b.scales, transposed, m, n, kp, c.data_ptr(), dtype_code(type), n, ptr(bias), ptr(ws), bytes, stream_of(c)), "f8mi_block_gemm");
     return c;
 }
+
 // The weight needs one copy if the backward product can read it transposed
 bool one_weight_copy(int64_t k, int64_t n) { return k % 128 == 0 && n % 128 == 0; }
+
+// What a layer keeps for backward, in one allocation: x transposed and its scales for the gradient of the weight; the weight, transposed or as it is,
+// and the scales of its transpose for the gradient of x.
+struct Kept {
+    Parts parts;
+    BlocksAt xt, w, wt;
+    Kept(int64_t m, int64_t k, int64_t n, bool need_dx, bool need_dw) {
+        if (need_dw) xt = BlocksAt(parts, k, m);
+        if (need_dx) {
+            const bool one = one_weight_copy(k, n);
+            if (one) w = BlocksAt(parts, n, k, true, false);
+            wt = BlocksAt(parts, k, n, !one);
+        }
+    }
+};
 
 // An argument that may be absent: autograd gives it an edge only where it is there.
 using MaybeTensor = std::optional<at::Tensor>;
 MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
-    // `saved`: what backward needs (x's transposed copy and scales, the weight's), or null
-    static at::Tensor compute(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, bool need_dx, bool need_dw, variable_list* saved) {
+    // kept: see Kept; null: nothing is
+    static at::Tensor compute(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, bool need_dx, bool need_dw, at::Tensor* kept) {
         const c10::DeviceGuard guard(x.device());
         const at::AutoDispatchBelowADInplaceOrView below;
         const int64_t k = weight.size(1), n = weight.size(0);
@@ -135,24 +166,32 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
         std::vector<int64_t> y_shape(x.sizes().begin(), x.sizes().end());
         y_shape.back() = n;
         if (m == 0) return at::empty(y_shape, x.options());
-        const bool one = one_weight_copy(k, n);
-        const Blocks x8 = Blocks::make(x, m, k), x8t = need_dw ? Blocks::make(x, k, m) : Blocks();
-        const Blocks w8 = Blocks::make(x, n, k), w8t = need_dx ? Blocks::make(x, k, n, !one) : Blocks();
-        const f8mi_block_cast_job jobs[2] = {job_of(xr, false, x8, x8t), job_of(wr, true, w8, w8t)};
+        const Kept k_at(m, k, n, need_dx, need_dw);
+        Parts parts;
+        const BlocksAt x8_at(parts, m, k), w8_at(parts, n, k, k_at.w.data < 0);
+        const at::Tensor mem = bytes_on(x, parts);
+        Blocks xt, wt, w8 = w8_at.in(mem);
+        const Blocks x8 = x8_at.in(mem);
+        if (k_at.parts.bytes) {
+            *kept = bytes_on(x, k_at.parts);
+            xt = k_at.xt.in(*kept);
+            wt = k_at.wt.in(*kept);
+            if (k_at.w.data >= 0) w8.data = k_at.w.in(*kept).data;
+        }
+        const f8mi_block_cast_job jobs[2] = {job_of(xr, false, x8, xt), job_of(wr, true, w8, wt)};
         check(L.block_cast(jobs, 2, stream_of(x)), "f8mi_block_cast");
         const at::Tensor b = bias.defined() ? bias.to(x.scalar_type()).contiguous() : at::Tensor();
-        at::Tensor y = block_gemm(x8, w8.data, w8.scales, false, m, n, k, x.scalar_type(), b);
-        if (saved) *saved = {x8t.data, x8t.scales, one && need_dx ? w8.data : w8t.data, w8t.scales};
+        at::Tensor y = block_gemm(x, x8, w8, false, m, n, k, x.scalar_type(), b);
         return x.dim() == 2 ? y : at::_unsafe_view(y, y_shape);
     }
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& bias_, bool need_dx, bool need_dw) {
         const at::Tensor bias = bias_.value_or(at::Tensor());
-        variable_list saved;
-        at::Tensor y = compute(x, weight, bias, need_dx, need_dw, &saved);
+        at::Tensor kept;
+        at::Tensor y = compute(x, weight, bias, need_dx, need_dw, &kept);
         ctx->saved_data["x_shape"] = x.sizes().vec();
-        ctx->saved_data["types"] = (int64_t)x.scalar_type() | (int64_t)weight.scalar_type() << 8 | (bias.defined() ? (int64_t)bias.scalar_type() + 1 : 0) << 16;
+        ctx->saved_data["types"] = (int64_t)x.scalar_type() | (int64_t)weight.scalar_type() << 8 | (bias.defined() ? (int64_t)bias.scalar_type() + 1 : 0) << 16 | (int64_t)need_dx << 24 | (int64_t)need_dw << 25;
         ctx->saved_data["n"] = weight.size(0);
-        ctx->save_for_backward(std::move(saved));
+        ctx->save_for_backward({kept});
         return y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -160,9 +199,10 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
         const auto saved = ctx->get_saved_variables();
         const auto x_shape = ctx->saved_data["x_shape"].toIntVector();
         const int64_t k = x_shape.back(), n = ctx->saved_data["n"].toInt(), types = ctx->saved_data["types"].toInt();
-        const at::ScalarType xt = (at::ScalarType)(types & 255), wt = (at::ScalarType)(types >> 8 & 255), bt = (at::ScalarType)((types >> 16) - 1);
+        const at::ScalarType xt = (at::ScalarType)(types & 255), wt = (at::ScalarType)(types >> 8 & 255), bt = (at::ScalarType)((types >> 16 & 255) - 1);
+        const bool kept_dx = types >> 24 & 1, kept_dw = types >> 25 & 1;
         const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
-        const bool need_db = types >> 16 && ctx->needs_input_grad(2);
+        const bool need_db = (types >> 16 & 255) && ctx->needs_input_grad(2);
         at::Tensor dx, dw, db;
         if (!grads[0].defined()) return {dx, dw, db, at::Tensor(), at::Tensor()};
         const c10::DeviceGuard guard(grads[0].device());
@@ -176,19 +216,29 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
             return {dx, dw, db, at::Tensor(), at::Tensor()};
         }
         if (!(need_dx || need_dw || need_db)) return {dx, dw, db, at::Tensor(), at::Tensor()};
-        TORCH_CHECK((!need_dx || saved[3].defined()) && (!need_dw || saved[0].defined()), "blockwise_linear: a gradient is asked for that the forward pass was not told of");
-        const Blocks g8 = need_dx ? Blocks::make(dy.t, m, n) : Blocks(), g8t = need_dw ? Blocks::make(dy.t, n, m) : Blocks();
-        const at::Tensor sums = need_db ? at::empty({(m + 127) / 128, n}, dy.t.options().dtype(at::kFloat)) : at::Tensor();
-        const f8mi_block_cast_job job = job_of(dy, false, g8, g8t, sums);
+        TORCH_CHECK((!need_dx || kept_dx) && (!need_dw || kept_dw), "blockwise_linear: a gradient is asked for that the forward pass was not told of");
+        const Kept k_at(m, k, n, kept_dx, kept_dw);
+        const at::Tensor& kept = saved[0];
+        if (need_dx || need_dw)  // (hooks on saved tensors hand back what they like)
+            TORCH_CHECK(kept.defined() && kept.is_cuda() && kept.is_contiguous() && kept.scalar_type() == at::kByte && kept.numel() == k_at.parts.bytes, "blockwise_linear: what was saved for backward is not what came back");
+        Parts parts;
+        const BlocksAt g8_at = need_dx ? BlocksAt(parts, m, n) : BlocksAt(), gt_at = need_dw ? BlocksAt(parts, n, m) : BlocksAt();
+        const int64_t sum_rows = (m + 127) / 128, sums_at = need_db ? parts.take(sum_rows * n * 4) : 0;
+        const at::Tensor mem = bytes_on(dy.t, parts);
+        const Blocks g8 = g8_at.in(mem), gt = gt_at.in(mem);
+        float* sums = need_db ? (float*)((uint8_t*)mem.data_ptr() + sums_at) : nullptr;
+        const f8mi_block_cast_job job = job_of(dy, false, g8, gt, sums);
         check(L.block_cast(&job, 1, stream_of(dy.t)), "f8mi_block_cast");
         if (need_dx) {
-            dx = block_gemm(g8, saved[2], saved[3], one_weight_copy(k, n), m, k, n, xt);
+            const bool one = one_weight_copy(k, n);
+            const Blocks w{one ? k_at.w.in(kept).data : k_at.wt.in(kept).data, k_at.wt.in(kept).scales};
+            dx = block_gemm(dy.t, g8, w, one, m, k, n, xt);
             if (x_shape.size() != 2) dx = dx.view(x_shape);
         }
-        if (need_dw) dw = block_gemm(g8t, saved[0], saved[1], false, n, k, m, wt);
+        if (need_dw) dw = block_gemm(dy.t, gt, k_at.xt.in(kept), false, n, k, m, wt);
         if (need_db) {
             db = at::empty({n}, dy.t.options().dtype(bt));
-            check(L.column_sum_finish((const float*)sums.data_ptr(), sums.size(0), n, dy.dtype(), db.data_ptr(), dtype_code(bt), stream_of(dy.t)), "f8mi_column_sum_finish");
+            check(L.column_sum_finish(sums, sum_rows, n, dy.dtype(), db.data_ptr(), dtype_code(bt), stream_of(dy.t)), "f8mi_column_sum_finish");
         }
         return {dx, dw, db, at::Tensor(), at::Tensor()};
     }
@@ -346,10 +396,13 @@ PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n
                 check(L.block_linear_few_rows(xr.t.data_ptr(), xr.ld, xr.dtype(), data.data_ptr(), scales.data_ptr(), xr.rows, n, k, y.data_ptr(), n, ptr(b), stream_of(x)),
                       "f8mi_block_linear_few_rows");
             } else {
-                const Blocks x8 = Blocks::make(x, xr.rows, k);
+                Parts parts;
+                const BlocksAt x8_at(parts, xr.rows, k);
+                const at::Tensor mem = bytes_on(x, parts);
+                const Blocks x8 = x8_at.in(mem);
                 const f8mi_block_cast_job job = job_of(xr, false, x8, Blocks());
                 check(L.block_cast(&job, 1, stream_of(x)), "f8mi_block_cast");
-                y = block_gemm(x8, data, scales, false, xr.rows, n, k, x.scalar_type(), b);
+                y = block_gemm(x, x8, {(uint8_t*)data.data_ptr(), (uint8_t*)scales.data_ptr()}, false, xr.rows, n, k, x.scalar_type(), b);
                 if (x.dim() != 2) y = y.view(y_shape);
             }
         }
