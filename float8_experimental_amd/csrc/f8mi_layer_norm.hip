@@ -6,9 +6,14 @@
 // (number of workgroups)-th row, so that w and b are read once and, backward, a lane sums the columns it owns over its rows in
 // registers.  Backward's workgroups write those sums, fp32, and a second launch adds them in a fixed order.  Statistics and sums are fp32.
 //
-// Rows that do not fit (more than 16384 values of 16 bits, 8192 of fp32) are read once for each statistic and once for the result, out of the
-// L2 after the first time, and the column sums have a kernel of their own.
+// Measured, both passes, of the bytes of x, y, x, dy and dx: 8192 rows of 4096 bf16 73 us (4.6 TB/s; a copy: 4.9), 4099 of 4097 fp32 77 us (4.4), 4096 of 8192
+// bf16 87 us (3.9), 12252 of 15170 fp32 784 us (4.7); the launches, the first rows' latency and the sums' rows are what is left at these sizes.
+//
+// Rows that do not fit (backward more than 16384 values, forward those whose parameters do not fit in LDS or more than 32768 of 16 bits, 16384 of fp32)
+// are read once for each statistic and once for the result, out of the L2 after the first time, and the column sums have a kernel of their own:
+// 1683 us where the rows of 15170 fp32 values above now take 784.
 #include <algorithm>
+#include <type_traits>
 
 #include "f8mi_gemm_util.h"
 
@@ -28,12 +33,12 @@ __device__ __forceinline__ void ln_unpack(uint4 q, float (&v)[Ln<DT>::V]) {
         else unpack2<DT>(w[i], v[2 * i], v[2 * i + 1]);
     }
 }
-// Values col .. col + V - 1 of a row, zeros past its end: there the last V values of the row are read and shifted (element by element that
+// Values col .. col + V - 1 of a row zeros past its end: there the last V values of the row are read and shifted (element by element that
 // part held 30 registers more, in every lane).  I: int, or int64_t where columns may need it.
 template <int DT, typename I>
 __device__ __forceinline__ uint4 ln_load(const uint8_t* row, I col, I cols) {
     constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
-    if (col + V <= cols) return load_nt16_any(row + col * SIZE);
+    if (col + V <= cols) return load_nt16_any(row + std::make_unsigned_t<I>(col * SIZE));
     uint64_t lo = 0, hi = 0;
     if (col < cols && cols >= V) {
         const uint4 q = load_nt16_any(row + (cols - V) * SIZE);
@@ -53,20 +58,25 @@ __device__ __forceinline__ uint4 ln_load(const uint8_t* row, I col, I cols) {
     }
     return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
-template <int DT, typename I>
-__device__ __forceinline__ void ln_store(uint8_t* row, I col, I cols, const float (&v)[Ln<DT>::V]) {
-    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+template <int DT>
+__device__ __forceinline__ uint4 ln_pack(const float (&v)[Ln<DT>::V]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if constexpr (DT == F8MI_FP32) w[i] = __float_as_uint(v[i]);
         else w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int DT, typename I>
+__device__ __forceinline__ void ln_store(uint8_t* row, I col, I cols, const float (&v)[Ln<DT>::V]) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+    const uint4 w = ln_pack<DT>(v);
     if (col + V <= cols) {
-        store16_any(row + col * SIZE, make_uint4(w[0], w[1], w[2], w[3]));
+        store16_any(row + std::make_unsigned_t<I>(col * SIZE), w);
         return;
     }
-    uint64_t lo = w[0] | (uint64_t)w[1] << 32, hi = w[2] | (uint64_t)w[3] << 32;
+    uint64_t lo = w.x | (uint64_t)w.y << 32, hi = w.z | (uint64_t)w.w << 32;
 #pragma unroll 1
     for (; col < cols; col++) {
         if constexpr (DT == F8MI_FP32) ((uint32_t*)row)[col] = (uint32_t)lo;
@@ -162,51 +172,123 @@ __device__ __forceinline__ void row_moments(float& mean, float& m2, int cols, fl
     }
 }
 
+// Rows of one 16-byte piece a lane have the parameters in registers (64 a lane up to 512 lanes, so that a CU holds 2048).  Longer ones have up to four
+// pieces and the parameters in LDS, in their own type, which leaves registers to have the next row on its way while this one's sums are
+// waited for (2048 rows of 8192 fp32 values, both passes: 117 -> 77 us, of 16384 bf16 values 118 -> 99).
+constexpr int LN_ROW_LANES = 1024;
 constexpr int ln_threads(int t) { return t < 256 ? 256 : t; }
-// One piece of 16 bytes a lane: 64 registers do, and a CU holds 2048 lanes; more pieces, or 16 waves that wait for each other: 1024 lanes.
-constexpr int ln_lanes(int t, int vpt) { return vpt == 1 && t < 1024 ? 2048 : 1024; }
-// Whether a row is asked for while the one before is waited for; the others have no registers for it.
-constexpr bool ln_ahead(int vpt) { return vpt == 1; }
-// Of a workgroup of the backward kernel, which writes a row of sums: one a CU, or two whose waits overlap where a row takes many pieces a lane.
-constexpr int ln_backward_threads(int vpt) { return vpt > 2 ? 512 : 1024; }
+constexpr int ln_waves_a_simd(int t, int vpt) { return t < LN_ROW_LANES && vpt == 1 ? 8 : 4; }
+constexpr int ln_backward_threads(int t, int vpt) { return vpt > 1 ? t : LN_ROW_LANES; }
+// rows asked for ahead, forward
+constexpr int ln_ahead(int t, int vpt) { return t == LN_ROW_LANES && vpt < 3 ? 2 : 1; }
 
-// T lanes a row, VPT pieces of 16 bytes a lane
-template <int DT, int PT, int T, int VPT>
-__global__ __launch_bounds__(ln_threads(T), ln_lanes(T, VPT) / 256) void layer_norm_kernel(const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int cols, const void* __restrict__ weight,
-                                                                   const void* __restrict__ bias, float eps, uint8_t* __restrict__ y, float2* __restrict__ stats) {
-    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_threads(T) / T;
-    __shared__ float2 slots[2][ln_threads(T) / 64];
-    const int t = threadIdx.x % T, group = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
-    const float inv_cols = 1.0f / (float)cols;
-    float w[VPT][V], b[VPT][V];
+// What a lane holds of a row: VPT pieces of V values, T * V apart.  The last may lie past the end of the row: it is moved back to end there
+// (no branch, nothing shifted; with those a lane's addresses and shifts took the registers of a piece), and `off` counts the values at
+// its start that the lane before holds too: they stay out of sums, and are stored twice, the same.  With 64 lanes a row may be shorter than a
+// piece: there values past the end are zeros, and `off` counts the others.
+template <int T, int VPT, int V>
+struct LnLane {
+    int t, last, off;
+    __device__ __forceinline__ LnLane(int t_, int cols) : t(t_), last(((VPT - 1) * T + t_) * V) {
+        if constexpr (T == 64) {
+            off = min(max(cols - last, 0), V);
+        } else {
+            const int col = last;
+            last = min(col, cols - V);
+            off = min(col - last, V);
+        }
+    }
+    __device__ __forceinline__ int col(int p) const { return p < VPT - 1 ? (p * T + t) * V : last; }
+    __device__ __forceinline__ bool has(int p, int i) const { return p < VPT - 1 || (T == 64 ? i < off : i >= off); }
+    __device__ __forceinline__ bool any(int p) const { return p < VPT - 1 || (T == 64 ? off > 0 : off < V); }
+    // row: the same in a wave, and kept apart from the lane's offset, or each piece has its own 64-bit address in registers for the whole loop
+    template <int DT>
+    __device__ __forceinline__ uint4 load(const uint8_t* row, int p, int cols) const {
+        if constexpr (T == 64) return ln_load<DT, int>(row, last, cols);
+        asm("" : "+s"(row));
+        return load_nt16_any(row + (uint32_t)(col(p) * Ln<DT>::SIZE));
+    }
+    template <int DT>
+    __device__ __forceinline__ void store(uint8_t* row, int p, int cols, const float (&v)[V]) const {
+        if (!any(p)) return;
+        if constexpr (T == 64) return ln_store<DT, int>(row, last, cols, v);
+        asm("" : "+s"(row));
+        store16_any(row + (uint32_t)(col(p) * Ln<DT>::SIZE), ln_pack<DT>(v));
+    }
+};
+
+// A parameter in LDS: 16-byte parts of a piece of V values lie `pieces` apart, so that lanes next to each other read without conflicts.
+template <int PT, int V>
+struct LnShared {
+    static constexpr int PV = Ln<PT>::V, PARTS = V / PV;
+    uint4* at;
+    int pieces;
+    __device__ __forceinline__ void fill(const void* p, int cols, float otherwise) {
+        for (int i = threadIdx.x; i < pieces * PARTS; i += blockDim.x) {
+            const int part = i / pieces, piece = i - part * pieces;
+            uint4 q;
+            if (p) {
+                q = load_nt16_any((const uint8_t*)p + (uint32_t)((min(piece * V, cols - V) + part * PV) * Ln<PT>::SIZE));
+            } else {
+                const uint32_t one = PT == F8MI_FP32 ? __float_as_uint(otherwise) : pack2<PT == F8MI_FP32 ? F8MI_BF16 : PT>(otherwise, otherwise);
+                q = make_uint4(one, one, one, one);
+            }
+            at[i] = q;
+        }
+    }
+    __device__ __forceinline__ void read(int piece, float (&v)[V]) const {
+        piece = min(piece, pieces - 1);
 #pragma unroll
-    for (int p = 0; p < VPT; p++) {
-        ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[p]);
-        ln_param<PT, V, int>(bias, (p * T + t) * V, cols, 0.f, b[p]);
+        for (int part = 0; part < PARTS; part++) {
+            float f[PV];
+            ln_unpack<PT>(at[part * pieces + piece], f);
+#pragma unroll
+            for (int j = 0; j < PV; j++) v[part * PV + j] = f[j];
+        }
+    }
+};
+
+// T lanes a row, VPT pieces of 16 bytes a lane (only the last of them can lie past the end of the row: ln_shape)
+template <int DT, int PT, int T, int VPT>
+__global__ __launch_bounds__(ln_threads(T), ln_waves_a_simd(T, VPT)) void layer_norm_kernel(const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int cols, const void* __restrict__ weight,
+                                                                   const void* __restrict__ bias, float eps, uint8_t* __restrict__ y, float2* __restrict__ stats) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_threads(T) / T, AHEAD = ln_ahead(T, VPT);
+    constexpr bool SHARED = VPT > 1;
+    __shared__ float2 slots[2][ln_threads(T) / 64];
+    extern __shared__ uint4 ln_shared[];
+    const int t = threadIdx.x % T, group = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
+    const LnLane<T, VPT, V> lane(t, cols);
+    const float inv_cols = 1.0f / (float)cols;
+    const int64_t stride = (int64_t)gridDim.x * GROUPS, first = (int64_t)blockIdx.x * GROUPS;
+    uint4 next[AHEAD][VPT];  // rows after this one: asked for before this one's sums have to wait for each other
+    auto fetch = [&](uint4 (&q)[VPT], int64_t row) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < VPT; p++) q[p] = row < rows ? lane.template load<DT>(x + row * ld * SIZE, p, cols) : make_uint4(0u, 0u, 0u, 0u);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) fetch(next[i], first + i * stride + group);
+    LnShared<PT, V> ws{ln_shared, (cols + V - 1) / V}, bs{ln_shared + ws.pieces * ws.PARTS, ws.pieces};
+    float w[V], b[V];
+    if constexpr (SHARED) {
+        ws.fill(weight, cols, 1.f);
+        bs.fill(bias, cols, 0.f);
+        __syncthreads();
+    } else {
+        ln_param<PT, V, int>(weight, lane.last, cols, 1.f, w);
+        ln_param<PT, V, int>(bias, lane.last, cols, 0.f, b);
     }
     const float inv_count = 1.0f / (float)max(wave_count<T, VPT, V>(t >> 6, cols), 1);
-    int parity = 0;
-    const int64_t stride = (int64_t)gridDim.x * GROUPS;
-    uint4 next[VPT];  // of the row after this one: asked for before this one's sums have to wait for each other
-    auto fetch = [&](int64_t row) __attribute__((always_inline)) {
-#pragma unroll
-        for (int p = 0; p < VPT; p++) next[p] = row < rows ? ln_load<DT, int>(x + row * ld * SIZE, (p * T + t) * V, cols) : make_uint4(0u, 0u, 0u, 0u);
-    };
-    if (ln_ahead(VPT)) fetch((int64_t)blockIdx.x * GROUPS + group);
-    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += stride) {
-        const int64_t row = r0 + group;
-        if (!ln_ahead(VPT)) fetch(row);
-        const bool in = row < rows;
+    auto one = [&](uint4 (&ahead)[VPT], int64_t row, float2* slot) __attribute__((always_inline)) {
         uint4 q[VPT];  // the row as it came: unpacking it again costs less than registers that keep waves from running
 #pragma unroll
-        for (int p = 0; p < VPT; p++) q[p] = next[p];
-        if (ln_ahead(VPT) && r0 + stride < rows) fetch(row + stride);
+        for (int p = 0; p < VPT; p++) q[p] = ahead[p];
+        if (row - group + AHEAD * stride < rows) fetch(ahead, row + AHEAD * stride);
         float s = 0.f, v[V];
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
             ln_unpack<DT>(q[p], v);
 #pragma unroll
-            for (int i = 0; i < V; i++) s += v[i];
+            for (int i = 0; i < V; i++) s += T == 64 || lane.has(p, i) ? v[i] : 0.f;
         }
         float mean = wave_sum(s) * inv_count;
         s = 0.f;
@@ -217,103 +299,121 @@ __global__ __launch_bounds__(ln_threads(T), ln_lanes(T, VPT) / 256) void layer_n
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 v[i] -= mean;
-                if ((p * T + t) * V + i < cols) s = __builtin_fmaf(v[i], v[i], s);
+                if (lane.has(p, i)) s = __builtin_fmaf(v[i], v[i], s);
             }
         }
         s = wave_sum(s);
-        row_moments<T, VPT, V>(mean, s, cols, inv_cols, slots[parity]);
-        parity ^= 1;
+        row_moments<T, VPT, V>(mean, s, cols, inv_cols, slot);
         const float rstd = 1.0f / __builtin_sqrtf(s * inv_cols + eps);
-        if (!in) continue;
+        if (row >= rows) return;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
             set_apart<DT>(q[p]);
             ln_unpack<DT>(q[p], v);
+            if constexpr (SHARED) {
+                ws.read(p * T + t, w);
+                bs.read(p * T + t, b);
+            }
 #pragma unroll
-            for (int i = 0; i < V; i++) v[i] = __builtin_fmaf((v[i] - mean) * rstd, w[p][i], b[p][i]);
-            const int col = (p * T + t) * V;
-            if (col < cols) ln_store<DT, int>(y + row * cols * SIZE, col, cols, v);
+            for (int i = 0; i < V; i++) v[i] = __builtin_fmaf((v[i] - mean) * rstd, w[i], b[i]);
+            lane.template store<DT>(y + row * cols * SIZE, p, cols, v);
         }
         if (stats && t == 0) stats[row] = make_float2(mean, rstd);
+    };
+    int parity = 0;
+    for (int64_t r0 = first; r0 < rows; r0 += AHEAD * stride, parity ^= 1) {
+        one(next[0], r0 + group, slots[AHEAD == 1 ? parity : 0]);
+        if constexpr (AHEAD == 2)
+            if (r0 + stride < rows) one(next[1], r0 + stride + group, slots[1]);
     }
 }
 
 template <int DT, int PT, int T, int VPT>
-__global__ __launch_bounds__(ln_backward_threads(VPT), 4) void layer_norm_backward_kernel(const uint8_t* __restrict__ dy, int64_t ld_dy, const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int cols,
+__global__ __launch_bounds__(ln_backward_threads(T, VPT), 4) void layer_norm_backward_kernel(const uint8_t* __restrict__ dy, int64_t ld_dy, const uint8_t* __restrict__ x, int64_t ld, int64_t rows, int cols,
                                                                             const void* __restrict__ weight, const float2* __restrict__ stats, uint8_t* __restrict__ dx,
                                                                             float* __restrict__ partial) {
-    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_backward_threads(VPT) / T;
-    __shared__ float2 slots[2][ln_backward_threads(VPT) / 64];
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = ln_backward_threads(T, VPT) / T;
+    constexpr bool SHARED = VPT > 1;
+    __shared__ float2 slots[2][ln_backward_threads(T, VPT) / 64];
     __shared__ float sums[GROUPS > 1 ? (GROUPS - 1) * T * 2 * V : 1];
+    extern __shared__ uint4 ln_shared[];
     const int t = threadIdx.x % T, group = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
+    const LnLane<T, VPT, V> lane(t, cols);
     const float inv_cols = 1.0f / (float)cols;
-    constexpr bool KEEP_W = VPT == 1 || DT == F8MI_FP32;  // else it is read again for each row, out of the L2: there are no registers for it
-    float w[KEEP_W ? VPT : 1][V], dw[VPT][V], db[VPT][V];
-#pragma unroll
-    for (int p = 0; p < VPT; p++) {
-        if constexpr (KEEP_W) ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[p]);
-#pragma unroll
-        for (int i = 0; i < V; i++) dw[p][i] = db[p][i] = 0.f;
-    }
-    int parity = 0;
-    const int64_t stride = (int64_t)gridDim.x * GROUPS;
-    uint4 nx[VPT], ng[VPT];  // of the row after this one: asked for before this one's sums have to wait for each other
-    float2 ns;
+    const int64_t stride = (int64_t)gridDim.x * GROUPS, first = (int64_t)blockIdx.x * GROUPS;
+    struct Next {  // of rows after this one: asked for before this one's sums have to wait for each other
+        uint4 x[VPT], g[VPT];
+        float2 stats;
+    } next;
     auto fetch = [&](int64_t row) __attribute__((always_inline)) {
         const bool in = row < rows;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
-            const int col = (p * T + t) * V;
-            nx[p] = in ? ln_load<DT, int>(x + row * ld * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
-            ng[p] = in ? ln_load<DT, int>(dy + row * ld_dy * SIZE, col, cols) : make_uint4(0u, 0u, 0u, 0u);
+            next.x[p] = in ? lane.template load<DT>(x + row * ld * SIZE, p, cols) : make_uint4(0u, 0u, 0u, 0u);
+            next.g[p] = in ? lane.template load<DT>(dy + row * ld_dy * SIZE, p, cols) : make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (VPT > 1) __builtin_amdgcn_sched_barrier(0);
         }
-        ns = in ? stats[row] : make_float2(0.f, 0.f);
+        next.stats = in ? stats[row] : make_float2(0.f, 0.f);
     };
-    if (ln_ahead(VPT)) fetch((int64_t)blockIdx.x * GROUPS + group);
-    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += stride, parity ^= 1) {
+    fetch(first + group);
+    LnShared<PT, V> ws{ln_shared, (cols + V - 1) / V};
+    float w[V], dw[VPT][V], db[VPT][V];
+    if constexpr (SHARED) {
+        ws.fill(weight, cols, 1.f);
+        __syncthreads();
+    } else {
+        ln_param<PT, V, int>(weight, lane.last, cols, 1.f, w);
+    }
+#pragma unroll
+    for (int p = 0; p < VPT; p++)
+#pragma unroll
+        for (int i = 0; i < V; i++) dw[p][i] = db[p][i] = 0.f;
+    int parity = 0;
+    for (int64_t r0 = first; r0 < rows; r0 += stride, parity ^= 1) {
         const int64_t row = r0 + group;
-        if (!ln_ahead(VPT)) fetch(row);
-        const bool in = row < rows;
         uint4 qx[VPT], qg[VPT];
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
-            qx[p] = nx[p];
-            qg[p] = ng[p];
+            qx[p] = next.x[p];
+            qg[p] = next.g[p];
         }
-        const float2 st = ns;
-        if (ln_ahead(VPT) && r0 + stride < rows) fetch(row + stride);
+        const float2 st = next.stats;
+        if (r0 + stride < rows) fetch(row + stride);
         float xh[V], g[V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
+            if constexpr (VPT > 1) __builtin_amdgcn_sched_barrier(0);  // one piece at a time: unpacked together they do not fit in registers
             ln_unpack<DT>(qx[p], xh);
             ln_unpack<DT>(qg[p], g);
-            if constexpr (!KEEP_W) ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[0]);
+            if constexpr (SHARED) ws.read(p * T + t, w);
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 xh[i] = (xh[i] - st.x) * st.y;
+                if (T > 64 && !lane.has(p, i)) g[i] = 0.f;
                 dw[p][i] = __builtin_fmaf(g[i], xh[i], dw[p][i]);
                 db[p][i] += g[i];
-                g[i] *= w[KEEP_W ? p : 0][i];  // (past the end dy, and so g, is zero)
+                g[i] *= w[i];
                 s1 += g[i];
                 s2 = __builtin_fmaf(g[i], xh[i], s2);
+                asm volatile("" : "+v"(dw[p][i]), "+v"(db[p][i]));  // added here: behind the barrier, where the compiler moves it, everything waits for it (8192 values: 98 -> 87 us)
             }
         }
         if (!dx) continue;
         row_sums<T>(s1, s2, slots[parity]);
         s1 *= inv_cols;
         s2 *= inv_cols;
-        if (!in) continue;
+        if (row >= rows) continue;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {
+            if constexpr (VPT > 1) __builtin_amdgcn_sched_barrier(0);
             set_apart<DT>(qx[p]);
             set_apart<DT>(qg[p]);
             ln_unpack<DT>(qx[p], xh);
             ln_unpack<DT>(qg[p], g);
-            if constexpr (!KEEP_W) ln_param<PT, V, int>(weight, (p * T + t) * V, cols, 1.f, w[0]);
+            if constexpr (SHARED) ws.read(p * T + t, w);
 #pragma unroll
-            for (int i = 0; i < V; i++) g[i] = st.y * (g[i] * w[KEEP_W ? p : 0][i] - s1 - (xh[i] - st.x) * st.y * s2);
-            const int col = (p * T + t) * V;
-            if (col < cols) ln_store<DT, int>(dx + row * cols * SIZE, col, cols, g);
+            for (int i = 0; i < V; i++) g[i] = st.y * (g[i] * w[i] - s1 - (xh[i] - st.x) * st.y * s2);
+            lane.template store<DT>(dx + row * cols * SIZE, p, cols, g);
         }
     }
     if (!partial) return;
@@ -339,10 +439,10 @@ __global__ __launch_bounds__(ln_backward_threads(VPT), 4) void layer_norm_backwa
                     db[p][i] += sums[((k * 2 + 1) * V + i) * T + t];
                 }
         }
-        const int col = (p * T + t) * V;
+        const int col = lane.col(p);
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (col + i < cols) {
+            if (lane.has(p, i)) {
                 out[col + i] = dw[p][i];
                 out[cols + col + i] = db[p][i];
             }
@@ -488,17 +588,23 @@ struct LnArgs {
     hipStream_t stream;
 };
 
-// Lanes of a row and pieces a lane, by the number of 16-byte pieces of a row; 0: does not fit.
+// Lanes of a row and pieces a lane, by the number of 16-byte pieces of a row; 0: does not fit.  Forward's weight and bias have to fit in LDS
+// with it, in backward the column sums of 16-bit rows take the registers of a third piece (20000 bf16 values with one spilled: 194 us, as by columns).
 struct LnShape {
     int t, vpt;
 };
-static LnShape ln_shape(int64_t cols, int dtype, bool backward) {
-    const int64_t pieces = (cols + (dtype == F8MI_FP32 ? 3 : 7)) / (dtype == F8MI_FP32 ? 4 : 8);
-    for (int t = 64; t <= 1024; t *= 2)
+constexpr int LN_MAX_LDS = (160 << 10) - 512;
+static int64_t ln_pieces(int64_t cols, int dtype) { return (cols + (dtype == F8MI_FP32 ? 3 : 7)) / (dtype == F8MI_FP32 ? 4 : 8); }
+// of the parameters that a workgroup of 1024 lanes keeps
+static int64_t ln_lds(int64_t cols, int dtype, int p_dtype, bool backward) { return ln_pieces(cols, dtype) * 16 * (dtype == p_dtype ? 1 : 2) * (backward ? 1 : 2); }
+static LnShape ln_shape(int64_t cols, int dtype, int p_dtype, bool backward) {
+    const int64_t pieces = ln_pieces(cols, dtype);
+    for (int t = 64; t <= LN_ROW_LANES; t *= 2)
         if (pieces <= t) return {t, 1};
-    if (pieces > 2048) return {0, 0};
-    if (backward && dtype != F8MI_FP32) return {1024, 2};
-    return {512, pieces <= 1536 ? 3 : 4};
+    if (dtype == F8MI_FP32 && pieces <= 3 * 512) return {512, 3};  // two workgroups a CU, and fewer idle lanes (4097 values: 88 us with 1024 lanes, 77)
+    const int64_t vpt = (pieces + LN_ROW_LANES - 1) / LN_ROW_LANES;
+    if (vpt > (backward && dtype != F8MI_FP32 ? 2 : 4) || ln_lds(cols, dtype, p_dtype, backward) > LN_MAX_LDS) return {0, 0};
+    return {LN_ROW_LANES, (int)vpt};
 }
 // Workgroups of `threads` lanes, `per_cu` of them on every CU, no more than the rows need
 static int64_t ln_workgroups(LnShape s, int64_t rows, int threads, int per_cu) {
@@ -510,25 +616,34 @@ static int64_t ln_chunk_rows(int64_t rows, int64_t cols, int dtype) {  // of the
     return std::max<int64_t>(8, (rows + want - 1) / want);
 }
 static int64_t ln_parts(int64_t rows, int64_t cols, int dtype) {
-    const LnShape s = ln_shape(cols, dtype, true);
-    if (s.t) return ln_workgroups(s, rows, ln_backward_threads(s.vpt), 1024 / ln_backward_threads(s.vpt));
+    const LnShape s = ln_shape(cols, dtype, F8MI_FP32, true);  // (a weight of fewer bits fits where one of fp32 does, and no row of fp32 ones does not)
+    if (s.t) return ln_workgroups(s, rows, ln_backward_threads(s.t, s.vpt), LN_ROW_LANES / ln_backward_threads(s.t, s.vpt));
     const int64_t chunk = ln_chunk_rows(rows, cols, dtype);
     return (rows + chunk - 1) / chunk;
 }
 
 template <int DT, int PT, int T, int VPT>
 static int launch_ln(const LnArgs& a, bool backward) {
-    const LnShape s{T, VPT};
-    constexpr bool HAS_BACKWARD = VPT == 1 || (VPT > 2) == (DT == F8MI_FP32), HAS_FORWARD = VPT != 2;  // (ln_shape)
-    if constexpr (HAS_BACKWARD)
+    const int64_t lds = VPT > 1 ? ln_lds(a.cols, DT, PT, backward) : 0;
     if (backward) {
-        hipLaunchKernelGGL((layer_norm_backward_kernel<DT, PT, T, VPT>), dim3((unsigned)a.parts), dim3(ln_backward_threads(VPT)), 0, a.stream, a.dy, a.ld_dy, a.x, a.ld, a.rows, (int)a.cols, a.weight,
-                           a.stats, a.out, a.partial);
+        if constexpr (VPT <= (DT == F8MI_FP32 ? 4 : 2)) {  // (ln_shape)
+            const auto kernel = layer_norm_backward_kernel<DT, PT, T, VPT>;
+            if constexpr (VPT > 1) {
+                static std::atomic<uint64_t> allowed{0};
+                if (int rc = allow_big_lds(kernel, LN_MAX_LDS, allowed)) return rc;
+            }
+            hipLaunchKernelGGL(kernel, dim3((unsigned)a.parts), dim3(ln_backward_threads(T, VPT)), (unsigned)lds, a.stream, a.dy, a.ld_dy, a.x, a.ld, a.rows, (int)a.cols, a.weight, a.stats, a.out, a.partial);
+        }
         return check_hip(hipGetLastError(), "layer norm backward kernel launch");
     }
-    if constexpr (HAS_FORWARD)
-    hipLaunchKernelGGL((layer_norm_kernel<DT, PT, T, VPT>), dim3((unsigned)ln_workgroups(s, a.rows, ln_threads(T), ln_lanes(T, VPT) / ln_threads(T))), dim3(ln_threads(T)), 0, a.stream, a.x, a.ld, a.rows, (int)a.cols,
-                       a.weight, a.bias, a.eps, a.out, a.stats);
+    const auto kernel = layer_norm_kernel<DT, PT, T, VPT>;
+    if constexpr (VPT > 1) {
+        static std::atomic<uint64_t> allowed{0};
+        if (int rc = allow_big_lds(kernel, LN_MAX_LDS, allowed)) return rc;
+    }
+    const int per_cu = ln_waves_a_simd(T, VPT) * 256 / ln_threads(T);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)ln_workgroups({T, VPT}, a.rows, ln_threads(T), per_cu)), dim3(ln_threads(T)), (unsigned)lds, a.stream, a.x, a.ld, a.rows, (int)a.cols, a.weight,
+                       a.bias, a.eps, a.out, a.stats);
     return check_hip(hipGetLastError(), "layer norm kernel launch");
 }
 template <int DT, int PT>
@@ -548,13 +663,17 @@ static int launch_ln_wide(const LnArgs& a, bool backward) {
 }
 template <int DT, int PT>
 static int launch_ln_by_size(const LnArgs& a, bool backward) {
-    const LnShape s = ln_shape(a.cols, DT, backward);
+    const LnShape s = ln_shape(a.cols, DT, PT, backward);
     if (s.t == 64) return launch_ln<DT, PT, 64, 1>(a, backward);
     if (s.t == 128) return launch_ln<DT, PT, 128, 1>(a, backward);
     if (s.t == 256) return launch_ln<DT, PT, 256, 1>(a, backward);
     if (s.t == 512 && s.vpt == 1) return launch_ln<DT, PT, 512, 1>(a, backward);
-    if (s.t == 512) return s.vpt == 3 ? launch_ln<DT, PT, 512, 3>(a, backward) : launch_ln<DT, PT, 512, 4>(a, backward);
-    if (s.t == 1024) return s.vpt == 1 ? launch_ln<DT, PT, 1024, 1>(a, backward) : launch_ln<DT, PT, 1024, 2>(a, backward);
+    if constexpr (DT == F8MI_FP32)
+        if (s.t == 512) return launch_ln<DT, PT, 512, 3>(a, backward);
+    if (s.vpt == 1) return launch_ln<DT, PT, LN_ROW_LANES, 1>(a, backward);
+    if (s.vpt == 2) return launch_ln<DT, PT, LN_ROW_LANES, 2>(a, backward);
+    if (s.vpt == 3) return launch_ln<DT, PT, LN_ROW_LANES, 3>(a, backward);
+    if (s.vpt == 4) return launch_ln<DT, PT, LN_ROW_LANES, 4>(a, backward);
     return launch_ln_wide<DT, PT>(a, backward);
 }
 static int launch_ln_by_type(int dtype, int p_dtype, const LnArgs& a, bool backward) {
