@@ -993,10 +993,11 @@ def block_gemm(a: Blocks, b: Blocks, out_dtype: torch.dtype, bias: Optional[torc
     bias = _checked_bias(bias, n, out_dtype, a.data.device)
     out = torch.empty((m, n), dtype=out_dtype, device=a.data.device)
     _check_device(a.data.device)
-    ws_ptr, ws_bytes = gemm_workspace(a.data.device, m, k, n)
+    ws_bytes = lib().f8mi_block_gemm_workspace_bytes(m, n, k)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=a.data.device) if ws_bytes else None
     rc = lib().f8mi_block_gemm(a.data.data_ptr(), a.scales.data_ptr(), (transposed if transposed is not None else b).data.data_ptr(), b.scales.data_ptr(),
                                int(transposed is not None), m, n, k, out.data_ptr(), _DT[out_dtype], n, bias.data_ptr() if bias is not None else None,
-                               ws_ptr, ws_bytes, _stream(a.data))
+                               workspace.data_ptr() if workspace is not None else None, ws_bytes, _stream(a.data))
     _check(rc, "f8mi_block_gemm")
     return out
 

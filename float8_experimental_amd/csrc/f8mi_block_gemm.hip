@@ -1,5 +1,7 @@
 // Products of operands with block scales (f8mi_block.h) on 128-row tiles, and the choice of kernel.  Main loop, LDS layout and epilogue are
 // those of f8mi_gemm_mid_impl.h, the choice that of f8mi_gemm.hip; a stage brings 256 bytes of scales more for each wave, and the matrix instruction applies them.
+#include <algorithm>
+
 #include "f8mi_block_gemm.h"
 #include "f8mi_gemm_mid_impl.h"
 
@@ -40,15 +42,38 @@ static int launch_mid2(const BlockGemm& g, bool wide) {
     return launch_mid3<C_DT, false, false>(g, wide, 1, g.C, g.ldc, g.bias);
 }
 
-// k_splits > 1: the parts go to `partial` (k_splits x M x N floats) and are added by a second launch
+// k_splits > 1: the parts go to `partial` (k_splits x M x N floats, N rounded up to a multiple of four) and are added by a second launch
 int launch_block_mid(const BlockGemm& g, bool wide, int k_splits, float* partial) {
     if (k_splits > 1) {
-        if (int rc = launch_mid3<F8MI_FP32, false, false>(g, wide, k_splits, partial, g.N, nullptr)) return rc;
-        return launch_splitk_reduce(g.c_dtype, k_splits, partial, g.stream, g.M, g.N, nullptr, nullptr, g.C, g.ldc, g.bias, g.c_vec_ok);
+        const int pitch = (g.N + 3) / 4 * 4;
+        BlockGemm part = g;
+        part.c_vec_ok = 1;
+        if (int rc = g.b_tr ? launch_mid4<F8MI_FP32, 4, true, false>(part, k_splits, partial, pitch, nullptr) : launch_mid4<F8MI_FP32, 4, false, false>(part, k_splits, partial, pitch, nullptr)) return rc;
+        return launch_splitk_reduce(g.c_dtype, k_splits, partial, pitch, g.stream, g.M, g.N, nullptr, nullptr, g.C, g.ldc, g.bias, g.c_vec_ok);
     }
     if (g.c_dtype == F8MI_BF16) return launch_mid2<F8MI_BF16>(g, wide);
     if (g.c_dtype == F8MI_FP16) return launch_mid2<F8MI_FP16>(g, wide);
     return launch_mid2<F8MI_FP32>(g, wide);
+}
+
+// Into how many parts a long contraction of at most 128 tiles of 128 x 128 is split so that the CUs get one each; 0: it is not.  Estimates: a
+// round of tiles takes 5 us and 2.4 ns for each unit of k with few tiles, 4.2 with one on every CU; the split costs another launch and the parts
+// written and read.  Any number of parts, of whole steps, and any width, unlike with one scale for an operand (whole / split, us:
+// 640 x 427 over 27648: 72 / 23; 128 x 5632 over 16640: 45 / 25; 267 x 4522 over 9728: 29 / 25; 2002 x 256 over 13312: 36 / 20; 512 x 256 over 4096: 14.2 / 11.9;
+// the number taken is within 5 % of the best of 2 - 8 at each).
+static int block_k_splits(int64_t m, int64_t n, int64_t k, bool b_tr, int64_t ws_bytes) {
+    if (use_mid_tiles(m, n, k) != 1 || m <= 16) return 0;
+    const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128), part = m * ((n + 3) / 4 * 4) * 4;
+    if (tiles > 128) return 0;
+    const auto round = [&](int s) { return 5.0 + (2.4 + 1.8 * (double)(tiles * s) / 256.0) * 1e-3 * (double)((k / 128 + s - 1) / s * 128); };
+    const double whole = round(1), few = !b_tr && use_skinny(m, n, k) ? skinny_time_us(m, n, k) : whole;
+    double best_time = 0.9 * std::min(whole, few);  // the estimates are not better than that
+    int best = 0;
+    for (int s = 2; s <= 8 && tiles * s <= 256 && k / s >= 1024 && s * part <= ws_bytes; s++) {
+        const double t = round(s) + 4.0 + (double)s * (double)part * 2.0 / 5e6;
+        if (t < best_time) { best_time = t; best = s; }
+    }
+    return best;
 }
 
 }  // namespace f8mi
@@ -56,8 +81,9 @@ int launch_block_mid(const BlockGemm& g, bool wide, int k_splits, float* partial
 using namespace f8mi;
 
 extern "C" int64_t f8mi_block_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    const int splits = m > 0 && n > 0 && k > 0 ? pick_k_splits(m, n, k, F8MI_GEMM_WORKSPACE_BYTES) : 0;
-    return splits > 1 ? splits * m * n * 4 : 0;
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    const int as_is = block_k_splits(m, n, k, false, F8MI_GEMM_WORKSPACE_BYTES), transposed = n % 128 == 0 ? block_k_splits(m, n, k, true, F8MI_GEMM_WORKSPACE_BYTES) : 0;
+    return std::max(as_is, transposed) * m * ((n + 3) / 4 * 4) * 4;
 }
 
 extern "C" int f8mi_block_gemm(const void* a, const void* a_scales, const void* bt, const void* b_scales, int b_transposed, int64_t m, int64_t n, int64_t k,
@@ -74,8 +100,8 @@ extern "C" int f8mi_block_gemm(const void* a, const void* a_scales, const void* 
     const BlockGemm g{(const uint8_t*)a, (const uint8_t*)a_scales, (const uint8_t*)bt, (const uint8_t*)b_scales, (int)m, (int)n, (int)k, c, ldc, bias_dev, c_dtype,
                       b_transposed != 0, (uintptr_t)c % (c_dtype == F8MI_FP32 ? 4 : 2) == 0, (hipStream_t)stream_, (int)m};
     ProfScope prof(F8MI_K_GEMM, 2.0 * (double)m * (double)n * (double)k, g.stream);
-    const int splits = workspace && !b_transposed ? pick_k_splits(m, n, k, workspace_bytes) : 0;
-    if (splits > 1) return launch_block_mid(g, use_mid_tiles(m, n, k) == 2, splits, (float*)workspace);
+    const int splits = workspace ? block_k_splits(m, n, k, b_transposed != 0, workspace_bytes) : 0;
+    if (splits > 1) return launch_block_mid(g, false, splits, (float*)workspace);
     if (!b_transposed && use_skinny(m, n, k)) return launch_block_few(g);
     if (const int mid = use_mid_tiles(m, n, k)) return launch_block_mid(g, mid == 2, 1, nullptr);
     if (k < 384) return launch_block_mid(g, true, 1, nullptr);

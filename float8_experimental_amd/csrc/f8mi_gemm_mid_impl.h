@@ -134,7 +134,9 @@ __device__ __forceinline__ void gemm_mid_tile(
     const int m0 = tm * MID_TILE_M, n0 = tn * Cfg::TILE_N;
     // k_splits > 1 (host: fp32 output, no bias): takes the split-th part of k and writes its partial sums,
     // unscaled, to the split-th M x ldc slab of C; a second kernel adds the slabs in a fixed order.
-    const int K_part = K / k_splits;
+    // (Block scales: parts may differ by a step.)
+    const int first_step = BLK ? split * (K / 128) / k_splits : 0;
+    const int K_part = BLK ? ((split + 1) * (K / 128) / k_splits - first_step) * 128 : K / k_splits;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
@@ -157,7 +159,7 @@ __device__ __forceinline__ void gemm_mid_tile(
         if constexpr (B_TR) b_voff[i] = mid_tr_voff<Cfg::TILE_N>(wave * 2 * Cfg::BI + i, ldb, b_unit, n0 / 64, N / 64 - 1);
         else b_voff[i] = (uint32_t)(min((wave * Cfg::BI + i) * 16 + (lane >> 2), N - 1 - n0) * ldb) + piece;
     }
-    const int64_t k0 = (int64_t)split * K_part;
+    const int64_t k0 = BLK ? (int64_t)first_step * 128 : (int64_t)split * K_part;
     const uint8_t* a_ptr = A_TR ? A + (int64_t)(m0 / 64) * a_unit + k0 * lda : A + (int64_t)m0 * lda + k0 / 64 * a_unit;
     const uint8_t* b_ptr = B_TR ? Bt + (int64_t)(n0 / 64) * b_unit + k0 * ldb : Bt + (int64_t)n0 * ldb + k0 / 64 * b_unit;
     // Block scales, 256 bytes a wave: lanes 0 - 31 bring those of A's 128 rows, the others those of the 128 rows of Bt that hold the wave's

@@ -443,8 +443,8 @@ inline int pick_k_splits(int64_t m, int64_t n, int64_t k, int64_t ws_bytes) {
 int launch_gemm_mid_splitk(int a_fmt, int b_fmt, int c_dtype, bool wide, int k_splits, float* partial, hipStream_t stream, const uint8_t* A,
                            int64_t lda, int64_t a_unit, const uint8_t* Bt, int64_t ldb, int64_t b_unit, int M, int N, int K, const float* sa,
                            const float* sb, void* C, int64_t ldc, const void* bias, int c_vec_ok);
-// The sum of the parts of a split product, for operands with block scales too (sa and sb null).
-int launch_splitk_reduce(int c_dtype, int k_splits, const float* partial, hipStream_t stream, int M, int N, const float* sa, const float* sb, void* C,
+// The sum of the parts of a split product, whose rows are `pitch` floats, for operands with block scales too (sa and sb null).
+int launch_splitk_reduce(int c_dtype, int k_splits, const float* partial, int pitch, hipStream_t stream, int M, int N, const float* sa, const float* sb, void* C,
                          int64_t ldc, const void* bias, int c_vec_ok);
 int launch_gemm_skinny(int a_fmt, int b_fmt, int c_dtype, hipStream_t stream, const uint8_t* A, int64_t lda, int64_t a_unit,
                        const uint8_t* Bt, int64_t ldb, int64_t b_unit, int M, int N, int K, const float* sa, const float* sb, void* C,

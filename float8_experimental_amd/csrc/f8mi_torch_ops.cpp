@@ -127,7 +127,7 @@ f8mi_block_cast_job job_of(const Rows& x, bool square, const Blocks& a, const Bl
 at::Tensor block_gemm(const at::Tensor& like, const Blocks& a, const Blocks& b, bool transposed, int64_t m, int64_t n, int64_t k, at::ScalarType type, const at::Tensor& bias = {}) {
     const int64_t kp = (k + 127) / 128 * 128;
     at::Tensor c = at::empty({m, n}, like.options().dtype(type).memory_format(at::MemoryFormat::Contiguous));
-    const int64_t bytes = transposed ? 0 : L.block_gemm_workspace_bytes(m, n, kp);
+    const int64_t bytes = L.block_gemm_workspace_bytes(m, n, kp);
     const at::Tensor ws = bytes ? at::empty({bytes / 4}, like.options().dtype(at::kFloat)) : at::Tensor();
     check(L.block_gemm(a.data, a.scales, b.data, b.scales, transposed, m, n, kp, c.data_ptr(), dtype_code(type), n, ptr(bias), ptr(ws), bytes, stream_of(c)), "f8mi_block_gemm");
     return c;

@@ -481,7 +481,7 @@ int f8mi_block_cast(const f8mi_block_cast_job* jobs, int count, void* stream);
 /* c [m][n] = a bt^T + bias, added in fp32 and rounded once.  a: copy of m rows, bt: copy of n rows, both contracting over k (padded: a
  * multiple of 128).  b_transposed: bt is the copy of another product instead, of k rows contracting over n (n a multiple of 128), read transposed;
  * b_scales are those of n rows contracting over k all the same.  bias: n values of c_dtype or NULL.  workspace (16-byte aligned, may be
- * NULL): with F8MI_GEMM_WORKSPACE_BYTES of it a long contraction of few tiles is split over workgroups, the parts added in a fixed order. */
+ * NULL): with f8mi_block_gemm_workspace_bytes() of it a long contraction of few tiles is split over workgroups, the parts added in a fixed order. */
 int f8mi_block_gemm(const void* a, const void* a_scales, const void* bt, const void* b_scales, int b_transposed, int64_t m, int64_t n, int64_t k,
                     void* c, int c_dtype, int64_t ldc, const void* bias_dev, void* workspace, int64_t workspace_bytes, void* stream);
 /* A whole linear of at most 16 rows and F8MI_FEW_ROWS_ELEMS activations (k rounded up to a multiple of 128) in one kernel: the values of
@@ -490,7 +490,7 @@ int f8mi_block_gemm(const void* a, const void* a_scales, const void* bt, const v
 int f8mi_block_linear_few_rows(const void* x, int64_t ldx, int dtype, const void* w, const void* w_scales, int64_t m, int64_t n, int64_t k, void* c, int64_t ldc,
                                const void* bias_dev, void* stream);
 
-/* Bytes of workspace that this product makes use of (0: none).  Needs no GPU. */
+/* Bytes of workspace that this product, b transposed or not, makes use of (0: none; at most F8MI_GEMM_WORKSPACE_BYTES).  Needs no GPU. */
 int64_t f8mi_block_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
 
 /* ---- layer norm over the last dimension ---------------------------------------------------------------------------------------------

@@ -375,3 +375,24 @@ def test_one_kernel_linears_have_the_values_of_cast_and_product(nat, m, k, n):
         product_close(got, a.dequant().cpu(), b.dequant().cpu(), bias)
         if nat.lib().f8mi_block_gemm_workspace_bytes(m, n, nat.padded_k(k)) == 0:  # both few-row kernels split k the same way
             assert torch.equal(got, want)
+
+
+# (m, n, k): parts of different numbers of steps, outputs that are multiples of nothing, one tile and many
+@pytest.mark.parametrize("m,n,k", [(400, 1, 9000), (300, 131, 12345), (640, 427, 9100), (257, 2050, 8200), (300, 1023, 20000), (2048, 129, 8191)])
+def test_products_split_over_k(nat, m, n, k):
+    assert nat.lib().f8mi_block_gemm_workspace_bytes(m, n, nat.padded_k(k)) > 0
+    for dtype in (BF16, FP16, FP32):
+        x, w, bias = values((m, k), dtype, m + k).cuda(), values((n, k), dtype, n + k, k**-0.5).cuda(), values((n,), dtype, 7).cuda()
+        (a, _), (b, _) = nat.block_cast([(x, False, True, False), (w, True, True, False)])
+        y = nat.block_gemm(a, b, dtype, bias)
+        product_close(y, a.dequant().double().cpu(), b.dequant().double().cpu(), bias)
+        assert torch.equal(y, nat.block_gemm(a, b, dtype, bias))
+
+
+@pytest.mark.parametrize("m,n,k", [(128, 9088, 256), (200, 16640, 384), (77, 27648, 128)])
+def test_products_split_over_k_that_read_the_weight_transposed(nat, m, n, k):
+    assert nat.lib().f8mi_block_gemm_workspace_bytes(m, k, n) > 0
+    g, w = values((m, n), BF16, m).cuda(), values((n, k), BF16, n).cuda()
+    ((a, _),) = nat.block_cast([(g, False, True, False)])
+    ((b, bt),) = nat.block_cast([(w, True, True, True)])
+    product_close(nat.block_gemm(a, nat.Blocks(None, bt.scales, k, n), BF16, transposed=b), a.dequant().double().cpu(), bt.dequant().double().cpu())
