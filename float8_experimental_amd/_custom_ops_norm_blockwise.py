@@ -1,5 +1,6 @@
 """The blockwise scaled linear and layer norm as ``torch.library`` custom ops, for ``torch.compile`` and whoever else has to see operators: opaque
 nodes with known shapes, one per direction, with the numbers of the eager path."""
+import contextlib
 from typing import Optional, Tuple
 
 import torch
@@ -89,8 +90,40 @@ class _BlockwiseLinearFn(torch.autograd.Function):
         return dx if need_dx else None, dw if need_dw else None, db if need_db else None
 
 
+# What a trace holds: one operator with its history, the same with gradients and without, that can be saved (an autograd function cannot).
+_traced = torch.library.Library("f8mi", "FRAGMENT")
+_traced.define("blockwise_linear(Tensor x2, Tensor weight, Tensor? bias) -> Tensor")
+_traced.define("layer_norm(Tensor x2, Tensor? weight, Tensor? bias, float eps) -> Tensor")
+
+
+@contextlib.contextmanager
+def _untraced():
+    """What an operator does is not in the trace that holds the operator."""
+    state = torch._C._get_tracing_state()
+    torch._C._set_tracing_state(None)
+    try:
+        yield
+    finally:
+        torch._C._set_tracing_state(state)
+
+
+def _records(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+@torch.library.impl(_traced, "blockwise_linear", "CompositeImplicitAutograd")
+def _traced_blockwise_linear(x2, weight, bias):
+    with _untraced():
+        y = _native.ops().blockwise_linear(x2, weight, bias)
+        return _blockwise_linear(x2, weight, bias) if y is None else y
+
+
+def _blockwise_linear(x2: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    return _BlockwiseLinearFn.apply(x2, weight, bias) if _records(x2, weight, bias) else blockwise_linear_fwd(x2, weight, bias, False, False)[0]
+
+
 def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
-    y = _BlockwiseLinearFn.apply(x.reshape(-1, x.shape[-1]), weight, bias)
+    y = (torch.ops.f8mi.blockwise_linear if torch.jit.is_tracing() else _blockwise_linear)(x.reshape(-1, x.shape[-1]), weight, bias)
     return y.reshape(*x.shape[:-1], weight.shape[0])
 
 
@@ -99,10 +132,17 @@ def _blockwise_inference_linear(x2: torch.Tensor, data: torch.Tensor, scales: to
     n = data.shape[1]
     if x2.shape[0] == 0:
         return x2.new_empty((0, n))
-    y = _native.ops().blockwise_inference_linear(x2.detach(), data, scales, n, x2.shape[1], bias)
-    if y is None:
-        raise _native.Float8NativeError("blockwise_inference_linear: a weight of another shape or device than its scales")
-    return y
+    k = x2.shape[1]
+    y = _native.ops().blockwise_inference_linear(x2.detach(), data, scales, n, k, bias)
+    if y is not None:
+        return y
+    if data.dtype is not _e4m3 or data.shape != _data_shape(n, k) or scales.dtype is not torch.uint8 or scales.shape != _scales_shape(n, k) or not (
+            x2.device == data.device == scales.device and data.is_contiguous() and scales.is_contiguous()):
+        raise _native.Float8NativeError(f"blockwise_inference_linear: {k} in_features on {x2.device} for a weight {tuple(data.shape)} ({data.dtype}) on {data.device} with scales "
+                                        f"{tuple(scales.shape)} ({scales.dtype}) on {scales.device}")
+    # a mode that is still on inside the operator
+    ((x8, _),) = _native.block_cast([(x2.detach(), False, True, False)])
+    return _native.block_gemm(x8, _native.Blocks(data, scales, n, k), x2.dtype, None if bias is None else bias.to(x2.dtype).contiguous())
 
 
 @_blockwise_inference_linear.register_fake
@@ -157,6 +197,18 @@ class _LayerNormFn(torch.autograd.Function):
         return tuple(g if need else None for g, need in zip((dx, dw, db), ctx.needs_input_grad)) + (None,)
 
 
+@torch.library.impl(_traced, "layer_norm", "CompositeImplicitAutograd")
+def _traced_layer_norm(x2, weight, bias, eps):
+    with _untraced():
+        y = _native.ops().layer_norm(x2, x2.shape[1], weight, bias, eps)
+        return _layer_norm(x2, weight, bias, eps) if y is None else y
+
+
+def _layer_norm(x2: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float) -> torch.Tensor:
+    return _LayerNormFn.apply(x2, weight, bias, eps) if _records(x2, weight, bias) else layer_norm_fwd(x2, weight, bias, eps)[0]
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], cols: int, eps: float) -> torch.Tensor:
     flat = lambda p: None if p is None else p.reshape(-1)
-    return _LayerNormFn.apply(x.reshape(-1, cols), flat(weight), flat(bias), eps).reshape(x.shape)
+    y = (torch.ops.f8mi.layer_norm if torch.jit.is_tracing() else _layer_norm)(x.reshape(-1, cols), flat(weight), flat(bias), eps)
+    return y.reshape(x.shape)

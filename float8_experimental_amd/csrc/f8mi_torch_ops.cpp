@@ -3,19 +3,22 @@
 // interpreter.  Host code only.
 //
 // Every function returns None, without having queued or allocated anything, for tensors that it does not take (subclasses, other devices or
-// types): the caller then goes through the registered operators, or raises.  Workspaces are temporaries of torch's caching allocator, which
+// types) and while somebody has to see operators (modes, traces): the caller then goes through the registered operators, or raises.  Workspaces are temporaries of torch's caching allocator, which
 // hands their memory out again in stream order: calls on any number of threads, streams and captures share nothing.
 #include <dlfcn.h>
 
 #include <optional>
 
 #include <ATen/ATen.h>
+#include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
@@ -57,9 +60,20 @@ int dtype_code(at::ScalarType t) {
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// Undefined: not taken.  A plain tensor (or Parameter) of a type that the kernels read, on the current device, whose memory holds its values
+// Whether somebody has to see operators: a dispatch or function mode, a trace (functional transforms show in the tensors).  A kernel's launch is none, and
+// a trace would hold the allocation of its output alone.  torch.set_default_device is a function mode that asks for nothing.
+PyObject* device_context = nullptr;  // torch.utils._device.DeviceContext
+bool watched() {
+    if (c10::impl::TorchDispatchModeTLS::any_modes_set() || at::tracer::impl::is_dispatch_enabled()) return true;
+    if (at::impl::torch_function_mode_enabled())
+        for (int64_t i = 0; i < at::impl::PythonTorchFunctionTLS::stack_len(); i++)
+            if ((PyObject*)Py_TYPE(at::impl::PythonTorchFunctionTLS::get_stack_at(i)->ptr(getPyInterpreter())) != device_context) return true;
+    return false;
+}
+
+// Undefined: not taken.  A plain tensor (or Parameter) of a type that the kernels read, on `device`, whose memory holds its values
 at::Tensor plain(PyObject* o, int device) {
-    if (!THPVariable_CheckExact(o) || c10::impl::TorchDispatchModeTLS::any_modes_set()) return {};
+    if (!THPVariable_CheckExact(o)) return {};
     const at::Tensor& t = THPVariable_Unpack(o);
     using K = c10::DispatchKey;
     constexpr c10::DispatchKeySet others({K::Python, K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Batched, K::Functionalize, K::Negative, K::ZeroTensor});
@@ -331,10 +345,11 @@ bool optional(PyObject* o, int device, at::Tensor& t) {
 }
 bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
-// The current device as torch has it for this thread, without a call into Python.
-int current_device() {
+// The device whose tensors a call takes: the current one as torch has it for this thread, without a call into Python.  -1, which no tensor is on, where
+// nothing is taken.
+int device_taken() {
     static const bool any = c10::hip::device_count() > 0;
-    return any ? (int)c10::hip::current_device() : -1;
+    return any && !watched() ? (int)c10::hip::current_device() : -1;
 }
 
 // blockwise_linear(x [..., k], weight [n, k], bias or None) -> y, with its history, or None (also for shapes that do not fit: the caller says what is
@@ -342,7 +357,7 @@ int current_device() {
 PyObject* blockwise_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!expect(n_args, 3, "blockwise_linear")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int device = current_device();
+        const int device = device_taken();
         const at::Tensor x = plain(a[0], device), w = plain(a[1], device);
         at::Tensor bias;
         if (!x.defined() || !w.defined() || !optional(a[2], device, bias)) Py_RETURN_NONE;
@@ -369,7 +384,7 @@ bool one_kernel_pays(int64_t m, int64_t n, int64_t kp, int dt) {
 PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!expect(n_args, 6, "blockwise_inference_linear")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int device = current_device();
+        const int device = device_taken();
         const int64_t n = PyLong_AsLongLong(a[3]), k = PyLong_AsLongLong(a[4]);
         const at::Tensor x = plain(a[0], device);
         at::Tensor bias;
@@ -415,7 +430,7 @@ PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n
 PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!expect(n_args, 5, "layer_norm")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int device = current_device();
+        const int device = device_taken();
         const at::Tensor x = plain(a[0], device);
         at::Tensor w, b;
         if (!x.defined() || !optional(a[2], device, w) || !optional(a[3], device, b)) Py_RETURN_NONE;
@@ -450,7 +465,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!expect(n_args, 4, "grad_clip")) return nullptr;
     return guarded([&]() -> PyObject* {
-        const int kind = (int)PyLong_AsLong(a[2]), device = current_device();
+        const int kind = (int)PyLong_AsLong(a[2]), device = device_taken();
         const double max_norm = PyFloat_AsDouble(a[3]);
         const bool of_params = PyUnicode_Check(a[1]) && PyUnicode_CompareWithASCIIString(a[1], "grads") == 0;
         const bool to_new = !PyUnicode_Check(a[1]);
@@ -530,6 +545,12 @@ PyObject* load(PyObject*, PyObject* args) {
     if (missing) {
         L.last_error = nullptr;
         return PyErr_Format(PyExc_ImportError, "%s does not export %s", path, missing);
+    }
+    THPObjectPtr module(PyImport_ImportModule("torch.utils._device"));
+    device_context = module ? PyObject_GetAttrString(module.get(), "DeviceContext") : nullptr;
+    if (!device_context) {
+        L.last_error = nullptr;
+        return nullptr;
     }
     Py_INCREF(error);
     native_error = error;

@@ -1,4 +1,5 @@
 """The global norm of many gradients and their clipping, in two launches for each 96 tensors (csrc/f8mi_grad_clip.hip)."""
+import functools
 import math
 from typing import Iterable, List, Optional, Tuple, Union
 
@@ -45,10 +46,23 @@ def _call(tensors: List[torch.Tensor], what, kind: int, max_norm: float):
 
 def _must(result):
     if result is None:
-        raise _native.Float8NativeError("gradient clipping under a dispatch mode or a functional transform is not implemented")
+        raise _native.Float8NativeError("gradient clipping under a dispatch mode, a trace or a functional transform is not implemented")
     return result
 
 
+def _shown_to_function_modes(fn):
+    """A ``TorchFunctionMode`` sees a call of ``fn`` as one operation."""
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        if not torch.compiler.is_compiling() and torch._C._is_torch_function_mode_enabled() and _native._function_mode_active():
+            return torch.overrides.handle_torch_function(call, (), *args, **kwargs)
+        return fn(*args, **kwargs)
+
+    return call
+
+
+@_shown_to_function_modes
 def grad_norm(grads: Iterable[torch.Tensor], norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """The norm (2, 1 or inf) of all values of all tensors as if they were one vector: a 0-dim float32 tensor.  Sums are kept in 64 bits
     and have a fixed order."""
@@ -59,6 +73,7 @@ def grad_norm(grads: Iterable[torch.Tensor], norm_type: float = 2.0, error_if_no
     return norm
 
 
+@_shown_to_function_modes
 def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
                out_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, List[torch.Tensor]]:
     """(norm, ``[g * min(1, max_norm / (norm + 1e-6)) for g in grads]``) in new tensors of ``out_dtype`` (default: each gradient's own), for
@@ -71,6 +86,7 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
     return _call(grads, out_dtype, kind, float(max_norm)) or _must(_call(_readable(grads), out_dtype, kind, float(max_norm)))
 
 
+@_shown_to_function_modes
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_``: scales the gradients of ``parameters`` in place so that their norm as one vector is at most
