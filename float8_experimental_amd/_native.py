@@ -316,6 +316,12 @@ def operators_are_watched() -> bool:
             or (torch._C._len_torch_function_stack() != 0 and _function_mode_active()) or torch.jit.is_tracing())
 
 
+def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises for a tensor with a forward-mode derivative, which an operator without one would drop."""
+    if torch.autograd.forward_ad._current_level >= 0 and any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 _checked_devices = set()
 
 

@@ -71,13 +71,14 @@ bool watched() {
     return false;
 }
 
-// Undefined: not taken.  A plain tensor (or Parameter) of a type that the kernels read, on `device`, whose memory holds its values
+// Undefined: not taken.  A plain tensor (or Parameter) of a type that the kernels read, on `device`, whose memory holds its values, without a forward-mode
+// derivative (which would be dropped)
 at::Tensor plain(PyObject* o, int device) {
     if (!THPVariable_CheckExact(o)) return {};
     const at::Tensor& t = THPVariable_Unpack(o);
     using K = c10::DispatchKey;
     constexpr c10::DispatchKeySet others({K::Python, K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Batched, K::Functionalize, K::Negative, K::ZeroTensor});
-    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(others) && t.get_device() == device && dtype_code(t.scalar_type()) >= 0 ? t : at::Tensor();
+    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(others) && t.get_device() == device && dtype_code(t.scalar_type()) >= 0 && !t._fw_grad(0).defined() ? t : at::Tensor();
 }
 
 // A matrix as the kernels read it: unit column stride, `ld` from row to row (0: the same row throughout); copied where its layout needs it.

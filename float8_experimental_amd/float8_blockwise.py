@@ -50,6 +50,7 @@ def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         y = _native.ops().blockwise_linear(x, weight, bias)
         if y is not None:
             return y
+        _native.refuse_tangents("blockwise_linear", x, weight, bias)
     if weight.dim() != 2:
         raise ValueError(f"blockwise_linear: weight of shape {tuple(weight.shape)} is no matrix")
     n, k = weight.shape
@@ -105,6 +106,7 @@ class Float8BlockwiseInferenceLinear(nn.Module):
             y = _native.ops().blockwise_inference_linear(input, self.weight_data, self.weight_scales, self.out_features, self.in_features, self.bias)
             if y is not None:
                 return y
+            _native.refuse_tangents("Float8BlockwiseInferenceLinear", input, self.bias)
         _checked(input, self.out_features, self.in_features, self.bias, "Float8BlockwiseInferenceLinear")
         if torch.is_grad_enabled() and input.requires_grad:
             raise RuntimeError("Float8BlockwiseInferenceLinear has no backward pass: call it under torch.no_grad() or torch.inference_mode()")

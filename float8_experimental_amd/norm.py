@@ -21,6 +21,7 @@ def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], wei
         y = _native.ops().layer_norm(x, normalized_shape, weight, bias, eps)
         if y is not None:
             return y
+        _native.refuse_tangents("layer_norm", x, weight, bias)
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     _native._require_gpu(x, "x")
     if x.dtype not in _HP_DTYPES:
