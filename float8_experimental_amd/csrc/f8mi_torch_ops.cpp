@@ -81,6 +81,13 @@ at::Tensor plain(PyObject* o, int device) {
     return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(others) && t.get_device() == device && dtype_code(t.scalar_type()) >= 0 && !t._fw_grad(0).defined() ? t : at::Tensor();
 }
 
+// What hooks on saved tensors hand back (they hand back what they like) is what was saved, or the kernels would read other memory
+bool as_saved(const at::Tensor& t, const c10::Device& device, at::ScalarType type, at::IntArrayRef sizes) {
+    using K = c10::DispatchKey;
+    constexpr c10::DispatchKeySet others({K::Python, K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Batched, K::Functionalize, K::ZeroTensor});
+    return t.defined() && t.device() == device && t.layout() == at::kStrided && t.scalar_type() == type && t.sizes() == sizes && !t.key_set().has_any(others);
+}
+
 // A matrix as the kernels read it: unit column stride, `ld` from row to row (0: the same row throughout); copied where its layout needs it.
 struct Rows {
     at::Tensor t;
@@ -234,8 +241,8 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
         TORCH_CHECK((!need_dx || kept_dx) && (!need_dw || kept_dw), "blockwise_linear: a gradient is asked for that the forward pass was not told of");
         const Kept k_at(m, k, n, kept_dx, kept_dw);
         const at::Tensor& kept = saved[0];
-        if (need_dx || need_dw)  // (hooks on saved tensors hand back what they like)
-            TORCH_CHECK(kept.defined() && kept.is_cuda() && kept.is_contiguous() && kept.scalar_type() == at::kByte && kept.numel() == k_at.parts.bytes, "blockwise_linear: what was saved for backward is not what came back");
+        if (need_dx || need_dw)
+            TORCH_CHECK(as_saved(kept, grads[0].device(), at::kByte, {k_at.parts.bytes}) && kept.is_contiguous(), "blockwise_linear: what was saved for backward is not what came back");
         Parts parts;
         const BlocksAt g8_at = need_dx ? BlocksAt(parts, m, n) : BlocksAt(), gt_at = need_dw ? BlocksAt(parts, n, m) : BlocksAt();
         const int64_t sum_rows = (m + 127) / 128, sums_at = need_db ? parts.take(sum_rows * n * 4) : 0;
@@ -278,6 +285,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         at::Tensor stats;
         at::Tensor y = compute(x, weight, bias, cols, eps, &stats);
         ctx->save_for_backward({x, weight, stats});
+        ctx->saved_data["x_shape"] = x.sizes().vec();
+        ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
         ctx->saved_data["cols"] = cols;
         ctx->saved_data["has_weight"] = weight.defined();
         ctx->saved_data["has_bias"] = bias.defined();
@@ -294,12 +303,16 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         if (!grads[0].defined() || !(need_dx || need_dw || need_db)) return {dx, dw, db, at::Tensor(), at::Tensor()};
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &stats = saved[2];
-        const c10::DeviceGuard guard(x.device());
+        const c10::DeviceGuard guard(grads[0].device());
         const at::AutoDispatchBelowADInplaceOrView below;
         const int64_t cols = ctx->saved_data["cols"].toInt();
         const at::ScalarType pt = (at::ScalarType)ctx->saved_data["p_type"].toInt();
+        TORCH_CHECK(as_saved(x, grads[0].device(), (at::ScalarType)ctx->saved_data["x_type"].toInt(), ctx->saved_data["x_shape"].toIntVector()) &&
+                        as_saved(stats, grads[0].device(), at::kFloat, {x.numel() / cols, 2}) && stats.is_contiguous() && !stats.is_neg() && saved[1].defined() == has_weight &&
+                        (!has_weight || as_saved(saved[1], grads[0].device(), pt, ctx->saved_data["w_shape"].toIntVector())),
+                    "layer_norm: what was saved for backward is not what came back");
         const Rows r(x, cols), dy(grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type()), cols);
-        const at::Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
+        const at::Tensor w = has_weight ? saved[1].resolve_neg().contiguous() : saved[1];
         if (need_dx) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
         if (need_dw) dw = at::empty(ctx->saved_data["w_shape"].toIntVector(), x.options().dtype(pt));
         if (need_db) db = at::empty(ctx->saved_data["b_shape"].toIntVector(), x.options().dtype(pt));
