@@ -100,57 +100,13 @@ class Float8BlockwiseInferenceLinear(nn.Module):
         self.bias = None if bias is None else nn.Parameter(bias, requires_grad=False)
 
     def _apply(self, fn, recurse=True):
-        # to(dtype), half() and the like convert buffers of floating types, which e4m3 is one of; type() converts all.  What is kept here moves, but its
-        # type is what it stands in
+        # to(dtype), half() and the like convert buffers of floating types, e4m3 among them, and type() all of them: the weight moves, and stays what it is
         kept = {name: self._buffers[name] for name in ("weight_data", "weight_scales")}
         super()._apply(fn, recurse)
         for name, t in kept.items():
             if self._buffers[name].dtype is not t.dtype:
                 self._buffers[name] = t.to(self._buffers[name].device)
         return self
-
-    def forward(self, input: torch.Tensor) -> torch.Tensor:
-        return blockwise_linear(input, self.weight, self.bias)
-
-    def extra_repr(self):
-        return f'{super().extra_repr()}, scaling="i:blk,w:blk,go:blk"'
-
-    @classmethod
-    def from_float(cls, mod: nn.Linear, config=None) -> "Float8BlockwiseLinear":
-        """A layer sharing ``mod``'s parameters."""
-        if config is not None and config.emulate:
-            raise NotImplementedError("blockwise scaling has no emulated products")
-        if config is not None and config.enable_fsdp_float8_all_gather:
-            raise NotImplementedError("blockwise scaling has no weight scales to compute ahead of the forward pass")
-        with torch.device("meta"):
-            new_mod = cls(mod.in_features, mod.out_features, bias=False)
-        new_mod.weight, new_mod.bias = mod.weight, mod.bias
-        new_mod.train(mod.training)
-        return new_mod
-
-
-class Float8BlockwiseInferenceLinear(nn.Module):
-    """A linear whose weight is kept as block-scaled e4m3, one byte a value and one for each 128 x 128 of them (repeated for its rows); the activations
-    are cast per call.  Construct through ``from_float`` / ``quantize_to_float8``.
-
-    ``weight_data`` [padded in_features / 64, out_features, 64] and ``weight_scales`` are buffers in the placement that the products read
-    (``f8mi_block_gemm`` of include/f8mi.h); ``dequantized_weight`` gives the values back."""
-
-    def __init__(self, in_features: int, out_features: int, bias: Optional[torch.Tensor] = None, device=None):
-        super().__init__()
-        self.in_features, self.out_features = in_features, out_features
-        blocks = _native._blocks_alloc(out_features, in_features, device)
-        self.register_buffer("weight_data", blocks.data)
-        self.register_buffer("weight_scales", blocks.scales)
-        self.bias = None if bias is None else nn.Parameter(bias, requires_grad=False)
-
-    def _apply(self, fn, recurse=True):
-        # to(dtype), half() and the like convert what is of a floating type, which e4m3 is: the weight goes through as the bytes that it is
-        self.weight_data = self.weight_data.view(torch.uint8)
-        try:
-            return super()._apply(fn, recurse)
-        finally:
-            self.weight_data = self.weight_data.view(torch.float8_e4m3fn)
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         if torch.is_autocast_enabled():
