@@ -30,8 +30,8 @@ def blockwise_linear_fwd(x2: torch.Tensor, weight: torch.Tensor, bias: Optional[
     (m, k), n = x2.shape, weight.shape[0]
     one = _one_weight_copy(k, n)
     empty = lambda dt: torch.empty(0, dtype=dt, device=x2.device)
-    if m == 0:
-        return (x2.new_empty((0, n)), empty(_e4m3), empty(torch.uint8), empty(_e4m3), empty(torch.uint8))
+    if m == 0:  # nothing is read in backward, but the shapes are those of any number of tokens
+        return _blockwise_linear_shapes(x2, weight, need_dx, need_dw)
     with _native.transient_workspaces():
         (x8, x8t), (w8, w8t) = _native.block_cast([(x2, False, True, need_dw), (weight, True, True, need_dx and ("scales" if one else True))])
         y = _native.block_gemm(x8, w8, x2.dtype, None if bias is None else bias.to(x2.dtype).contiguous())
@@ -39,13 +39,17 @@ def blockwise_linear_fwd(x2: torch.Tensor, weight: torch.Tensor, bias: Optional[
             (w8.data if one else w8t.data) if need_dx else empty(_e4m3), w8t.scales if need_dx else empty(torch.uint8))
 
 
-@blockwise_linear_fwd.register_fake
-def _(x2, weight, bias, need_dx, need_dw):
+def _blockwise_linear_shapes(x2, weight, need_dx, need_dw):
     (m, k), n = x2.shape, weight.shape[0]
     make = lambda shape, dt, wanted: torch.empty(shape if wanted else (0,), dtype=dt, device=x2.device)
     w_shape = _data_shape(n, k) if _one_weight_copy(k, n) else _data_shape(k, n)
     return (torch.empty((m, n), dtype=x2.dtype, device=x2.device), make(_data_shape(k, m), _e4m3, need_dw), make(_scales_shape(k, m), torch.uint8, need_dw),
             make(w_shape, _e4m3, need_dx), make(_scales_shape(k, n), torch.uint8, need_dx))
+
+
+@blockwise_linear_fwd.register_fake
+def _(x2, weight, bias, need_dx, need_dw):
+    return _blockwise_linear_shapes(x2, weight, need_dx, need_dw)
 
 
 @torch.library.custom_op("f8mi::blockwise_linear_bwd", mutates_args=())
