@@ -173,16 +173,17 @@ def _(x2, weight, bias, eps):
 
 
 @torch.library.custom_op("f8mi::layer_norm_bwd", mutates_args=())
-def layer_norm_bwd(dy2: torch.Tensor, x2: torch.Tensor, weight: Optional[torch.Tensor], p_dtype: torch.dtype, stats: torch.Tensor) -> Tuple[
-        torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dx, dweight, dbias)"""
-    return _native.layer_norm_backward(dy2, x2, weight, p_dtype, stats)
+def layer_norm_bwd(dy2: torch.Tensor, x2: torch.Tensor, weight: Optional[torch.Tensor], p_dtype: torch.dtype, stats: torch.Tensor, need_dx: bool, need_dw: bool,
+                   need_db: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias); an unneeded gradient is empty."""
+    grads = _native.layer_norm_backward(dy2, x2, weight, p_dtype, stats, need_dx, need_dw, need_db)
+    return tuple(torch.empty(0, dtype=dt, device=x2.device) if g is None else g for g, dt in zip(grads, (x2.dtype, p_dtype, p_dtype)))
 
 
 @layer_norm_bwd.register_fake
-def _(dy2, x2, weight, p_dtype, stats):
-    p = lambda: torch.empty(x2.shape[1], dtype=p_dtype, device=x2.device)
-    return torch.empty(x2.shape, dtype=x2.dtype, device=x2.device), p(), p()
+def _(dy2, x2, weight, p_dtype, stats, need_dx, need_dw, need_db):
+    p = lambda need: torch.empty(x2.shape[1] if need else 0, dtype=p_dtype, device=x2.device)
+    return torch.empty(x2.shape if need_dx else (0,), dtype=x2.dtype, device=x2.device), p(need_dw), p(need_db)
 
 
 class _LayerNormFn(torch.autograd.Function):
@@ -197,8 +198,9 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gy):
         x2, stats, *weight = ctx.saved_tensors
-        dx, dw, db = layer_norm_bwd(gy, x2, weight[0] if ctx.has_weight else None, ctx.p_dtype, stats)
-        return tuple(g if need else None for g, need in zip((dx, dw, db), ctx.needs_input_grad)) + (None,)
+        needs = ctx.needs_input_grad[:3]
+        grads = layer_norm_bwd(gy, x2, weight[0] if ctx.has_weight else None, ctx.p_dtype, stats, *needs)
+        return tuple(g if need else None for g, need in zip(grads, needs)) + (None,)
 
 
 @torch.library.impl(_traced, "layer_norm", "CompositeImplicitAutograd")

@@ -1023,18 +1023,20 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
     return y, stats
 
 
-def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], p_dtype: torch.dtype, stats: torch.Tensor):
-    """(dx, dweight, dbias) of a matrix, the latter two in ``p_dtype``.  See f8mi_layer_norm_backward."""
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], p_dtype: torch.dtype, stats: torch.Tensor, need_dx: bool = True,
+                        need_dw: bool = True, need_db: bool = True):
+    """(dx, dweight, dbias) of a matrix, the latter two in ``p_dtype``, None where not needed.  See f8mi_layer_norm_backward."""
     _require_gpu(dy, "dy")
     xs, rows, cols, ld = _as_2d(x)
     gs, _, _, ld_dy = _as_2d(dy)
     weight = None if weight is None else weight.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw, db = (torch.empty(cols, dtype=p_dtype, device=x.device) for _ in range(2))
-    need = lib().f8mi_layer_norm_workspace_bytes(rows, cols, _DT[x.dtype])
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
+    dw, db = (torch.empty(cols, dtype=p_dtype, device=x.device) if needed else None for needed in (need_dw, need_db))
+    need = lib().f8mi_layer_norm_workspace_bytes(rows, cols, _DT[x.dtype]) if need_dw or need_db else 0
     ws = torch.empty(max(need // 4, 1), dtype=torch.float32, device=x.device)
-    rc = lib().f8mi_layer_norm_backward(gs.data_ptr(), ld_dy, xs.data_ptr(), ld, rows, cols, _DT[x.dtype], weight.data_ptr() if weight is not None else None,
-                                        _DT[p_dtype], stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), need, _stream(x))
+    ptr = lambda t: None if t is None else t.data_ptr()
+    rc = lib().f8mi_layer_norm_backward(gs.data_ptr(), ld_dy, xs.data_ptr(), ld, rows, cols, _DT[x.dtype], ptr(weight), _DT[p_dtype], stats.data_ptr(), ptr(dx), ptr(dw),
+                                        ptr(db), ws.data_ptr(), need, _stream(x))
     _check(rc, "f8mi_layer_norm_backward")
     return dx, dw, db
 
