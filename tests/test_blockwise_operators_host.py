@@ -1,8 +1,11 @@
 """The registered operators of the blockwise linear and layer norm, as a compiler sees them: no GPU needed."""
+import inspect
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
+import float8_experimental_amd as f8
 from float8_experimental_amd import _custom_ops_norm_blockwise as ops
 from float8_experimental_amd import _native
 
@@ -53,3 +56,7 @@ def test_compiled_layer_norm_computes_what_is_asked_for(monkeypatch):
             fake = ops.layer_norm_bwd(x.detach(), x.detach(), w.detach(), BF16, stats, *map(bool, which))
         assert shapes(real) == shapes(fake)
         asked.clear()
+
+
+def test_clip_grad_norm_takes_the_arguments_of_torch():
+    assert list(inspect.signature(f8.clip_grad_norm_).parameters) == list(inspect.signature(torch.nn.utils.clip_grad_norm_).parameters)
