@@ -960,7 +960,7 @@ def block_cast(jobs):
     """[(copy contracting over the columns or None, copy contracting over the rows or None)] of one or two 2-D tensors, in one pass over
     each.  A job is ``(x, square, want, want_t)``: ``square`` gives every 128 x 128 values one scale, otherwise blocks are 128
     values along the contraction of each copy; ``want_t`` may be ``"scales"`` for a square tensor that another product reads transposed.  A fifth entry of
-    a job, a dtype, asks for the columns summed up in that type (see ``column_sum``) as the third of its results.  See f8mi_block_cast."""
+    a job, a dtype, asks for the columns summed up, in fp32 and rounded once to that type, as the third of its results.  See f8mi_block_cast."""
     structs, out = (BlockCastJob * len(jobs))(), []
     held = []
     for s, (x, square, want, want_t, *sum_dtype) in zip(structs, jobs):
@@ -985,7 +985,7 @@ def block_cast(jobs):
         if sum_dtype:
             a, b, sums = out[i]
             total = torch.empty(sums.shape[1], dtype=sum_dtype[0], device=x.device)
-            _check(lib().f8mi_column_sum_finish(sums.data_ptr(), *sums.shape, _DT[x.dtype], total.data_ptr(), _DT[total.dtype], stream), "f8mi_column_sum_finish")
+            _check(lib().f8mi_column_sum_finish(sums.data_ptr(), *sums.shape, _DT[torch.float32], total.data_ptr(), _DT[total.dtype], stream), "f8mi_column_sum_finish")
             out[i] = (a, b, total)
     return out
 

@@ -260,7 +260,7 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
         if (need_dw) dw = block_gemm(dy.t, gt, k_at.xt.in(kept), false, n, k, m, wt);
         if (need_db) {
             db = at::empty({n}, dy.t.options().dtype(bt));
-            check(L.column_sum_finish(sums, sum_rows, n, dy.dtype(), db.data_ptr(), dtype_code(bt), stream_of(dy.t)), "f8mi_column_sum_finish");
+            check(L.column_sum_finish(sums, sum_rows, n, F8MI_FP32, db.data_ptr(), dtype_code(bt), stream_of(dy.t)), "f8mi_column_sum_finish");
         }
         return {dx, dw, db, at::Tensor(), at::Tensor()};
     }

@@ -42,8 +42,9 @@ def _checked(x: torch.Tensor, n: int, k: int, bias: Optional[torch.Tensor], what
 def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ weight.t() + bias`` with every product of forward and backward on block-scaled e4m3 operands.
 
-    ``x`` [..., k] and ``weight`` [n, k] in bfloat16, float16 or float32 (the weight may have another type than x), ``bias`` [n]; the result and
-    the gradient of x have x's type, those of weight and bias the parameters' own.  Under autocast x takes the autocast type first."""
+    ``x`` [..., k] and ``weight`` [n, k] in bfloat16, float16 or float32 (the weight may have another type than x), ``bias`` [n], which is rounded to x's
+    type before it is added; the result and the gradient of x have x's type, those of weight and bias the parameters' own, to which their fp32 sums are
+    rounded once.  Under autocast x takes the autocast type first."""
     if torch.is_autocast_enabled():
         x = x.to(torch.get_autocast_dtype("cuda"))
     if not torch.compiler.is_compiling():
