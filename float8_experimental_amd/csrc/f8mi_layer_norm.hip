@@ -166,8 +166,8 @@ __device__ __forceinline__ void row_moments(float& mean, float& m2, int cols, fl
 #pragma unroll 4
         for (int i = 0; i < T / 64; i++) {
             const float2 w = slots[first + i];
-            const float d = w.x - mean;
-            m2 += __builtin_fmaf(d * d, (float)wave_count<T, VPT, V>(i, cols), w.y);
+            const float d = w.x - mean, n = (float)wave_count<T, VPT, V>(i, cols);
+            m2 += n > 0.f ? __builtin_fmaf(d * d, n, w.y) : 0.f;  // (the square of a large mean is infinite, and zero times that a NaN)
         }
     }
 }
