@@ -389,7 +389,7 @@ __global__ __launch_bounds__(ln_backward_threads(T, VPT), 4) void layer_norm_bac
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 xh[i] = (xh[i] - st.x) * st.y;
-                if (T > 64 && !lane.has(p, i)) g[i] = 0.f;
+                if (!lane.has(p, i)) (T > 64 ? g[i] : xh[i]) = 0.f;  // (past the end of a row g is zero, but xh may be infinite)
                 dw[p][i] = __builtin_fmaf(g[i], xh[i], dw[p][i]);
                 db[p][i] += g[i];
                 g[i] *= w[i];
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(LN_WIDE_THREADS) void layer_norm_backward_wide_kern
         for (int i = 0; i < V; i++) {
             g[i] *= w[i];
             s1 += g[i];
-            s2 = __builtin_fmaf(g[i], (xv[i] - st.x) * st.y, s2);
+            if (col + i < cols) s2 = __builtin_fmaf(g[i], (xv[i] - st.x) * st.y, s2);  // (past the end of a row xhat may be infinite)
         }
     }
     row_sums<LN_WIDE_THREADS>(s1, s2, slots);

@@ -25,3 +25,19 @@ def test_means_whose_square_overflows(f8, cols, mean):
     # 96 roundings in the mean, which the spread divides, as many in the spread
     tol = 2 * 96 * FP * (v.abs().mean(1, keepdim=True) * rstd + want.abs()) + 4 * FP * v.abs() * rstd
     assert got.isfinite().all() and ((got - want).abs() <= tol).all()
+
+
+# (columns, log2 of the values, eps): the sum of a row is finite, a value times 1 / sqrt(eps) is not
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols,log2,eps", [(8, 120, 1e-5), (64, 121, 1e-5), (128, 113, 1e-12), (20001, 112, 1e-12)])
+def test_gradients_of_constant_rows_of_large_values(f8, cols, log2, eps, dtype):
+    """Their mean is exact and their variance zero: xhat is zero and dx is (dy - mean(dy)) / sqrt(eps), in rows that end inside a lane's piece too."""
+    x = torch.full((3, cols), 2.0**log2, dtype=dtype, device="cuda", requires_grad=True)
+    w = torch.ones(cols, dtype=dtype, device="cuda", requires_grad=True)
+    dy = (torch.randn(3, cols, generator=torch.Generator().manual_seed(cols)) * 2.0**-10).to(dtype).cuda()
+    f8.layer_norm(x, cols, w, eps=eps).backward(dy)
+    d = dy.double()
+    want = (d - d.mean(1, keepdim=True)) / eps**0.5
+    # one rounding to the output's type, and sums of 96 roundings
+    tol = (2.0**-8 if dtype is torch.bfloat16 else 2.0**-23) * want.abs() + 96 * FP * (d.abs() + d.abs().mean(1, keepdim=True)) / eps**0.5
+    assert ((x.grad.double() - want).abs() <= tol).all() and (w.grad == 0).all()
