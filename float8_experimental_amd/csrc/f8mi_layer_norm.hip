@@ -151,6 +151,12 @@ __device__ __forceinline__ int wave_count(int wave, int cols) {  // values of th
     for (int p = 0; p < VPT; p++) n += min(max(cols - (p * T + wave * 64) * V, 0), 64 * V);
     return n;
 }
+// a / n by inv, 1 / n rounded: the rounded quotient, where the product alone is an ulp off for one n in seven.  The mean of a constant row is then its
+// value: an ulp of a large one, squared, would be its variance.
+__device__ __forceinline__ float quotient(float a, float n, float inv) {
+    const float q = a * inv;
+    return __builtin_fmaf(__builtin_fmaf(-q, n, a), inv, q);
+}
 template <int T, int VPT, int V>
 __device__ __forceinline__ void row_moments(float& mean, float& m2, int cols, float inv_cols, float2* slots) {
     if constexpr (T > 64) {
@@ -161,7 +167,7 @@ __device__ __forceinline__ void row_moments(float& mean, float& m2, int cols, fl
         float total = 0.f;
 #pragma unroll 4
         for (int i = 0; i < T / 64; i++) total = __builtin_fmaf(slots[first + i].x, (float)wave_count<T, VPT, V>(i, cols), total);
-        mean = total * inv_cols;
+        mean = quotient(total, (float)cols, inv_cols);
         m2 = 0.f;
 #pragma unroll 4
         for (int i = 0; i < T / 64; i++) {
@@ -277,7 +283,7 @@ __global__ __launch_bounds__(ln_threads(T), ln_waves_a_simd(T, VPT)) void layer_
         ln_param<PT, V, int>(weight, lane.last, cols, 1.f, w);
         ln_param<PT, V, int>(bias, lane.last, cols, 0.f, b);
     }
-    const float inv_count = 1.0f / (float)max(wave_count<T, VPT, V>(t >> 6, cols), 1);
+    const float count = (float)max(wave_count<T, VPT, V>(t >> 6, cols), 1), inv_count = 1.0f / count;
     auto one = [&](uint4 (&ahead)[VPT], int64_t row, float2* slot) __attribute__((always_inline)) {
         uint4 q[VPT];  // the row as it came: unpacking it again costs less than registers that keep waves from running
 #pragma unroll
@@ -290,7 +296,7 @@ __global__ __launch_bounds__(ln_threads(T), ln_waves_a_simd(T, VPT)) void layer_
 #pragma unroll
             for (int i = 0; i < V; i++) s += T == 64 || lane.has(p, i) ? v[i] : 0.f;
         }
-        float mean = wave_sum(s) * inv_count;
+        float mean = quotient(wave_sum(s), count, inv_count);
         s = 0.f;
 #pragma unroll
         for (int p = 0; p < VPT; p++) {

@@ -41,3 +41,19 @@ def test_gradients_of_constant_rows_of_large_values(f8, cols, log2, eps, dtype):
     # one rounding to the output's type, and sums of 96 roundings
     tol = (2.0**-8 if dtype is torch.bfloat16 else 2.0**-23) * want.abs() + 96 * FP * (d.abs() + d.abs().mean(1, keepdim=True)) / eps**0.5
     assert ((x.grad.double() - want).abs() <= tol).all() and (w.grad == 0).all()
+
+
+@pytest.mark.parametrize("cols", [7, 63, 109, 379, 500, 731, 1000, 2035, 4093])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_constant_rows_have_no_variance(f8, cols, dtype):
+    """Eight significant bits, so that every sum is exact: the mean is the value itself, and not an ulp beside it (whose square is 1.5e-5, more than eps)."""
+    x = torch.full((3, cols), 98816.0, dtype=dtype, device="cuda", requires_grad=True)
+    b = torch.randn(cols, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    dy = torch.randn(3, cols, generator=torch.Generator().manual_seed(cols)).to(dtype).cuda()
+    y = f8.layer_norm(x, cols, None, b)
+    assert torch.equal(y, b.expand(3, cols))
+    y.backward(dy)
+    d = dy.double()
+    want = (d - d.mean(1, keepdim=True)) / 1e-5**0.5
+    tol = (2.0**-8 if dtype is torch.bfloat16 else 2.0**-23) * want.abs() + 96 * FP * (d.abs() + d.abs().mean(1, keepdim=True)) / 1e-5**0.5
+    assert ((x.grad.double() - want).abs() <= tol).all()
