@@ -7,7 +7,9 @@
 // hands their memory out again in stream order: calls on any number of threads, streams and captures share nothing.
 #include <dlfcn.h>
 
+#include <algorithm>
 #include <optional>
+#include <utility>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -473,6 +475,18 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
+// Whether two of them share memory: one read while the other is written, in place, would be scaled or not as it happens.
+bool overlapping(const std::vector<at::Tensor>& ts) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> at;
+    at.reserve(ts.size());
+    for (const at::Tensor& t : ts)
+        if (t.numel()) at.emplace_back((uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.nbytes());
+    std::sort(at.begin(), at.end());
+    for (size_t i = 1; i < at.size(); i++)
+        if (at[i].first < at[i - 1].second) return true;
+    return false;
+}
+
 // grad_clip(list, what, kind, max_norm) -> (norm (fp32, 0-dim), list or None), or None: something in the list is not taken.
 // what: "norm" of the tensors; "grads": the gradients of the tensors are clipped in place; None: clipped into new tensors of the tensors' own
 // types; a dtype: of that type.
@@ -502,6 +516,7 @@ PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             if (!g.defined() || !g.is_non_overlapping_and_dense()) Py_RETURN_NONE;
             xs.push_back(g);
         }
+        if (of_params && overlapping(xs)) Py_RETURN_NONE;
         at::Tensor norm;
         {
             const WithoutGil no_gil;

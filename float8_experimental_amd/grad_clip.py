@@ -89,9 +89,10 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
 @_shown_to_function_modes
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> torch.Tensor:
-    """``torch.nn.utils.clip_grad_norm_`` for the norms 2, 1 and inf (``foreach`` chooses nothing: there is one implementation): scales the gradients of ``parameters`` in place so that their norm as one vector is at most
-    ``max_norm``, and returns the norm before (0-dim float32).  Nothing is written where nothing is clipped, and nothing waits for the GPU
-    unless ``error_if_nonfinite``, which raises before a gradient is changed."""
+    """``torch.nn.utils.clip_grad_norm_`` for the norms 2, 1 and inf (``foreach`` chooses nothing: there is one implementation): scales the
+    gradients of ``parameters`` in place so that their norm as one vector is at most ``max_norm``, and returns the norm before (0-dim
+    float32).  A gradient that is listed more than once counts in the norm as often and is scaled once.  Nothing is written where nothing is
+    clipped, and nothing waits for the GPU unless ``error_if_nonfinite``, which raises before a gradient is changed."""
     parameters, kind = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters), _kind(norm_type)
     if error_if_nonfinite:
         grad_norm([p.grad for p in parameters if p.grad is not None], norm_type, True)
