@@ -15,6 +15,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -62,7 +63,7 @@ int dtype_code(at::ScalarType t) {
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// Whether somebody has to see operators: a dispatch or function mode, a trace (functional transforms show in the tensors).  A kernel's launch is none, and
+// Whether somebody has to see operators: a dispatch or function mode, a trace (what a functional transform follows shows in the tensors).  A kernel's launch is none, and
 // a trace would hold the allocation of its output alone.  torch.set_default_device is a function mode that asks for nothing.
 PyObject* device_context = nullptr;  // torch.utils._device.DeviceContext
 bool watched() {
@@ -89,6 +90,13 @@ bool as_saved(const at::Tensor& t, const c10::Device& device, at::ScalarType typ
     constexpr c10::DispatchKeySet others({K::Python, K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Batched, K::Functionalize, K::ZeroTensor});
     return t.defined() && t.device() == device && t.layout() == at::kStrided && t.scalar_type() == type && t.sizes() == sizes && !t.key_set().has_any(others);
 }
+
+// Below autograd, and below functional transforms: what is plain is a constant to them (what they follow is not taken), but what is allocated inside one
+// would be a tensor of it, without memory.
+struct Below {
+    const at::AutoDispatchBelowADInplaceOrView autograd;
+    const c10::impl::ExcludeDispatchKeyGuard transforms{c10::DispatchKeySet({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode})};
+};
 
 // A matrix as the kernels read it: unit column stride, `ld` from row to row (0: the same row throughout); copied where its layout needs it.
 struct Rows {
@@ -183,7 +191,7 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
     // kept: see Kept; null: nothing is
     static at::Tensor compute(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, bool need_dx, bool need_dw, at::Tensor* kept) {
         const c10::DeviceGuard guard(x.device());
-        const at::AutoDispatchBelowADInplaceOrView below;
+        const Below below;
         const int64_t k = weight.size(1), n = weight.size(0);
         const Rows xr(x, k), wr(weight, k);
         const int64_t m = xr.rows;
@@ -230,7 +238,7 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
         at::Tensor dx, dw, db;
         if (!grads[0].defined()) return {dx, dw, db, at::Tensor(), at::Tensor()};
         const c10::DeviceGuard guard(grads[0].device());
-        const at::AutoDispatchBelowADInplaceOrView below;
+        const Below below;
         const Rows dy(grads[0].scalar_type() == xt ? grads[0] : grads[0].to(xt), n);
         const int64_t m = dy.rows;
         if (m == 0) {
@@ -273,7 +281,7 @@ struct BlockwiseLinear : torch::autograd::Function<BlockwiseLinear> {
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static at::Tensor compute(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, int64_t cols, double eps, at::Tensor* stats_out) {
         const c10::DeviceGuard guard(x.device());
-        const at::AutoDispatchBelowADInplaceOrView below;
+        const Below below;
         const Rows r(x, cols);
         const int pt = weight.defined() ? dtype_code(weight.scalar_type()) : bias.defined() ? dtype_code(bias.scalar_type()) : r.dtype();
         const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
@@ -306,7 +314,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &stats = saved[2];
         const c10::DeviceGuard guard(grads[0].device());
-        const at::AutoDispatchBelowADInplaceOrView below;
+        const Below below;
         const int64_t cols = ctx->saved_data["cols"].toInt();
         const at::ScalarType pt = (at::ScalarType)ctx->saved_data["p_type"].toInt();
         TORCH_CHECK(as_saved(x, grads[0].device(), (at::ScalarType)ctx->saved_data["x_type"].toInt(), ctx->saved_data["x_shape"].toIntVector()) &&
@@ -415,7 +423,7 @@ PyObject* blockwise_inference_linear(PyObject*, PyObject* const* a, Py_ssize_t n
         {
             const WithoutGil no_gil;
             const c10::DeviceGuard guard(x.device());
-            const at::AutoDispatchBelowADInplaceOrView below;
+            const Below below;
             std::vector<int64_t> y_shape(x.sizes().begin(), x.sizes().end());
             y_shape.back() = n;
             const Rows xr(x, k);
@@ -520,7 +528,7 @@ PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         at::Tensor norm;
         {
             const WithoutGil no_gil;
-            const at::AutoDispatchBelowADInplaceOrView below;
+            const Below below;
             const c10::DeviceGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
             const auto options = at::TensorOptions().device(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
             std::vector<f8mi_grad> grads(xs.size());

@@ -43,13 +43,13 @@ class Function(torch.overrides.TorchFunctionMode):
         return func(*args, **(kwargs or {}))
 
 
-def forwards(f8):
+def forwards(f8, trains=True):
     """(name, name of its operator, call, x): what a model runs forward"""
     w, b = normal(128, 256, seed=1), normal(128, seed=2)
     p, q = normal(256, seed=3, dtype=torch.float32), normal(256, seed=4, dtype=torch.float32)
     lin = nn.Linear(256, 128, device="cuda", dtype=BF16)
     served = f8.Float8BlockwiseInferenceLinear.from_float(lin)
-    norm = f8.LayerNorm.from_float(nn.LayerNorm(256, device="cuda", dtype=BF16))
+    norm = f8.LayerNorm.from_float(nn.LayerNorm(256, device="cuda", dtype=BF16).requires_grad_(trains))
     return [("linear", "f8mi.blockwise_linear_fwd", lambda x: f8.blockwise_linear(x, w, b), normal(40, 256)),
             ("linear, 3-D", "f8mi.blockwise_linear_fwd", lambda x: f8.blockwise_linear(x, w), normal(2, 20, 256)),
             ("served, few", "f8mi.blockwise_inference_linear", served, normal(3, 256)),
@@ -157,3 +157,18 @@ def test_clipping_is_not_traced(f8):
         with pytest.raises(RuntimeError, match="trace"), warnings.catch_warnings():
             warnings.simplefilter("ignore")
             torch.jit.trace(call, g)
+
+
+def test_calls_inside_functional_transforms_of_something_else(f8):
+    """Tensors that a transform does not know are constants to it; a history inside one is refused, as by any C++ autograd function."""
+    scale = torch.tensor([1.0, 2.0], device="cuda")
+    for name, op, call, x in forwards(f8, trains=False):
+        with torch.no_grad():
+            want = call(x).float()
+            for got in (torch.func.grad(lambda s: (call(x).float() * s).sum())(scale[0]), torch.func.jvp(lambda s: (call(x).float() * s).sum(), (scale[0],), (scale[0],))[1]):
+                assert abs(got - want.sum()) <= 2.0**-7 * want.abs().sum(), name
+            batch = torch.func.vmap(lambda s: call(x).float() * s)(scale)
+            assert torch.equal(batch, want * scale.view(2, *[1] * want.dim())), name
+    x, w = normal(40, 256), normal(128, 256, seed=1).requires_grad_()
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.vmap(lambda s: f8.blockwise_linear(x, w).float() * s)(scale)
