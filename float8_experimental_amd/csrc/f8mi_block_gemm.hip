@@ -1,5 +1,6 @@
 // Products of operands with block scales (f8mi_block.h) on 128-row tiles, and the choice of kernel.  Main loop, LDS layout and epilogue are
-// those of f8mi_gemm_mid_impl.h, the choice that of f8mi_gemm.hip; a stage brings 256 bytes of scales more for each wave, and the matrix instruction applies them.
+// those of f8mi_gemm_mid_impl.h; the choice is by the estimates of f8mi_gemm_util.h, fitted to products with one scale: for these only the split of k
+// (block_k_splits) was measured.  A stage brings 256 bytes of scales more for each wave, and the matrix instruction applies them.
 // Bound by the loads into LDS and their latency.  Measured, bf16: 2048 x 4096 over 4096 30 us (2.3 PFLOP/s), the weight read transposed 32 us, 512 x 1024
 // over 1024 7.7 us.
 #include <algorithm>

@@ -598,7 +598,8 @@ struct LnArgs {
 };
 
 // Lanes of a row and pieces a lane, by the number of 16-byte pieces of a row; 0: does not fit.  Forward's weight and bias have to fit in LDS
-// with it, in backward the column sums of 16-bit rows take the registers of a third piece (20000 bf16 values with one spilled: 194 us, as by columns).
+// with it, in backward the column sums of 16-bit rows take the registers of a third piece (with one it spilled and was no faster than by columns: 2048
+// rows of 20000 bf16 values, both passes, 169 us, 8192 of them 581).
 struct LnShape {
     int t, vpt;
 };
@@ -610,7 +611,9 @@ static LnShape ln_shape(int64_t cols, int dtype, int p_dtype, bool backward) {
     const int64_t pieces = ln_pieces(cols, dtype);
     for (int t = 64; t <= LN_ROW_LANES; t *= 2)
         if (pieces <= t) return {t, 1};
-    if (dtype == F8MI_FP32 && pieces <= 3 * 512) return {512, 3};  // two workgroups a CU, and fewer idle lanes (4097 values: 88 us with 1024 lanes, 77)
+    // two workgroups a CU, and fewer idle lanes (both passes, us, 1024 lanes / 512: 4099 rows of 4097 96 / 78, 8192 of 4352 169 / 142, 4096 of 5120 97 / 85,
+    // 4096 of 6144 108 / 100, 2048 of 4100 71 / 69, 16384 of 6000 398 / 402)
+    if (dtype == F8MI_FP32 && pieces <= 3 * 512) return {512, 3};
     const int64_t vpt = (pieces + LN_ROW_LANES - 1) / LN_ROW_LANES;
     if (vpt > (backward && dtype != F8MI_FP32 ? 2 : 4) || ln_lds(cols, dtype, p_dtype, backward) > LN_MAX_LDS) return {0, 0};
     return {LN_ROW_LANES, (int)vpt};

@@ -398,7 +398,7 @@ PyObject* blockwise_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 // Cast and product of a few rows in one kernel: every workgroup converts all of the activations for itself, which costs more than the launch it saves
-// once there are many of them and many rows (the lines of the linears with one scale).
+// once there are many of them and many rows.  The lines are those measured for the linears with one scale; for block scales they were not measured.
 bool one_kernel_pays(int64_t m, int64_t n, int64_t kp, int dt) {
     if (m > 16 || m * kp > F8MI_FEW_ROWS_ELEMS) return false;
     return dt == F8MI_FP32 ? n <= 16384 || m * n <= 65536 : m * n <= 262144;

@@ -8,7 +8,9 @@ each tensor once.
 
     y = q(x) q(w)^T + bias,   dx = q(dy) q(w),   dw = q'(dy)^T q'(x)
 
-with q' in blocks along the tokens, which the backward's contraction runs over.  Products add in fp32 and are rounded once.
+with q' in blocks along the tokens, which the backward's contraction runs over.  The matrix cores add products: the eight of neighbouring k
+are cut to multiples of 2^-13 of the largest of them, the groups of eight are added in fp32 (about 1.3e-5 of a result's size altogether, as in
+``torch._scaled_mm``), and the result is rounded once.
 
 ``convert_to_float8_training`` with ``ScalingType.BLOCKWISE`` for all three tensors swaps ``nn.Linear`` for ``Float8BlockwiseLinear``,
 ``quantize_to_float8`` with ``ActivationCasting.BLOCKWISE`` for ``Float8BlockwiseInferenceLinear``; ``blockwise_linear`` is the function
