@@ -465,14 +465,20 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 if (!PyLong_Check(PyTuple_GET_ITEM(a[1], i))) Py_RETURN_NONE;
                 shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(a[1], i)));
             }
+        if (PyErr_Occurred()) {  // a number that no dimension has
+            PyErr_Clear();
+            Py_RETURN_NONE;
+        }
+        const int64_t d = (int64_t)shape.size();
+        if (d == 0 || x.dim() < d || x.sizes().slice(x.dim() - d) != at::IntArrayRef(shape)) Py_RETURN_NONE;
         int64_t cols = 1;
         for (const int64_t s : shape) cols *= s;
-        const int64_t d = (int64_t)shape.size();
-        if (d == 0 || cols <= 0 || x.dim() < d || x.sizes().slice(x.dim() - d) != at::IntArrayRef(shape)) Py_RETURN_NONE;
+        if (cols <= 0) Py_RETURN_NONE;
         for (const at::Tensor* p : {&w, &b})
             if (p->defined() && (p->sizes() != at::IntArrayRef(shape) || (p->scalar_type() != x.scalar_type() && p->scalar_type() != at::kFloat))) Py_RETURN_NONE;
         if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()) Py_RETURN_NONE;
         const double eps = PyFloat_AsDouble(a[4]);
+        if (eps == -1.0 && PyErr_Occurred()) return nullptr;
         at::Tensor y;
         {
             const WithoutGil no_gil;
