@@ -23,9 +23,13 @@ from .float8_tensor import Float8Tensor, GemmInputRole, LinearMMConfig, ScaledMM
 from .fsdp_utils import precompute_float8_dynamic_scale_for_fsdp  # all weight scales in one pass
 
 # beside the reference's names: linears with a scale for each block of 128, and the operators around them in a training step
-from .float8_blockwise import Float8BlockwiseInferenceLinear, Float8BlockwiseLinear, blockwise_linear
-from .norm import LayerNorm, convert_layer_norms, layer_norm
+from .float8_blockwise import BlockwiseActivations, Float8BlockwiseInferenceLinear, Float8BlockwiseLinear, blockwise_linear
+from .norm import LayerNorm, RMSNorm, convert_layer_norms, convert_rms_norms, layer_norm, rms_norm, rms_norm_blockwise
+from .residual_dropout import Dropout, convert_dropouts, dropout
 from .grad_clip import clip_grad_norm_, clip_grads, grad_norm
+
+# low-rank adapters beside any of the linears: trained, and many of them served at once
+from .low_rank import AdaptedLinear, AdapterRows, adapt_linears, low_rank_adapters, select_adapters
 
 # checkpoints holding Float8Tensors load with torch.load(..., weights_only=True)
 _serialization.add_safe_globals([Float8Tensor, GemmInputRole, LinearMMConfig, ScaledMMConfig])

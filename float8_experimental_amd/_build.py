@@ -18,6 +18,9 @@ EXT_LIB = os.path.join(HERE, "_f8mi_torch.so")
 # ... and that of the blockwise scaled linear, layer norm and gradient clipping
 OPS_SRC = os.path.join(CSRC, "f8mi_torch_ops.cpp")
 OPS_LIB = os.path.join(HERE, "_f8mi_torch_ops.so")
+# ... and that of RMS norm, dropout, low-rank adapters and the served blockwise linear on activations that have been cast
+MODEL_SRC = os.path.join(CSRC, "f8mi_torch_model.cpp")
+MODEL_LIB = os.path.join(HERE, "_f8mi_torch_model.so")
 OBJ_DIR = os.path.join(CSRC, "build")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -62,7 +65,7 @@ def build(verbose: bool = True, out: str = LIB, defines=()) -> str:
     os.makedirs(obj_dir, exist_ok=True)
     srcs = sources()
     with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
-        exts = [ex.submit(build_extension, *e) for e in ((EXT_SRC, EXT_LIB), (OPS_SRC, OPS_LIB))] if out == LIB else []
+        exts = [ex.submit(build_extension, *e) for e in ((EXT_SRC, EXT_LIB), (OPS_SRC, OPS_LIB), (MODEL_SRC, MODEL_LIB))] if out == LIB else []
         objs = list(ex.map(lambda src: _compile(src, obj_dir, tuple(defines)), srcs))
         for ext in exts:
             ext.result()

@@ -77,6 +77,17 @@ EXPORTS = (
     "f8mi_layer_norm_workspace_bytes",
     "f8mi_grad_clip",
     "f8mi_grad_clip_workspace_bytes",
+    "f8mi_rms_norm",
+    "f8mi_rms_norm_block",
+    "f8mi_rms_norm_workspace_bytes",
+    "f8mi_rms_norm_backward",
+    "f8mi_dropout",
+    "f8mi_adapter_rows_words",
+    "f8mi_adapter_rows",
+    "f8mi_adapters_workspace_bytes",
+    "f8mi_adapters",
+    "f8mi_adapters_backward_workspace_bytes",
+    "f8mi_adapters_backward",
     "f8mi_prof_enable",
     "f8mi_prof_reset",
     "f8mi_prof_read",
@@ -212,6 +223,28 @@ def lib() -> C.CDLL:
         L.f8mi_grad_clip_workspace_bytes.argtypes = [i64]
         L.f8mi_grad_clip.restype = i32
         L.f8mi_grad_clip.argtypes = [C.POINTER(Grad), i64, i32, C.c_float, i32, fp, vp, i64, vp]
+        L.f8mi_rms_norm.restype = i32
+        L.f8mi_rms_norm.argtypes = [vp, i64, vp, i64, i64, i64, i32, vp, i32, C.c_float, vp, vp, fp, vp]
+        L.f8mi_rms_norm_block.restype = i32
+        L.f8mi_rms_norm_block.argtypes = [vp, i64, vp, i64, i64, i64, i32, vp, i32, C.c_float, vp, vp, vp, vp]
+        L.f8mi_rms_norm_workspace_bytes.restype = i64
+        L.f8mi_rms_norm_workspace_bytes.argtypes = [i64, i64, i32, i32]
+        L.f8mi_rms_norm_backward.restype = i32
+        L.f8mi_rms_norm_backward.argtypes = [vp, i64, vp, i64, vp, i64, i64, i64, i32, vp, i32, fp, vp, vp, vp, i64, vp]
+        L.f8mi_dropout.restype = i32
+        L.f8mi_dropout.argtypes = [vp, vp, i64, i32, C.c_double, vp, vp, vp]
+        L.f8mi_adapter_rows_words.restype = i64
+        L.f8mi_adapter_rows_words.argtypes = [i64, i64]
+        L.f8mi_adapter_rows.restype = i32
+        L.f8mi_adapter_rows.argtypes = [vp, i32, i64, i64, vp, vp]
+        L.f8mi_adapters_workspace_bytes.restype = i64
+        L.f8mi_adapters_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i32]
+        L.f8mi_adapters.restype = i32
+        L.f8mi_adapters.argtypes = [vp, i64, vp, vp, fp, C.c_float, vp, i64, i64, i64, i64, i64, i32, vp, i64, vp, fp, vp, i64, vp]
+        L.f8mi_adapters_backward_workspace_bytes.restype = i64
+        L.f8mi_adapters_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i32, i32, i32, i32]
+        L.f8mi_adapters_backward.restype = i32
+        L.f8mi_adapters_backward.argtypes = [vp, i64, vp, i64, vp, vp, fp, C.c_float, vp, fp, i64, i64, i64, i64, i64, i32, vp, vp, vp, i32, vp, i64, vp]
         L.f8mi_prof_enable.restype = i32
         L.f8mi_prof_enable.argtypes = [i32]
         L.f8mi_prof_reset.restype = i32
@@ -229,8 +262,10 @@ def lib() -> C.CDLL:
 
 _EXT_PATH = os.path.join(_HERE, "_f8mi_torch.so")
 _OPS_PATH = os.path.join(_HERE, "_f8mi_torch_ops.so")
+_MODEL_PATH = os.path.join(_HERE, "_f8mi_torch_model.so")
 _ext = None
 _ops = None
+_model_ops = None
 
 
 def _load_extension(name: str, path: str):
@@ -268,6 +303,21 @@ def ops():
                     _check_device(torch.device("cuda", torch.cuda.current_device()))
                 _ops = module
     return _ops
+
+
+def model_ops():
+    """The CPython module with the host path of RMS norm, dropout, low-rank adapters and the served blockwise linear on activations that have been cast
+    (csrc/f8mi_torch_model.cpp), on the loaded library."""
+    global _model_ops
+    if _model_ops is None:
+        lib()
+        with _lock:
+            if _model_ops is None:
+                module = _load_extension("_f8mi_torch_model", _MODEL_PATH)
+                if torch.cuda.is_available():  # (without a GPU nothing is taken, and the callers say so)
+                    _check_device(torch.device("cuda", torch.cuda.current_device()))
+                _model_ops = module
+    return _model_ops
 
 
 def build_knobs() -> str:
@@ -1039,6 +1089,111 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
                                         ptr(db), ws.data_ptr(), need, _stream(x))
     _check(rc, "f8mi_layer_norm_backward")
     return dx, dw, db
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor], eps: float):
+    """(y, sum or None, rstd of each row [rows]) of matrices.  See f8mi_rms_norm."""
+    _require_gpu(x, "x")
+    xs, rows, cols, ld = _as_2d(x)
+    rs, _, _, ld_r = (None, 0, 0, 0) if residual is None else _as_2d(residual)
+    weight = None if weight is None else weight.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _check_device(x.device)
+    _check(lib().f8mi_rms_norm(xs.data_ptr(), ld, _ptr(rs), ld_r, rows, cols, _DT[x.dtype], _ptr(weight), _DT[x.dtype if weight is None else weight.dtype], eps, y.data_ptr(), _ptr(total),
+                               rstd.data_ptr(), _stream(x)), "f8mi_rms_norm")
+    return y, total, rstd
+
+
+def rms_norm_block(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor], eps: float):
+    """(the normed rows in block scales, sum or None) of matrices.  See f8mi_rms_norm_block."""
+    _require_gpu(x, "x")
+    xs, rows, cols, ld = _as_2d(x)
+    rs, _, _, ld_r = (None, 0, 0, 0) if residual is None else _as_2d(residual)
+    weight = None if weight is None else weight.contiguous()
+    out = _blocks_alloc(rows, cols, x.device)
+    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _check_device(x.device)
+    _check(lib().f8mi_rms_norm_block(xs.data_ptr(), ld, _ptr(rs), ld_r, rows, cols, _DT[x.dtype], _ptr(weight), _DT[x.dtype if weight is None else weight.dtype], eps, out.data.data_ptr(),
+                                     out.scales.data_ptr(), _ptr(total), _stream(x)), "f8mi_rms_norm_block")
+    return out, total
+
+
+def rms_norm_backward(dy: torch.Tensor, s: torch.Tensor, ds: Optional[torch.Tensor], weight: Optional[torch.Tensor], rstd: torch.Tensor, need_dx: bool = True, need_dw: bool = True):
+    """(dx, dweight) of matrices, None where not needed.  See f8mi_rms_norm_backward."""
+    _require_gpu(dy, "dy")
+    ss, rows, cols, ld = _as_2d(s)
+    gs, _, _, ld_dy = _as_2d(dy)
+    es, _, _, ld_ds = (None, 0, 0, 0) if ds is None else _as_2d(ds)
+    p_dtype = s.dtype if weight is None else weight.dtype
+    weight = None if weight is None else weight.contiguous()
+    dx = torch.empty(s.shape, dtype=s.dtype, device=s.device) if need_dx else None
+    dw = torch.empty(cols, dtype=p_dtype, device=s.device) if need_dw else None
+    need = lib().f8mi_rms_norm_workspace_bytes(rows, cols, _DT[s.dtype], _DT[p_dtype]) if need_dw else 0
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=s.device)
+    _check(lib().f8mi_rms_norm_backward(gs.data_ptr(), ld_dy, ss.data_ptr(), ld, _ptr(es), ld_ds, rows, cols, _DT[s.dtype], _ptr(weight), _DT[p_dtype], rstd.data_ptr(), _ptr(dx), _ptr(dw),
+                                        ws.data_ptr(), need, _stream(s)), "f8mi_rms_norm_backward")
+    return dx, dw
+
+
+def dropout(x: torch.Tensor, residual: Optional[torch.Tensor], seed: torch.Tensor, p: float) -> torch.Tensor:
+    """See f8mi_dropout."""
+    _require_gpu(x, "x")
+    x, residual = x.contiguous(), None if residual is None else residual.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _check_device(x.device)
+    _check(lib().f8mi_dropout(x.data_ptr(), _ptr(residual), x.numel(), _DT[x.dtype], p, seed.data_ptr(), out.data_ptr(), _stream(x)), "f8mi_dropout")
+    return out
+
+
+def adapter_rows(ids: torch.Tensor, count: int) -> torch.Tensor:
+    """The table of a batch whose row i has the adapter ids[i], int32 or int64.  See f8mi_adapter_rows."""
+    _require_gpu(ids, "ids")
+    ids, m = ids.contiguous(), ids.numel()
+    table = torch.empty(lib().f8mi_adapter_rows_words(m, count), dtype=torch.int32, device=ids.device)
+    _check_device(ids.device)
+    _check(lib().f8mi_adapter_rows(ids.data_ptr(), ids.element_size(), m, count, table.data_ptr(), _stream(ids)), "f8mi_adapter_rows")
+    return table
+
+
+def adapters(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, y: Optional[torch.Tensor], scale: Optional[torch.Tensor], factor: float, need_h: bool = False):
+    """(out, h or None) of matrices.  See f8mi_adapters."""
+    _require_gpu(x, "x")
+    xs, m, k, ld = _as_2d(x)
+    ys, _, n, ld_y = (None, 0, b.shape[1], 0) if y is None else _as_2d(y)
+    count, rank = a.shape[:2]
+    a, b = (t.to(x.dtype).contiguous() for t in (a, b))
+    out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    h = torch.empty((m, -(-rank // 16) * 16), dtype=torch.float32, device=x.device) if need_h else None
+    _check_device(x.device)
+    need = lib().f8mi_adapters_workspace_bytes(m, k, n, rank, count, _DT[x.dtype])
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
+    _check(lib().f8mi_adapters(xs.data_ptr(), ld, a.data_ptr(), b.data_ptr(), _ptr(scale), factor, table.data_ptr(), m, k, n, rank, count, _DT[x.dtype], _ptr(ys), ld_y, out.data_ptr(), _ptr(h),
+                               ws.data_ptr(), need, _stream(x)), "f8mi_adapters")
+    return out, h
+
+
+def adapters_backward(dout: torch.Tensor, x: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, scale: Optional[torch.Tensor], factor: float, h: Optional[torch.Tensor],
+                      need_dx: bool, need_da: bool, need_db: bool):
+    """(dx, da, db) of matrices, None where not needed; x is read for da, h for db.  See f8mi_adapters_backward."""
+    _require_gpu(dout, "dout")
+    gs, m, n, ld_g = _as_2d(dout)
+    count, rank, k = a.shape
+    xs, _, _, ld = _as_2d(x) if need_da else (None, 0, 0, 0)
+    p_dtype = a.dtype
+    a, b = (t.to(dout.dtype).contiguous() for t in (a, b))
+    dx = torch.empty((m, k), dtype=dout.dtype, device=dout.device) if need_dx else None
+    da, db = (torch.empty(t.shape, dtype=p_dtype, device=dout.device) if needed else None for t, needed in ((a, need_da), (b, need_db)))
+    need = lib().f8mi_adapters_backward_workspace_bytes(m, k, n, rank, count, _DT[dout.dtype], need_dx, need_da, need_db)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dout.device)
+    _check(lib().f8mi_adapters_backward(gs.data_ptr(), ld_g, _ptr(xs), ld, a.data_ptr(), b.data_ptr(), _ptr(scale), factor, table.data_ptr(), _ptr(h), m, k, n, rank, count, _DT[dout.dtype], _ptr(dx),
+                                        _ptr(da), _ptr(db), _DT[p_dtype], ws.data_ptr(), need, _stream(dout)), "f8mi_adapters_backward")
+    return dx, da, db
 
 
 def sync_table(entries, device: torch.device) -> torch.Tensor:

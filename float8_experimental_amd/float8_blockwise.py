@@ -16,11 +16,12 @@ are cut to multiples of 2^-13 of the largest of them, the groups of eight are ad
 ``quantize_to_float8`` with ``ActivationCasting.BLOCKWISE`` for ``Float8BlockwiseInferenceLinear``; ``blockwise_linear`` is the function
 behind the former.
 """
-from typing import Optional
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
 
+from . import _custom_ops_model as _compiled_model
 from . import _custom_ops_norm_blockwise as _compiled
 from . import _native
 
@@ -87,6 +88,20 @@ class Float8BlockwiseLinear(nn.Linear):
         return new_mod
 
 
+class BlockwiseActivations(NamedTuple):
+    """Activations [..., k] as ``Float8BlockwiseInferenceLinear`` multiplies them: e4m3 with a scale for each 128 values of a row, in the placement of its weight.  What
+    ``rms_norm_blockwise`` gives."""
+
+    data: torch.Tensor  # [padded k / 64, rows, 64]
+    scales: torch.Tensor
+    shape: Tuple[int, ...]
+    dtype: torch.dtype  # of the activations before, and of a linear's result
+
+    def dequantized(self) -> torch.Tensor:
+        """The values that the activations stand for, in fp32."""
+        return _native.Blocks(self.data, self.scales, self.data.shape[1], self.shape[-1]).dequant().float().reshape(self.shape)
+
+
 class Float8BlockwiseInferenceLinear(nn.Module):
     """A linear whose weight is kept as block-scaled e4m3, one byte a value and one for each 128 x 128 of them (repeated for its rows); the activations
     are cast per call.  Construct through ``from_float`` / ``quantize_to_float8``.
@@ -111,7 +126,9 @@ class Float8BlockwiseInferenceLinear(nn.Module):
                 self._buffers[name] = t.to(self._buffers[name].device)
         return self
 
-    def forward(self, input: torch.Tensor) -> torch.Tensor:
+    def forward(self, input: Union[torch.Tensor, BlockwiseActivations]) -> torch.Tensor:
+        if isinstance(input, BlockwiseActivations):
+            return self._forward_cast(input)
         if torch.is_autocast_enabled():
             input = input.to(torch.get_autocast_dtype("cuda"))
         if not torch.compiler.is_compiling():
@@ -123,6 +140,25 @@ class Float8BlockwiseInferenceLinear(nn.Module):
         if torch.is_grad_enabled() and input.requires_grad:
             raise RuntimeError("Float8BlockwiseInferenceLinear has no backward pass: call it under torch.no_grad() or torch.inference_mode()")
         return _compiled.blockwise_inference_linear(input, self.weight_data, self.weight_scales, self.bias)
+
+    def _forward_cast(self, input: BlockwiseActivations) -> torch.Tensor:
+        k, n = self.in_features, self.out_features
+        if input.shape[-1] != k:
+            raise ValueError(f"Float8BlockwiseInferenceLinear: activations of shape {input.shape} do not end in the {k} in_features of the weight")
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else input.dtype
+        y = None
+        if not torch.compiler.is_compiling():
+            y = _native.model_ops().blockwise_inference_linear_cast(input.data, input.scales, input.data.shape[1], dtype, self.weight_data, self.weight_scales, n, k, self.bias)
+        if y is None:
+            if not torch.compiler.is_compiling():
+                _native.refuse_tangents("Float8BlockwiseInferenceLinear", self.bias)
+            _native._require_gpu(input.data, "input")
+            if self.bias is not None:
+                _native._require_gpu(self.bias, "bias")
+                if self.bias.shape != (n,) or self.bias.dtype not in _HP_DTYPES:
+                    raise ValueError(f"Float8BlockwiseInferenceLinear: bias of shape {tuple(self.bias.shape)} ({self.bias.dtype}) for {n} out_features")
+            y = _compiled_model.blockwise_inference_linear_cast(input.data, input.scales, self.weight_data, self.weight_scales, k, dtype, self.bias)
+        return y.reshape(*input.shape[:-1], n)
 
     def dequantized_weight(self) -> torch.Tensor:
         """[out_features, in_features] in fp32: the values that the weight stands for."""

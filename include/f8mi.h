@@ -524,6 +524,47 @@ int64_t f8mi_grad_clip_workspace_bytes(int64_t count);
 int f8mi_grad_clip(const f8mi_grad* grads, int64_t count, int norm_kind, float max_norm, int scale, float* norm_dev, void* workspace, int64_t workspace_bytes,
                    void* stream);
 
+/* ---- RMS norm over the last dimension, with the addition in front of it -------------------------------------------------------------
+ * sum [rows][cols] = x + residual, rounded to their type; y = sum * rstd * weight, rstd = 1 / sqrt(mean(sum^2) + eps), statistics in fp32.  residual NULL: sum is
+ * x, and nothing is written there.  weight: cols values of p_dtype (x's dtype or F8MI_FP32), or NULL (1).  ld, ld_residual: elements from row to row, or 0: one row
+ * throughout; y and sum are dense and overlap no input but for sum == residual == dense.  rstd: [rows] for the backward pass, or NULL. */
+int f8mi_rms_norm(const void* x, int64_t ld, const void* residual, int64_t ld_residual, int64_t rows, int64_t cols, int dtype, const void* weight, int p_dtype, float eps,
+                  void* y, void* sum, float* rstd, void* stream);
+/* ... and y, not rounded before, kept in block scales (f8mi_block_cast's copy of `rows` rows contracting over the columns): out and out_scales, 16-byte aligned.  Scales of
+ * rows past the last are not written. */
+int f8mi_rms_norm_block(const void* x, int64_t ld, const void* residual, int64_t ld_residual, int64_t rows, int64_t cols, int dtype, const void* weight, int p_dtype, float eps,
+                        void* out, void* out_scales, void* sum, void* stream);
+/* dx (dense, x's dtype: the gradient of x and of the residual) = ds + rstd * (g - xhat * mean(g * xhat)), g = dy * weight, xhat = s * rstd; s: what was normed; ds: the
+ * gradient of the sum, or NULL.  dweight (p_dtype) = sum over rows of dy * xhat, in a fixed order.  Either may be NULL.  workspace: for dweight, 16-byte aligned, contents
+ * arbitrary. */
+int64_t f8mi_rms_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype, int p_dtype);
+int f8mi_rms_norm_backward(const void* dy, int64_t ld_dy, const void* s, int64_t ld, const void* ds, int64_t ld_ds, int64_t rows, int64_t cols, int dtype, const void* weight,
+                           int p_dtype, const float* rstd, void* dx, void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- dropout without a stored mask ------------------------------------------------------------------------------------------------------
+ * out = residual + (kept ? x / (1 - p) : 0) of n dense values (residual NULL: 0), in fp32 and rounded once; its own backward pass with the output's gradient as x.
+ * Value i is kept if word i % 4 of Philox 4x32 with 7 rounds, counter i / 4 and the 64 bits at seed_dev as the key, is at least p * 2^32, rounded.  0 <= p < 1. */
+int f8mi_dropout(const void* x, const void* residual, int64_t n, int dtype, double p, const int64_t* seed_dev, void* out, void* stream);
+
+/* ---- low-rank adapters of many requests beside one projection -------------------------------------------------------------------------
+ * out_i = y_i + scale_e B_e (A_e x_i), e the adapter of row i; a row without one keeps y_i.  a [count][r][k], b [count][n][r] dense, of x's dtype; scale_e = factor * scale[e],
+ * scale [count] fp32 or NULL (1); y [m][n] of x's dtype or NULL (0); out dense.
+ * table: what f8mi_adapter_rows made of the rows' adapters (int32 or int64 ids; a number that is no adapter's means none) for this m and count:
+ * f8mi_adapter_rows_words() 32-bit words, 16-byte aligned.  h: [m][r rounded up to 16] fp32 for the backward pass, or NULL.  workspace: 16-byte
+ * aligned, contents arbitrary.  Sums are fp32, in a fixed order. */
+#define F8MI_ADAPTER_MAX_ROWS (1 << 24)
+#define F8MI_ADAPTER_MAX_COUNT 32768
+#define F8MI_ADAPTER_MAX_RANK 256
+int64_t f8mi_adapter_rows_words(int64_t m, int64_t count);
+int f8mi_adapter_rows(const void* ids, int id_bytes, int64_t m, int64_t count, void* table, void* stream);
+int64_t f8mi_adapters_workspace_bytes(int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype);
+int f8mi_adapters(const void* x, int64_t ldx, const void* a, const void* b, const float* scale, float factor, const void* table, int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype,
+                  const void* y, int64_t ldy, void* out, float* h, void* workspace, int64_t workspace_bytes, void* stream);
+/* dx (dense, without what comes through y), da, db (p_dtype, whole: zeros for an adapter without rows); each may be NULL.  workspace: 256-byte aligned. */
+int64_t f8mi_adapters_backward_workspace_bytes(int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype, int need_dx, int need_da, int need_db);
+int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const void* a, const void* b, const float* scale, float factor, const void* table, const float* h, int64_t m,
+                           int64_t k, int64_t n, int64_t r, int64_t count, int dtype, void* dx, void* da, void* db, int p_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
