@@ -6,7 +6,7 @@
 //
 // HBM-bound: x, y and dout are read once each, out and dx written, an adapter is read by each of its tiles out of the L2.  The products run
 // on the matrix cores straight from registers: a lane's 16 bytes of a row, loaded as they lie, are its operand.  The order of a contraction is free as long
-// as both operands have the same one, so a lane takes 32 neighbouring bytes of a row and four lanes whole lines of the cache.
+// as both operands have the same one, so the four lanes that share a row take 64 neighbouring bytes of it, two instructions a line of the cache.
 //
 // h and dh are sums and stay in 32 bits: 16-bit matrix instructions get them as the sum of two 16-bit values (an error of 2^-17 of h, where one alone
 // would be off by as much as the rounding of the result), fp16 ones after a power of two for each row, so that nothing overflows or falls among the
@@ -37,6 +37,31 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p) {
     return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// V values of a row of r, from column col on, zeros past its end: `from` is their place in a tensor of `total` values.  WHOLE: r is a multiple of V, so that they all lie in the
+// row or none does.  No branch, so that many are on their way at once: past the end of the tensor its last 16 bytes are read and shifted.
+template <int DT, bool WHOLE>
+__device__ __forceinline__ uint4 load_of_row(const uint8_t* base, int64_t from, int64_t total, int col, int r) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
+    if constexpr (WHOLE) {
+        const bool in = col < r;
+        const uint4 q = load16_any(base + (in ? from : from - col) * SIZE);
+        return in ? q : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        if (total < V) return ln_load<DT, int>(base + (from - col) * SIZE, col, r);  // (nothing to read 16 bytes of)
+        const int64_t at = min(from, total - V);
+        const uint4 q = load16_any(base + at * SIZE);
+        uint64_t lo = q.x | (uint64_t)q.y << 32, hi = q.z | (uint64_t)q.w << 32;
+        const int shift = (int)min(from - at, (int64_t)V) * SIZE * 8, keep = min(max(r - col, 0), V) * SIZE * 8;  // bits
+        if (shift) {
+            lo = shift >= 64 ? (shift >= 128 ? 0 : hi >> (shift - 64)) : lo >> shift | hi << (64 - shift);
+            hi = shift >= 64 ? 0 : hi >> shift;
+        }
+        lo = keep >= 64 ? lo : keep ? lo & ~0ull >> (64 - keep) : 0;
+        hi = keep >= 128 ? hi : keep > 64 ? hi & ~0ull >> (128 - keep) : 0;
+        return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    }
+}
+
 struct AdapterArgs {
     const uint8_t* x;  // [m][k], k: contracted (shrink)
     int64_t ld;
@@ -53,239 +78,438 @@ struct AdapterArgs {
     int64_t ld_y;
     uint8_t* out;      // [m][n]
     float* h;          // [m][rp]: the parts added up, or null
-    int n, cols;       // cols: of out that a workgroup has, a multiple of 256
+    int n, cols, chunks;  // cols: of out that a workgroup has; chunks: workgroups a tile
 };
 
-// ---- shrink: a wave has 16 MT rows of one adapter, 16 RT of its rank and a part of the contraction
-template <int DT, int MT, int RT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void adapter_shrink_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+// ---- shrink: a wave has 16 rows of one adapter, 16 RT of its rank and a part of the contraction; those of a workgroup's waves are added up in LDS
+constexpr int SHRINK_WAVES = 8;
+template <int DT, int RT>
+__global__ __launch_bounds__(64 * SHRINK_WAVES) void adapter_shrink_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
     constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2, STEP = 128 / SIZE;  // values of a step: a line of the cache of each row
-    constexpr int DEPTH = MT * RT >= 8 ? 1 : 2;                       // steps in flight
-    __shared__ float4 part[WAVES][MT * RT][64];
-    const AdapterTile tile = tiles[blockIdx.x];
+    constexpr int DEPTH = 2;                                          // steps in flight
+    constexpr int WAVES = SHRINK_WAVES;
+    __shared__ float4 part[WAVES][RT][64];
+    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), split = id % g.splits;  // a tile's workgroups, and those of the next ones, on one XCD: A stays in its L2
+    const AdapterTile tile = tiles[id / g.splits];
     if (tile.rows == 0 || tile.group >= g.count) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lm = lane & 15, lq = lane >> 4;
-    const int j0 = blockIdx.z * (16 * RT);
+    const int j0 = blockIdx.y * (16 * RT);
     const int32_t* order = g.table + AdapterTable(g.m, g.count).order() + tile.first;
-    const int64_t steps = g.k / STEP, unit = (int64_t)blockIdx.y * WAVES + wave, units = (int64_t)g.splits * WAVES;
+    const int64_t steps = g.k / STEP, unit = (int64_t)split * WAVES + wave, units = (int64_t)g.splits * WAVES;
     const int s0 = (int)(steps * unit / units), s1 = (int)(steps * (unit + 1) / units);
-    const uint8_t *px[MT], *pa[RT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) px[i] = g.x + (int64_t)order[min(i * 16 + lm, tile.rows - 1)] * g.ld * SIZE;
+    const uint8_t *px = g.x + (int64_t)order[min(lm, tile.rows - 1)] * g.ld * SIZE, *pa[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) pa[i] = g.a + ((int64_t)tile.group * g.r + min(j0 + i * 16 + lm, g.r - 1)) * g.k * SIZE;
 
-    v4f_l acc[RT][MT];
+    v4f_l acc[RT] = {};
+    uint4 fx[DEPTH][2], fa[DEPTH][RT][2];
+    auto load = [&](int d, int h, int s) __attribute__((always_inline)) {
+        const int64_t at = (int64_t)s * 128 + h * 64 + lq * 16;
 #pragma unroll
-    for (int i = 0; i < RT * MT; i++) acc[i / MT][i % MT] = (v4f_l){0.f, 0.f, 0.f, 0.f};
-    uint4 fx[DEPTH][MT][2], fa[DEPTH][RT][2];
-    auto load = [&](int d, int s) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)s * 128 + lq * 32;
-#pragma unroll
-        for (int i = 0; i < RT; i++) {
-            fa[d][i][0] = load16_any(pa[i] + at);
-            fa[d][i][1] = load16_any(pa[i] + at + 16);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            fx[d][i][0] = load16_any(px[i] + at);
-            fx[d][i][1] = load16_any(px[i] + at + 16);
-        }
+        for (int i = 0; i < RT; i++) fa[d][i][h] = load16_any(pa[i] + at);
+        fx[d][h] = load16_any(px + at);
     };
-    auto multiply = [&](int d) __attribute__((always_inline)) {
+    auto multiply = [&](int d, int h) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-#pragma unroll
-                for (int j = 0; j < MT; j++) acc[i][j] = mfma_16<DT>(fa[d][i][h], fx[d][j][h], acc[i][j]);
+        for (int i = 0; i < RT; i++) acc[i] = mfma_16<DT>(fa[d][i][h], fx[d][h], acc[i]);
     };
     if (s0 < s1) {
 #pragma unroll
-        for (int d = 0; d < DEPTH; d++) load(d, min(s0 + d, s1 - 1));
+        for (int i = 0; i < 2 * DEPTH; i++) load(i / 2, i % 2, min(s0 + i / 2, s1 - 1));
         int s = s0;
         for (; s + DEPTH < s1; s += DEPTH) {
 #pragma unroll
-            for (int d = 0; d < DEPTH; d++) {
-                multiply(d);
-                load(d, min(s + DEPTH + d, s1 - 1));
+            for (int i = 0; i < 2 * DEPTH; i++) {  // what has been multiplied is asked for again at once
+                multiply(i / 2, i % 2);
+                load(i / 2, i % 2, min(s + DEPTH + i / 2, s1 - 1));
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
-        for (int d = 0; d < DEPTH; d++)
-            if (s + d < s1) multiply(d);
+        for (int i = 0; i < 2 * DEPTH; i++)
+            if (s + i / 2 < s1) multiply(i / 2, i % 2);
     }
     if (unit == units - 1 && steps * STEP < g.k) {  // what is left of the rows
-        const int at = (int)steps * STEP + lq * (STEP / 4);
+        const int at = (int)steps * STEP + lq * (STEP / 8);
 #pragma unroll 1
         for (int h = 0; h < 2; h++) {
-            uint4 ta[RT], tx[MT];
+            const uint4 tx = ln_load<DT, int>(px, at + h * (STEP / 2), g.k);
 #pragma unroll
-            for (int i = 0; i < RT; i++) ta[i] = ln_load<DT, int>(pa[i], at + h * (STEP / 8), g.k);
-#pragma unroll
-            for (int i = 0; i < MT; i++) tx[i] = ln_load<DT, int>(px[i], at + h * (STEP / 8), g.k);
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-#pragma unroll
-                for (int j = 0; j < MT; j++) acc[i][j] = mfma_16<DT>(ta[i], tx[j], acc[i][j]);
+            for (int i = 0; i < RT; i++) acc[i] = mfma_16<DT>(ln_load<DT, int>(pa[i], at + h * (STEP / 2), g.k), tx, acc[i]);
         }
     }
     // lane l: row l % 16, 4 (l / 16) + e of the rank
 #pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int j = 0; j < MT; j++) part[wave][i * MT + j][lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+    for (int i = 0; i < RT; i++) part[wave][i][lane] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
     __syncthreads();
-    for (int item = threadIdx.x; item < RT * MT * 64; item += 64 * WAVES) {
-        const int at = item >> 6, l = item & 63, row = (at % MT) * 16 + (l & 15), j = j0 + (at / MT) * 16 + 4 * (l >> 4);
+    for (int item = threadIdx.x; item < RT * 64; item += 64 * WAVES) {
+        const int at = item >> 6, l = item & 63, row = l & 15, j = j0 + at * 16 + 4 * (l >> 4);
         float4 s = part[0][at][l];
 #pragma unroll
         for (int w = 1; w < WAVES; w++) {
             const float4 p = part[w][at][l];
             s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
         }
-        if (row < tile.rows && j < g.rp) *(float4*)(g.partial + ((int64_t)blockIdx.y * g.m + tile.first + row) * g.rp + j) = s;
+        if (row < tile.rows && j < g.rp) *(float4*)(g.partial + ((int64_t)split * g.m + tile.first + row) * g.rp + j) = s;
     }
 }
 
-// ---- expand: a workgroup has 16 MT rows of one adapter and `cols` columns of out
-constexpr int EXPAND_THREADS = 256;
-template <int DT>
-constexpr int expand_pitch(int rp) { return DT == F8MI_FP32 ? rp + 4 : (rp <= 16 ? 16 : (rp + 31) / 32 * 32) * 2 + 8; }  // elements of a row of h in LDS: high parts, then low ones
-
-template <int DT, int MT>
-__global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
-    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, ROWS = 16 * MT;
-    extern __shared__ __align__(16) uint8_t expand_lds[];  // h [ROWS][pitch], then fp32 [ROWS][rp] while it is converted
-    __shared__ float row_factor[ROWS];
-    const AdapterTile tile = tiles[blockIdx.x];
-    if (tile.rows == 0) return;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, lm = lane & 15, lq = lane >> 4;
-    const bool none = tile.group >= g.count;
-    const int32_t* order = g.table + AdapterTable(g.m, g.count).order() + tile.first;
-    const int rp = g.rp, pitch = expand_pitch<DT>(rp), half = (pitch - 8) / 2;  // half: of a row's high parts (16-bit types)
-    float* sums = DT == F8MI_FP32 ? (float*)expand_lds : (float*)(expand_lds + ROWS * pitch * 2);
-    const int sums_pitch = DT == F8MI_FP32 ? pitch : rp;
-    if (!none) {
-        const float scale = g.factor * (g.scale ? g.scale[tile.group] : 1.f);
-        for (int item = t; item < ROWS * (rp / 4); item += EXPAND_THREADS) {
-            const int row = item / (rp / 4), j = (item % (rp / 4)) * 4;
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row < tile.rows) {
-                const float* p = g.partial + ((int64_t)tile.first + row) * rp + j;
-#pragma unroll 4
-                for (int i = 0; i < g.splits; i++) {
-                    const float4 q = *(const float4*)(p + i * g.m * rp);
-                    s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
-                }
-                if (j >= g.r) s.x = 0.f;  // (rows of A past the last are the last again)
-                if (j + 1 >= g.r) s.y = 0.f;
-                if (j + 2 >= g.r) s.z = 0.f;
-                if (j + 3 >= g.r) s.w = 0.f;
-                if (g.h && blockIdx.y == 0) *(float4*)(g.h + ((int64_t)tile.first + row) * rp + j) = s;
-            }
-            *(float4*)(sums + row * sums_pitch + j) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+// 64 rows of one adapter and 16 RT of its rank a workgroup: a wave has 16 of the rows and brings them itself, all four multiply them by the same part of A, which goes through LDS: BYTES
+// of each of its rows at a time, the next ones (and the next ones of x) on their way meanwhile.  A workgroup has a part of the contraction; nothing is left to add up inside it.
+constexpr int TALL_THREADS = 256;
+template <int DT, int RT, int BYTES>
+__global__ __launch_bounds__(TALL_THREADS, 4) void adapter_shrink_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, PIECES = BYTES / 16, KP = RT * 16 * PIECES / TALL_THREADS, PITCH = BYTES + 16, STEP = BYTES / SIZE;
+    __shared__ __align__(16) uint8_t lds_a[2][RT * 16 * PITCH];
+    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), split = id % g.splits;  // a tile's workgroups, and those of the next ones, on one XCD: A stays in its L2
+    const AdapterTile tile = tiles[id / g.splits];
+    if (tile.rows == 0 || tile.group >= g.count) return;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, lm = lane & 15, lq = lane >> 4, j0 = blockIdx.y * (16 * RT);
+    const int steps = (g.k + STEP - 1) / STEP, s0 = (int)((int64_t)steps * split / g.splits), s1 = (int)((int64_t)steps * (split + 1) / g.splits);
+    const int64_t x_row = (int64_t)g.table[AdapterTable(g.m, g.count).order() + tile.first + min(wave * 16 + lm, tile.rows - 1)] * g.ld, x_total = (g.m - 1) * g.ld + g.k;
+    const int64_t a_first = ((int64_t)tile.group * g.r + j0) * g.k, a_total = (int64_t)g.count * g.r * g.k;
+    v4f_l acc[RT] = {};
+    uint4 fa[KP], fx[PIECES / 4], next_x[PIECES / 4];
+    // (a step that ends with the row or before it, the same for the workgroup, needs no edges)
+    auto load_x = [&](int s, uint4 (&q)[PIECES / 4]) __attribute__((always_inline)) {
+        const int k0 = s * STEP + lq * V;
+        if ((s + 1) * STEP <= g.k) {
+#pragma unroll
+            for (int i = 0; i < PIECES / 4; i++) q[i] = load16_any(g.x + (x_row + k0 + i * 4 * V) * SIZE);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES / 4; i++) q[i] = load_of_row<DT, false>(g.x, x_row + k0 + i * 4 * V, x_total, k0 + i * 4 * V, g.k);
         }
+    };
+    auto load_a = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < KP; i++) {
+            const int item = i * TALL_THREADS + t, row = min(item / PIECES, g.r - 1 - j0), k = s * STEP + item % PIECES * V;
+            if ((s + 1) * STEP <= g.k) fa[i] = load16_any(g.a + (a_first + (int64_t)row * g.k + k) * SIZE);
+            else fa[i] = load_of_row<DT, false>(g.a, a_first + (int64_t)row * g.k + k, a_total, k, g.k);
+        }
+    };
+    auto keep_a = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < KP; i++) {
+            const int item = i * TALL_THREADS + t;
+            *(uint4*)(lds_a[buffer] + item / PIECES * PITCH + item % PIECES * 16) = fa[i];
+        }
+    };
+    if (s0 < s1) {
+        load_a(s0);
+        load_x(s0, fx);
+        keep_a(0);
         __syncthreads();
-        if constexpr (DT != F8MI_FP32) {
-            if constexpr (DT == F8MI_FP16) {  // a power of two that brings the row's largest to [1, 2)
-                if (t < ROWS) {
-                    uint32_t most = 0u;
-                    for (int j = 0; j < g.r; j++) most = max(most, __float_as_uint(sums[t * rp + j]) & 0x7fffffffu);
-                    const int e = min(max((int)(most >> 23), 1), 253);
-                    row_factor[t] = __uint_as_float((uint32_t)e << 23);  // 2^(e - 127)
-                }
-                __syncthreads();
-            }
-            uint16_t* kept = (uint16_t*)expand_lds;
-            for (int item = t; item < ROWS * half; item += EXPAND_THREADS) {
-                const int row = item / half, j = item % half;
-                float v = j < rp ? sums[row * rp + j] : 0.f;
-                if constexpr (DT == F8MI_FP16) v *= __uint_as_float((254u << 23) - __float_as_uint(row_factor[row]));  // times 2^(127 - e)
-                const uint32_t high = pack2<DT>(v, 0.f) & 0xffffu;
-                float back, zero;
-                unpack2<DT>(high, back, zero);
-                kept[row * pitch + j] = (uint16_t)high;
-                kept[row * pitch + half + j] = (uint16_t)pack2<DT>(back - back == 0.f ? v - back : 0.f, 0.f);  // (nothing is left of an infinity)
-            }
-            __syncthreads();
+    }
+    for (int s = s0, buffer = 0; s < s1; s++, buffer ^= 1) {
+        const bool more = s + 1 < s1;
+        if (more) {
+            load_x(s + 1, next_x);
+            load_a(s + 1);
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES / 4; i++)
+#pragma unroll
+            for (int j = 0; j < RT; j++) acc[j] = mfma_16<DT>(*(const uint4*)(lds_a[buffer] + (j * 16 + lm) * PITCH + i * 64 + lq * 16), fx[i], acc[j]);
+        if (more) {
+            keep_a(buffer ^ 1);
+            lds_barrier();
+#pragma unroll
+            for (int i = 0; i < PIECES / 4; i++) fx[i] = next_x[i];
         }
     }
-    const uint8_t* hrow[MT];  // of the lane's row in LDS
-    float factor[MT];
-    int64_t at_row[MT];
+    const int row = wave * 16 + lm;
+    if (row < tile.rows)
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        hrow[i] = expand_lds + (i * 16 + lm) * pitch * SIZE;
-        factor[i] = DT == F8MI_FP16 && !none ? row_factor[i * 16 + lm] : 1.f;
-        at_row[i] = order[min(i * 16 + lm, tile.rows - 1)];
+        for (int j = 0; j < RT; j++)
+            if (j0 + j * 16 < g.rp) *(float4*)(g.partial + ((int64_t)split * g.m + tile.first + row) * g.rp + j0 + j * 16 + 4 * lq) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+}
+
+// ---- expand: a workgroup has 16 WR rows of one adapter and `cols` columns of out
+constexpr int EXPAND_THREADS = 256;
+// Of a row of h in LDS: 16-bit types have its high parts, then its low ones, `half` elements each: whole instructions of 32, or 16, where one instruction takes both.
+__host__ __device__ constexpr int expand_half(int rp) { return rp <= 16 ? 16 : (rp + 31) / 32 * 32; }
+template <int DT>
+__host__ __device__ constexpr int expand_pitch(int rp) { return DT == F8MI_FP32 ? rp + 4 : expand_half(rp) * 2 + 8; }
+
+// The parts of h that the contraction's parts gave, added up, scaled and kept in LDS as the products take them: rows first .. of the table's order.  `sums` (fp16 alone): fp32
+// [ROWS][half] beside them, free afterwards.
+template <int DT, int ROWS>
+__device__ __forceinline__ void stage_h(const AdapterArgs& g, const AdapterTile& tile, bool first, uint8_t* kept_bytes, float* sums, uint32_t* row_most, float& factor, int my_row) {
+    const int t = threadIdx.x, rp = g.rp, pitch = expand_pitch<DT>(rp), half = DT == F8MI_FP32 ? rp : expand_half(rp), quads = half / 4;
+    const float scale = g.factor * (g.scale ? g.scale[tile.group] : 1.f);
+    auto keep = [&](int row, int j, const float (&v)[4]) __attribute__((always_inline)) {
+        uint32_t high[2], low[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float a, b;
+            high[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+            unpack2<DT>(high[i], a, b);
+            low[i] = pack2<DT>(a - a == 0.f ? v[2 * i] - a : 0.f, b - b == 0.f ? v[2 * i + 1] - b : 0.f);  // (nothing is left of an infinity)
+        }
+        uint16_t* at = (uint16_t*)kept_bytes + row * pitch + j;
+        *(uint2*)at = make_uint2(high[0], high[1]);
+        *(uint2*)(at + half) = make_uint2(low[0], low[1]);
+    };
+    if constexpr (DT == F8MI_FP16) {
+        if (t < ROWS) row_most[t] = 0u;
+        __syncthreads();
     }
-    const int end = min(g.n, (int)(blockIdx.y + 1) * g.cols);
-    for (int n0 = blockIdx.y * g.cols + wave * 64; n0 < end; n0 += 256) {
-        const int col = n0 + lq * 16;  // of out: 16 neighbouring ones of each of the lane's rows
-        uint4 fy[MT][16 / V];
+    for (int item = t; item < ROWS * quads; item += EXPAND_THREADS) {
+        const int row = item / quads, j = (item - row * quads) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (row < tile.rows && j < rp) {
+            const float* p = g.partial + ((int64_t)tile.first + row) * rp + j;
+#pragma unroll 4
+            for (int i = 0; i < g.splits; i++) {
+                const float4 q = *(const float4*)(p + i * g.m * rp);
+                v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+            }
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+            for (int e = 0; e < 4; e++)
+                if (j + e >= g.r) v[e] = 0.f;  // (rows of A past the last are the last again)
+            if (g.h && first) *(float4*)(g.h + ((int64_t)tile.first + row) * rp + j) = make_float4(v[0], v[1], v[2], v[3]);
+        }
 #pragma unroll
-            for (int p = 0; p < 16 / V; p++)
-                fy[i][p] = g.y ? ln_load<DT, int>(g.y + at_row[i] * g.ld_y * SIZE, col + p * V, g.n) : make_uint4(0u, 0u, 0u, 0u);
-        v4f_l acc[MT][4];
+        for (int e = 0; e < 4; e++) v[e] *= scale;
+        if constexpr (DT == F8MI_BF16) keep(row, j, v);
+        else *(float4*)(DT == F8MI_FP32 ? (float*)kept_bytes + row * pitch + j : sums + item * 4) = make_float4(v[0], v[1], v[2], v[3]);
+        if constexpr (DT == F8MI_FP16) {
+            uint32_t most = 0u;
 #pragma unroll
-        for (int i = 0; i < MT * 4; i++) acc[i / 4][i % 4] = (v4f_l){0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; e++) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+            atomicMax(&row_most[row], most);  // (in LDS; a maximum has no order)
+        }
+    }
+    __syncthreads();
+    factor = 1.f;
+    if constexpr (DT == F8MI_FP16) {  // a power of two, 2^(e - 127), that brings the row's largest to [1, 2)
+        auto exponent = [&](int row) __attribute__((always_inline)) { return (uint32_t)min(max((int)(row_most[row] >> 23), 1), 253); };
+        for (int item = t; item < ROWS * quads; item += EXPAND_THREADS) {
+            const int row = item / quads;
+            const float4 q = *(const float4*)(sums + item * 4);
+            const float f = __uint_as_float((254u - exponent(row)) << 23);
+            const float v[4] = {q.x * f, q.y * f, q.z * f, q.w * f};
+            keep(row, (item - row * quads) * 4, v);
+        }
+        factor = __uint_as_float(exponent(my_row) << 23);
+        __syncthreads();
+    }
+}
+
+// Of out and y, 64 columns from n0: a lane's pieces of 16 bytes of its row, those of the four lanes that share it next to each other, so that an instruction takes 64 bytes of each row.
+// (Not past the caches: these are half lines; a copy of 8192 x 14336 in such pieces takes 95 us, past the caches 122.)
+// EDGE: some may lie past the last.
+template <int DT, bool EDGE>
+struct ExpandCols {
+    static constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, PIECES = 16 / V;
+    int n0, n, lq, lm;
+    __device__ __forceinline__ int col(int p) const { return n0 + p * 4 * V + lq * V; }
+    // row q of the matrix instructions' tile c: four columns of piece c / (V / 4) of the lane q / 4
+    __device__ __forceinline__ int of_tile(int c) const { return n0 + c / (V / 4) * 4 * V + (lm >> 2) * V + c % (V / 4) * 4 + (lm & 3); }
+    __device__ __forceinline__ bool inside() const { return !EDGE || n0 + 64 <= n; }  // the same for the wave
+    __device__ __forceinline__ void load(const uint8_t* row, uint4 (&q)[PIECES]) const {
+        if (inside()) {
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) q[p] = load16_any(row + (int64_t)col(p) * SIZE);
+        } else {
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) q[p] = ln_load<DT, int>(row, col(p), n);
+        }
+    }
+    // y + acc * factor (adapted: a row without an adapter keeps y's bits)
+    __device__ __forceinline__ void store(uint8_t* row, const uint4 (&q)[PIECES], const v4f_l* acc, float factor, bool adapted) const {
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+            float v[V];
+            ln_unpack<DT>(q[p], v);
+            if (adapted)
+#pragma unroll
+                for (int e = 0; e < V; e++) v[e] = __builtin_fmaf(acc[(p * V + e) / 4][e % 4], factor, v[e]);
+            if (inside()) store16_any(row + (int64_t)col(p) * SIZE, ln_pack<DT>(v));
+            else if (col(p) < n) ln_store<DT, int>(row, col(p), n, v);
+        }
+    }
+};
+
+// A wave has 16 rows and 64 columns at a time, the waves below each other (WR 4) or side by side (1); B straight out of the caches.
+template <int DT, int WR, bool WHOLE>
+__global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+    constexpr int SIZE = Ln<DT>::SIZE, ROWS = 16 * WR, STEP = WR > 1 ? 64 : 256;
+    extern __shared__ __align__(16) uint8_t expand_lds[];  // h [ROWS][pitch], then (fp16) fp32 [ROWS][half] while it is converted
+    __shared__ uint32_t row_most[DT == F8MI_FP16 ? ROWS : 1];
+    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), chunk = id % g.chunks;  // a tile's workgroups, and those of the next ones, on one XCD: B stays in its L2
+    const AdapterTile tile = tiles[id / g.chunks];
+    if (tile.rows == 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lm = lane & 15, lq = lane >> 4;
+    const bool none = tile.group >= g.count;
+    const int rp = g.rp, pitch = expand_pitch<DT>(rp), half = expand_half(rp);
+    const int my_row = (WR > 1 ? wave * 16 : 0) + lm;
+    float factor = 1.f;
+    if (!none) stage_h<DT, ROWS>(g, tile, chunk == 0, expand_lds, (float*)(expand_lds + ROWS * pitch * SIZE), row_most, factor, my_row);
+    if (WR > 1 && wave * 16 >= tile.rows) return;
+    const int64_t at_row = g.table[AdapterTable(g.m, g.count).order() + tile.first + min(my_row, tile.rows - 1)];
+    const uint8_t *hrow = expand_lds + my_row * pitch * SIZE, *y_row = g.y + at_row * g.ld_y * SIZE;
+    uint8_t* out_row = g.out + at_row * g.n * SIZE;
+    const int end = min(g.n, (chunk + 1) * g.cols);
+    const int64_t b_total = (int64_t)g.count * g.n * g.r;
+    for (int n0 = chunk * g.cols + (WR > 1 ? 0 : wave * 64); n0 < end; n0 += STEP) {
+        const ExpandCols<DT, true> at{n0, g.n, lq, lm};
+        uint4 fy[ExpandCols<DT, true>::PIECES] = {};
+        if (g.y) at.load(y_row, fy);
+        v4f_l acc[4] = {};
         if (!none) {
-            // tile c's row q of B: column n0 + 16 (q / 4) + 4 c + q % 4, so that a lane's four tiles give it neighbours
-            const uint8_t* pb[4];
+            int64_t pb[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) pb[c] = g.b + ((int64_t)tile.group * g.n + min(n0 + 16 * (lm >> 2) + 4 * c + (lm & 3), g.n - 1)) * g.r * SIZE;
+            for (int c = 0; c < 4; c++) pb[c] = ((int64_t)tile.group * g.n + min(at.of_tile(c), g.n - 1)) * g.r;
+            auto load_b = [&](uint4 (&fb)[4], int j) __attribute__((always_inline)) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) fb[c] = load_of_row<DT, WHOLE>(g.b, pb[c] + j, b_total, j, g.r);
+            };
             if constexpr (DT == F8MI_FP32) {
                 for (int j = 0; j < rp; j += 16) {
                     uint4 fb[4];
+                    load_b(fb, j + lq * 4);
+                    const uint4 fh = *(const uint4*)(hrow + (j + lq * 4) * 4);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) fb[c] = ln_load<DT, int>(pb[c], j + lq * 4, g.r);
-#pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        const uint4 fh = *(const uint4*)(hrow[i] + (j + lq * 4) * 4);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) acc[i][c] = mfma_16<DT>(fb[c], fh, acc[i][c]);
-                    }
+                    for (int c = 0; c < 4; c++) acc[c] = mfma_16<DT>(fb[c], fh, acc[c]);
                 }
             } else if (half == 16) {  // both parts of h in one instruction, B twice
                 uint4 fb[4];
+                load_b(fb, (lq & 1) * 8);
+                const uint4 fh = *(const uint4*)(hrow + lq * 16);
 #pragma unroll
-                for (int c = 0; c < 4; c++) fb[c] = ln_load<DT, int>(pb[c], (lq & 1) * 8, g.r);
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    const uint4 fh = *(const uint4*)(hrow[i] + lq * 16);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) acc[i][c] = mfma_16<DT>(fb[c], fh, acc[i][c]);
-                }
+                for (int c = 0; c < 4; c++) acc[c] = mfma_16<DT>(fb[c], fh, acc[c]);
             } else {
-                for (int j = 0; j < half; j += 32) {
-                    uint4 fb[4];
+                uint4 fb[2][4];  // the next part of the rank is on its way while one is multiplied
+                load_b(fb[0], lq * 8);
+                for (int j = 0; j < half; j += 64) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) fb[c] = ln_load<DT, int>(pb[c], j + lq * 8, g.r);
+                    for (int d = 0; d < 2; d++) {
+                        const int k = j + d * 32;
+                        if (k >= half) break;
+                        if (k + 32 < half) load_b(fb[d ^ 1], k + 32 + lq * 8);
+                        const uint4 high = *(const uint4*)(hrow + (k + lq * 8) * 2), low = *(const uint4*)(hrow + (half + k + lq * 8) * 2);
 #pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        const uint4 high = *(const uint4*)(hrow[i] + (j + lq * 8) * 2), low = *(const uint4*)(hrow[i] + (half + j + lq * 8) * 2);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) acc[i][c] = mfma_16<DT>(fb[c], low, mfma_16<DT>(fb[c], high, acc[i][c]));
+                        for (int c = 0; c < 4; c++) acc[c] = mfma_16<DT>(fb[d][c], low, mfma_16<DT>(fb[d][c], high, acc[c]));
                     }
                 }
             }
         }
+        if (my_row < tile.rows) at.store(out_row, fy, acc, factor, !none);
+    }
+}
+
+// 64 rows and B through LDS, 16-bit types: the four waves have 16 rows each and the same columns, CB of them at a time, so that B is read once a workgroup.  The next
+// CB columns of B and of y are on their way while these are multiplied.  The last of them are moved back to end with the last column (their first are
+// then computed twice, the same): no access has an edge.  MOST: the largest expand_half.
+template <int DT, int MOST, int CB, bool WHOLE>
+__global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+    constexpr int SIZE = 2, ROWS = 64, SUB = CB / 64, PIECES = ExpandCols<DT, false>::PIECES;
+    constexpr int KP = CB * MOST / 8 / EXPAND_THREADS;  // pieces of 16 bytes of B that a lane brings
+    constexpr int KH = MOST <= 64 ? (MOST + 31) / 32 : 0;  // of a rank of up to 64 the wave's h stays in registers
+    extern __shared__ __align__(16) uint8_t expand_lds[];  // h [ROWS][pitch], then (fp16) fp32 [ROWS][half] while it is converted and B [2][CB][half + 8] from then on
+    __shared__ uint32_t row_most[DT == F8MI_FP16 ? ROWS : 1];
+    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), chunk = id % g.chunks;  // a tile's workgroups, and those of the next ones, on one XCD: B stays in its L2
+    const AdapterTile tile = tiles[id / g.chunks];
+    if (tile.rows == 0) return;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, lm = lane & 15, lq = lane >> 4;
+    const bool none = tile.group >= g.count;
+    const int rp = g.rp, half = KH ? MOST : expand_half(rp), pitch = 2 * half + 8, b_pitch = half + 8, row_pieces = half / 8;
+    uint8_t* const behind = expand_lds + ROWS * pitch * 2;
+    uint16_t* const lds_b = (uint16_t*)behind;
+    const int my_row = wave * 16 + lm;
+    const int64_t at_row = g.table[AdapterTable(g.m, g.count).order() + tile.first + min(my_row, tile.rows - 1)];
+    const uint8_t* y_row = g.y + at_row * g.ld_y * SIZE;
+    uint8_t* out_row = g.out + at_row * g.n * SIZE;
+    const int begin = chunk * g.cols, end = min(g.n, begin + g.cols), last = g.n - CB;
+    const int64_t b_total = (int64_t)g.count * g.n * g.r;
+    uint4 fb[KP], fy[SUB][PIECES] = {}, next_y[SUB][PIECES] = {};
+    auto load_b = [&](int n0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-            if (i * 16 + lm >= tile.rows) continue;
+        for (int i = 0; i < KP; i++) {
+            const int item = i * EXPAND_THREADS + t, row = item / row_pieces, j = (item - row * row_pieces) * 8;
+            if (item < CB * row_pieces) fb[i] = load_of_row<DT, WHOLE>(g.b, ((int64_t)tile.group * g.n + n0 + row) * g.r + j, b_total, j, g.r);
+        }
+    };
+    auto keep_b = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
-            for (int p = 0; p < 16 / V; p++) {
-                if (col + p * V >= g.n) continue;
-                float v[V];
-                ln_unpack<DT>(fy[i][p], v);
-                if (!none)  // (-0 + 0 is 0: a row without an adapter keeps its bits)
+        for (int i = 0; i < KP; i++) {
+            const int item = i * EXPAND_THREADS + t, row = item / row_pieces, j = (item - row * row_pieces) * 8;
+            if (item < CB * row_pieces) *(uint4*)(lds_b + (buffer * CB + row) * b_pitch + j) = fb[i];
+        }
+    };
+    auto load_y = [&](int n0, uint4 (&q)[SUB][PIECES]) __attribute__((always_inline)) {
+        if (g.y)
 #pragma unroll
-                    for (int e = 0; e < V; e++) v[e] = __builtin_fmaf(acc[i][(p * V + e) / 4][e % 4], factor[i], v[e]);
-                ln_store<DT, int>(g.out + at_row[i] * g.n * SIZE, col + p * V, g.n, v);
+            for (int u = 0; u < SUB; u++) ExpandCols<DT, false>{n0 + u * 64, g.n, lq, lm}.load(y_row, q[u]);
+    };
+    load_y(min(begin, last), fy);
+    float factor = 1.f;
+    if (!none) {
+        load_b(min(begin, last));
+        stage_h<DT, ROWS>(g, tile, chunk == 0, expand_lds, (float*)behind, row_most, factor, my_row);
+        keep_b(0);
+        __syncthreads();
+    }
+    const uint16_t* hrow = (const uint16_t*)expand_lds + my_row * pitch;
+    uint4 fh[KH ? KH : 1][2] = {};
+    if (!none)
+#pragma unroll
+        for (int k = 0; k < KH; k++) {
+            fh[k][0] = *(const uint4*)(hrow + k * 32 + lq * 8);
+            if constexpr (MOST > 16) fh[k][1] = *(const uint4*)(hrow + half + k * 32 + lq * 8);
+        }
+    int buffer = 0;
+    for (int n0 = begin; n0 < end; n0 += CB, buffer ^= 1) {
+        const bool more = n0 + CB < end;  // the same for the workgroup
+        if (more) {
+            load_y(min(n0 + CB, last), next_y);
+            if (!none) load_b(min(n0 + CB, last));
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; u++) {
+            const ExpandCols<DT, false> at{min(n0, last) + u * 64, g.n, lq, lm};
+            v4f_l acc[4] = {};
+            if (!none) {
+                const uint16_t* pb[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) pb[c] = lds_b + (buffer * CB + at.of_tile(c) - min(n0, last)) * b_pitch;
+                if constexpr (MOST == 16) {  // a rank of up to 16: both parts of h in one instruction, B twice
+#pragma unroll
+                    for (int c = 0; c < 4; c++) acc[c] = mfma_16<DT>(*(const uint4*)(pb[c] + (lq & 1) * 8), fh[0][0], acc[c]);
+                } else if constexpr (KH > 0) {
+#pragma unroll
+                    for (int k = 0; k < KH; k++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const uint4 q = *(const uint4*)(pb[c] + k * 32 + lq * 8);
+                            acc[c] = mfma_16<DT>(q, fh[k][1], mfma_16<DT>(q, fh[k][0], acc[c]));
+                        }
+                } else {
+#pragma unroll 1
+                    for (int k = lq * 8; k < half; k += 32) {
+                        const uint4 high = *(const uint4*)(hrow + k), low = *(const uint4*)(hrow + half + k);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const uint4 q = *(const uint4*)(pb[c] + k);
+                            acc[c] = mfma_16<DT>(q, low, mfma_16<DT>(q, high, acc[c]));
+                        }
+                    }
+                }
             }
+            if (my_row < tile.rows) at.store(out_row, fy[u], acc, factor, !none);
+        }
+        if (more) {
+            if (!none) {
+                keep_b(buffer ^ 1);
+                lds_barrier();
+            }
+#pragma unroll
+            for (int u = 0; u < SUB; u++)
+#pragma unroll
+                for (int p = 0; p < PIECES; p++) fy[u][p] = next_y[u][p];
         }
     }
 }
@@ -400,29 +624,33 @@ struct AdapterShape {
     // Tiles of 64 rows where an adapter has that many on average: x is read once for each 64 of the rank, an adapter once a tile.
     bool tall() const { return m >= 48 * (count < m ? count : m); }
     int64_t tiles() const { return table().tiles(tall() ? 64 : 16); }
-    // Parts of a contraction of this length: two workgroups a CU, and two steps a wave
+    // Parts of a contraction of this length: four workgroups a CU, and two steps at least (of a workgroup, of each wave of one for short tiles)
     int64_t splits(int64_t contracted) const {
-        const int64_t steps = contracted * (dtype == F8MI_FP32 ? 4 : 2) / 128, waves = tall() ? 4 : 8, want = 2 * (int64_t)cu_count() / std::max<int64_t>(1, tiles() * ((rp() + 63) / 64));
-        return std::max<int64_t>(1, std::min({want, steps / (2 * waves), (int64_t)32}));
+        const int64_t bytes = contracted * (dtype == F8MI_FP32 ? 4 : 2), steps = tall() ? bytes / (rp() <= 16 ? 512 : 256) : bytes / (128 * SHRINK_WAVES);
+        const int64_t want = 4 * (int64_t)cu_count() / std::max<int64_t>(1, tiles() * ((rp() + 63) / 64));
+        return std::max<int64_t>(1, std::min({want, steps / 2, (int64_t)32}));
     }
     int64_t partial_bytes(int64_t contracted) const { return splits(contracted) * m * rp() * 4; }
 };
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-template <int DT, int MT, int WAVES>
-static int launch_shrink3(const AdapterArgs& g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
-    const int rt = g.rp / 16;
-    const dim3 grid((unsigned)n_tiles, (unsigned)g.splits, (unsigned)(rt <= 4 ? 1 : (rt + 3) / 4));
-    if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<DT, MT, 1, WAVES>), grid, dim3(64 * WAVES), 0, stream, g, tiles);
-    else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_kernel<DT, MT, 2, WAVES>), grid, dim3(64 * WAVES), 0, stream, g, tiles);
-    else hipLaunchKernelGGL((adapter_shrink_kernel<DT, MT, 4, WAVES>), grid, dim3(64 * WAVES), 0, stream, g, tiles);
-    return check_hip(hipGetLastError(), "adapter shrink kernel launch");
-}
 template <int DT>
 static int launch_shrink2(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     const AdapterTable table = s.table();
-    if (s.tall()) return launch_shrink3<DT, 4, 4>(g, (const AdapterTile*)(g.table + table.tiles64()), s.tiles(), stream);
-    return launch_shrink3<DT, 1, 8>(g, (const AdapterTile*)(g.table + table.tiles16()), s.tiles(), stream);
+    const int rt = g.rp / 16;
+    const dim3 grid((unsigned)(s.tiles() * g.splits), (unsigned)(rt <= 4 ? 1 : (rt + 3) / 4));
+    if (s.tall()) {
+        const AdapterTile* tiles = (const AdapterTile*)(g.table + table.tiles64());
+        if (rt == 1) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 512>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 2, 256>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        else hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 4, 256>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+    } else {
+        const AdapterTile* tiles = (const AdapterTile*)(g.table + table.tiles16());
+        if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<DT, 1>), grid, dim3(64 * SHRINK_WAVES), 0, stream, g, tiles);
+        else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_kernel<DT, 2>), grid, dim3(64 * SHRINK_WAVES), 0, stream, g, tiles);
+        else hipLaunchKernelGGL((adapter_shrink_kernel<DT, 4>), grid, dim3(64 * SHRINK_WAVES), 0, stream, g, tiles);
+    }
+    return check_hip(hipGetLastError(), "adapter shrink kernel launch");
 }
 static int launch_shrink(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     if (s.dtype == F8MI_BF16) return launch_shrink2<F8MI_BF16>(g, s, stream);
@@ -430,23 +658,50 @@ static int launch_shrink(const AdapterArgs& g, const AdapterShape& s, hipStream_
     return launch_shrink2<F8MI_FP32>(g, s, stream);
 }
 
-template <int DT, int MT>
-static int launch_expand3(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
-    // four workgroups a CU, each with as many columns as that leaves
-    const int64_t want = std::max<int64_t>(1, 4 * (int64_t)cu_count() / n_tiles), blocks = std::max(1, (g.n + 255) / 256);  // (one, without columns, where h alone is asked for)
-    g.cols = (int)((blocks + want - 1) / want * 256);
-    const int lds = 16 * MT * (DT == F8MI_FP32 ? expand_pitch<DT>(g.rp) * 4 : expand_pitch<DT>(g.rp) * 2 + g.rp * 4);
-    const auto kernel = adapter_expand_kernel<DT, MT>;
-    static std::atomic<uint64_t> allowed{0};
+// Columns of out a workgroup: `per_cu` workgroups a CU in all, whole blocks of `block` columns
+static int expand_cols(const AdapterArgs& g, int64_t n_tiles, int per_cu, int block) {
+    const int64_t want = std::max<int64_t>(1, per_cu * (int64_t)cu_count() / n_tiles), blocks = std::max(1, (g.n + block - 1) / block);  // (one where h alone is asked for)
+    return (int)((blocks + want - 1) / want * block);
+}
+template <typename K>
+static int launch_expand_kernel(K kernel, std::atomic<uint64_t>& allowed, AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, int lds, hipStream_t stream) {
     if (int rc = allow_big_lds(kernel, (160 << 10) - 1024, allowed)) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)n_tiles, (unsigned)((blocks * 256 + g.cols - 1) / g.cols)), dim3(EXPAND_THREADS), (unsigned)lds, stream, g, tiles);
+    g.chunks = std::max(1, (g.n + g.cols - 1) / g.cols);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(n_tiles * g.chunks)), dim3(EXPAND_THREADS), (unsigned)lds, stream, g, tiles);
     return check_hip(hipGetLastError(), "adapter expand kernel launch");
+}
+template <int DT, int WR, bool WHOLE>
+static int launch_expand_direct(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
+    static std::atomic<uint64_t> allowed{0};
+    g.cols = expand_cols(g, n_tiles, WR > 1 ? 8 : 4, 256);
+    return launch_expand_kernel(adapter_expand_kernel<DT, WR, WHOLE>, allowed, g, tiles, n_tiles, 16 * WR * (expand_pitch<DT>(g.rp) * Ln<DT>::SIZE + (DT == F8MI_FP16 ? expand_half(g.rp) * 4 : 0)), stream);
+}
+template <int DT, int MOST, int CB, bool WHOLE>
+static int launch_expand_tall(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
+    static std::atomic<uint64_t> allowed{0};
+    g.cols = expand_cols(g, n_tiles, 8, CB);
+    const int lds = 64 * expand_pitch<DT>(g.rp) * 2 + std::max(DT == F8MI_FP16 ? 64 * expand_half(g.rp) * 4 : 0, 2 * CB * (expand_half(g.rp) + 8) * 2);
+    return launch_expand_kernel(adapter_expand_tall_kernel<DT, MOST, CB, WHOLE>, allowed, g, tiles, n_tiles, lds, stream);
+}
+template <int DT, bool WHOLE>
+static int launch_expand3(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
+    const AdapterTable table = s.table();
+    const AdapterTile *short_tiles = (const AdapterTile*)(g.table + table.tiles16()), *tall_tiles = (const AdapterTile*)(g.table + table.tiles64());
+    if (!s.tall()) return launch_expand_direct<DT, 1, WHOLE>(g, short_tiles, s.tiles(), stream);
+    const int half = expand_half(g.rp);
+    if (DT == F8MI_FP32 || g.n < (half <= 32 ? 128 : 64)) return launch_expand_direct<DT, 4, WHOLE>(g, tall_tiles, s.tiles(), stream);
+    if constexpr (DT != F8MI_FP32) {
+        if (half == 16) return launch_expand_tall<DT, 16, 128, WHOLE>(g, tall_tiles, s.tiles(), stream);
+        if (half == 32) return launch_expand_tall<DT, 32, 128, WHOLE>(g, tall_tiles, s.tiles(), stream);
+        if (half == 64) return launch_expand_tall<DT, 64, 64, WHOLE>(g, tall_tiles, s.tiles(), stream);
+        if (half <= 128) return launch_expand_tall<DT, 128, 64, WHOLE>(g, tall_tiles, s.tiles(), stream);
+        return launch_expand_tall<DT, 256, 64, WHOLE>(g, tall_tiles, s.tiles(), stream);
+    }
+    return F8MI_ERR_UNSUPPORTED;  // (not reached)
 }
 template <int DT>
 static int launch_expand2(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
-    const AdapterTable table = s.table();
-    if (s.tall()) return launch_expand3<DT, 4>(g, (const AdapterTile*)(g.table + table.tiles64()), s.tiles(), stream);
-    return launch_expand3<DT, 1>(g, (const AdapterTile*)(g.table + table.tiles16()), s.tiles(), stream);
+    return g.r % Ln<DT>::V == 0 ? launch_expand3<DT, true>(g, s, stream) : launch_expand3<DT, false>(g, s, stream);
 }
 static int launch_expand(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     if (s.dtype == F8MI_BF16) return launch_expand2<F8MI_BF16>(g, s, stream);
@@ -517,7 +772,7 @@ extern "C" int f8mi_adapters(const void* x, int64_t ldx, const void* a, const vo
     const int64_t need = s.partial_bytes(k);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0 || (uintptr_t)table % 16 != 0 || (uintptr_t)h % 16 != 0) { set_error("f8mi_adapters: 16-byte aligned workspace of %lld bytes, table and h", (long long)need); return F8MI_ERR_INVALID_ARG; }
     const AdapterArgs g{(const uint8_t*)x, ldx, (const uint8_t*)a, (const int32_t*)table, (float*)workspace, m, (int)k, (int)r, (int)s.rp(), (int)count, (int)s.splits(k),
-                        (const uint8_t*)b, scale, factor, (const uint8_t*)y, ldy, (uint8_t*)out, h, (int)n, 0};
+                        (const uint8_t*)b, scale, factor, (const uint8_t*)y, ldy, (uint8_t*)out, h, (int)n, 0, 0};
     if (int rc = launch_shrink(g, s, stream)) return rc;
     return launch_expand(g, s, stream);
 }
@@ -540,7 +795,7 @@ extern "C" int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const v
         if (dx)
             if (int rc = launch_transpose(a, ws + space.at, count, (int)r, (int)k, dtype, stream)) return rc;
         const AdapterArgs g{(const uint8_t*)dout, ld_dout, ws + space.bt, (const int32_t*)table, (float*)(ws + space.partial), m, (int)n, (int)r, (int)s.rp(), (int)count, (int)s.splits(n),
-                            dx ? ws + space.at : nullptr, scale, factor, nullptr, 0, (uint8_t*)dx, dh, dx ? (int)k : 0, 0};
+                            dx ? ws + space.at : nullptr, scale, factor, nullptr, 0, (uint8_t*)dx, dh, dx ? (int)k : 0, 0, 0};
         if (int rc = launch_shrink(g, s, stream)) return rc;
         if (int rc = launch_expand(g, s, stream)) return rc;
     }
