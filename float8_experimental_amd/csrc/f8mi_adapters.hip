@@ -579,6 +579,135 @@ __global__ __launch_bounds__(OUTER_THREADS) void adapter_outer_kernel(const Oute
             }
 }
 
+// The same for 16-bit types on their matrix instructions.  Both operands are wanted eight rows a lane and lie in LDS by rows: the reads turn them (ds_read_b64_tr_b16: of 4 rows x 16 columns
+// each of 16 lanes gets a column).  small goes in as two bf16 values, high and low; fp16 values of big too, exactly, so that neither overflows or falls among the subnormals: bf16 has the
+// exponents of fp32.  A row of 128 columns is 256 bytes; a pitch of 288 and rows 8 .. 15 of 16 turned by half a row let the 32 lanes that read at a time reach all banks.
+// COLS_FIRST: sums [cols][r], so that a lane has four neighbours of the rank, else of the columns.
+constexpr int OUTER_STEP = 64, OUTER_PITCH = 288;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ int outer_at(int row, int byte) { return row * OUTER_PITCH + (byte ^ ((row >> 3 & 1) * 128)); }
+// rows row .. row + 7 of the lane's column of the 16 from `byte` on
+__device__ __forceinline__ uint4 outer_read(const uint8_t* lds, int row, int byte, int lm) {
+    typedef __attribute__((address_space(3))) s16x4* at;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(lds + outer_at(row + (lm >> 2), byte + (lm & 3) * 8)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(lds + outer_at(row + 4 + (lm >> 2), byte + (lm & 3) * 8)));
+    const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+    return make_uint4(l.x, l.y, h.x, h.y);
+}
+// two values as two bf16 each
+__device__ __forceinline__ void split2(float a, float b, uint32_t& high, uint32_t& low) {
+    high = pack_bf16x2(a, b);
+    const float x = __uint_as_float(high << 16), y = __uint_as_float(high & 0xffff0000u);
+    low = pack_bf16x2(x - x == 0.f ? a - x : 0.f, y - y == 0.f ? b - y : 0.f);  // (nothing is left of an infinity)
+}
+template <int DT, int RT, bool COLS_FIRST>
+__global__ __launch_bounds__(OUTER_THREADS) void adapter_outer16_kernel(const OuterArgs g, const AdapterTile* __restrict__ chunks, int col_blocks) {
+    constexpr int PARTS = DT == F8MI_FP16 ? 2 : 1;  // of big
+    __shared__ __align__(16) uint8_t big[PARTS][OUTER_STEP * OUTER_PITCH], small[OUTER_STEP * OUTER_PITCH];  // small: a row's high parts, from byte 128 on its low ones
+    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x);  // a chunk's workgroups on one XCD: small stays in its L2
+    const AdapterTile chunk = chunks[id / col_blocks];
+    if (chunk.rows == 0 || chunk.group >= g.count) return;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, lm = lane & 15, lq = lane >> 4;
+    const int c0 = min(id % col_blocks * OUTER_COLS, g.cols - OUTER_COLS), j0 = blockIdx.y * OUTER_RANK;  // (the last columns are moved back: some are computed twice, the same)
+    const int32_t* order = g.table + AdapterTable(g.m, g.count).order() + chunk.first;
+    const int my_row = t >> 4, my_col = (t & 15) * 8;
+    int at_row[4];
+    uint4 fb[4];
+    float4 fs[RT];
+    auto load_order = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) at_row[i] = order[min(r0 + my_row + 16 * i, chunk.rows - 1)];
+    };
+    auto load = [&](int r0) __attribute__((always_inline)) {  // of rows past the last: that one again, not kept
+#pragma unroll
+        for (int i = 0; i < 4; i++) fb[i] = load16_any(g.big + (at_row[i] * g.ld + c0 + my_col) * 2);
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int item = i * OUTER_THREADS + t, row = min(r0 + item / (RT * 4), chunk.rows - 1), j = min(j0 + item % (RT * 4) * 4, g.rp - 4);
+            fs[i] = *(const float4*)(g.small + ((int64_t)chunk.first + row) * g.rp + j);
+        }
+    };
+    auto keep = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = my_row + 16 * i, at = outer_at(row, my_col * 2);
+            const uint4 q = r0 + row < chunk.rows ? fb[i] : make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (DT == F8MI_BF16) {
+                *(uint4*)(big[0] + at) = q;
+            } else {
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                uint32_t high[4], low[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x, y;
+                    unpack2<F8MI_FP16>(w[e], x, y);
+                    split2(x, y, high[e], low[e]);
+                }
+                *(uint4*)(big[0] + at) = make_uint4(high[0], high[1], high[2], high[3]);
+                *(uint4*)(big[PARTS - 1] + at) = make_uint4(low[0], low[1], low[2], low[3]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int item = i * OUTER_THREADS + t, row = item / (RT * 4), j = item % (RT * 4) * 4;
+            const bool in = r0 + row < chunk.rows && j0 + j < g.rp;
+            uint32_t high[2], low[2];
+            split2(in ? fs[i].x : 0.f, in ? fs[i].y : 0.f, high[0], low[0]);
+            split2(in ? fs[i].z : 0.f, in ? fs[i].w : 0.f, high[1], low[1]);
+            *(uint2*)(small + outer_at(row, j * 2)) = make_uint2(high[0], high[1]);
+            *(uint2*)(small + outer_at(row, 128 + j * 2)) = make_uint2(low[0], low[1]);
+        }
+    };
+    v4f_l acc[2][RT] = {};
+    load_order(0);
+    load(0);
+    load_order(OUTER_STEP);
+    for (int r0 = 0; r0 < chunk.rows; r0 += OUTER_STEP) {
+        lds_barrier();  // (what was kept has been read)
+        keep(r0);
+        lds_barrier();
+        if (r0 + OUTER_STEP < chunk.rows) {
+            load(r0 + OUTER_STEP);
+            load_order(r0 + 2 * OUTER_STEP);
+        }
+#pragma unroll
+        for (int k = 0; k < OUTER_STEP; k += 32) {
+            const int row = k + lq * 8;
+            uint4 b[PARTS][2];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) b[p][u] = outer_read(big[p], row, (wave * 32 + u * 16) * 2, lm);
+#pragma unroll
+            for (int j = 0; j < RT; j++) {
+                const uint4 high = outer_read(small, row, j * 32, lm), low = outer_read(small, row, 128 + j * 32, lm);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    auto add = [&](uint4 x, uint4 y) __attribute__((always_inline)) { acc[u][j] = COLS_FIRST ? mfma_16<F8MI_BF16>(y, x, acc[u][j]) : mfma_16<F8MI_BF16>(x, y, acc[u][j]); };
+                    add(b[0][u], high);
+                    add(b[0][u], low);
+                    if constexpr (PARTS == 2) add(b[1][u], high);
+                }
+            }
+        }
+    }
+    float* out = g.partial + (int64_t)(id / col_blocks) * g.cols * g.r;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int j = 0; j < RT; j++) {
+            const int col = c0 + wave * 32 + u * 16 + (COLS_FIRST ? lm : 4 * lq), rank = j0 + j * 16 + (COLS_FIRST ? 4 * lq : lm);
+            if (rank >= g.r) continue;
+            float* at = out + (COLS_FIRST ? (int64_t)col * g.r + rank : (int64_t)rank * g.cols + col);
+            const v4f_l v = acc[u][j];
+            if (!COLS_FIRST || rank + 4 <= g.r) store16_any(at, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+            else
+#pragma unroll
+                for (int e = 0; e < 3; e++)
+                    if (rank + e < g.r) at[e] = v[e];
+        }
+}
+
 // the chunks of an adapter added up in their order; no chunk: zeros
 __global__ __launch_bounds__(256) void adapter_outer_finish_kernel(const float* __restrict__ partial, const int32_t* __restrict__ chunk_start, const float* __restrict__ scale, float factor, int64_t size,
                                                                    void* __restrict__ out, int dtype) {
@@ -708,14 +837,28 @@ static int launch_expand(const AdapterArgs& g, const AdapterShape& s, hipStream_
     if (s.dtype == F8MI_FP16) return launch_expand2<F8MI_FP16>(g, s, stream);
     return launch_expand2<F8MI_FP32>(g, s, stream);
 }
+template <int DT, bool COLS_FIRST>
+static void launch_outer16(const OuterArgs& g, const AdapterTile* chunks, int64_t n_chunks, hipStream_t stream) {
+    const int blocks = (g.cols + OUTER_COLS - 1) / OUTER_COLS, rt = g.rp / 16;
+    const dim3 grid((unsigned)(n_chunks * blocks), (unsigned)((g.rp + OUTER_RANK - 1) / OUTER_RANK));
+    if (rt == 1) hipLaunchKernelGGL((adapter_outer16_kernel<DT, 1, COLS_FIRST>), grid, dim3(OUTER_THREADS), 0, stream, g, chunks, blocks);
+    else if (rt == 2) hipLaunchKernelGGL((adapter_outer16_kernel<DT, 2, COLS_FIRST>), grid, dim3(OUTER_THREADS), 0, stream, g, chunks, blocks);
+    else hipLaunchKernelGGL((adapter_outer16_kernel<DT, 4, COLS_FIRST>), grid, dim3(OUTER_THREADS), 0, stream, g, chunks, blocks);
+}
+template <int DT>
+static void launch_outer2(const OuterArgs& g, const AdapterTile* chunks, int64_t n_chunks, hipStream_t stream) {
+    if constexpr (DT != F8MI_FP32)
+        if (g.cols >= OUTER_COLS) return g.cols_first ? launch_outer16<DT, true>(g, chunks, n_chunks, stream) : launch_outer16<DT, false>(g, chunks, n_chunks, stream);
+    const dim3 grid((unsigned)n_chunks, (unsigned)((g.cols + OUTER_COLS - 1) / OUTER_COLS), (unsigned)((g.rp + OUTER_RANK - 1) / OUTER_RANK));
+    hipLaunchKernelGGL(adapter_outer_kernel<DT>, grid, dim3(OUTER_THREADS), 0, stream, g, chunks);
+}
 static int launch_outer(const OuterArgs& g, int dtype, const float* scale, float factor, void* out, int out_dtype, hipStream_t stream) {
     const AdapterTable table(g.m, g.count);
     const int64_t chunks = table.tiles(adapter_chunk_rows(g.m)), size = (int64_t)g.cols * g.r;
     const AdapterTile* list = (const AdapterTile*)(g.table + table.chunks());
-    const dim3 grid((unsigned)chunks, (unsigned)((g.cols + OUTER_COLS - 1) / OUTER_COLS), (unsigned)((g.rp + OUTER_RANK - 1) / OUTER_RANK));
-    if (dtype == F8MI_BF16) hipLaunchKernelGGL(adapter_outer_kernel<F8MI_BF16>, grid, dim3(OUTER_THREADS), 0, stream, g, list);
-    else if (dtype == F8MI_FP16) hipLaunchKernelGGL(adapter_outer_kernel<F8MI_FP16>, grid, dim3(OUTER_THREADS), 0, stream, g, list);
-    else hipLaunchKernelGGL(adapter_outer_kernel<F8MI_FP32>, grid, dim3(OUTER_THREADS), 0, stream, g, list);
+    if (dtype == F8MI_BF16) launch_outer2<F8MI_BF16>(g, list, chunks, stream);
+    else if (dtype == F8MI_FP16) launch_outer2<F8MI_FP16>(g, list, chunks, stream);
+    else launch_outer2<F8MI_FP32>(g, list, chunks, stream);
     if (int rc = check_hip(hipGetLastError(), "adapter gradient kernel launch")) return rc;
     hipLaunchKernelGGL(adapter_outer_finish_kernel, dim3((unsigned)((size + 255) / 256), (unsigned)g.count), dim3(256), 0, stream, g.partial, g.table + table.chunk_start(), scale, factor, size, out, out_dtype);
     return check_hip(hipGetLastError(), "adapter gradient sum kernel launch");
