@@ -37,6 +37,18 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p) {
     return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// Rows of 16-bit values with an odd pitch begin at odd multiples of two bytes every other time, where an access of 16 bytes takes three times as long (4099 x 4097: 32 us to read instead
+// of 10).  ODD: the words around them instead, moved by half a word.  No word is read that holds none of the 16 bytes.
+template <bool ODD>
+__device__ __forceinline__ uint4 load16_at(const uint8_t* p) {
+    if constexpr (!ODD) return load16_any(p);
+    const uint32_t off = (uint32_t)(uintptr_t)p & 2u, shift = off * 8;
+    const uint4 q = load16_any(p - off);
+    const uint32_t next = *(const u32_any*)(p - off + (off ? 16 : 12));
+    return make_uint4(__builtin_amdgcn_alignbit(q.y, q.x, shift), __builtin_amdgcn_alignbit(q.z, q.y, shift), __builtin_amdgcn_alignbit(q.w, q.z, shift),
+                      __builtin_amdgcn_alignbit(off ? next : 0u, q.w, shift));
+}
+
 // V values of a row of r, from column col on, zeros past its end: `from` is their place in a tensor of `total` values.  WHOLE: r is a multiple of V, so that they all lie in the
 // row or none does.  No branch, so that many are on their way at once: past the end of the tensor its last 16 bytes are read and shifted.
 template <int DT, bool WHOLE>
@@ -157,8 +169,10 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void adapter_shrink_kernel(const
 // 64 rows of one adapter and 16 RT of its rank a workgroup: a wave has 16 of the rows and brings them itself, all four multiply them by the same part of A, which goes through LDS: BYTES
 // of each of its rows at a time, the next ones (and the next ones of x) on their way meanwhile.  A workgroup has a part of the contraction; nothing is left to add up inside it.
 constexpr int TALL_THREADS = 256;
-template <int DT, int RT, int BYTES>
-__global__ __launch_bounds__(TALL_THREADS, 4) void adapter_shrink_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+// ODD: some rows of x begin at odd multiples of two bytes (load16_at): the words around a lane's values are brought, and the last one is the first of the lane that has the next 16 bytes, but for
+// one word a step.
+template <int DT, int RT, int BYTES, bool ODD>
+__global__ __launch_bounds__(TALL_THREADS, ODD ? 3 : 4) void adapter_shrink_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
     constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, PIECES = BYTES / 16, KP = RT * 16 * PIECES / TALL_THREADS, PITCH = BYTES + 16, STEP = BYTES / SIZE;
     __shared__ __align__(16) uint8_t lds_a[2][RT * 16 * PITCH];
     const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), split = id % g.splits;  // a tile's workgroups, and those of the next ones, on one XCD: A stays in its L2
@@ -170,12 +184,16 @@ __global__ __launch_bounds__(TALL_THREADS, 4) void adapter_shrink_tall_kernel(co
     const int64_t a_first = ((int64_t)tile.group * g.r + j0) * g.k, a_total = (int64_t)g.count * g.r * g.k;
     v4f_l acc[RT] = {};
     uint4 fa[KP], fx[PIECES / 4], next_x[PIECES / 4];
+    const uint32_t off = ODD ? (uint32_t)(uintptr_t)(g.x + x_row * SIZE) & 2u : 0u;
+    uint32_t edge = 0u, next_edge = 0u;  // the word behind the step's values of the row
     // (a step that ends with the row or before it, the same for the workgroup, needs no edges)
-    auto load_x = [&](int s, uint4 (&q)[PIECES / 4]) __attribute__((always_inline)) {
+    auto load_x = [&](int s, uint4 (&q)[PIECES / 4], uint32_t& e) __attribute__((always_inline)) {
         const int k0 = s * STEP + lq * V;
         if ((s + 1) * STEP <= g.k) {
 #pragma unroll
-            for (int i = 0; i < PIECES / 4; i++) q[i] = load16_any(g.x + (x_row + k0 + i * 4 * V) * SIZE);
+            for (int i = 0; i < PIECES / 4; i++) q[i] = load16_any(g.x + (x_row + k0 + i * 4 * V) * SIZE - off);
+            if constexpr (ODD)
+                if (off && lq == 3) e = *(const u32_any*)(g.x + (x_row + (s + 1) * STEP) * SIZE - off);
         } else {
 #pragma unroll
             for (int i = 0; i < PIECES / 4; i++) q[i] = load_of_row<DT, false>(g.x, x_row + k0 + i * 4 * V, x_total, k0 + i * 4 * V, g.k);
@@ -198,16 +216,31 @@ __global__ __launch_bounds__(TALL_THREADS, 4) void adapter_shrink_tall_kernel(co
     };
     if (s0 < s1) {
         load_a(s0);
-        load_x(s0, fx);
+        load_x(s0, fx, edge);
         keep_a(0);
         __syncthreads();
     }
     for (int s = s0, buffer = 0; s < s1; s++, buffer ^= 1) {
         const bool more = s + 1 < s1;
         if (more) {
-            load_x(s + 1, next_x);
+            load_x(s + 1, next_x, next_edge);
             load_a(s + 1);
         }
+        if constexpr (ODD)
+            if ((s + 1) * STEP <= g.k) {  // (the same for the workgroup)
+                const uint32_t shift = off * 8;
+                uint32_t got[PIECES / 4 + 1];
+#pragma unroll
+                for (int i = 0; i < PIECES / 4; i++) got[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((lane + 16) * 4, (int)fx[i].x);
+                got[PIECES / 4] = edge;
+#pragma unroll
+                for (int i = 0; i < PIECES / 4; i++) {
+                    const uint4 q = fx[i];
+                    const uint32_t next = lq == 3 ? got[i + 1] : got[i];
+                    fx[i] = make_uint4(__builtin_amdgcn_alignbit(q.y, q.x, shift), __builtin_amdgcn_alignbit(q.z, q.y, shift), __builtin_amdgcn_alignbit(q.w, q.z, shift),
+                                       __builtin_amdgcn_alignbit(next, q.w, shift));
+                }
+            }
 #pragma unroll
         for (int i = 0; i < PIECES / 4; i++)
 #pragma unroll
@@ -217,6 +250,7 @@ __global__ __launch_bounds__(TALL_THREADS, 4) void adapter_shrink_tall_kernel(co
             lds_barrier();
 #pragma unroll
             for (int i = 0; i < PIECES / 4; i++) fx[i] = next_x[i];
+            edge = next_edge;
         }
     }
     const int row = wave * 16 + lm;
@@ -300,8 +334,8 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& g, const AdapterTile&
 
 // Of out and y, 64 columns from n0: a lane's pieces of 16 bytes of its row, those of the four lanes that share it next to each other, so that an instruction takes 64 bytes of each row.
 // (Not past the caches: these are half lines; a copy of 8192 x 14336 in such pieces takes 95 us, past the caches 122.)
-// EDGE: some may lie past the last.
-template <int DT, bool EDGE>
+// EDGE: some may lie past the last.  ODD: load16_at, and stores of whole words, a value moved on from lane to lane, where a row begins at an odd multiple of two bytes.
+template <int DT, bool EDGE, bool ODD = false>
 struct ExpandCols {
     static constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, PIECES = 16 / V;
     int n0, n, lq, lm;
@@ -312,7 +346,7 @@ struct ExpandCols {
     __device__ __forceinline__ void load(const uint8_t* row, uint4 (&q)[PIECES]) const {
         if (inside()) {
 #pragma unroll
-            for (int p = 0; p < PIECES; p++) q[p] = load16_any(row + (int64_t)col(p) * SIZE);
+            for (int p = 0; p < PIECES; p++) q[p] = load16_at<ODD>(row + (int64_t)col(p) * SIZE);
         } else {
 #pragma unroll
             for (int p = 0; p < PIECES; p++) q[p] = ln_load<DT, int>(row, col(p), n);
@@ -320,6 +354,7 @@ struct ExpandCols {
     }
     // y + acc * factor (adapted: a row without an adapter keeps y's bits)
     __device__ __forceinline__ void store(uint8_t* row, const uint4 (&q)[PIECES], const v4f_l* acc, float factor, bool adapted) const {
+        uint32_t before = 0u;
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
             float v[V];
@@ -327,7 +362,25 @@ struct ExpandCols {
             if (adapted)
 #pragma unroll
                 for (int e = 0; e < V; e++) v[e] = __builtin_fmaf(acc[(p * V + e) / 4][e % 4], factor, v[e]);
-            if (inside()) store16_any(row + (int64_t)col(p) * SIZE, ln_pack<DT>(v));
+            if constexpr (ODD) {
+                uint4 w = ln_pack<DT>(v);
+                const bool odd = (uintptr_t)row & 2;
+                const bool first = odd && p == 0 && lq == 0, last = odd && p == PIECES - 1 && lq == 3;
+                // the value before these eight: of the lane 16 before, or that of the piece before 48 after
+                const uint32_t got = (uint32_t)__builtin_amdgcn_ds_bpermute((int)((threadIdx.x & 63) - 16) * 4, (int)w.w), own = w.w;
+                const uint32_t prev = lq == 0 ? before : got;
+                before = got;
+                uint8_t* at = row + (int64_t)col(p) * SIZE;
+                if (first) *(uint16_t*)at = (uint16_t)w.x;
+                if (odd) w = make_uint4(w.x << 16 | prev >> 16, __builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16), __builtin_amdgcn_alignbit(w.w, w.z, 16));
+                if (first) {
+                    store8_any(at + 2, w.y, w.z);
+                    *(u32_any*)(at + 10) = w.w;
+                } else {
+                    store16_any(at - (odd ? 2 : 0), w);
+                }
+                if (last) *(uint16_t*)(at + 14) = (uint16_t)(own >> 16);
+            } else if (inside()) store16_any(row + (int64_t)col(p) * SIZE, ln_pack<DT>(v));
             else if (col(p) < n) ln_store<DT, int>(row, col(p), n, v);
         }
     }
@@ -404,9 +457,9 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_kernel(const Ad
 // 64 rows and B through LDS, 16-bit types: the four waves have 16 rows each and the same columns, CB of them at a time, so that B is read once a workgroup.  The next
 // CB columns of B and of y are on their way while these are multiplied.  The last of them are moved back to end with the last column (their first are
 // then computed twice, the same): no access has an edge.  MOST: the largest expand_half.
-template <int DT, int MOST, int CB, bool WHOLE>
+template <int DT, int MOST, int CB, bool WHOLE, bool ODD>
 __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
-    constexpr int SIZE = 2, ROWS = 64, SUB = CB / 64, PIECES = ExpandCols<DT, false>::PIECES;
+    constexpr int SIZE = 2, ROWS = 64, SUB = CB / 64, PIECES = ExpandCols<DT, false, ODD>::PIECES;
     constexpr int KP = CB * MOST / 8 / EXPAND_THREADS;  // pieces of 16 bytes of B that a lane brings
     constexpr int KH = MOST <= 64 ? (MOST + 31) / 32 : 0;  // of a rank of up to 64 the wave's h stays in registers
     extern __shared__ __align__(16) uint8_t expand_lds[];  // h [ROWS][pitch], then (fp16) fp32 [ROWS][half] while it is converted and B [2][CB][half + 8] from then on
@@ -443,7 +496,7 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(con
     auto load_y = [&](int n0, uint4 (&q)[SUB][PIECES]) __attribute__((always_inline)) {
         if (g.y)
 #pragma unroll
-            for (int u = 0; u < SUB; u++) ExpandCols<DT, false>{n0 + u * 64, g.n, lq, lm}.load(y_row, q[u]);
+            for (int u = 0; u < SUB; u++) ExpandCols<DT, false, ODD>{n0 + u * 64, g.n, lq, lm}.load(y_row, q[u]);
     };
     load_y(min(begin, last), fy);
     float factor = 1.f;
@@ -470,7 +523,7 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(con
         }
 #pragma unroll
         for (int u = 0; u < SUB; u++) {
-            const ExpandCols<DT, false> at{min(n0, last) + u * 64, g.n, lq, lm};
+            const ExpandCols<DT, false, ODD> at{min(n0, last) + u * 64, g.n, lq, lm};
             v4f_l acc[4] = {};
             if (!none) {
                 const uint16_t* pb[4];
@@ -763,16 +816,18 @@ struct AdapterShape {
 };
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-template <int DT>
-static int launch_shrink2(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
+// 16-bit rows that begin at odd multiples of two bytes
+static bool odd_rows(const void* p, int64_t ld, int dtype) { return dtype != F8MI_FP32 && ((ld & 1) || ((uintptr_t)p & 2)); }
+template <int DT, bool ODD>
+static int launch_shrink3(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     const AdapterTable table = s.table();
     const int rt = g.rp / 16;
     const dim3 grid((unsigned)(s.tiles() * g.splits), (unsigned)(rt <= 4 ? 1 : (rt + 3) / 4));
     if (s.tall()) {
         const AdapterTile* tiles = (const AdapterTile*)(g.table + table.tiles64());
-        if (rt == 1) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 512>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
-        else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 2, 256>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
-        else hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 4, 256>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        if (rt == 1) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 512, ODD>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 2, 256, ODD>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        else hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 4, 256, ODD>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
     } else {
         const AdapterTile* tiles = (const AdapterTile*)(g.table + table.tiles16());
         if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<DT, 1>), grid, dim3(64 * SHRINK_WAVES), 0, stream, g, tiles);
@@ -780,6 +835,12 @@ static int launch_shrink2(const AdapterArgs& g, const AdapterShape& s, hipStream
         else hipLaunchKernelGGL((adapter_shrink_kernel<DT, 4>), grid, dim3(64 * SHRINK_WAVES), 0, stream, g, tiles);
     }
     return check_hip(hipGetLastError(), "adapter shrink kernel launch");
+}
+template <int DT>
+static int launch_shrink2(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
+    if constexpr (DT != F8MI_FP32)
+        if (odd_rows(g.x, g.ld, DT)) return launch_shrink3<DT, true>(g, s, stream);
+    return launch_shrink3<DT, false>(g, s, stream);
 }
 static int launch_shrink(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     if (s.dtype == F8MI_BF16) return launch_shrink2<F8MI_BF16>(g, s, stream);
@@ -805,12 +866,17 @@ static int launch_expand_direct(AdapterArgs g, const AdapterTile* tiles, int64_t
     g.cols = expand_cols(g, n_tiles, WR > 1 ? 8 : 4, 256);
     return launch_expand_kernel(adapter_expand_kernel<DT, WR, WHOLE>, allowed, g, tiles, n_tiles, 16 * WR * (expand_pitch<DT>(g.rp) * Ln<DT>::SIZE + (DT == F8MI_FP16 ? expand_half(g.rp) * 4 : 0)), stream);
 }
-template <int DT, int MOST, int CB, bool WHOLE>
-static int launch_expand_tall(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
+template <int DT, int MOST, int CB, bool WHOLE, bool ODD>
+static int launch_expand_tall2(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
     g.cols = expand_cols(g, n_tiles, 8, CB);
     const int lds = 64 * expand_pitch<DT>(g.rp) * 2 + std::max(DT == F8MI_FP16 ? 64 * expand_half(g.rp) * 4 : 0, 2 * CB * (expand_half(g.rp) + 8) * 2);
-    return launch_expand_kernel(adapter_expand_tall_kernel<DT, MOST, CB, WHOLE>, allowed, g, tiles, n_tiles, lds, stream);
+    return launch_expand_kernel(adapter_expand_tall_kernel<DT, MOST, CB, WHOLE, ODD>, allowed, g, tiles, n_tiles, lds, stream);
+}
+template <int DT, int MOST, int CB, bool WHOLE>
+static int launch_expand_tall(const AdapterArgs& g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
+    return odd_rows(g.out, g.n, DT) || (g.y && odd_rows(g.y, g.ld_y, DT)) ? launch_expand_tall2<DT, MOST, CB, WHOLE, true>(g, tiles, n_tiles, stream)
+                                                                          : launch_expand_tall2<DT, MOST, CB, WHOLE, false>(g, tiles, n_tiles, stream);
 }
 template <int DT, bool WHOLE>
 static int launch_expand3(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
