@@ -37,6 +37,14 @@ __device__ __forceinline__ uint4 load16_any(const uint8_t* p) {
     return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// ds_read_b64_tr_b16: the 16 lanes of a group address 8 bytes each, lane l row l / 4 of four and four of its columns; a lane gets the four rows of one column, that of lane l / 4's
+// bytes l % 4.  Two of them, of rows and of the four rows after, are a lane's operand.
+__device__ __forceinline__ uint4 read_turned(const uint8_t* rows, const uint8_t* after) {
+    typedef __attribute__((address_space(3))) s16x4* at;
+    const uint2 l = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)rows)), h = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)after));
+    return make_uint4(l.x, l.y, h.x, h.y);
+}
 // Rows of 16-bit values with an odd pitch begin at odd multiples of two bytes every other time, where an access of 16 bytes takes three times as long (4099 x 4097: 32 us to read instead
 // of 10).  ODD: the words around them instead, moved by half a word.  No word is read that holds none of the 16 bytes.
 template <bool ODD>
@@ -91,6 +99,7 @@ struct AdapterArgs {
     uint8_t* out;      // [m][n]
     float* h;          // [m][rp]: the parts added up, or null
     int n, cols, chunks;  // cols: of out that a workgroup has; chunks: workgroups a tile
+    bool a_turned, b_turned;  // a is [count][k][r], b [count][r][n]: the adapters' other matrices as they lie
 };
 
 // ---- shrink: a wave has 16 rows of one adapter, 16 RT of its rank and a part of the contraction; those of a workgroup's waves are added up in LDS
@@ -170,18 +179,22 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void adapter_shrink_kernel(const
 // of each of its rows at a time, the next ones (and the next ones of x) on their way meanwhile.  A workgroup has a part of the contraction; nothing is left to add up inside it.
 constexpr int TALL_THREADS = 256;
 // ODD: some rows of x begin at odd multiples of two bytes (load16_at): the words around a lane's values are brought, and the last one is the first of the lane that has the next 16 bytes, but for
-// one word a step.
-template <int DT, int RT, int BYTES, bool ODD>
-__global__ __launch_bounds__(TALL_THREADS, ODD ? 3 : 4) void adapter_shrink_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
-    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, PIECES = BYTES / 16, KP = RT * 16 * PIECES / TALL_THREADS, PITCH = BYTES + 16, STEP = BYTES / SIZE;
-    __shared__ __align__(16) uint8_t lds_a[2][RT * 16 * PITCH];
+// one word a step.  TURNED (16-bit types): A is [count][k][r], the other matrix of an adapter as it lies, and is turned on the way out of LDS.
+template <int DT, int RT, int BYTES, bool ODD, bool TURNED>
+__global__ __launch_bounds__(TALL_THREADS, ODD || (TURNED && RT == 1) ? 3 : 4) void adapter_shrink_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+    constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, PIECES = BYTES / 16, KP = RT * 16 * PIECES / TALL_THREADS, STEP = BYTES / SIZE;
+    // turned, the rows of 32 RT bytes that 32 lanes read at a time (0 .. 3 and 8 .. 11) lie in different banks: by a half turn of every second eight, or by padding (two of eight meet)
+    constexpr int PITCH = !TURNED ? BYTES + 16 : RT == 4 ? 160 : RT * 32;
+    __shared__ __align__(16) uint8_t lds_a[2][(TURNED ? STEP : RT * 16) * PITCH];
+    auto turned_at = [](int row, int byte) __attribute__((always_inline)) { return (row * PITCH + byte) ^ (RT == 4 ? 0 : (row >> 3 & 1) * (RT == 1 ? 128 : 32)); };
     const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), split = id % g.splits;  // a tile's workgroups, and those of the next ones, on one XCD: A stays in its L2
     const AdapterTile tile = tiles[id / g.splits];
     if (tile.rows == 0 || tile.group >= g.count) return;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, lm = lane & 15, lq = lane >> 4, j0 = blockIdx.y * (16 * RT);
     const int steps = (g.k + STEP - 1) / STEP, s0 = (int)((int64_t)steps * split / g.splits), s1 = (int)((int64_t)steps * (split + 1) / g.splits);
     const int64_t x_row = (int64_t)g.table[AdapterTable(g.m, g.count).order() + tile.first + min(wave * 16 + lm, tile.rows - 1)] * g.ld, x_total = (g.m - 1) * g.ld + g.k;
-    const int64_t a_first = ((int64_t)tile.group * g.r + j0) * g.k, a_total = (int64_t)g.count * g.r * g.k;
+    const int64_t a_first = TURNED ? (int64_t)tile.group * g.k * g.r : ((int64_t)tile.group * g.r + j0) * g.k, a_total = (int64_t)g.count * g.r * g.k;
+    const bool whole = g.r % V == 0;
     v4f_l acc[RT] = {};
     uint4 fa[KP], fx[PIECES / 4], next_x[PIECES / 4];
     const uint32_t off = ODD ? (uint32_t)(uintptr_t)(g.x + x_row * SIZE) & 2u : 0u;
@@ -202,7 +215,17 @@ __global__ __launch_bounds__(TALL_THREADS, ODD ? 3 : 4) void adapter_shrink_tall
     auto load_a = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < KP; i++) {
-            const int item = i * TALL_THREADS + t, row = min(item / PIECES, g.r - 1 - j0), k = s * STEP + item % PIECES * V;
+            const int item = i * TALL_THREADS + t;
+            if constexpr (TURNED) {  // (zeros behind the last row)
+                const int row = s * STEP + item / (2 * RT), j = j0 + item % (2 * RT) * 8;
+                fa[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (row < g.k) {
+                    if (whole) fa[i] = j < g.r ? load16_any(g.a + (a_first + (int64_t)row * g.r + j) * SIZE) : fa[i];
+                    else fa[i] = load_of_row<DT, false>(g.a, a_first + (int64_t)row * g.r + j, a_total, j, g.r);
+                }
+                continue;
+            }
+            const int row = min(item / PIECES, g.r - 1 - j0), k = s * STEP + item % PIECES * V;
             if ((s + 1) * STEP <= g.k) fa[i] = load16_any(g.a + (a_first + (int64_t)row * g.k + k) * SIZE);
             else fa[i] = load_of_row<DT, false>(g.a, a_first + (int64_t)row * g.k + k, a_total, k, g.k);
         }
@@ -211,7 +234,7 @@ __global__ __launch_bounds__(TALL_THREADS, ODD ? 3 : 4) void adapter_shrink_tall
 #pragma unroll
         for (int i = 0; i < KP; i++) {
             const int item = i * TALL_THREADS + t;
-            *(uint4*)(lds_a[buffer] + item / PIECES * PITCH + item % PIECES * 16) = fa[i];
+            *(uint4*)(lds_a[buffer] + (TURNED ? turned_at(item / (2 * RT), item % (2 * RT) * 16) : item / PIECES * PITCH + item % PIECES * 16)) = fa[i];
         }
     };
     if (s0 < s1) {
@@ -244,7 +267,16 @@ __global__ __launch_bounds__(TALL_THREADS, ODD ? 3 : 4) void adapter_shrink_tall
 #pragma unroll
         for (int i = 0; i < PIECES / 4; i++)
 #pragma unroll
-            for (int j = 0; j < RT; j++) acc[j] = mfma_16<DT>(*(const uint4*)(lds_a[buffer] + (j * 16 + lm) * PITCH + i * 64 + lq * 16), fx[i], acc[j]);
+            for (int j = 0; j < RT; j++) {
+                uint4 q;
+                if constexpr (TURNED) {
+                    const int row = i * 32 + lq * 8 + (lm >> 2), byte = j * 32 + (lm & 3) * 8;
+                    q = read_turned(lds_a[buffer] + turned_at(row, byte), lds_a[buffer] + turned_at(row + 4, byte));
+                } else {
+                    q = *(const uint4*)(lds_a[buffer] + (j * 16 + lm) * PITCH + i * 64 + lq * 16);
+                }
+                acc[j] = mfma_16<DT>(q, fx[i], acc[j]);
+            }
         if (more) {
             keep_a(buffer ^ 1);
             lds_barrier();
@@ -262,6 +294,8 @@ __global__ __launch_bounds__(TALL_THREADS, ODD ? 3 : 4) void adapter_shrink_tall
 
 // ---- expand: a workgroup has 16 WR rows of one adapter and `cols` columns of out
 constexpr int EXPAND_THREADS = 256;
+// Columns that the kernel for 64 rows needs: a whole block
+constexpr int expand_least(int rp) { return rp <= 32 ? 128 : 64; }
 // Of a row of h in LDS: 16-bit types have its high parts, then its low ones, `half` elements each: whole instructions of 32, or 16, where one instruction takes both.
 __host__ __device__ constexpr int expand_half(int rp) { return rp <= 16 ? 16 : (rp + 31) / 32 * 32; }
 template <int DT>
@@ -456,8 +490,9 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_kernel(const Ad
 
 // 64 rows and B through LDS, 16-bit types: the four waves have 16 rows each and the same columns, CB of them at a time, so that B is read once a workgroup.  The next
 // CB columns of B and of y are on their way while these are multiplied.  The last of them are moved back to end with the last column (their first are
-// then computed twice, the same): no access has an edge.  MOST: the largest expand_half.
-template <int DT, int MOST, int CB, bool WHOLE, bool ODD>
+// then computed twice, the same): no access has an edge.  MOST: the largest expand_half.  TURNED: B is
+// [count][r][n], the other matrix of an adapter as it lies: CB values of each of its rows go to LDS and are turned on the way out.
+template <int DT, int MOST, int CB, bool WHOLE, bool ODD, bool TURNED>
 __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
     constexpr int SIZE = 2, ROWS = 64, SUB = CB / 64, PIECES = ExpandCols<DT, false, ODD>::PIECES;
     constexpr int KP = CB * MOST / 8 / EXPAND_THREADS;  // pieces of 16 bytes of B that a lane brings
@@ -469,7 +504,8 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(con
     if (tile.rows == 0) return;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, lm = lane & 15, lq = lane >> 4;
     const bool none = tile.group >= g.count;
-    const int rp = g.rp, half = KH ? MOST : expand_half(rp), pitch = 2 * half + 8, b_pitch = half + 8, row_pieces = half / 8;
+    const int rp = g.rp, half = KH ? MOST : expand_half(rp), pitch = 2 * half + 8, b_pitch = TURNED ? CB + 32 : half + 8, row_pieces = TURNED ? CB / 8 : half / 8, pieces = CB / 8 * half;
+    const int buffer_values = TURNED ? half * b_pitch : CB * b_pitch;
     uint8_t* const behind = expand_lds + ROWS * pitch * 2;
     uint16_t* const lds_b = (uint16_t*)behind;
     const int my_row = wave * 16 + lm;
@@ -483,14 +519,19 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(con
 #pragma unroll
         for (int i = 0; i < KP; i++) {
             const int item = i * EXPAND_THREADS + t, row = item / row_pieces, j = (item - row * row_pieces) * 8;
-            if (item < CB * row_pieces) fb[i] = load_of_row<DT, WHOLE>(g.b, ((int64_t)tile.group * g.n + n0 + row) * g.r + j, b_total, j, g.r);
+            if (item >= pieces) continue;
+            if constexpr (TURNED) fb[i] = row < g.r ? load16_any(g.b + (((int64_t)tile.group * g.r + row) * g.n + n0 + j) * SIZE) : make_uint4(0u, 0u, 0u, 0u);
+            else fb[i] = load_of_row<DT, WHOLE>(g.b, ((int64_t)tile.group * g.n + n0 + row) * g.r + j, b_total, j, g.r);
         }
     };
     auto keep_b = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < KP; i++) {
             const int item = i * EXPAND_THREADS + t, row = item / row_pieces, j = (item - row * row_pieces) * 8;
-            if (item < CB * row_pieces) *(uint4*)(lds_b + (buffer * CB + row) * b_pitch + j) = fb[i];
+            if (item >= pieces) continue;
+            uint4 q = fb[i];
+            if (TURNED && (row >> 3 & 1)) q = make_uint4(q.z, q.w, q.x, q.y);  // (every second eight rows: 32 lanes read the first or the second half of 16 bytes of rows 0 .. 3, and the other of 8 .. 11)
+            *(uint4*)(lds_b + buffer * buffer_values + row * b_pitch + j) = q;
         }
     };
     auto load_y = [&](int n0, uint4 (&q)[SUB][PIECES]) __attribute__((always_inline)) {
@@ -527,17 +568,26 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(con
             v4f_l acc[4] = {};
             if (!none) {
                 const uint16_t* pb[4];
+                if constexpr (!TURNED)
 #pragma unroll
-                for (int c = 0; c < 4; c++) pb[c] = lds_b + (buffer * CB + at.of_tile(c) - min(n0, last)) * b_pitch;
+                    for (int c = 0; c < 4; c++) pb[c] = lds_b + buffer * buffer_values + (at.of_tile(c) - min(n0, last)) * b_pitch;
+                auto read_b = [&](int c, int k) __attribute__((always_inline)) {  // eight of the rank from k on, k a multiple of 8, of column c of the lane
+                    if constexpr (TURNED) {
+                        const uint8_t* rows = (const uint8_t*)(lds_b + buffer * buffer_values + (k + (lm >> 2)) * b_pitch + u * 64 + c / 2 * 32 + (lm & 3) * 8) + ((c & 1) ^ (k >> 3 & 1)) * 8;
+                        return read_turned(rows, rows + 4 * b_pitch * 2);
+                    } else {
+                        return *(const uint4*)(pb[c] + k);
+                    }
+                };
                 if constexpr (MOST == 16) {  // a rank of up to 16: both parts of h in one instruction, B twice
 #pragma unroll
-                    for (int c = 0; c < 4; c++) acc[c] = mfma_16<DT>(*(const uint4*)(pb[c] + (lq & 1) * 8), fh[0][0], acc[c]);
+                    for (int c = 0; c < 4; c++) acc[c] = mfma_16<DT>(read_b(c, (lq & 1) * 8), fh[0][0], acc[c]);
                 } else if constexpr (KH > 0) {
 #pragma unroll
                     for (int k = 0; k < KH; k++)
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
-                            const uint4 q = *(const uint4*)(pb[c] + k * 32 + lq * 8);
+                            const uint4 q = read_b(c, k * 32 + lq * 8);
                             acc[c] = mfma_16<DT>(q, fh[k][1], mfma_16<DT>(q, fh[k][0], acc[c]));
                         }
                 } else {
@@ -546,7 +596,7 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(con
                         const uint4 high = *(const uint4*)(hrow + k), low = *(const uint4*)(hrow + half + k);
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
-                            const uint4 q = *(const uint4*)(pb[c] + k);
+                            const uint4 q = read_b(c, k);
                             acc[c] = mfma_16<DT>(q, low, mfma_16<DT>(q, high, acc[c]));
                         }
                     }
@@ -637,15 +687,10 @@ __global__ __launch_bounds__(OUTER_THREADS) void adapter_outer_kernel(const Oute
 // exponents of fp32.  A row of 128 columns is 256 bytes; a pitch of 288 and rows 8 .. 15 of 16 turned by half a row let the 32 lanes that read at a time reach all banks.
 // COLS_FIRST: sums [cols][r], so that a lane has four neighbours of the rank, else of the columns.
 constexpr int OUTER_STEP = 64, OUTER_PITCH = 288;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ int outer_at(int row, int byte) { return row * OUTER_PITCH + (byte ^ ((row >> 3 & 1) * 128)); }
 // rows row .. row + 7 of the lane's column of the 16 from `byte` on
 __device__ __forceinline__ uint4 outer_read(const uint8_t* lds, int row, int byte, int lm) {
-    typedef __attribute__((address_space(3))) s16x4* at;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(lds + outer_at(row + (lm >> 2), byte + (lm & 3) * 8)));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(lds + outer_at(row + 4 + (lm >> 2), byte + (lm & 3) * 8)));
-    const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
-    return make_uint4(l.x, l.y, h.x, h.y);
+    return read_turned(lds + outer_at(row + (lm >> 2), byte + (lm & 3) * 8), lds + outer_at(row + 4 + (lm >> 2), byte + (lm & 3) * 8));
 }
 // two values as two bf16 each
 __device__ __forceinline__ void split2(float a, float b, uint32_t& high, uint32_t& low) {
@@ -809,25 +854,28 @@ struct AdapterShape {
     // Parts of a contraction of this length: four workgroups a CU, and two steps at least (of a workgroup, of each wave of one for short tiles)
     int64_t splits(int64_t contracted) const {
         const int64_t bytes = contracted * (dtype == F8MI_FP32 ? 4 : 2), steps = tall() ? bytes / (rp() <= 16 ? 512 : 256) : bytes / (128 * SHRINK_WAVES);
-        const int64_t want = 4 * (int64_t)cu_count() / std::max<int64_t>(1, tiles() * ((rp() + 63) / 64));
+        const int64_t want = 2 * (int64_t)cu_count() / std::max<int64_t>(1, tiles() * ((rp() + 63) / 64));
         return std::max<int64_t>(1, std::min({want, steps / 2, (int64_t)32}));
     }
+    // Backward reads the adapters' matrices as they lie; short tiles and fp32 have their transposes made (4.6 us each for four adapters of 4096 x 16)
+    bool turns_b() const { return tall() && dtype != F8MI_FP32; }
+    bool turns_a() const { return turns_b() && rp() <= 128 && k >= expand_least((int)rp()); }  // (of a larger rank the rows of two blocks do not fit in LDS beside h)
     int64_t partial_bytes(int64_t contracted) const { return splits(contracted) * m * rp() * 4; }
 };
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // 16-bit rows that begin at odd multiples of two bytes
 static bool odd_rows(const void* p, int64_t ld, int dtype) { return dtype != F8MI_FP32 && ((ld & 1) || ((uintptr_t)p & 2)); }
-template <int DT, bool ODD>
+template <int DT, bool ODD, bool TURNED>
 static int launch_shrink3(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     const AdapterTable table = s.table();
     const int rt = g.rp / 16;
     const dim3 grid((unsigned)(s.tiles() * g.splits), (unsigned)(rt <= 4 ? 1 : (rt + 3) / 4));
     if (s.tall()) {
         const AdapterTile* tiles = (const AdapterTile*)(g.table + table.tiles64());
-        if (rt == 1) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 512, ODD>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
-        else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 2, 256, ODD>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
-        else hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 4, 256, ODD>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        if (rt == 1) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 512, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 2, 256, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        else hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 4, 256, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
     } else {
         const AdapterTile* tiles = (const AdapterTile*)(g.table + table.tiles16());
         if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<DT, 1>), grid, dim3(64 * SHRINK_WAVES), 0, stream, g, tiles);
@@ -839,8 +887,10 @@ static int launch_shrink3(const AdapterArgs& g, const AdapterShape& s, hipStream
 template <int DT>
 static int launch_shrink2(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     if constexpr (DT != F8MI_FP32)
-        if (odd_rows(g.x, g.ld, DT)) return launch_shrink3<DT, true>(g, s, stream);
-    return launch_shrink3<DT, false>(g, s, stream);
+        if (odd_rows(g.x, g.ld, DT)) return g.a_turned ? launch_shrink3<DT, true, true>(g, s, stream) : launch_shrink3<DT, true, false>(g, s, stream);
+    if constexpr (DT != F8MI_FP32)
+        if (g.a_turned) return launch_shrink3<DT, false, true>(g, s, stream);
+    return launch_shrink3<DT, false, false>(g, s, stream);
 }
 static int launch_shrink(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     if (s.dtype == F8MI_BF16) return launch_shrink2<F8MI_BF16>(g, s, stream);
@@ -866,17 +916,19 @@ static int launch_expand_direct(AdapterArgs g, const AdapterTile* tiles, int64_t
     g.cols = expand_cols(g, n_tiles, WR > 1 ? 8 : 4, 256);
     return launch_expand_kernel(adapter_expand_kernel<DT, WR, WHOLE>, allowed, g, tiles, n_tiles, 16 * WR * (expand_pitch<DT>(g.rp) * Ln<DT>::SIZE + (DT == F8MI_FP16 ? expand_half(g.rp) * 4 : 0)), stream);
 }
-template <int DT, int MOST, int CB, bool WHOLE, bool ODD>
+template <int DT, int MOST, int CB, bool WHOLE, bool ODD, bool TURNED>
 static int launch_expand_tall2(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
     g.cols = expand_cols(g, n_tiles, 8, CB);
-    const int lds = 64 * expand_pitch<DT>(g.rp) * 2 + std::max(DT == F8MI_FP16 ? 64 * expand_half(g.rp) * 4 : 0, 2 * CB * (expand_half(g.rp) + 8) * 2);
-    return launch_expand_kernel(adapter_expand_tall_kernel<DT, MOST, CB, WHOLE, ODD>, allowed, g, tiles, n_tiles, lds, stream);
+    const int lds = 64 * expand_pitch<DT>(g.rp) * 2 + std::max(DT == F8MI_FP16 ? 64 * expand_half(g.rp) * 4 : 0, 2 * 2 * (TURNED ? expand_half(g.rp) * (CB + 32) : CB * (expand_half(g.rp) + 8)));
+    return launch_expand_kernel(adapter_expand_tall_kernel<DT, MOST, CB, WHOLE, ODD, TURNED>, allowed, g, tiles, n_tiles, lds, stream);
 }
 template <int DT, int MOST, int CB, bool WHOLE>
 static int launch_expand_tall(const AdapterArgs& g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
-    return odd_rows(g.out, g.n, DT) || (g.y && odd_rows(g.y, g.ld_y, DT)) ? launch_expand_tall2<DT, MOST, CB, WHOLE, true>(g, tiles, n_tiles, stream)
-                                                                          : launch_expand_tall2<DT, MOST, CB, WHOLE, false>(g, tiles, n_tiles, stream);
+    const bool odd = odd_rows(g.out, g.n, DT) || (g.y && odd_rows(g.y, g.ld_y, DT));
+    if constexpr (WHOLE && MOST <= 128)  // (turned, it is not asked)
+        if (g.b_turned) return odd ? launch_expand_tall2<DT, MOST, CB, true, true, true>(g, tiles, n_tiles, stream) : launch_expand_tall2<DT, MOST, CB, true, false, true>(g, tiles, n_tiles, stream);
+    return odd ? launch_expand_tall2<DT, MOST, CB, WHOLE, true, false>(g, tiles, n_tiles, stream) : launch_expand_tall2<DT, MOST, CB, WHOLE, false, false>(g, tiles, n_tiles, stream);
 }
 template <int DT, bool WHOLE>
 static int launch_expand3(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
@@ -884,7 +936,7 @@ static int launch_expand3(const AdapterArgs& g, const AdapterShape& s, hipStream
     const AdapterTile *short_tiles = (const AdapterTile*)(g.table + table.tiles16()), *tall_tiles = (const AdapterTile*)(g.table + table.tiles64());
     if (!s.tall()) return launch_expand_direct<DT, 1, WHOLE>(g, short_tiles, s.tiles(), stream);
     const int half = expand_half(g.rp);
-    if (DT == F8MI_FP32 || g.n < (half <= 32 ? 128 : 64)) return launch_expand_direct<DT, 4, WHOLE>(g, tall_tiles, s.tiles(), stream);
+    if (DT == F8MI_FP32 || g.n < expand_least(g.rp)) return launch_expand_direct<DT, 4, WHOLE>(g, tall_tiles, s.tiles(), stream);
     if constexpr (DT != F8MI_FP32) {
         if (half == 16) return launch_expand_tall<DT, 16, 128, WHOLE>(g, tall_tiles, s.tiles(), stream);
         if (half == 32) return launch_expand_tall<DT, 32, 128, WHOLE>(g, tall_tiles, s.tiles(), stream);
@@ -896,7 +948,7 @@ static int launch_expand3(const AdapterArgs& g, const AdapterShape& s, hipStream
 }
 template <int DT>
 static int launch_expand2(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
-    return g.r % Ln<DT>::V == 0 ? launch_expand3<DT, true>(g, s, stream) : launch_expand3<DT, false>(g, s, stream);
+    return g.b_turned || g.r % Ln<DT>::V == 0 ? launch_expand3<DT, true>(g, s, stream) : launch_expand3<DT, false>(g, s, stream);
 }
 static int launch_expand(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
     if (s.dtype == F8MI_BF16) return launch_expand2<F8MI_BF16>(g, s, stream);
@@ -951,8 +1003,8 @@ struct AdapterBackwardSpace {
         auto take = [&](int64_t n) { const int64_t o = at_byte; at_byte += up256(n); return o; };
         partial = take(inner ? s.partial_bytes(s.n) : 0);
         dh = take(inner ? s.m * s.rp() * 4 : 0);
-        bt = take(inner ? s.count * s.n * s.r * size : 0);
-        at = take(need_dx ? s.count * s.k * s.r * size : 0);
+        bt = take(inner && !s.turns_b() ? s.count * s.n * s.r * size : 0);
+        at = take(need_dx && !s.turns_a() ? s.count * s.k * s.r * size : 0);
         sums = take(std::max(need_da ? chunks * s.k * s.r * 4 : 0, need_db ? chunks * s.n * s.r * 4 : 0));
         bytes = at_byte;
     }
@@ -981,7 +1033,7 @@ extern "C" int f8mi_adapters(const void* x, int64_t ldx, const void* a, const vo
     const int64_t need = s.partial_bytes(k);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0 || (uintptr_t)table % 16 != 0 || (uintptr_t)h % 16 != 0) { set_error("f8mi_adapters: 16-byte aligned workspace of %lld bytes, table and h", (long long)need); return F8MI_ERR_INVALID_ARG; }
     const AdapterArgs g{(const uint8_t*)x, ldx, (const uint8_t*)a, (const int32_t*)table, (float*)workspace, m, (int)k, (int)r, (int)s.rp(), (int)count, (int)s.splits(k),
-                        (const uint8_t*)b, scale, factor, (const uint8_t*)y, ldy, (uint8_t*)out, h, (int)n, 0, 0};
+                        (const uint8_t*)b, scale, factor, (const uint8_t*)y, ldy, (uint8_t*)out, h, (int)n, 0, 0, false, false};
     if (int rc = launch_shrink(g, s, stream)) return rc;
     return launch_expand(g, s, stream);
 }
@@ -1000,11 +1052,12 @@ extern "C" int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const v
     uint8_t* ws = (uint8_t*)workspace;
     float* dh = (float*)(ws + space.dh);
     if (dx || da) {
-        if (int rc = launch_transpose(b, ws + space.bt, count, (int)n, (int)r, dtype, stream)) return rc;
-        if (dx)
+        if (!s.turns_b())
+            if (int rc = launch_transpose(b, ws + space.bt, count, (int)n, (int)r, dtype, stream)) return rc;
+        if (dx && !s.turns_a())
             if (int rc = launch_transpose(a, ws + space.at, count, (int)r, (int)k, dtype, stream)) return rc;
-        const AdapterArgs g{(const uint8_t*)dout, ld_dout, ws + space.bt, (const int32_t*)table, (float*)(ws + space.partial), m, (int)n, (int)r, (int)s.rp(), (int)count, (int)s.splits(n),
-                            dx ? ws + space.at : nullptr, scale, factor, nullptr, 0, (uint8_t*)dx, dh, dx ? (int)k : 0, 0, 0};
+        const AdapterArgs g{(const uint8_t*)dout, ld_dout, s.turns_b() ? (const uint8_t*)b : ws + space.bt, (const int32_t*)table, (float*)(ws + space.partial), m, (int)n, (int)r, (int)s.rp(), (int)count, (int)s.splits(n),
+                            !dx ? nullptr : s.turns_a() ? (const uint8_t*)a : ws + space.at, scale, factor, nullptr, 0, (uint8_t*)dx, dh, dx ? (int)k : 0, 0, 0, s.turns_b(), dx && s.turns_a()};
         if (int rc = launch_shrink(g, s, stream)) return rc;
         if (int rc = launch_expand(g, s, stream)) return rc;
     }
