@@ -105,7 +105,7 @@ struct AdapterArgs {
 // ---- shrink: a wave has 16 rows of one adapter, 16 RT of its rank and a part of the contraction; those of a workgroup's waves are added up in LDS
 constexpr int SHRINK_WAVES = 8;
 template <int DT, int RT>
-__global__ __launch_bounds__(64 * SHRINK_WAVES) void adapter_shrink_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+__global__ __launch_bounds__(64 * SHRINK_WAVES, 4) void adapter_shrink_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
     constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2, STEP = 128 / SIZE;  // values of a step: a line of the cache of each row
     constexpr int DEPTH = 2;                                          // steps in flight
     constexpr int WAVES = SHRINK_WAVES;
@@ -118,31 +118,38 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void adapter_shrink_kernel(const
     const int32_t* order = g.table + AdapterTable(g.m, g.count).order() + tile.first;
     const int64_t steps = g.k / STEP, unit = (int64_t)split * WAVES + wave, units = (int64_t)g.splits * WAVES;
     const int s0 = (int)(steps * unit / units), s1 = (int)(steps * (unit + 1) / units);
-    const uint8_t *px = g.x + (int64_t)order[min(lm, tile.rows - 1)] * g.ld * SIZE, *pa[RT];
+    const int at_row = order[min(lm, tile.rows - 1)];  // (waited for behind the first loads of A)
+    const uint8_t *px = nullptr, *pa[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) pa[i] = g.a + ((int64_t)tile.group * g.r + min(j0 + i * 16 + lm, g.r - 1)) * g.k * SIZE;
 
     v4f_l acc[RT] = {};
     uint4 fx[DEPTH][2], fa[DEPTH][RT][2];
-    auto load = [&](int d, int h, int s) __attribute__((always_inline)) {
+    auto load_a = [&](int d, int h, int s) __attribute__((always_inline)) {
         const int64_t at = (int64_t)s * 128 + h * 64 + lq * 16;
 #pragma unroll
         for (int i = 0; i < RT; i++) fa[d][i][h] = load16_any(pa[i] + at);
-        fx[d][h] = load16_any(px + at);
     };
+    auto load_x = [&](int d, int h, int s) __attribute__((always_inline)) { fx[d][h] = load16_any(px + (int64_t)s * 128 + h * 64 + lq * 16); };
     auto multiply = [&](int d, int h) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < RT; i++) acc[i] = mfma_16<DT>(fa[d][i][h], fx[d][h], acc[i]);
     };
+    if (s0 < s1)
+#pragma unroll
+        for (int i = 0; i < 2 * DEPTH; i++) load_a(i / 2, i % 2, min(s0 + i / 2, s1 - 1));
+    __builtin_amdgcn_sched_barrier(0);
+    px = g.x + (int64_t)at_row * g.ld * SIZE;
     if (s0 < s1) {
 #pragma unroll
-        for (int i = 0; i < 2 * DEPTH; i++) load(i / 2, i % 2, min(s0 + i / 2, s1 - 1));
+        for (int i = 0; i < 2 * DEPTH; i++) load_x(i / 2, i % 2, min(s0 + i / 2, s1 - 1));
         int s = s0;
         for (; s + DEPTH < s1; s += DEPTH) {
 #pragma unroll
             for (int i = 0; i < 2 * DEPTH; i++) {  // what has been multiplied is asked for again at once
                 multiply(i / 2, i % 2);
-                load(i / 2, i % 2, min(s + DEPTH + i / 2, s1 - 1));
+                load_a(i / 2, i % 2, min(s + DEPTH + i / 2, s1 - 1));
+                load_x(i / 2, i % 2, min(s + DEPTH + i / 2, s1 - 1));
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -421,8 +428,9 @@ struct ExpandCols {
 };
 
 // A wave has 16 rows and 64 columns at a time, the waves below each other (WR 4) or side by side (1); B straight out of the caches.
-template <int DT, int WR, bool WHOLE>
-__global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+// The last 64 columns are moved back to end with the last one (those before are computed twice, the same); EDGE: there are less than 64.
+template <int DT, int WR, bool WHOLE, bool EDGE>
+__global__ __launch_bounds__(EXPAND_THREADS, WHOLE && !EDGE ? 4 : 1) void adapter_expand_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
     constexpr int SIZE = Ln<DT>::SIZE, ROWS = 16 * WR, STEP = WR > 1 ? 64 : 256;
     extern __shared__ __align__(16) uint8_t expand_lds[];  // h [ROWS][pitch], then (fp16) fp32 [ROWS][half] while it is converted
     __shared__ uint32_t row_most[DT == F8MI_FP16 ? ROWS : 1];
@@ -442,14 +450,14 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_kernel(const Ad
     const int end = min(g.n, (chunk + 1) * g.cols);
     const int64_t b_total = (int64_t)g.count * g.n * g.r;
     for (int n0 = chunk * g.cols + (WR > 1 ? 0 : wave * 64); n0 < end; n0 += STEP) {
-        const ExpandCols<DT, true> at{n0, g.n, lq, lm};
-        uint4 fy[ExpandCols<DT, true>::PIECES] = {};
+        const ExpandCols<DT, EDGE> at{EDGE ? n0 : min(n0, g.n - 64), g.n, lq, lm};
+        uint4 fy[ExpandCols<DT, EDGE>::PIECES] = {};
         if (g.y) at.load(y_row, fy);
         v4f_l acc[4] = {};
         if (!none) {
             int64_t pb[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) pb[c] = ((int64_t)tile.group * g.n + min(at.of_tile(c), g.n - 1)) * g.r;
+            for (int c = 0; c < 4; c++) pb[c] = ((int64_t)tile.group * g.n + (EDGE ? min(at.of_tile(c), g.n - 1) : at.of_tile(c))) * g.r;
             auto load_b = [&](uint4 (&fb)[4], int j) __attribute__((always_inline)) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) fb[c] = load_of_row<DT, WHOLE>(g.b, pb[c] + j, b_total, j, g.r);
@@ -910,11 +918,15 @@ static int launch_expand_kernel(K kernel, std::atomic<uint64_t>& allowed, Adapte
     hipLaunchKernelGGL(kernel, dim3((unsigned)(n_tiles * g.chunks)), dim3(EXPAND_THREADS), (unsigned)lds, stream, g, tiles);
     return check_hip(hipGetLastError(), "adapter expand kernel launch");
 }
-template <int DT, int WR, bool WHOLE>
-static int launch_expand_direct(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
+template <int DT, int WR, bool WHOLE, bool EDGE>
+static int launch_expand_direct2(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
-    g.cols = expand_cols(g, n_tiles, WR > 1 ? 8 : 4, 256);
-    return launch_expand_kernel(adapter_expand_kernel<DT, WR, WHOLE>, allowed, g, tiles, n_tiles, 16 * WR * (expand_pitch<DT>(g.rp) * Ln<DT>::SIZE + (DT == F8MI_FP16 ? expand_half(g.rp) * 4 : 0)), stream);
+    g.cols = expand_cols(g, n_tiles, 4, 256);
+    return launch_expand_kernel(adapter_expand_kernel<DT, WR, WHOLE, EDGE>, allowed, g, tiles, n_tiles, 16 * WR * (expand_pitch<DT>(g.rp) * Ln<DT>::SIZE + (DT == F8MI_FP16 ? expand_half(g.rp) * 4 : 0)), stream);
+}
+template <int DT, int WR, bool WHOLE>
+static int launch_expand_direct(const AdapterArgs& g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
+    return g.n < 64 ? launch_expand_direct2<DT, WR, WHOLE, true>(g, tiles, n_tiles, stream) : launch_expand_direct2<DT, WR, WHOLE, false>(g, tiles, n_tiles, stream);
 }
 template <int DT, int MOST, int CB, bool WHOLE, bool ODD, bool TURNED>
 static int launch_expand_tall2(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
