@@ -814,20 +814,27 @@ __global__ __launch_bounds__(OUTER_THREADS) void adapter_outer16_kernel(const Ou
         }
 }
 
-// the chunks of an adapter added up in their order; no chunk: zeros
-__global__ __launch_bounds__(256) void adapter_outer_finish_kernel(const float* __restrict__ partial, const int32_t* __restrict__ chunk_start, const float* __restrict__ scale, float factor, int64_t size,
-                                                                   void* __restrict__ out, int dtype) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int e = blockIdx.y, first = chunk_start[e], end = chunk_start[e + 1];
-    if (at >= size) return;
+// The chunks of an adapter added up in their order; no chunk: zeros.  Both gradients in one launch.
+struct OuterSums {
+    const float* partial;
+    int64_t size;  // of one adapter's gradient; 0: not asked for
+    void* out;
+};
+__global__ __launch_bounds__(256) void adapter_outer_finish_kernel(const OuterSums first, const OuterSums second, int first_blocks, const int32_t* __restrict__ chunk_start, const float* __restrict__ scale,
+                                                                   float factor, int dtype) {
+    const bool in_first = (int)blockIdx.x < first_blocks;
+    const OuterSums g{in_first ? first.partial : second.partial, in_first ? first.size : second.size, in_first ? first.out : second.out};
+    const int64_t at = (int64_t)(blockIdx.x - (in_first ? 0 : first_blocks)) * 256 + threadIdx.x;
+    const int e = blockIdx.y, begin = chunk_start[e], end = chunk_start[e + 1];
+    if (at >= g.size) return;
     float s = 0.f;
 #pragma unroll 8
-    for (int i = first; i < end; i++) s += partial[(int64_t)i * size + at];
-    if (first < end) s *= factor * (scale ? scale[e] : 1.f);
-    const int64_t to = (int64_t)e * size + at;
-    if (dtype == F8MI_FP32) ((float*)out)[to] = s;
-    else if (dtype == F8MI_BF16) ((uint16_t*)out)[to] = (uint16_t)pack2<F8MI_BF16>(s, 0.f);
-    else ((uint16_t*)out)[to] = (uint16_t)pack2<F8MI_FP16>(s, 0.f);
+    for (int i = begin; i < end; i++) s += g.partial[(int64_t)i * g.size + at];
+    if (begin < end) s *= factor * (scale ? scale[e] : 1.f);
+    const int64_t to = (int64_t)e * g.size + at;
+    if (dtype == F8MI_FP32) ((float*)g.out)[to] = s;
+    else if (dtype == F8MI_BF16) ((uint16_t*)g.out)[to] = (uint16_t)pack2<F8MI_BF16>(s, 0.f);
+    else ((uint16_t*)g.out)[to] = (uint16_t)pack2<F8MI_FP16>(s, 0.f);
 }
 
 // ---- [batch][rows][cols] -> [batch][cols][rows]
@@ -982,15 +989,18 @@ static void launch_outer2(const OuterArgs& g, const AdapterTile* chunks, int64_t
     const dim3 grid((unsigned)n_chunks, (unsigned)((g.cols + OUTER_COLS - 1) / OUTER_COLS), (unsigned)((g.rp + OUTER_RANK - 1) / OUTER_RANK));
     hipLaunchKernelGGL(adapter_outer_kernel<DT>, grid, dim3(OUTER_THREADS), 0, stream, g, chunks);
 }
-static int launch_outer(const OuterArgs& g, int dtype, const float* scale, float factor, void* out, int out_dtype, hipStream_t stream) {
+static int launch_outer(const OuterArgs& g, int dtype, hipStream_t stream) {
     const AdapterTable table(g.m, g.count);
-    const int64_t chunks = table.tiles(adapter_chunk_rows(g.m)), size = (int64_t)g.cols * g.r;
+    const int64_t chunks = table.tiles(adapter_chunk_rows(g.m));
     const AdapterTile* list = (const AdapterTile*)(g.table + table.chunks());
     if (dtype == F8MI_BF16) launch_outer2<F8MI_BF16>(g, list, chunks, stream);
     else if (dtype == F8MI_FP16) launch_outer2<F8MI_FP16>(g, list, chunks, stream);
     else launch_outer2<F8MI_FP32>(g, list, chunks, stream);
-    if (int rc = check_hip(hipGetLastError(), "adapter gradient kernel launch")) return rc;
-    hipLaunchKernelGGL(adapter_outer_finish_kernel, dim3((unsigned)((size + 255) / 256), (unsigned)g.count), dim3(256), 0, stream, g.partial, g.table + table.chunk_start(), scale, factor, size, out, out_dtype);
+    return check_hip(hipGetLastError(), "adapter gradient kernel launch");
+}
+static int launch_outer_finish(const AdapterShape& s, const OuterSums& da, const OuterSums& db, const int32_t* table, const float* scale, float factor, int out_dtype, hipStream_t stream) {
+    const int64_t first = (da.size + 255) / 256, second = (db.size + 255) / 256;
+    hipLaunchKernelGGL(adapter_outer_finish_kernel, dim3((unsigned)(first + second), (unsigned)s.count), dim3(256), 0, stream, da, db, (int)first, table + s.table().chunk_start(), scale, factor, out_dtype);
     return check_hip(hipGetLastError(), "adapter gradient sum kernel launch");
 }
 
@@ -1007,7 +1017,7 @@ static bool bad_stride(int64_t ld, int64_t cols) { return ld < 0 || (ld < cols &
 
 // parts of backward's workspace
 struct AdapterBackwardSpace {
-    int64_t partial, dh, at, bt, sums, bytes;
+    int64_t partial, dh, at, bt, sums_a, sums_b, bytes;
     AdapterBackwardSpace(const AdapterShape& s, bool need_dx, bool need_da, bool need_db) {
         const int64_t size = s.dtype == F8MI_FP32 ? 4 : 2, chunks = s.table().tiles(adapter_chunk_rows(s.m));
         const bool inner = need_dx || need_da;
@@ -1017,7 +1027,8 @@ struct AdapterBackwardSpace {
         dh = take(inner ? s.m * s.rp() * 4 : 0);
         bt = take(inner && !s.turns_b() ? s.count * s.n * s.r * size : 0);
         at = take(need_dx && !s.turns_a() ? s.count * s.k * s.r * size : 0);
-        sums = take(std::max(need_da ? chunks * s.k * s.r * 4 : 0, need_db ? chunks * s.n * s.r * 4 : 0));
+        sums_a = take(need_da ? chunks * s.k * s.r * 4 : 0);
+        sums_b = take(need_db ? chunks * s.n * s.r * 4 : 0);
         bytes = at_byte;
     }
 };
@@ -1073,16 +1084,18 @@ extern "C" int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const v
         if (int rc = launch_shrink(g, s, stream)) return rc;
         if (int rc = launch_expand(g, s, stream)) return rc;
     }
-    const OuterArgs o{nullptr, 0, nullptr, (const int32_t*)table, m, 0, (int)r, (int)s.rp(), (int)count, 0, (float*)(ws + space.sums)};
+    float *sums_a = (float*)(ws + space.sums_a), *sums_b = (float*)(ws + space.sums_b);
+    const OuterArgs o{nullptr, 0, nullptr, (const int32_t*)table, m, 0, (int)r, (int)s.rp(), (int)count, 0, nullptr};
     if (da) {
         OuterArgs q = o;
-        q.big = (const uint8_t*)x; q.ld = ldx; q.small = dh; q.cols = (int)k;
-        if (int rc = launch_outer(q, dtype, scale, factor, da, p_dtype, stream)) return rc;
+        q.big = (const uint8_t*)x; q.ld = ldx; q.small = dh; q.cols = (int)k; q.partial = sums_a;
+        if (int rc = launch_outer(q, dtype, stream)) return rc;
     }
     if (db) {
         OuterArgs q = o;
-        q.big = (const uint8_t*)dout; q.ld = ld_dout; q.small = h; q.cols = (int)n; q.cols_first = 1;
-        if (int rc = launch_outer(q, dtype, scale, factor, db, p_dtype, stream)) return rc;
+        q.big = (const uint8_t*)dout; q.ld = ld_dout; q.small = h; q.cols = (int)n; q.cols_first = 1; q.partial = sums_b;
+        if (int rc = launch_outer(q, dtype, stream)) return rc;
     }
+    if (da || db) return launch_outer_finish(s, {sums_a, da ? k * r : 0, da}, {sums_b, db ? n * r : 0, db}, (const int32_t*)table, scale, factor, p_dtype, stream);
     return F8MI_OK;
 }

@@ -191,10 +191,12 @@ struct RmsBackwardArgs {
     hipStream_t stream;
 };
 
+// Sums of columns in registers, of more pieces a lane than those have room for in LDS
+constexpr bool rms_sums_in_lds(int dtype, int vpt) { return vpt > (dtype == F8MI_FP32 ? 3 : 2); }
 template <int DT, int PT, int T, int VPT, bool DS>
 __global__ __launch_bounds__(rms_backward_threads(T, VPT), 4) void rms_norm_backward_kernel(const RmsBackwardArgs a) {
     constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE, GROUPS = rms_backward_threads(T, VPT) / T;
-    constexpr bool SHARED = VPT > 1;
+    constexpr bool SHARED = VPT > 1, IN_LDS = rms_sums_in_lds(DT, VPT);
     __shared__ float slots[2][rms_backward_threads(T, VPT) / 64];
     __shared__ float sums[GROUPS > 1 ? (GROUPS - 1) * T * V : 1];
     extern __shared__ uint4 rms_shared[];
@@ -218,7 +220,8 @@ __global__ __launch_bounds__(rms_backward_threads(T, VPT), 4) void rms_norm_back
     };
     fetch(first + group);
     LnShared<PT, V> ws{rms_shared, (cols + V - 1) / V};
-    float w[V], dw[VPT][V];
+    float4* const lds_sums = (float4*)(rms_shared + ws.pieces * ws.PARTS);  // of V columns, the four from part * 4 on, at [part][piece]; a lane's own
+    float w[V], dw[IN_LDS ? 1 : VPT][V];
     if constexpr (SHARED) {
         ws.fill(a.weight, cols, 1.f);
         __syncthreads();
@@ -226,9 +229,16 @@ __global__ __launch_bounds__(rms_backward_threads(T, VPT), 4) void rms_norm_back
         ln_param<PT, V, int>(a.weight, lane.last, cols, 1.f, w);
     }
 #pragma unroll
-    for (int p = 0; p < VPT; p++)
+    for (int p = 0; p < VPT; p++) {
+        if constexpr (IN_LDS) {
+            if (p * T + t < ws.pieces)
 #pragma unroll
-        for (int i = 0; i < V; i++) dw[p][i] = 0.f;
+                for (int part = 0; part < V / 4; part++) lds_sums[part * ws.pieces + p * T + t] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) dw[p][i] = 0.f;
+        }
+    }
     int parity = 0;
     for (int64_t r0 = first; r0 < rows; r0 += stride, parity ^= 1) {
         const int64_t row = r0 + group;
@@ -237,7 +247,7 @@ __global__ __launch_bounds__(rms_backward_threads(T, VPT), 4) void rms_norm_back
         for (int p = 0; p < VPT; p++) {
             qs[p] = next.s[p];
             qg[p] = next.g[p];
-            if constexpr (DS) qd[p] = row < rows ? lane.template load<DT>(a.ds + row * a.ld_ds * SIZE, p, cols) : make_uint4(0u, 0u, 0u, 0u);  // needed behind the sum
+            if constexpr (DS && !IN_LDS) qd[p] = row < rows ? lane.template load<DT>(a.ds + row * a.ld_ds * SIZE, p, cols) : make_uint4(0u, 0u, 0u, 0u);  // needed behind the sum
         }
         const float rstd = next.rstd;
         if (r0 + stride < rows) fetch(row + stride);
@@ -252,12 +262,28 @@ __global__ __launch_bounds__(rms_backward_threads(T, VPT), 4) void rms_norm_back
             for (int i = 0; i < V; i++) {
                 xh[i] *= rstd;
                 if (!lane.has(p, i)) g[i] = xh[i] = 0.f;
-                dw[p][i] = __builtin_fmaf(g[i], xh[i], dw[p][i]);
                 s2 = __builtin_fmaf(g[i] * w[i], xh[i], s2);
-                asm volatile("" : "+v"(dw[p][i]));  // added here, not behind the barrier
+                if constexpr (!IN_LDS) {
+                    dw[p][i] = __builtin_fmaf(g[i], xh[i], dw[p][i]);
+                    asm volatile("" : "+v"(dw[p][i]));  // added here, not behind the barrier
+                }
             }
+            if constexpr (IN_LDS)
+                if (p * T + t < ws.pieces)
+#pragma unroll
+                    for (int part = 0; part < V / 4; part++) {
+                        float4& d = lds_sums[part * ws.pieces + p * T + t];
+                        const float4 v = d;
+                        d = make_float4(__builtin_fmaf(g[4 * part], xh[4 * part], v.x), __builtin_fmaf(g[4 * part + 1], xh[4 * part + 1], v.y),
+                                        __builtin_fmaf(g[4 * part + 2], xh[4 * part + 2], v.z), __builtin_fmaf(g[4 * part + 3], xh[4 * part + 3], v.w));
+                    }
         }
         if (!a.dx) continue;
+        if constexpr (DS && IN_LDS) {  // (no registers for it before)
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < VPT; p++) qd[p] = row < rows ? lane.template load<DT>(a.ds + row * a.ld_ds * SIZE, p, cols) : make_uint4(0u, 0u, 0u, 0u);
+        }
         s2 = rms_row_sum<T>(s2, slots[parity]) * inv_cols;
         if (row >= rows) continue;
 #pragma unroll
@@ -295,9 +321,21 @@ __global__ __launch_bounds__(rms_backward_threads(T, VPT), 4) void rms_norm_back
                 for (int i = 0; i < V; i++) dw[p][i] += sums[(k * V + i) * T + t];
         }
         const int col = lane.col(p);
+        if constexpr (IN_LDS) {
+            if (p * T + t >= ws.pieces) continue;
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (lane.has(p, i)) out[col + i] = dw[p][i];
+            for (int part = 0; part < V / 4; part++) {
+                const float4 d = lds_sums[part * ws.pieces + p * T + t];
+                const float v[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (lane.has(p, part * 4 + e)) out[col + part * 4 + e] = v[e];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (lane.has(p, i)) out[col + i] = dw[p][i];
+        }
     }
 }
 
@@ -351,33 +389,69 @@ __global__ __launch_bounds__(RMS_WIDE_THREADS) void rms_norm_wide_kernel(const R
     if (!CAST && a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
 }
 
-template <int DT, int PT>
+// SUMS: the sums of the columns too, in LDS; a workgroup takes every (number of workgroups)-th row.  Else a workgroup a row, and a kernel of their own.
+template <int DT, int PT, bool SUMS>
 __global__ __launch_bounds__(RMS_WIDE_THREADS) void rms_norm_backward_wide_kernel(const RmsBackwardArgs a) {
     constexpr int V = Ln<DT>::V, SIZE = Ln<DT>::SIZE;
     constexpr int64_t STEP = RMS_WIDE_THREADS * V;
-    __shared__ float slots[RMS_WIDE_THREADS / 64];
-    const int64_t row = blockIdx.x, cols = a.cols;
-    const uint8_t *srow = a.s + row * a.ld * SIZE, *grow = a.dy + row * a.ld_dy * SIZE;
-    const float rstd = a.rstd[row];
-    float s[V], g[V], w[V], s2 = 0.f;
-    for (int64_t col = threadIdx.x * V; col < cols; col += STEP) {
-        ln_unpack<DT>(ln_load<DT, int64_t>(srow, col, cols), s);
-        ln_unpack<DT>(ln_load<DT, int64_t>(grow, col, cols), g);
-        ln_param<PT, V, int64_t>(a.weight, col, cols, 1.f, w);
+    __shared__ float slots[2][RMS_WIDE_THREADS / 64];
+    extern __shared__ uint4 rms_shared[];  // SUMS: of V columns, the four from part * 4 on, at [part][piece]
+    const int64_t cols = a.cols, pieces = (cols + V - 1) / V;
+    float4* sums = (float4*)rms_shared;
+    if constexpr (SUMS)
+        for (int64_t i = threadIdx.x; i < pieces; i += RMS_WIDE_THREADS)
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (col + i < cols) s2 = __builtin_fmaf(g[i] * w[i], s[i] * rstd, s2);
+            for (int part = 0; part < V / 4; part++) sums[part * pieces + i] = make_float4(0.f, 0.f, 0.f, 0.f);  // (a lane's own)
+    int parity = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+        const uint8_t *srow = a.s + row * a.ld * SIZE, *grow = a.dy + row * a.ld_dy * SIZE;
+        const float rstd = a.rstd[row];
+        float s2 = 0.f;
+#pragma unroll 2
+        for (int64_t col = threadIdx.x * V; col < cols; col += STEP) {
+            float s[V], g[V], w[V];
+            ln_unpack<DT>(ln_load<DT, int64_t>(srow, col, cols), s);
+            ln_unpack<DT>(ln_load<DT, int64_t>(grow, col, cols), g);
+            ln_param<PT, V, int64_t>(a.weight, col, cols, 1.f, w);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                s[i] *= rstd;
+                if (col + i >= cols) s[i] = 0.f;  // (there g is zero, but rstd may be infinite)
+                s2 = __builtin_fmaf(g[i] * w[i], s[i], s2);
+            }
+            if constexpr (SUMS)
+#pragma unroll
+                for (int part = 0; part < V / 4; part++) {
+                    float4& d = sums[part * pieces + col / V];
+                    d = make_float4(__builtin_fmaf(g[4 * part], s[4 * part], d.x), __builtin_fmaf(g[4 * part + 1], s[4 * part + 1], d.y), __builtin_fmaf(g[4 * part + 2], s[4 * part + 2], d.z),
+                                    __builtin_fmaf(g[4 * part + 3], s[4 * part + 3], d.w));
+                }
+        }
+        if (!a.dx) continue;
+        s2 = rms_row_sum<RMS_WIDE_THREADS>(s2, slots[parity]) / (float)cols;
+#pragma unroll 2
+        for (int64_t col = threadIdx.x * V; col < cols; col += STEP) {
+            float s[V], g[V], w[V], d[V] = {};
+            ln_unpack<DT>(ln_load<DT, int64_t>(srow, col, cols), s);
+            ln_unpack<DT>(ln_load<DT, int64_t>(grow, col, cols), g);
+            ln_param<PT, V, int64_t>(a.weight, col, cols, 1.f, w);
+            if (a.ds) ln_unpack<DT>(ln_load<DT, int64_t>(a.ds + row * a.ld_ds * SIZE, col, cols), d);
+#pragma unroll
+            for (int i = 0; i < V; i++) g[i] = __builtin_fmaf(rstd, __builtin_fmaf(s[i] * rstd, -s2, g[i] * w[i]), d[i]);
+            ln_store<DT, int64_t>(a.dx + row * cols * SIZE, col, cols, g);
+        }
     }
-    s2 = rms_row_sum<RMS_WIDE_THREADS>(s2, slots) / (float)cols;
-    for (int64_t col = threadIdx.x * V; col < cols; col += STEP) {
-        ln_unpack<DT>(ln_load<DT, int64_t>(srow, col, cols), s);
-        ln_unpack<DT>(ln_load<DT, int64_t>(grow, col, cols), g);
-        ln_param<PT, V, int64_t>(a.weight, col, cols, 1.f, w);
-        float d[V] = {};
-        if (a.ds) ln_unpack<DT>(ln_load<DT, int64_t>(a.ds + row * a.ld_ds * SIZE, col, cols), d);
+    if constexpr (SUMS) {
+        float* out = a.partial + (int64_t)blockIdx.x * cols;
+        for (int64_t i = threadIdx.x; i < pieces; i += RMS_WIDE_THREADS)
 #pragma unroll
-        for (int i = 0; i < V; i++) g[i] = __builtin_fmaf(rstd, __builtin_fmaf(s[i] * rstd, -s2, g[i] * w[i]), d[i]);
-        ln_store<DT, int64_t>(a.dx + row * cols * SIZE, col, cols, g);
+            for (int part = 0; part < V / 4; part++) {
+                const float4 d = sums[part * pieces + i];
+                const float v[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (i * V + part * 4 + e < cols) out[i * V + part * 4 + e] = v[e];
+            }
     }
 }
 
@@ -428,21 +502,22 @@ __global__ __launch_bounds__(64 * RMS_FINISH_WAVES) void rms_norm_finish_kernel(
 // ---- launches
 
 // Lanes of a row and pieces a lane, by the number of 16-byte pieces of a row; 0: does not fit.  The weight has to fit in LDS, and a lane's pieces in 128 registers: with
-// the conversion to block scales three of them, in backward, where each column has a sum, two of 16-bit values.
+// the conversion to block scales three of them, in backward three of 16-bit values.
 struct RmsShape {
     int t, vpt;
 };
 constexpr int RMS_MAX_LDS = (160 << 10) - 512;
 static int64_t rms_pieces(int64_t cols, int dtype) { return (cols + (dtype == F8MI_FP32 ? 3 : 7)) / (dtype == F8MI_FP32 ? 4 : 8); }
 static int64_t rms_lds(int64_t cols, int dtype, int p_dtype) { return rms_pieces(cols, dtype) * 16 * (dtype == p_dtype ? 1 : 2); }
-constexpr int rms_forward_pieces(bool cast) { return cast ? 3 : 4; }
-constexpr int rms_backward_pieces(int dtype) { return dtype == F8MI_FP32 ? 4 : 2; }
-static RmsShape rms_shape(int64_t cols, int dtype, int p_dtype, int most) {
+constexpr int rms_forward_pieces(int dtype, bool cast) { return cast ? 3 : dtype == F8MI_FP32 ? 5 : 4; }
+constexpr int rms_backward_pieces(int dtype) { return dtype == F8MI_FP32 ? 5 : 3; }
+static int64_t rms_sums_lds(int64_t cols, int dtype) { return rms_pieces(cols, dtype) * (dtype == F8MI_FP32 ? 16 : 32); }  // of the columns' sums
+static RmsShape rms_shape(int64_t cols, int dtype, int p_dtype, int most, bool sums) {
     const int64_t pieces = rms_pieces(cols, dtype);
     for (int t = 64; t <= RMS_LANES; t *= 2)
         if (pieces <= t) return {t, 1};
     const int64_t vpt = (pieces + RMS_LANES - 1) / RMS_LANES;
-    if (vpt > most || rms_lds(cols, dtype, p_dtype) > RMS_MAX_LDS) return {0, 0};
+    if (vpt > most || rms_lds(cols, dtype, p_dtype) + (sums && rms_sums_in_lds(dtype, (int)vpt) ? rms_sums_lds(cols, dtype) : 0) > RMS_MAX_LDS) return {0, 0};
     return {RMS_LANES, (int)vpt};
 }
 // Workgroups of `threads` lanes, `per_cu` of them on every CU, no more than the rows need
@@ -455,8 +530,9 @@ static int64_t rms_chunk_rows(int64_t rows, int64_t cols, int dtype) {  // of th
     return std::max<int64_t>(8, (rows + want - 1) / want);
 }
 static int64_t rms_parts(int64_t rows, int64_t cols, int dtype, int p_dtype) {
-    const RmsShape s = rms_shape(cols, dtype, p_dtype, rms_backward_pieces(dtype));
+    const RmsShape s = rms_shape(cols, dtype, p_dtype, rms_backward_pieces(dtype), true);
     if (s.t) return rms_workgroups(s, rows, rms_backward_threads(s.t, s.vpt), RMS_LANES / rms_backward_threads(s.t, s.vpt));
+    if (rms_sums_lds(cols, dtype) <= RMS_MAX_LDS) return std::min<int64_t>(cu_count(), rows);
     const int64_t chunk = rms_chunk_rows(rows, cols, dtype);
     return (rows + chunk - 1) / chunk;
 }
@@ -479,7 +555,7 @@ static int launch_rms_wide(const RmsArgs& a) {
 }
 template <int DT, int PT, bool RES, bool CAST>
 static int launch_rms_by_size(const RmsArgs& a) {
-    const RmsShape s = rms_shape(CAST ? (a.cols + 127) & ~(int64_t)127 : a.cols, DT, PT, rms_forward_pieces(CAST));
+    const RmsShape s = rms_shape(CAST ? (a.cols + 127) & ~(int64_t)127 : a.cols, DT, PT, rms_forward_pieces(DT, CAST), false);
     if (s.t == 64) return launch_rms<DT, PT, 64, 1, RES, CAST>(a);
     if (s.t == 128) return launch_rms<DT, PT, 128, 1, RES, CAST>(a);
     if (s.t == 256) return launch_rms<DT, PT, 256, 1, RES, CAST>(a);
@@ -487,8 +563,10 @@ static int launch_rms_by_size(const RmsArgs& a) {
     if (s.vpt == 1) return launch_rms<DT, PT, RMS_LANES, 1, RES, CAST>(a);
     if (s.vpt == 2) return launch_rms<DT, PT, RMS_LANES, 2, RES, CAST>(a);
     if (s.vpt == 3) return launch_rms<DT, PT, RMS_LANES, 3, RES, CAST>(a);
-    if constexpr (rms_forward_pieces(CAST) == 4)
+    if constexpr (rms_forward_pieces(DT, CAST) >= 4)
         if (s.vpt == 4) return launch_rms<DT, PT, RMS_LANES, 4, RES, CAST>(a);
+    if constexpr (rms_forward_pieces(DT, CAST) == 5)
+        if (s.vpt == 5) return launch_rms<DT, PT, RMS_LANES, 5, RES, CAST>(a);
     return launch_rms_wide<DT, PT, CAST>(a);
 }
 template <bool CAST>
@@ -512,12 +590,20 @@ static int launch_rms_backward(const RmsBackwardArgs& a) {
         static std::atomic<uint64_t> allowed{0};
         if (int rc = allow_big_lds(kernel, RMS_MAX_LDS, allowed)) return rc;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)a.parts), dim3(rms_backward_threads(T, VPT)), (unsigned)(VPT > 1 ? rms_lds(a.cols, DT, PT) : 0), a.stream, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.parts), dim3(rms_backward_threads(T, VPT)),
+                       (unsigned)((VPT > 1 ? rms_lds(a.cols, DT, PT) : 0) + (rms_sums_in_lds(DT, VPT) ? rms_sums_lds(a.cols, DT) : 0)), a.stream, a);
     return check_hip(hipGetLastError(), "RMS norm backward kernel launch");
 }
 template <int DT, int PT>
 static int launch_rms_backward_wide(const RmsBackwardArgs& a) {
-    if (a.dx) hipLaunchKernelGGL((rms_norm_backward_wide_kernel<DT, PT>), dim3((unsigned)a.rows), dim3(RMS_WIDE_THREADS), 0, a.stream, a);
+    if (a.partial && rms_sums_lds(a.cols, DT) <= RMS_MAX_LDS) {
+        const auto kernel = rms_norm_backward_wide_kernel<DT, PT, true>;
+        static std::atomic<uint64_t> allowed{0};
+        if (int rc = allow_big_lds(kernel, RMS_MAX_LDS, allowed)) return rc;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)a.parts), dim3(RMS_WIDE_THREADS), (unsigned)rms_sums_lds(a.cols, DT), a.stream, a);
+        return check_hip(hipGetLastError(), "RMS norm backward kernel launch");
+    }
+    if (a.dx) hipLaunchKernelGGL((rms_norm_backward_wide_kernel<DT, PT, false>), dim3((unsigned)a.rows), dim3(RMS_WIDE_THREADS), 0, a.stream, a);
     if (a.partial) {
         const unsigned strips = (unsigned)((a.cols + 256 * Ln<DT>::V - 1) / (256 * Ln<DT>::V));
         hipLaunchKernelGGL(rms_norm_columns_kernel<DT>, dim3(strips, (unsigned)a.parts), dim3(256), 0, a.stream, a, rms_chunk_rows(a.rows, a.cols, DT));
@@ -526,16 +612,17 @@ static int launch_rms_backward_wide(const RmsBackwardArgs& a) {
 }
 template <int DT, int PT, bool DS>
 static int launch_rms_backward_by_size(const RmsBackwardArgs& a) {
-    const RmsShape s = rms_shape(a.cols, DT, PT, rms_backward_pieces(DT));
+    const RmsShape s = rms_shape(a.cols, DT, PT, rms_backward_pieces(DT), true);
     if (s.t == 64) return launch_rms_backward<DT, PT, 64, 1, DS>(a);
     if (s.t == 128) return launch_rms_backward<DT, PT, 128, 1, DS>(a);
     if (s.t == 256) return launch_rms_backward<DT, PT, 256, 1, DS>(a);
     if (s.t == 512) return launch_rms_backward<DT, PT, 512, 1, DS>(a);
     if (s.vpt == 1) return launch_rms_backward<DT, PT, RMS_LANES, 1, DS>(a);
     if (s.vpt == 2) return launch_rms_backward<DT, PT, RMS_LANES, 2, DS>(a);
-    if constexpr (rms_backward_pieces(DT) == 4) {
-        if (s.vpt == 3) return launch_rms_backward<DT, PT, RMS_LANES, 3, DS>(a);
+    if (s.vpt == 3) return launch_rms_backward<DT, PT, RMS_LANES, 3, DS>(a);
+    if constexpr (rms_backward_pieces(DT) == 5) {
         if (s.vpt == 4) return launch_rms_backward<DT, PT, RMS_LANES, 4, DS>(a);
+        if (s.vpt == 5) return launch_rms_backward<DT, PT, RMS_LANES, 5, DS>(a);
     }
     return launch_rms_backward_wide<DT, PT>(a);
 }
