@@ -514,8 +514,12 @@ constexpr int rms_backward_pieces(int dtype) { return dtype == F8MI_FP32 ? 5 : 3
 static int64_t rms_sums_lds(int64_t cols, int dtype) { return rms_pieces(cols, dtype) * (dtype == F8MI_FP32 ? 16 : 32); }  // of the columns' sums
 static RmsShape rms_shape(int64_t cols, int dtype, int p_dtype, int most, bool sums) {
     const int64_t pieces = rms_pieces(cols, dtype);
-    for (int t = 64; t <= RMS_LANES; t *= 2)
+    for (int t = 64; t <= 512; t *= 2)
         if (pieces <= t) return {t, 1};
+    // two workgroups a CU instead of one whose lanes are half idle (both passes, us, 1024 lanes / 512: 8192 rows of 4352 bf16 107 / 102, of 5120 118 / 113, 4096 of 6000 78 / 76, of 7000
+    // 87 / 88, of 8192 94 / 96; 4099 of 2050 fp32 45 / 42, of 3000 53 / 52, of 4096 62 / 65)
+    if (pieces <= 768) return {512, 2};
+    if (pieces <= RMS_LANES) return {RMS_LANES, 1};
     const int64_t vpt = (pieces + RMS_LANES - 1) / RMS_LANES;
     if (vpt > most || rms_lds(cols, dtype, p_dtype) + (sums && rms_sums_in_lds(dtype, (int)vpt) ? rms_sums_lds(cols, dtype) : 0) > RMS_MAX_LDS) return {0, 0};
     return {RMS_LANES, (int)vpt};
@@ -559,7 +563,8 @@ static int launch_rms_by_size(const RmsArgs& a) {
     if (s.t == 64) return launch_rms<DT, PT, 64, 1, RES, CAST>(a);
     if (s.t == 128) return launch_rms<DT, PT, 128, 1, RES, CAST>(a);
     if (s.t == 256) return launch_rms<DT, PT, 256, 1, RES, CAST>(a);
-    if (s.t == 512) return launch_rms<DT, PT, 512, 1, RES, CAST>(a);
+    if (s.t == 512 && s.vpt == 1) return launch_rms<DT, PT, 512, 1, RES, CAST>(a);
+    if (s.t == 512) return launch_rms<DT, PT, 512, 2, RES, CAST>(a);
     if (s.vpt == 1) return launch_rms<DT, PT, RMS_LANES, 1, RES, CAST>(a);
     if (s.vpt == 2) return launch_rms<DT, PT, RMS_LANES, 2, RES, CAST>(a);
     if (s.vpt == 3) return launch_rms<DT, PT, RMS_LANES, 3, RES, CAST>(a);
@@ -616,7 +621,8 @@ static int launch_rms_backward_by_size(const RmsBackwardArgs& a) {
     if (s.t == 64) return launch_rms_backward<DT, PT, 64, 1, DS>(a);
     if (s.t == 128) return launch_rms_backward<DT, PT, 128, 1, DS>(a);
     if (s.t == 256) return launch_rms_backward<DT, PT, 256, 1, DS>(a);
-    if (s.t == 512) return launch_rms_backward<DT, PT, 512, 1, DS>(a);
+    if (s.t == 512 && s.vpt == 1) return launch_rms_backward<DT, PT, 512, 1, DS>(a);
+    if (s.t == 512) return launch_rms_backward<DT, PT, 512, 2, DS>(a);
     if (s.vpt == 1) return launch_rms_backward<DT, PT, RMS_LANES, 1, DS>(a);
     if (s.vpt == 2) return launch_rms_backward<DT, PT, RMS_LANES, 2, DS>(a);
     if (s.vpt == 3) return launch_rms_backward<DT, PT, RMS_LANES, 3, DS>(a);
