@@ -22,7 +22,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: Optional[torch.Tensor] = None
         raise ValueError(f"dropout: p={p} is not a probability")
     if seed is None:
         _native._require_gpu(x, "x")
-        seed = torch.empty(1, dtype=torch.int64, device=x.device).random_()
+        seed = torch.randint(2**63 - 1, (1,), device=x.device)
     if not torch.compiler.is_compiling():
         out = _native.model_ops().dropout(x, p, seed, residual)
         if out is not None:

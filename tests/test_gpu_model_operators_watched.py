@@ -113,6 +113,38 @@ def test_gradients_through_modes_and_traces(f8, name):
     assert equal(tuple(grads(torch.compile(call, fullgraph=True, backend="aot_eager"))), tuple(want))
 
 
+def test_compiled_calls_without_gradients(f8):
+    for name, (_, _, call, args) in calls(f8).items():
+        with torch.no_grad():
+            assert equal(torch.compile(call, fullgraph=True, backend="aot_eager")(*args), call(*args)), name
+    x = torch.ones(100, 100, device="cuda")
+    drawn = torch.compile(lambda t: f8.dropout(t, 0.5), fullgraph=True, backend="aot_eager")
+    a, b = drawn(x), drawn(x)  # a seed of its own each time
+    assert 0.4 < (a == 0).float().mean() < 0.6 and not torch.equal(a, b)
+
+
+def test_autocast(f8):
+    """The norm and dropout keep x's type; the adapters and the served linear take the autocast type, as the linears do."""
+    x, w = normal(40, 256, dtype=FP32), normal(256, dtype=FP32, seed=1)
+    a, b, y = normal(3, 8, 256, seed=3, dtype=FP32), normal(3, 128, 8, seed=4, dtype=FP32), normal(40, 128, seed=5, dtype=FP32)
+    rows = f8.AdapterRows(torch.arange(40, device="cuda") % 3, 3)
+    served = f8.Float8BlockwiseInferenceLinear.from_float(nn.Linear(256, 64, device="cuda", dtype=FP32))
+    layer = f8.AdaptedLinear(nn.Linear(256, 128, device="cuda"), 3, 8)
+    f8.select_adapters(layer, rows)
+    with torch.no_grad():
+        layer.adapter_b.normal_()
+        plain = f8.low_rank_adapters(x.bfloat16(), a, b, rows, y.bfloat16())
+        with torch.autocast("cuda", dtype=BF16):
+            assert f8.rms_norm(x, 256, w).dtype == FP32 and f8.dropout(x, 0.5).dtype == FP32
+            out = f8.low_rank_adapters(x, a, b, rows, y)
+            assert out.dtype == BF16 and torch.equal(out, plain)
+            assert served(f8.rms_norm_blockwise(x, 256, w)).dtype == BF16 and layer(x).dtype == BF16
+    xs = x.clone().requires_grad_()
+    with torch.autocast("cuda", dtype=BF16):
+        layer(xs).sum().backward()
+    assert xs.grad.dtype == FP32 and layer.adapter_a.grad.dtype == FP32 and xs.grad.isfinite().all()
+
+
 @pytest.mark.parametrize("name", NAMES)
 def test_tangents_raise(f8, name):
     _, _, call, args = calls(f8)[name]
