@@ -866,11 +866,15 @@ struct AdapterShape {
     // Tiles of 64 rows where an adapter has that many on average: x is read once for each 64 of the rank, an adapter once a tile.
     bool tall() const { return m >= 48 * (count < m ? count : m); }
     int64_t tiles() const { return table().tiles(tall() ? 64 : 16); }
-    // Parts of a contraction of this length: four workgroups a CU, and two steps at least (of a workgroup, of each wave of one for short tiles)
+    // Parts of a contraction that two workgroups a CU want
+    int64_t wanted_splits() const { return std::max<int64_t>(1, 2 * (int64_t)cu_count() / std::max<int64_t>(1, tiles() * ((rp() + 63) / 64))); }
+    int64_t row_bytes(int64_t contracted) const { return contracted * (dtype == F8MI_FP32 ? 4 : 2); }
+    // Bytes of a row that a step of 64 rows takes: 512 where a rank of up to 16 leaves the registers and each part has two such steps, else 256
+    int shrink_bytes(int64_t contracted) const { return rp() <= 16 && row_bytes(contracted) >= 2 * 512 * wanted_splits() ? 512 : 256; }
+    // No more parts than steps (4099 tokens of 1000 fp16 values, 68 tiles: 11.5 us with one part, 7.0 with as many as there are steps); of short tiles two steps for each wave
     int64_t splits(int64_t contracted) const {
-        const int64_t bytes = contracted * (dtype == F8MI_FP32 ? 4 : 2), steps = tall() ? bytes / (rp() <= 16 ? 512 : 256) : bytes / (128 * SHRINK_WAVES);
-        const int64_t want = 2 * (int64_t)cu_count() / std::max<int64_t>(1, tiles() * ((rp() + 63) / 64));
-        return std::max<int64_t>(1, std::min({want, steps / 2, (int64_t)32}));
+        const int64_t steps = tall() ? (row_bytes(contracted) + shrink_bytes(contracted) - 1) / shrink_bytes(contracted) : row_bytes(contracted) / (128 * SHRINK_WAVES) / 2;
+        return std::max<int64_t>(1, std::min({wanted_splits(), steps, (int64_t)32}));
     }
     // Backward reads the adapters' matrices as they lie; short tiles and fp32 have their transposes made (4.6 us each for four adapters of 4096 x 16)
     bool turns_b() const { return tall() && dtype != F8MI_FP32; }
@@ -888,7 +892,8 @@ static int launch_shrink3(const AdapterArgs& g, const AdapterShape& s, hipStream
     const dim3 grid((unsigned)(s.tiles() * g.splits), (unsigned)(rt <= 4 ? 1 : (rt + 3) / 4));
     if (s.tall()) {
         const AdapterTile* tiles = (const AdapterTile*)(g.table + table.tiles64());
-        if (rt == 1) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 512, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        if (rt == 1 && s.shrink_bytes(g.k) == 512) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 512, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
+        else if (rt == 1) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 1, 256, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
         else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 2, 256, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
         else hipLaunchKernelGGL((adapter_shrink_tall_kernel<DT, 4, 256, ODD, TURNED>), grid, dim3(TALL_THREADS), 0, stream, g, tiles);
     } else {

@@ -527,7 +527,7 @@ int f8mi_grad_clip(const f8mi_grad* grads, int64_t count, int norm_kind, float m
 /* ---- RMS norm over the last dimension, with the addition in front of it -------------------------------------------------------------
  * sum [rows][cols] = x + residual, rounded to their type; y = sum * rstd * weight, rstd = 1 / sqrt(mean(sum^2) + eps), statistics in fp32.  residual NULL: sum is
  * x, and nothing is written there.  weight: cols values of p_dtype (x's dtype or F8MI_FP32), or NULL (1).  ld, ld_residual: elements from row to row, or 0: one row
- * throughout; y and sum are dense and overlap no input but for sum == residual == dense.  rstd: [rows] for the backward pass, or NULL. */
+ * throughout; y and sum are dense and overlap no input (a row's last values are read by two lanes, which do not wait for each other).  rstd: [rows] for the backward pass, or NULL. */
 int f8mi_rms_norm(const void* x, int64_t ld, const void* residual, int64_t ld_residual, int64_t rows, int64_t cols, int dtype, const void* weight, int p_dtype, float eps,
                   void* y, void* sum, float* rstd, void* stream);
 /* ... and y, not rounded before, kept in block scales (f8mi_block_cast's copy of `rows` rows contracting over the columns): out and out_scales, 16-byte aligned.  Scales of
@@ -543,7 +543,7 @@ int f8mi_rms_norm_backward(const void* dy, int64_t ld_dy, const void* s, int64_t
 
 /* ---- dropout without a stored mask ------------------------------------------------------------------------------------------------------
  * out = residual + (kept ? x / (1 - p) : 0) of n dense values (residual NULL: 0), in fp32 and rounded once; its own backward pass with the output's gradient as x.
- * Value i is kept if word i % 4 of Philox 4x32 with 7 rounds, counter i / 4 and the 64 bits at seed_dev as the key, is at least p * 2^32, rounded.  0 <= p < 1. */
+ * Value i is kept if word i % 4 of Philox 4x32 with 7 rounds, counter i / 4 and the 64 bits at seed_dev as the key, is at least p * 2^32, rounded.  0 <= p < 1.  out overlaps no input. */
 int f8mi_dropout(const void* x, const void* residual, int64_t n, int dtype, double p, const int64_t* seed_dev, void* out, void* stream);
 
 /* ---- low-rank adapters of many requests beside one projection -------------------------------------------------------------------------
@@ -551,7 +551,7 @@ int f8mi_dropout(const void* x, const void* residual, int64_t n, int dtype, doub
  * scale [count] fp32 or NULL (1); y [m][n] of x's dtype or NULL (0); out dense.
  * table: what f8mi_adapter_rows made of the rows' adapters (int32 or int64 ids; a number that is no adapter's means none) for this m and count:
  * f8mi_adapter_rows_words() 32-bit words, 16-byte aligned.  h: [m][r rounded up to 16] fp32 for the backward pass, or NULL.  workspace: 16-byte
- * aligned, contents arbitrary.  Sums are fp32, in a fixed order. */
+ * aligned, contents arbitrary.  out overlaps no input (its last columns may be computed twice).  Sums are fp32, in a fixed order. */
 #define F8MI_ADAPTER_MAX_ROWS (1 << 24)
 #define F8MI_ADAPTER_MAX_COUNT 32768
 #define F8MI_ADAPTER_MAX_RANK 256
