@@ -14,7 +14,7 @@ import torch.nn as nn
 
 from . import _custom_ops_model as _compiled
 from . import _native
-from .float8_blockwise import Float8BlockwiseInferenceLinear
+from .float8_blockwise import BlockwiseActivations, Float8BlockwiseInferenceLinear
 from .residual_dropout import dropout as _dropout
 
 _HP_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -24,7 +24,9 @@ MAX_RANK, MAX_COUNT, MAX_ROWS = 256, 32768, 1 << 24  # F8MI_ADAPTER_MAX_*
 
 class AdapterRows:
     """The rows of a batch by adapter: ``adapters`` has one whole number for each row (``x.numel() / k`` of them, in their order), that of its adapter among ``count``; any other
-    number, -1 for instance, means none.  Made once for a batch and used by all its layers; it keeps what the numbers were then."""
+    number, -1 for instance, means none.  Made once for a batch and used by all its layers; it keeps what the numbers were then.
+
+    A captured graph reads the table that it was captured with: it has to outlive the graph, or is made inside the capture, from numbers that are written between replays."""
 
     def __init__(self, adapters: torch.Tensor, count: int):
         _native._require_gpu(adapters, "adapters")
@@ -132,6 +134,8 @@ class AdaptedLinear(nn.Module):
         y = self.linear(input)
         if self.rows is None:
             return y
+        if isinstance(input, BlockwiseActivations):
+            raise TypeError("AdaptedLinear: the adapters need the activations in bfloat16, float16 or float32, not BlockwiseActivations")
         x = _dropout(input, self.dropout) if self.training and self.dropout > 0.0 else input
         return low_rank_adapters(x, self.adapter_a, self.adapter_b, self.rows, y, self.scaling)
 
@@ -141,9 +145,12 @@ class AdaptedLinear(nn.Module):
 
 def adapt_linears(module: nn.Module, count: int, rank: int, *, alpha: Optional[float] = None, dropout: float = 0.0, dtype: Optional[torch.dtype] = None,
                   module_filter_fn: Optional[Callable[[nn.Module, str], bool]] = None) -> nn.Module:
-    """Puts an ``AdaptedLinear`` around every linear of ``module`` that passes ``module_filter_fn(linear, fqn)``; no other parameter of ``module`` asks for gradients
-    any more.  A root-level linear is returned adapted."""
-    module.requires_grad_(False)
+    """Puts an ``AdaptedLinear`` around every linear of ``module`` that passes ``module_filter_fn(linear, fqn)``; no parameter of ``module`` but its adapters asks for
+    gradients any more.  A root-level linear is returned adapted; linears that have adapters already keep those."""
+    kept = {id(p) for m in module.modules() if isinstance(m, AdaptedLinear) for p in (m.adapter_a, m.adapter_b)}
+    for p in module.parameters():
+        if id(p) not in kept:
+            p.requires_grad_(False)
     wanted = lambda m, fqn: isinstance(m, (nn.Linear, Float8BlockwiseInferenceLinear)) and (module_filter_fn is None or module_filter_fn(m, fqn))
     around = lambda m: AdaptedLinear(m, count, rank, alpha, dropout, dtype).train(m.training)
     if wanted(module, ""):
@@ -159,7 +166,8 @@ def adapt_linears(module: nn.Module, count: int, rank: int, *, alpha: Optional[f
             else:
                 visit(child, fqn)
 
-    visit(module, "")
+    if not isinstance(module, AdaptedLinear):
+        visit(module, "")
     return module
 
 

@@ -31,6 +31,23 @@ def test_arguments_are_checked_before_tensors():
         f8.Dropout.from_float(nn.Dropout(0.5, inplace=True))
 
 
+def test_adapting_twice_keeps_the_first_adapters():
+    model = nn.Sequential(nn.Linear(8, 6), nn.Linear(6, 4))
+    f8.adapt_linears(model, 3, 2, module_filter_fn=lambda m, fqn: fqn == "0")
+    first = model[0]
+    assert f8.adapt_linears(model, 3, 4, module_filter_fn=lambda m, fqn: True) is model
+    assert model[0] is first and type(first.linear) is nn.Linear and type(model[1]) is f8.AdaptedLinear and (first.rank, model[1].rank) == (2, 4)
+    assert [n for n, p in model.named_parameters() if p.requires_grad] == ["0.adapter_a", "0.adapter_b", "1.adapter_a", "1.adapter_b"]
+    assert f8.adapt_linears(first, 3, 4) is first and type(first.linear) is nn.Linear
+
+
+def test_activations_that_have_been_cast_are_refused_beside_adapters():
+    layer = f8.AdaptedLinear(nn.Linear(8, 6), 2, 2)
+    layer.linear, layer.rows = nn.Identity(), object()  # (as a linear that takes them, and any rows)
+    with pytest.raises(TypeError, match="BlockwiseActivations"):
+        layer(f8.BlockwiseActivations(torch.empty(2, 1, 64), torch.empty(1), (1, 8), BF16))
+
+
 def test_modules_are_swapped_and_share_their_parameters():
     model = nn.Sequential(nn.RMSNorm(8, eps=1e-3), nn.Dropout(0.3), nn.Linear(8, 6), nn.Sequential(nn.RMSNorm(6), nn.Linear(6, 4, bias=False)))
     weights = dict(model.named_parameters())
