@@ -1,7 +1,7 @@
 // Low-rank adapters of many requests beside one projection (f8mi_adapters.h), forward and backward:
 //   h_i = A_e x_i,  out_i = y_i + scale_e B_e h_i,
 //   dh_i = B_e^T dout_i,  dx_i = scale_e A_e^T dh_i,  dA_e = scale_e sum_i dh_i x_i^T,  dB_e = scale_e sum_i dout_i h_i^T.
-// Three kernels: `shrink` (h from x and A, dh from dout and B^T), `expand` (out from y, h and B; dx from dh and A^T) and `outer` (dA, dB).  The
+// Three kernels: `shrink` (h from x and A, dh from dout and B^T), `expand` (out from y, h and B; dx from dh and A^T) and `outer` (dA, dB); for few rows `whole`, the first two in one.  The
 // transposed copies of the adapters that backward needs of short tiles and in fp32 are made by a fourth; they are small beside x.
 //
 // HBM-bound: x, y and dout are read once each, out and dx written, an adapter is read by each of its tiles out of the L2.  The products run
@@ -103,21 +103,15 @@ struct AdapterArgs {
 };
 
 // ---- shrink: a wave has 16 rows of one adapter, 16 RT of its rank and a part of the contraction; those of a workgroup's waves are added up in LDS
-// (16 rows a tile: an adapter of few rows.  64 rows with an adapter each, 8192 values, rank 16: 6.6 us out of HBM, one token of 4096 3.1; latency.)
+// (16 rows a tile: an adapter of few rows.  64 rows with an adapter each, 8192 values, rank 16: 6.6 us out of HBM; latency.)
 constexpr int SHRINK_WAVES = 8;
-template <int DT, int RT>
-__global__ __launch_bounds__(64 * SHRINK_WAVES, 4) void adapter_shrink_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+// The sums of part `split` of `splits` over the workgroup, of the rank from j0 on, to h [tile.rows][rp]
+template <int DT, int RT, int DEPTH, int WAVES>  // DEPTH: steps in flight
+__device__ __forceinline__ void shrink_rows(const AdapterArgs& g, const AdapterTile& tile, int split, int splits, int j0, float4 (&part)[WAVES][RT][64], float* h_out) {
     constexpr int SIZE = DT == F8MI_FP32 ? 4 : 2, STEP = 128 / SIZE;  // values of a step: a line of the cache of each row
-    constexpr int DEPTH = 2;                                          // steps in flight
-    constexpr int WAVES = SHRINK_WAVES;
-    __shared__ float4 part[WAVES][RT][64];
-    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), split = id % g.splits;  // a tile's workgroups, and those of the next ones, on one XCD: A stays in its L2
-    const AdapterTile tile = tiles[id / g.splits];
-    if (tile.rows == 0 || tile.group >= g.count) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lm = lane & 15, lq = lane >> 4;
-    const int j0 = blockIdx.y * (16 * RT);
     const int32_t* order = g.table + AdapterTable(g.m, g.count).order() + tile.first;
-    const int64_t steps = g.k / STEP, unit = (int64_t)split * WAVES + wave, units = (int64_t)g.splits * WAVES;
+    const int64_t steps = g.k / STEP, unit = (int64_t)split * WAVES + wave, units = (int64_t)splits * WAVES;
     const int s0 = (int)(steps * unit / units), s1 = (int)(steps * (unit + 1) / units);
     const int at_row = order[min(lm, tile.rows - 1)];  // (waited for behind the first loads of A)
     const uint8_t *px = nullptr, *pa[RT];
@@ -179,8 +173,16 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES, 4) void adapter_shrink_kernel(co
             const float4 p = part[w][at][l];
             s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
         }
-        if (row < tile.rows && j < g.rp) *(float4*)(g.partial + ((int64_t)split * g.m + tile.first + row) * g.rp + j) = s;
+        if (row < tile.rows && j < g.rp) *(float4*)(h_out + row * g.rp + j) = s;
     }
+}
+template <int DT, int RT>
+__global__ __launch_bounds__(64 * SHRINK_WAVES, 4) void adapter_shrink_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+    __shared__ float4 part[SHRINK_WAVES][RT][64];
+    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), split = id % g.splits;  // a tile's workgroups, and those of the next ones, on one XCD: A stays in its L2
+    const AdapterTile tile = tiles[id / g.splits];
+    if (tile.rows == 0 || tile.group >= g.count) return;
+    shrink_rows<DT, RT, 2, SHRINK_WAVES>(g, tile, split, g.splits, blockIdx.y * (16 * RT), part, g.partial + ((int64_t)split * g.m + tile.first) * g.rp);
 }
 
 // 64 rows of one adapter and 16 RT of its rank a workgroup: a wave has 16 of the rows and brings them itself, all four multiply them by the same part of A, which goes through LDS: BYTES
@@ -312,8 +314,8 @@ __host__ __device__ constexpr int expand_pitch(int rp) { return DT == F8MI_FP32 
 
 // The parts of h that the contraction's parts gave, added up, scaled and kept in LDS as the products take them: rows first .. of the table's order.  `sums` (fp16 alone): fp32
 // [ROWS][half] beside them, free afterwards.
-template <int DT, int ROWS>
-__device__ __forceinline__ void stage_h(const AdapterArgs& g, const AdapterTile& tile, bool first, uint8_t* kept_bytes, float* sums, uint32_t* row_most, float& factor, int my_row) {
+template <int DT, int ROWS, int THREADS = EXPAND_THREADS>
+__device__ __forceinline__ void stage_h(const AdapterArgs& g, const AdapterTile& tile, const float* parts, int splits, bool first, uint8_t* kept_bytes, float* sums, uint32_t* row_most, float& factor, int my_row) {
     const int t = threadIdx.x, rp = g.rp, pitch = expand_pitch<DT>(rp), half = DT == F8MI_FP32 ? rp : expand_half(rp), quads = half / 4;
     const float scale = g.factor * (g.scale ? g.scale[tile.group] : 1.f);
     auto keep = [&](int row, int j, const float (&v)[4]) __attribute__((always_inline)) {
@@ -333,13 +335,13 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& g, const AdapterTile&
         if (t < ROWS) row_most[t] = 0u;
         __syncthreads();
     }
-    for (int item = t; item < ROWS * quads; item += EXPAND_THREADS) {
+    for (int item = t; item < ROWS * quads; item += THREADS) {
         const int row = item / quads, j = (item - row * quads) * 4;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (row < tile.rows && j < rp) {
-            const float* p = g.partial + ((int64_t)tile.first + row) * rp + j;
+            const float* p = parts + row * rp + j;
 #pragma unroll 4
-            for (int i = 0; i < g.splits; i++) {
+            for (int i = 0; i < splits; i++) {
                 const float4 q = *(const float4*)(p + i * g.m * rp);
                 v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
             }
@@ -363,7 +365,7 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& g, const AdapterTile&
     factor = 1.f;
     if constexpr (DT == F8MI_FP16) {  // a power of two, 2^(e - 127), that brings the row's largest to [1, 2)
         auto exponent = [&](int row) __attribute__((always_inline)) { return (uint32_t)min(max((int)(row_most[row] >> 23), 1), 253); };
-        for (int item = t; item < ROWS * quads; item += EXPAND_THREADS) {
+        for (int item = t; item < ROWS * quads; item += THREADS) {
             const int row = item / quads;
             const float4 q = *(const float4*)(sums + item * 4);
             const float f = __uint_as_float((254u - exponent(row)) << 23);
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(EXPAND_THREADS, WHOLE && !EDGE ? 4 : 1) void adapte
     const int rp = g.rp, pitch = expand_pitch<DT>(rp), half = expand_half(rp);
     const int my_row = (WR > 1 ? wave * 16 : 0) + lm;
     float factor = 1.f;
-    if (!none) stage_h<DT, ROWS>(g, tile, chunk == 0, expand_lds, (float*)(expand_lds + ROWS * pitch * SIZE), row_most, factor, my_row);
+    if (!none) stage_h<DT, ROWS>(g, tile, g.partial + (int64_t)tile.first * rp, g.splits, chunk == 0, expand_lds, (float*)(expand_lds + ROWS * pitch * SIZE), row_most, factor, my_row);
     if (WR > 1 && wave * 16 >= tile.rows) return;
     const int64_t at_row = g.table[AdapterTable(g.m, g.count).order() + tile.first + min(my_row, tile.rows - 1)];
     const uint8_t *hrow = expand_lds + my_row * pitch * SIZE, *y_row = g.y + at_row * g.ld_y * SIZE;
@@ -496,6 +498,47 @@ __global__ __launch_bounds__(EXPAND_THREADS, WHOLE && !EDGE ? 4 : 1) void adapte
         }
         if (my_row < tile.rows) at.store(out_row, fy, acc, factor, !none);
     }
+}
+
+// Both products of 16 rows of one adapter of rank 16 or less in one launch: each workgroup of a tile has 64 columns a wave and finds all of h for itself, A out of the L2 but for the first of
+// them.  B and y are on their way meanwhile.
+constexpr int WHOLE_COLS = 64 * SHRINK_WAVES;
+template <int DT, bool WHOLE>
+__global__ __launch_bounds__(64 * SHRINK_WAVES, 4) void adapter_whole_kernel(const AdapterArgs g, const AdapterTile* __restrict__ tiles) {
+    constexpr int SIZE = Ln<DT>::SIZE, ROWS = 16, PITCH = expand_pitch<DT>(16);
+    __shared__ float4 part[SHRINK_WAVES][1][64];
+    __shared__ __align__(16) float h[ROWS * 16], sums[DT == F8MI_FP16 ? ROWS * 16 : 4];
+    __shared__ __align__(16) uint8_t kept[ROWS * PITCH * SIZE];
+    __shared__ uint32_t row_most[DT == F8MI_FP16 ? ROWS : 1];
+    const int id = xcd_contiguous_id(blockIdx.x, gridDim.x), chunk = id % g.chunks;
+    const AdapterTile tile = tiles[id / g.chunks];
+    if (tile.rows == 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lm = lane & 15, lq = lane >> 4;
+    const bool none = tile.group >= g.count;
+    const int64_t at_row = g.table[AdapterTable(g.m, g.count).order() + tile.first + min(lm, tile.rows - 1)];
+    const int n0 = chunk * WHOLE_COLS + wave * 64;
+    const ExpandCols<DT, false> at{min(n0, g.n - 64), g.n, lq, lm};  // (the last 64 columns are moved back as in the other kernels)
+    uint4 fy[ExpandCols<DT, false>::PIECES] = {}, fb[4] = {};
+    if (n0 < g.n) {
+        if (!none)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int j = DT == F8MI_FP32 ? lq * 4 : (lq & 1) * 8;  // (16-bit types: both parts of h in one instruction, B twice)
+                fb[c] = load_of_row<DT, WHOLE>(g.b, ((int64_t)tile.group * g.n + at.of_tile(c)) * g.r + j, (int64_t)g.count * g.n * g.r, j, g.r);
+            }
+        if (g.y) at.load(g.y + at_row * g.ld_y * SIZE, fy);
+    }
+    float factor = 1.f;
+    v4f_l acc[4] = {};
+    if (!none) {
+        shrink_rows<DT, 1, 4, SHRINK_WAVES>(g, tile, 0, 1, 0, part, h);
+        __syncthreads();
+        stage_h<DT, ROWS, 64 * SHRINK_WAVES>(g, tile, h, 1, chunk == 0, kept, sums, row_most, factor, lm);
+        const uint4 fh = *(const uint4*)(kept + lm * PITCH * SIZE + lq * 16);
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[c] = mfma_16<DT>(fb[c], fh, acc[c]);
+    }
+    if (n0 < g.n && lm < tile.rows) at.store(g.out + at_row * g.n * SIZE, fy, acc, factor, !none);
 }
 
 // 64 rows and B through LDS, 16-bit types: the four waves have 16 rows each and the same columns, CB of them at a time, so that B is read once a workgroup.  The next
@@ -554,7 +597,7 @@ __global__ __launch_bounds__(EXPAND_THREADS) void adapter_expand_tall_kernel(con
     float factor = 1.f;
     if (!none) {
         load_b(min(begin, last));
-        stage_h<DT, ROWS>(g, tile, chunk == 0, expand_lds, (float*)behind, row_most, factor, my_row);
+        stage_h<DT, ROWS>(g, tile, g.partial + (int64_t)tile.first * rp, g.splits, chunk == 0, expand_lds, (float*)behind, row_most, factor, my_row);
         keep_b(0);
         __syncthreads();
     }
@@ -883,7 +926,13 @@ struct AdapterShape {
     // Backward reads the adapters' matrices as they lie; short tiles and fp32 have their transposes made (4.6 us each for four adapters of 4096 x 16)
     bool turns_b() const { return tall() && dtype != F8MI_FP32; }
     bool turns_a() const { return turns_b() && rp() <= 128 && k >= expand_least((int)rp()); }  // (of a larger rank the rows of two blocks do not fit in LDS beside h)
-    int64_t partial_bytes(int64_t contracted) const { return splits(contracted) * m * rp() * 4; }
+    // Both products in one launch, where an adapter's rank and rows are few, its side of the contraction is short enough for each workgroup to read all of it and there is a workgroup a CU at most.
+    // Eager calls are bound by the host, 9.3 us with two launches and a workspace, 5.2 - 7 with one.  On the GPU (us a call in a captured graph, two launches / one): one row 2048 -> 2048 of rank 8
+    // 6.5 / 5.7, 4096 -> 4096 (128 KB) 6.7 / 7.3; 16 rows of 16 adapters 2048 -> 2048 8.1 / 7.0; 256 KB: one row 7.0 / 13; more workgroups: 64 rows of 64 adapters 1024 -> 4096 10.8 / 11.5.
+    bool whole(int64_t contracted, int64_t columns) const {
+        return !tall() && rp() <= 16 && 16 * row_bytes(contracted) <= (128 << 10) && (columns == 0 || columns >= 64) && tiles() * ((columns + WHOLE_COLS - 1) / WHOLE_COLS) <= cu_count();
+    }
+    int64_t partial_bytes(int64_t contracted, int64_t columns) const { return whole(contracted, columns) ? 0 : splits(contracted) * m * rp() * 4; }
 };
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -983,6 +1032,22 @@ static int launch_expand(const AdapterArgs& g, const AdapterShape& s, hipStream_
     if (s.dtype == F8MI_FP16) return launch_expand2<F8MI_FP16>(g, s, stream);
     return launch_expand2<F8MI_FP32>(g, s, stream);
 }
+template <int DT, bool WHOLE>
+static int launch_whole2(AdapterArgs g, const AdapterShape& s, hipStream_t stream) {
+    g.chunks = std::max(1, (g.n + WHOLE_COLS - 1) / WHOLE_COLS);
+    hipLaunchKernelGGL((adapter_whole_kernel<DT, WHOLE>), dim3((unsigned)(s.tiles() * g.chunks)), dim3(64 * SHRINK_WAVES), 0, stream, g, (const AdapterTile*)(g.table + s.table().tiles16()));
+    return check_hip(hipGetLastError(), "adapter kernel launch");
+}
+template <int DT>
+static int launch_whole(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
+    return g.r % Ln<DT>::V == 0 ? launch_whole2<DT, true>(g, s, stream) : launch_whole2<DT, false>(g, s, stream);
+}
+// h and out
+static int launch_products(const AdapterArgs& g, const AdapterShape& s, hipStream_t stream) {
+    if (s.whole(g.k, g.n)) return s.dtype == F8MI_BF16 ? launch_whole<F8MI_BF16>(g, s, stream) : s.dtype == F8MI_FP16 ? launch_whole<F8MI_FP16>(g, s, stream) : launch_whole<F8MI_FP32>(g, s, stream);
+    if (int rc = launch_shrink(g, s, stream)) return rc;
+    return launch_expand(g, s, stream);
+}
 template <int DT, bool COLS_FIRST>
 static void launch_outer16(const OuterArgs& g, const AdapterTile* chunks, int64_t n_chunks, hipStream_t stream) {
     const int blocks = (g.cols + OUTER_COLS - 1) / OUTER_COLS, rt = g.rp / 16;
@@ -1032,7 +1097,7 @@ struct AdapterBackwardSpace {
         const bool inner = need_dx || need_da;
         int64_t at_byte = 0;
         auto take = [&](int64_t n) { const int64_t o = at_byte; at_byte += up256(n); return o; };
-        partial = take(inner ? s.partial_bytes(s.n) : 0);
+        partial = take(inner ? s.partial_bytes(s.n, need_dx ? s.k : 0) : 0);
         dh = take(inner ? s.m * s.rp() * 4 : 0);
         bt = take(inner && !s.turns_b() ? s.count * s.n * s.r * size : 0);
         at = take(need_dx && !s.turns_a() ? s.count * s.k * s.r * size : 0);
@@ -1048,7 +1113,7 @@ using namespace f8mi;
 
 extern "C" int64_t f8mi_adapters_workspace_bytes(int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype) {
     const AdapterShape s{m, k, n, r, count, dtype};
-    return adapters_check("f8mi_adapters_workspace_bytes", s) || m == 0 ? 0 : s.partial_bytes(k);
+    return adapters_check("f8mi_adapters_workspace_bytes", s) || m == 0 ? 0 : s.partial_bytes(k, n);
 }
 extern "C" int64_t f8mi_adapters_backward_workspace_bytes(int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype, int need_dx, int need_da, int need_db) {
     const AdapterShape s{m, k, n, r, count, dtype};
@@ -1062,12 +1127,11 @@ extern "C" int f8mi_adapters(const void* x, int64_t ldx, const void* a, const vo
     if (int rc = adapters_check("f8mi_adapters", s)) return rc;
     if (m == 0) return F8MI_OK;
     if (!x || !a || !b || !table || !out || bad_stride(ldx, k) || (y && bad_stride(ldy, n))) { set_error("f8mi_adapters: null pointer or row stride"); return F8MI_ERR_INVALID_ARG; }
-    const int64_t need = s.partial_bytes(k);
-    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0 || (uintptr_t)table % 16 != 0 || (uintptr_t)h % 16 != 0) { set_error("f8mi_adapters: 16-byte aligned workspace of %lld bytes, table and h", (long long)need); return F8MI_ERR_INVALID_ARG; }
+    const int64_t need = s.partial_bytes(k, n);
+    if ((need && !workspace) || workspace_bytes < need || (uintptr_t)workspace % 16 != 0 || (uintptr_t)table % 16 != 0 || (uintptr_t)h % 16 != 0) { set_error("f8mi_adapters: 16-byte aligned workspace of %lld bytes, table and h", (long long)need); return F8MI_ERR_INVALID_ARG; }
     const AdapterArgs g{(const uint8_t*)x, ldx, (const uint8_t*)a, (const int32_t*)table, (float*)workspace, m, (int)k, (int)r, (int)s.rp(), (int)count, (int)s.splits(k),
                         (const uint8_t*)b, scale, factor, (const uint8_t*)y, ldy, (uint8_t*)out, h, (int)n, 0, 0, false, false};
-    if (int rc = launch_shrink(g, s, stream)) return rc;
-    return launch_expand(g, s, stream);
+    return launch_products(g, s, stream);
 }
 
 extern "C" int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const void* a, const void* b, const float* scale, float factor, const void* table, const float* h, int64_t m,
@@ -1090,8 +1154,7 @@ extern "C" int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const v
             if (int rc = launch_transpose(a, ws + space.at, count, (int)r, (int)k, dtype, stream)) return rc;
         const AdapterArgs g{(const uint8_t*)dout, ld_dout, s.turns_b() ? (const uint8_t*)b : ws + space.bt, (const int32_t*)table, (float*)(ws + space.partial), m, (int)n, (int)r, (int)s.rp(), (int)count, (int)s.splits(n),
                             !dx ? nullptr : s.turns_a() ? (const uint8_t*)a : ws + space.at, scale, factor, nullptr, 0, (uint8_t*)dx, dh, dx ? (int)k : 0, 0, 0, s.turns_b(), dx && s.turns_a()};
-        if (int rc = launch_shrink(g, s, stream)) return rc;
-        if (int rc = launch_expand(g, s, stream)) return rc;
+        if (int rc = launch_products(g, s, stream)) return rc;
     }
     float *sums_a = (float*)(ws + space.sums_a), *sums_b = (float*)(ws + space.sums_b);
     const OuterArgs o{nullptr, 0, nullptr, (const int32_t*)table, m, 0, (int)r, (int)s.rp(), (int)count, 0, nullptr};

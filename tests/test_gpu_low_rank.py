@@ -108,6 +108,28 @@ def test_forward_and_backward(f8, shape, dtype):
         assert all(torch.equal(got[name], again[name]) for name in got)
 
 
+FEW = [  # on both sides of what goes in one launch: the length of the contractions, the number of columns, the rank, the workgroups
+    (1, 4096, 513, 8, 3), (1, 4097, 513, 8, 3), (5, 2048, 1100, 5, 2), (5, 2056, 4096, 16, 2), (20, 300, 512, 16, 20), (20, 300, 63, 16, 20), (20, 63, 300, 16, 20), (20, 300, 64, 17, 20),
+    (16, 64, 7000, 16, 64), (16, 64, 9000, 16, 64), (33, 1, 64, 1, 40),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("shape", FEW, ids=lambda s: "x".join(map(str, s)))
+def test_few_rows_in_one_launch_and_in_two(f8, shape, dtype):
+    m, k, n, r, count = shape
+    x, a, b, y, scale, dout = made(m, k, n, r, count, dtype, m + n)
+    ids = whose("any", m, count, k)
+    rows, want = f8.AdapterRows(ids, count), formula(x, a, b, ids, y, scale, dout)
+    got = run(f8, x, a, b, rows, y, scale, dout)
+    check(got, want)
+    assert torch.equal(got["out"], f8.low_rank_adapters(x, a, b, rows, y, scale))  # (without h kept for backward)
+    for name, t in (("dx", x), ("da", a), ("db", b)):  # each gradient alone, the same bits
+        leaf = t.clone().requires_grad_()
+        f8.low_rank_adapters(*(leaf if u is t else u for u in (x, a, b)), rows, y, scale).backward(dout)
+        assert torch.equal(leaf.grad, got[name]), name
+
+
 @pytest.mark.parametrize("kind", ["one", "none"])
 @pytest.mark.parametrize("m", [1, 16, 200])
 def test_all_rows_of_one_adapter_and_of_none(f8, kind, m):
