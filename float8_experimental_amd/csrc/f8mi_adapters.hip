@@ -984,6 +984,19 @@ static int expand_cols(const AdapterArgs& g, int64_t n_tiles, int per_cu, int bl
     const int64_t want = std::max<int64_t>(1, per_cu * (int64_t)cu_count() / n_tiles), blocks = std::max(1, (g.n + block - 1) / block);  // (one where h alone is asked for)
     return (int)((blocks + want - 1) / want * block);
 }
+// The same for 64 rows, of which four workgroups run on a CU at once: eight a CU or four, whichever takes less by an estimate in blocks of columns.  A workgroup costs its blocks and what h costs it
+// (`before`: half a block for each block's bytes of parts, out of the L2, and one for the latency); a round that is less than a quarter full takes as long as a full one; a tenth of a workgroup is
+// lost at the end.  (us of the kernel, eight / four: 2048 rows of rank 16 to 4096 columns 15.0 / 12.8, 4099 fp16 of rank 12 to 4097 31 / 27, 4096 of rank 64 to 4096 36 / 30; 8192 of rank 16 to 4096 36 / 37, to 8192
+// 60.6 / 61.8, of rank 64 to 14336 140 / 147.)
+static int expand_tall_cols(const AdapterArgs& g, int64_t n_tiles, int block) {
+    auto cost = [&](int cols) {
+        const double blocks = cols / block, before = 1.0 + 0.5 * g.splits * g.rp / block, slots = 4.0 * cu_count();
+        const double rounds = std::max(1.0, (double)n_tiles * ((g.n + cols - 1) / cols) / slots), rest = rounds - (int64_t)rounds;
+        return (rest > 0.0 && rest < 0.25 ? (int64_t)rounds + 1.0 : rounds) * (blocks + before) + 0.1 * blocks;
+    };
+    const int eight = expand_cols(g, n_tiles, 8, block), four = expand_cols(g, n_tiles, 4, block);
+    return cost(four) < cost(eight) ? four : eight;
+}
 template <typename K>
 static int launch_expand_kernel(K kernel, std::atomic<uint64_t>& allowed, AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, int lds, hipStream_t stream) {
     if (int rc = allow_big_lds(kernel, (160 << 10) - 1024, allowed)) return rc;
@@ -1004,7 +1017,7 @@ static int launch_expand_direct(const AdapterArgs& g, const AdapterTile* tiles, 
 template <int DT, int MOST, int CB, bool WHOLE, bool ODD, bool TURNED>
 static int launch_expand_tall2(AdapterArgs g, const AdapterTile* tiles, int64_t n_tiles, hipStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
-    g.cols = expand_cols(g, n_tiles, 8, CB);
+    g.cols = expand_tall_cols(g, n_tiles, CB);
     const int lds = 64 * expand_pitch<DT>(g.rp) * 2 + std::max(DT == F8MI_FP16 ? 64 * expand_half(g.rp) * 4 : 0, 2 * 2 * (TURNED ? expand_half(g.rp) * (CB + 32) : CB * (expand_half(g.rp) + 8)));
     return launch_expand_kernel(adapter_expand_tall_kernel<DT, MOST, CB, WHOLE, ODD, TURNED>, allowed, g, tiles, n_tiles, lds, stream);
 }
