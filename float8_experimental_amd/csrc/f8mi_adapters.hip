@@ -739,7 +739,7 @@ __global__ __launch_bounds__(OUTER_THREADS) void adapter_outer_kernel(const Oute
 // The same for 16-bit types on their matrix instructions.  Both operands are wanted eight rows a lane and lie in LDS by rows: the reads turn them (ds_read_b64_tr_b16: of 4 rows x 16 columns
 // each of 16 lanes gets a column).  small goes in as two bf16 values, high and low; fp16 values of big too, exactly, so that neither overflows or falls among the subnormals: bf16 has the
 // exponents of fp32.  A row of 128 columns is 256 bytes; a pitch of 288 and rows 8 .. 15 of 16 turned by half a row let the 32 lanes that read at a time reach all banks.
-// Measured: 8192 rows of 4096 bf16 columns, rank 16, 23 us out of HBM and 16 of what the memory-side cache has; with fp32 matrix instructions, which fp32 takes, 39.
+// Measured: 8192 rows of 4096 bf16 columns, rank 16, 22 us out of HBM and 15.5 of what the memory-side cache has; with fp32 matrix instructions, which fp32 takes, 39.
 // COLS_FIRST: sums [cols][r], so that a lane has four neighbours of the rank, else of the columns.
 constexpr int OUTER_STEP = 64, OUTER_PITCH = 288;
 __device__ __forceinline__ int outer_at(int row, int byte) { return row * OUTER_PITCH + (byte ^ ((row >> 3 & 1) * 128)); }
@@ -757,7 +757,7 @@ template <int DT, int RT, bool COLS_FIRST>
 __global__ __launch_bounds__(OUTER_THREADS) void adapter_outer16_kernel(const OuterArgs g, const AdapterTile* __restrict__ chunks, int col_blocks) {
     constexpr int PARTS = DT == F8MI_FP16 ? 2 : 1;  // of big
     __shared__ __align__(16) uint8_t big[PARTS][OUTER_STEP * OUTER_PITCH], small[RT == 4 ? OUTER_STEP * OUTER_PITCH : OUTER_STEP * 64 * RT];
-    // of a row of small the high parts (0) or the low ones: of up to 32 of the rank apart and without gaps, so that five workgroups fit a CU (of 8192 rows of 4096 columns all run at once: 22.2 -> 21.4 us; fp16 four instead of two)
+    // of a row of small the high parts (0) or the low ones: of up to 32 of the rank apart and without gaps, so that five workgroups fit a CU (of 8192 rows of 4096 columns all run at once: 21.4 us, of a pitch as big's has 22.2; fp16 four instead of two)
     auto small_at = [](int row, int part, int byte) __attribute__((always_inline)) {
         if constexpr (RT == 4) return outer_at(row, part * 128 + byte);
         return part * OUTER_STEP * 32 * RT + ((row * 32 * RT + byte) ^ ((row >> 3 & 1) * (RT == 1 ? 128 : 32)));
