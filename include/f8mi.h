@@ -551,7 +551,7 @@ int f8mi_dropout(const void* x, const void* residual, int64_t n, int dtype, doub
  * scale [count] fp32 or NULL (1); y [m][n] of x's dtype or NULL (0); out dense.
  * table: what f8mi_adapter_rows made of the rows' adapters (int32 or int64 ids; a number that is no adapter's means none) for this m and count:
  * f8mi_adapter_rows_words() 32-bit words, 16-byte aligned.  h: [m][r rounded up to 16] fp32 for the backward pass, or NULL.  workspace: 16-byte
- * aligned, contents arbitrary.  out overlaps no input (its last columns may be computed twice).  Sums are fp32, in a fixed order. */
+ * aligned, contents arbitrary (NULL where f8mi_adapters_workspace_bytes is 0: few rows in one launch).  out overlaps no input (its last columns may be computed twice).  Sums are fp32, in a fixed order. */
 #define F8MI_ADAPTER_MAX_ROWS (1 << 24)
 #define F8MI_ADAPTER_MAX_COUNT 32768
 #define F8MI_ADAPTER_MAX_RANK 256
