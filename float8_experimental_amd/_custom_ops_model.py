@@ -5,7 +5,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native
-from ._custom_ops_norm_blockwise import _data_shape, _records, _scales_shape, _untraced
+from ._custom_ops_norm_blockwise import _HP_DTYPES, _check_operands, _data_shape, _records, _scales_shape, _untraced
 
 _e4m3 = torch.float8_e4m3fn
 
@@ -28,6 +28,7 @@ _traced.define("low_rank_adapters(Tensor x2, Tensor a, Tensor b, Tensor table, T
 @torch.library.custom_op("f8mi::rms_norm_fwd", mutates_args=())
 def rms_norm_fwd(x2: torch.Tensor, weight: Optional[torch.Tensor], residual2: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, x + residual (empty without one), rstd of each row)"""
+    _check_operands("rms_norm", x2, ("weight", weight, x2.shape[1:], (x2.dtype, torch.float32)), ("residual", residual2, x2.shape, (x2.dtype,)))
     y, total, rstd = _native.rms_norm(x2, weight, residual2, eps)
     return y, _empty(x2, 0) if total is None else total, rstd
 
@@ -41,7 +42,9 @@ def _(x2, weight, residual2, eps):
 def rms_norm_bwd(dy2: torch.Tensor, s2: torch.Tensor, ds2: Optional[torch.Tensor], weight: Optional[torch.Tensor], rstd: torch.Tensor, need_dx: bool, need_dw: bool) -> Tuple[
         torch.Tensor, torch.Tensor]:
     """(dx, dweight); an unneeded gradient is empty."""
-    dx, dw = _native.rms_norm_backward(dy2, s2, ds2, weight, rstd, need_dx, need_dw)
+    _check_operands("rms_norm, backward", s2, ("the gradient", dy2, s2.shape, (s2.dtype,)), ("the sum's gradient", ds2, s2.shape, (s2.dtype,)),
+                    ("weight", weight, s2.shape[1:], (s2.dtype, torch.float32)), ("rstd", rstd, s2.shape[:1], (torch.float32,)))
+    dx, dw = _native.rms_norm_backward(dy2, s2, ds2, weight, rstd.contiguous(), need_dx, need_dw)
     return _empty(s2, 0) if dx is None else dx, _empty(s2, 0, s2.dtype if weight is None else weight.dtype) if dw is None else dw
 
 
@@ -100,6 +103,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional
 @torch.library.custom_op("f8mi::rms_norm_blockwise", mutates_args=())
 def rms_norm_blockwise(x2: torch.Tensor, weight: Optional[torch.Tensor], residual2: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(data, scales, x + residual (empty without one))"""
+    _check_operands("rms_norm_blockwise", x2, ("weight", weight, x2.shape[1:], (x2.dtype, torch.float32)), ("residual", residual2, x2.shape, (x2.dtype,)))
     out, total = _native.rms_norm_block(x2, weight, residual2, eps)
     return out.data, out.scales, _empty(x2, 0) if total is None else total
 
@@ -134,6 +138,9 @@ def _(x_data, x_scales, data, scales, k, dtype, bias):
 @torch.library.custom_op("f8mi::dropout_masked", mutates_args=())
 def dropout_masked(x: torch.Tensor, residual: Optional[torch.Tensor], seed: torch.Tensor, p: float) -> torch.Tensor:
     """residual + x / (1 - p) where kept"""
+    if seed.dtype is not torch.int64 or seed.numel() != 1 or seed.device != x.device or (residual is not None and (residual.shape, residual.dtype, residual.device) != (x.shape, x.dtype, x.device)):
+        raise _native.Float8NativeError(f"dropout: a seed {tuple(seed.shape)} ({seed.dtype}) on {seed.device}" + (
+            "" if residual is None else f" and a residual {tuple(residual.shape)} ({residual.dtype}) on {residual.device}") + f" for x {tuple(x.shape)} ({x.dtype}) on {x.device}")
     return _native.dropout(x, residual, seed, p)
 
 
@@ -175,6 +182,8 @@ def dropout(x: torch.Tensor, residual: Optional[torch.Tensor], seed: torch.Tenso
 
 @torch.library.custom_op("f8mi::adapter_rows", mutates_args=())
 def adapter_rows(ids: torch.Tensor, count: int) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise _native.Float8NativeError(f"adapter_rows: ids of {ids.dtype}; int64 or int32 is needed")
     return _native.adapter_rows(ids, count)
 
 
@@ -193,11 +202,18 @@ def adapter_rows_words(m: int, count: int) -> int:
     return up4(groups) + up4(groups + 1) + up4(m) + 4 * tiles
 
 
+def _check_adapters(what: str, rows2: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, scale: Optional[torch.Tensor], *operands) -> None:
+    if a.dim() != 3 or b.dim() != 3 or a.dtype not in _HP_DTYPES or a.dtype is not b.dtype or a.device != rows2.device or b.device != rows2.device or (a.shape[0], a.shape[1]) != (b.shape[0], b.shape[2]):
+        raise _native.Float8NativeError(f"{what}: a {tuple(a.shape)} ({a.dtype}) on {a.device} and b {tuple(b.shape)} ({b.dtype}) on {b.device} for rows on {rows2.device}")
+    _check_operands(what, rows2, ("a batch's table", table, (adapter_rows_words(rows2.shape[0], a.shape[0]),), (torch.int32,)), ("scale", scale, a.shape[:1], (torch.float32,)), *operands)
+
+
 @torch.library.custom_op("f8mi::adapters_fwd", mutates_args=())
 def adapters_fwd(x2: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, y2: Optional[torch.Tensor], scale: Optional[torch.Tensor], factor: float, need_h: bool) -> Tuple[
         torch.Tensor, torch.Tensor]:
     """(out, h (empty unless needed))"""
-    out, h = _native.adapters(x2, a, b, table, y2, scale, factor, need_h)
+    _check_adapters("low_rank_adapters", x2, a, b, table, scale, ("x", x2, (x2.shape[0], a.shape[-1]), (x2.dtype,)), ("y", y2, (x2.shape[0], b.shape[1]), (x2.dtype,)))
+    out, h = _native.adapters(x2, a, b, table.contiguous(), y2, None if scale is None else scale.contiguous(), factor, need_h)
     return out, _empty(x2, 0, torch.float32) if h is None else h
 
 
@@ -212,7 +228,10 @@ def adapters_bwd(dout2: torch.Tensor, x2: Optional[torch.Tensor], a: torch.Tenso
     """(dx, da, db); an unneeded gradient is empty."""
     if dout2.shape[0] == 0:
         return _empty(dout2, (0, a.shape[2]) if need_dx else 0), torch.zeros_like(a) if need_da else _empty(a, 0), torch.zeros_like(b) if need_db else _empty(b, 0)
-    grads = _native.adapters_backward(dout2, x2, a, b, table, scale, factor, h, need_dx, need_da, need_db)
+    m, rank = dout2.shape[0], a.shape[1]
+    _check_adapters("low_rank_adapters, backward", dout2, a, b, table, scale, ("the gradient", dout2, (m, b.shape[1]), (dout2.dtype,)),
+                    ("x", x2 if need_da else None, (m, a.shape[-1]), (dout2.dtype,)), ("h", h if need_db else None, (m, (rank + 15) // 16 * 16), (torch.float32,)))
+    grads = _native.adapters_backward(dout2, x2, a, b, table.contiguous(), None if scale is None else scale.contiguous(), factor, h.contiguous(), need_dx, need_da, need_db)
     return tuple(_empty(t, 0) if g is None else g for g, t in zip(grads, (dout2, a, b)))
 
 

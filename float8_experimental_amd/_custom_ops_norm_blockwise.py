@@ -9,6 +9,7 @@ from . import _native
 
 _e4m3 = torch.float8_e4m3fn
 _KB, _BLOCK = _native.KB, _native.BLOCK
+_HP_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _data_shape(rows: int, k: int):
@@ -109,6 +110,16 @@ def _untraced():
         yield
     finally:
         torch._C._set_tracing_state(state)
+
+
+def _check_operands(what: str, x2: torch.Tensor, *operands) -> None:
+    """Each operand (name, tensor or None, shape, types) is what the kernels read beside the matrix x2.  The entry points have checked their arguments, but not those that a trace is
+    replayed with or that hooks on saved tensors hand back: without this their memory would be read past its end."""
+    if x2.dim() != 2 or x2.dtype not in _HP_DTYPES:
+        raise _native.Float8NativeError(f"{what}: {tuple(x2.shape)} ({x2.dtype}) is no matrix of bfloat16, float16 or float32")
+    for name, t, shape, dtypes in operands:
+        if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.device != x2.device):
+            raise _native.Float8NativeError(f"{what}: {name} {tuple(t.shape)} ({t.dtype}) on {t.device} beside {tuple(x2.shape)} ({x2.dtype}) on {x2.device}; {tuple(shape)} is needed")
 
 
 def _records(*tensors: Optional[torch.Tensor]) -> bool:
