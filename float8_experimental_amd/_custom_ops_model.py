@@ -19,7 +19,7 @@ _traced = torch.library.Library("f8mi", "FRAGMENT")
 _traced.define("rms_norm(Tensor x2, Tensor? weight, float eps) -> Tensor")
 _traced.define("rms_norm_add(Tensor x2, Tensor? weight, Tensor residual2, float eps) -> (Tensor, Tensor)")
 _traced.define("dropout(Tensor x, Tensor? residual, Tensor seed, float p) -> Tensor")
-_traced.define("low_rank_adapters(Tensor x2, Tensor a, Tensor b, Tensor table, Tensor? y2, Tensor? scale, float factor) -> Tensor")
+_traced.define("low_rank_adapters(Tensor x2, Tensor a, Tensor b, Tensor table, Tensor rows, int count, Tensor? y2, Tensor? scale, float factor) -> Tensor")
 
 
 # ---- RMS norm
@@ -202,48 +202,53 @@ def adapter_rows_words(m: int, count: int) -> int:
     return up4(groups) + up4(groups + 1) + up4(m) + 4 * tiles
 
 
-def _check_adapters(what: str, rows2: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, scale: Optional[torch.Tensor], *operands) -> None:
+def _check_adapters(what: str, rows2: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, rows: Optional[int], count: Optional[int], scale: Optional[torch.Tensor],
+                    *operands) -> None:
+    """``rows`` and ``count``: what the table was made for.  Its length alone does not say so (tables of 5 and of 8 rows are equally long), and the rows that it lists are read and written."""
     if a.dim() != 3 or b.dim() != 3 or a.dtype not in _HP_DTYPES or a.dtype is not b.dtype or a.device != rows2.device or b.device != rows2.device or (a.shape[0], a.shape[1]) != (b.shape[0], b.shape[2]):
         raise _native.Float8NativeError(f"{what}: a {tuple(a.shape)} ({a.dtype}) on {a.device} and b {tuple(b.shape)} ({b.dtype}) on {b.device} for rows on {rows2.device}")
+    if (rows2.shape[0] if rows is None else rows, a.shape[0] if count is None else count) != (rows2.shape[0], a.shape[0]):
+        raise _native.Float8NativeError(f"{what}: a table of {rows} rows and {count} adapters for {rows2.shape[0]} rows and {a.shape[0]} adapters")
     _check_operands(what, rows2, ("a batch's table", table, (adapter_rows_words(rows2.shape[0], a.shape[0]),), (torch.int32,)), ("scale", scale, a.shape[:1], (torch.float32,)), *operands)
 
 
 @torch.library.custom_op("f8mi::adapters_fwd", mutates_args=())
-def adapters_fwd(x2: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, y2: Optional[torch.Tensor], scale: Optional[torch.Tensor], factor: float, need_h: bool) -> Tuple[
-        torch.Tensor, torch.Tensor]:
-    """(out, h (empty unless needed))"""
-    _check_adapters("low_rank_adapters", x2, a, b, table, scale, ("x", x2, (x2.shape[0], a.shape[-1]), (x2.dtype,)), ("y", y2, (x2.shape[0], b.shape[1]), (x2.dtype,)))
+def adapters_fwd(x2: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, y2: Optional[torch.Tensor], scale: Optional[torch.Tensor], factor: float, need_h: bool,
+                 rows: Optional[int] = None, count: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out, h (empty unless needed)); ``rows`` and ``count``: of the table"""
+    _check_adapters("low_rank_adapters", x2, a, b, table, rows, count, scale, ("x", x2, (x2.shape[0], a.shape[-1]), (x2.dtype,)), ("y", y2, (x2.shape[0], b.shape[1]), (x2.dtype,)))
     out, h = _native.adapters(x2, a, b, table.contiguous(), y2, None if scale is None else scale.contiguous(), factor, need_h)
     return out, _empty(x2, 0, torch.float32) if h is None else h
 
 
 @adapters_fwd.register_fake
-def _(x2, a, b, table, y2, scale, factor, need_h):
+def _(x2, a, b, table, y2, scale, factor, need_h, rows=None, count=None):
     return _empty(x2, (x2.shape[0], b.shape[1])), _empty(x2, (x2.shape[0], (a.shape[1] + 15) // 16 * 16) if need_h else 0, torch.float32)
 
 
 @torch.library.custom_op("f8mi::adapters_bwd", mutates_args=())
 def adapters_bwd(dout2: torch.Tensor, x2: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, scale: Optional[torch.Tensor], factor: float, h: torch.Tensor, need_dx: bool,
-                 need_da: bool, need_db: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                 need_da: bool, need_db: bool, rows: Optional[int] = None, count: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, da, db); an unneeded gradient is empty."""
     if dout2.shape[0] == 0:
         return _empty(dout2, (0, a.shape[2]) if need_dx else 0), torch.zeros_like(a) if need_da else _empty(a, 0), torch.zeros_like(b) if need_db else _empty(b, 0)
     m, rank = dout2.shape[0], a.shape[1]
-    _check_adapters("low_rank_adapters, backward", dout2, a, b, table, scale, ("the gradient", dout2, (m, b.shape[1]), (dout2.dtype,)),
+    _check_adapters("low_rank_adapters, backward", dout2, a, b, table, rows, count, scale, ("the gradient", dout2, (m, b.shape[1]), (dout2.dtype,)),
                     ("x", x2 if need_da else None, (m, a.shape[-1]), (dout2.dtype,)), ("h", h if need_db else None, (m, (rank + 15) // 16 * 16), (torch.float32,)))
     grads = _native.adapters_backward(dout2, x2, a, b, table.contiguous(), None if scale is None else scale.contiguous(), factor, h.contiguous(), need_dx, need_da, need_db)
     return tuple(_empty(t, 0) if g is None else g for g, t in zip(grads, (dout2, a, b)))
 
 
 @adapters_bwd.register_fake
-def _(dout2, x2, a, b, table, scale, factor, h, need_dx, need_da, need_db):
+def _(dout2, x2, a, b, table, scale, factor, h, need_dx, need_da, need_db, rows=None, count=None):
     return _empty(dout2, (dout2.shape[0], a.shape[2]) if need_dx else 0), _empty(a, a.shape if need_da else 0), _empty(b, b.shape if need_db else 0)
 
 
 class _AdaptersFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x2, a, b, table, y2, scale, factor):
-        out, h = adapters_fwd(x2, a, b, table, y2, scale, factor, ctx.needs_input_grad[2])
+    def forward(ctx, x2, a, b, table, rows, count, y2, scale, factor):
+        out, h = adapters_fwd(x2, a, b, table, y2, scale, factor, ctx.needs_input_grad[2], rows, count)
+        ctx.rows, ctx.count = rows, count
         ctx.factor, ctx.has_scale, ctx.has_x = factor, scale is not None, ctx.needs_input_grad[1]
         ctx.save_for_backward(a, b, table, h, *([x2] if ctx.has_x else []), *([scale] if ctx.has_scale else []))
         return out
@@ -253,21 +258,27 @@ class _AdaptersFn(torch.autograd.Function):
         a, b, table, h, *rest = ctx.saved_tensors
         x2, scale = rest[0] if ctx.has_x else None, rest[-1] if ctx.has_scale else None
         needs = ctx.needs_input_grad[:3]
-        grads = adapters_bwd(g, x2, a, b, table, scale, ctx.factor, h, *needs) if any(needs) else (None,) * 3
-        return tuple(d if need else None for d, need in zip(grads, needs)) + (None, g if ctx.needs_input_grad[4] else None, None, None)
+        grads = adapters_bwd(g, x2, a, b, table, scale, ctx.factor, h, *needs, ctx.rows, ctx.count) if any(needs) else (None,) * 3
+        return tuple(d if need else None for d, need in zip(grads, needs)) + (None, None, None, g if ctx.needs_input_grad[6] else None, None, None)
 
 
-def _low_rank_adapters(x2, a, b, table, y2, scale, factor):
-    return _AdaptersFn.apply(x2, a, b, table, y2, scale, factor) if _records(x2, a, b, y2) else adapters_fwd(x2, a, b, table, y2, scale, factor, False)[0]
+def _low_rank_adapters(x2, a, b, table, rows, count, y2, scale, factor):
+    if _records(x2, a, b, y2):
+        return _AdaptersFn.apply(x2, a, b, table, rows, count, y2, scale, factor)
+    return adapters_fwd(x2, a, b, table, y2, scale, factor, False, rows, count)[0]
 
 
 @torch.library.impl(_traced, "low_rank_adapters", "CompositeImplicitAutograd")
-def _traced_low_rank_adapters(x2, a, b, table, y2, scale, factor):
+def _traced_low_rank_adapters(x2, a, b, table, rows, count, y2, scale, factor):
     with _untraced():
-        out = _native.model_ops().low_rank_adapters(x2, a, b, table, x2.shape[0], a.shape[0], y2, scale, factor)
-        return _low_rank_adapters(x2, a, b, table, y2, scale, factor) if out is None else out
+        rows = int(rows)
+        out = _native.model_ops().low_rank_adapters(x2, a, b, table, rows, count, y2, scale, factor)
+        return _low_rank_adapters(x2, a, b, table, rows, count, y2, scale, factor) if out is None else out
 
 
-def low_rank_adapters(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, y: Optional[torch.Tensor], scale: Optional[torch.Tensor], factor: float) -> torch.Tensor:
-    call = torch.ops.f8mi.low_rank_adapters if torch.jit.is_tracing() else _low_rank_adapters
-    return call(x.reshape(-1, x.shape[-1]), a, b, table, None if y is None else y.reshape(-1, y.shape[-1]), scale, factor).reshape(*x.shape[:-1], b.shape[1])
+def low_rank_adapters(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Tensor, rows: int, count: int, y: Optional[torch.Tensor], scale: Optional[torch.Tensor], factor: float) -> torch.Tensor:
+    """``rows``, ``count``: of the table.  A trace has the rows as a number on the host: a constant where the table is one, else the rows of the numbers that the table is made of in the trace."""
+    call = _low_rank_adapters
+    if torch.jit.is_tracing():
+        call, rows = torch.ops.f8mi.low_rank_adapters, torch.as_tensor(rows, device="cpu")
+    return call(x.reshape(-1, x.shape[-1]), a, b, table, rows, count, None if y is None else y.reshape(-1, y.shape[-1]), scale, factor).reshape(*x.shape[:-1], b.shape[1])

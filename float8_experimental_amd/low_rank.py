@@ -96,7 +96,7 @@ def low_rank_adapters(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter
         out = _native.model_ops().low_rank_adapters(x, a, b, adapters.table, adapters.rows, adapters.count, y, per_adapter, factor)  # with adapters and a scale of types that it takes
         if out is not None:
             return out
-    return _compiled.low_rank_adapters(x, a, b, adapters.table, y, per_adapter, float(factor))
+    return _compiled.low_rank_adapters(x, a, b, adapters.table, adapters.rows, adapters.count, y, per_adapter, float(factor))
 
 
 class AdaptedLinear(nn.Module):

@@ -2,7 +2,9 @@
 for, and none is reached."""
 import pytest
 import torch
+import torch.fx.experimental.proxy_tensor
 
+import float8_experimental_amd as f8
 from float8_experimental_amd import _custom_ops_model as ops
 from float8_experimental_amd import _native
 
@@ -91,3 +93,60 @@ def test_adapters_of_other_rows_beside_them(reached):
 def test_rows_of_numbers_that_are_not_whole(reached):
     for ids in (z(5, dtype=FP32), torch.zeros(5, dtype=torch.int16)):
         refused(reached, lambda: ops.adapter_rows(ids, 3), "ids")
+
+
+# ---- the rows that a table was made for
+
+
+@pytest.mark.parametrize("rows, count", [(8, 3), (6, 3), (5, 2), (5, 4), (0, 0)])
+def test_a_table_that_is_as_long_but_of_other_rows(reached, rows, count):
+    assert ops.adapter_rows_words(8, 3) == ops.adapter_rows_words(6, 3) == ops.adapter_rows_words(5, 3)
+    t = operands()
+    refused(reached, lambda: ops.adapters_fwd(t["x"], t["a"], t["b"], t["table"], t["y"], None, 1.0, True, rows, count), f"table of {rows} rows and {count} adapters")
+    refused(reached, lambda: ops.adapters_bwd(t["g"], t["x"], t["a"], t["b"], t["table"], None, 1.0, t["h"], True, True, True, rows, count), f"table of {rows} rows and {count} adapters")
+
+
+@pytest.fixture
+def stand_ins(monkeypatch):
+    """The adapters' kernels, on the CPU: (rows of x, rows of the ids that the table was made of) of each call."""
+    seen = []
+
+    def adapters(x, a, b, table, y, scale, factor, need_h):
+        seen.append((len(x), int(table[0])))
+        return torch.zeros(len(x), b.shape[1], dtype=x.dtype), torch.zeros(len(x), 16) if need_h else None
+
+    def adapter_rows(ids, count):
+        table = torch.zeros(ops.adapter_rows_words(ids.numel(), count), dtype=torch.int32)
+        table[0] = ids.numel()
+        return table
+
+    monkeypatch.setattr(_native, "_require_gpu", lambda t, name: None)
+    monkeypatch.setattr(_native, "adapters", adapters)
+    monkeypatch.setattr(_native, "adapter_rows", adapter_rows)
+    return seen
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traces_with_a_table_from_outside_take_its_rows_alone(stand_ins):
+    a, b, rows = z(2, 4, 8), z(2, 6, 4), f8.AdapterRows(torch.zeros(8, dtype=torch.int64), 2)
+    graphed = torch.fx.experimental.proxy_tensor.make_fx(lambda x, a, b: f8.low_rank_adapters(x, a, b, rows))(z(8, 8), a, b)
+    traced = torch.jit.trace(lambda x, a, b: f8.low_rank_adapters(x, a, b, rows), (z(8, 8), a, b))
+    stand_ins.clear()
+    for call in (graphed, traced):
+        assert call(z(8, 8), a, b).shape == (8, 6)
+        for x, p, q in ((z(5, 8), a, b), (z(9, 8), a, b), (z(8, 8), z(3, 4, 8), z(3, 6, 4)), (z(8, 8), a[:1], b[:1])):
+            with pytest.raises(RuntimeError, match="table of 8 rows and 2 adapters"):
+                call(x, p, q)
+    assert stand_ins == [(8, 8)] * 2
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traces_that_make_the_table_take_any_rows(stand_ins):
+    a, b = z(2, 4, 8), z(2, 6, 4)
+    traced = torch.jit.trace(lambda x, ids: f8.low_rank_adapters(x, a, b, f8.AdapterRows(ids, 2)), (z(5, 8), torch.zeros(5, dtype=torch.int64)))
+    stand_ins.clear()
+    for m in (5, 6, 8, 70, 1):
+        assert traced(z(m, 8), torch.zeros(m, dtype=torch.int64)).shape == (m, 6)
+    assert stand_ins == [(m, m) for m in (5, 6, 8, 70, 1)]
+    with pytest.raises(RuntimeError, match="table of 8 rows"):
+        traced(z(5, 8), torch.zeros(8, dtype=torch.int64))
