@@ -24,6 +24,16 @@ def _one_weight_copy(k: int, n: int) -> bool:
     return k % _BLOCK == 0 and n % _BLOCK == 0
 
 
+def _check_operands(what: str, x2: torch.Tensor, *operands) -> None:
+    """Each operand (name, tensor or None, shape, types) is what the kernels read beside the matrix x2.  The entry points have checked their arguments, but not those that a trace is
+    replayed with or that hooks on saved tensors hand back: without this their memory would be read past its end."""
+    if x2.dim() != 2 or x2.dtype not in _HP_DTYPES:
+        raise _native.Float8NativeError(f"{what}: {tuple(x2.shape)} ({x2.dtype}) is no matrix of bfloat16, float16 or float32")
+    for name, t, shape, dtypes in operands:
+        if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.device != x2.device):
+            raise _native.Float8NativeError(f"{what}: {name} {tuple(t.shape)} ({t.dtype}) on {t.device} beside {tuple(x2.shape)} ({x2.dtype}) on {x2.device}; {tuple(shape)} is needed")
+
+
 @torch.library.custom_op("f8mi::blockwise_linear_fwd", mutates_args=())
 def blockwise_linear_fwd(x2: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], need_dx: bool, need_dw: bool) -> Tuple[
         torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -62,6 +72,10 @@ def blockwise_linear_bwd(dy2: torch.Tensor, xt: torch.Tensor, xt_scales: torch.T
     if m == 0:
         return (dy2.new_empty((0, k)) if need_dx else empty(dy2.dtype), dy2.new_zeros((n, k), dtype=w_dtype) if need_dw else empty(w_dtype),
                 dy2.new_zeros(n, dtype=b_dtype) if b_dtype is not None else empty(dy2.dtype))
+    w_shape = _data_shape(n, k) if _one_weight_copy(k, n) else _data_shape(k, n)
+    _check_operands("blockwise_linear, backward", dy2, ("x", xt if need_dw else None, _data_shape(k, m), (_e4m3,)), ("x's scales", xt_scales if need_dw else None, _scales_shape(k, m), (torch.uint8,)),
+                    ("weight", w if need_dx else None, w_shape, (_e4m3,)), ("the weight's scales", w_scales if need_dx else None, _scales_shape(k, n), (torch.uint8,)))
+    xt, xt_scales, w, w_scales = (t.contiguous() for t in (xt, xt_scales, w, w_scales))
     with _native.transient_workspaces():
         ((g8, g8t, *db),) = _native.block_cast([(dy2, False, need_dx, need_dw, *([b_dtype] if b_dtype is not None else []))])
         dx, dw = empty(dy2.dtype), empty(w_dtype)
@@ -110,16 +124,6 @@ def _untraced():
         yield
     finally:
         torch._C._set_tracing_state(state)
-
-
-def _check_operands(what: str, x2: torch.Tensor, *operands) -> None:
-    """Each operand (name, tensor or None, shape, types) is what the kernels read beside the matrix x2.  The entry points have checked their arguments, but not those that a trace is
-    replayed with or that hooks on saved tensors hand back: without this their memory would be read past its end."""
-    if x2.dim() != 2 or x2.dtype not in _HP_DTYPES:
-        raise _native.Float8NativeError(f"{what}: {tuple(x2.shape)} ({x2.dtype}) is no matrix of bfloat16, float16 or float32")
-    for name, t, shape, dtypes in operands:
-        if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.device != x2.device):
-            raise _native.Float8NativeError(f"{what}: {name} {tuple(t.shape)} ({t.dtype}) on {t.device} beside {tuple(x2.shape)} ({x2.dtype}) on {x2.device}; {tuple(shape)} is needed")
 
 
 def _records(*tensors: Optional[torch.Tensor]) -> bool:
@@ -175,6 +179,8 @@ def blockwise_inference_linear(x: torch.Tensor, data: torch.Tensor, scales: torc
 @torch.library.custom_op("f8mi::layer_norm_fwd", mutates_args=())
 def layer_norm_fwd(x2: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
     """(y, (mean, rstd) of each row)"""
+    p_dtypes = (x2.dtype, torch.float32) if weight is None or bias is None else (weight.dtype,) if weight.dtype in (x2.dtype, torch.float32) else ()
+    _check_operands("layer_norm", x2, ("weight", weight, x2.shape[1:], p_dtypes), ("bias", bias, x2.shape[1:], p_dtypes))
     return _native.layer_norm(x2, weight, bias, eps)
 
 
@@ -187,6 +193,8 @@ def _(x2, weight, bias, eps):
 def layer_norm_bwd(dy2: torch.Tensor, x2: torch.Tensor, weight: Optional[torch.Tensor], p_dtype: torch.dtype, stats: torch.Tensor, need_dx: bool, need_dw: bool,
                    need_db: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dweight, dbias); an unneeded gradient is empty."""
+    _check_operands("layer_norm, backward", x2, ("the gradient", dy2, x2.shape, (x2.dtype,)), ("weight", weight, x2.shape[1:], (p_dtype,)), ("statistics", stats, (x2.shape[0], 2), (torch.float32,)))
+    stats = stats.contiguous()
     grads = _native.layer_norm_backward(dy2, x2, weight, p_dtype, stats, need_dx, need_dw, need_db)
     return tuple(torch.empty(0, dtype=dt, device=x2.device) if g is None else g for g, dt in zip(grads, (x2.dtype, p_dtype, p_dtype)))
 
