@@ -284,8 +284,9 @@ PyObject* rms_norm_blockwise(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!expect(n_args, 5, "rms_norm_blockwise")) return nullptr;
     return guarded([&]() -> PyObject* {
         RmsCall c;
-        if (!c.taken(a) || c.cols != c.x.size(-1) || wants_grad(c.x) || wants_grad(c.weight) || wants_grad(c.residual)) Py_RETURN_NONE;
+        if (!c.taken(a)) Py_RETURN_NONE;
         if (c.eps == -1.0 && PyErr_Occurred()) return nullptr;
+        if (c.cols != c.x.size(-1) || wants_grad(c.x) || wants_grad(c.weight) || wants_grad(c.residual)) Py_RETURN_NONE;
         at::Tensor data, scales, sum;
         {
             const WithoutGil no_gil;
