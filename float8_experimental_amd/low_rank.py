@@ -104,7 +104,9 @@ class AdaptedLinear(nn.Module):
 
     ``linear`` (its parameters no longer ask for gradients), ``adapter_a`` [count, rank, in_features] as ``nn.Linear`` initialises a weight and ``adapter_b`` [count,
     out_features, rank] of zeros, in ``dtype`` (None: that of the linear's weight, bfloat16 where that is float8).  ``alpha / rank`` (alpha None: rank) scales
-    what they add, ``dropout`` of their input is dropped in training.  ``rows`` says which adapter each row of the batch has (``select_adapters``); None: no row has one."""
+    what they add, ``dropout`` of their input is dropped in training.  ``rows`` says which adapter each row of the batch has (``select_adapters``); None: no row has one.
+
+    It is called as a linear is, and has no ``weight`` and no ``bias``: who multiplied by those would leave the adapters out."""
 
     def __init__(self, linear: nn.Module, count: int, rank: int, alpha: Optional[float] = None, dropout: float = 0.0, dtype: Optional[torch.dtype] = None):
         super().__init__()
@@ -143,31 +145,49 @@ class AdaptedLinear(nn.Module):
         return f"count={self.count}, rank={self.rank}, scaling={self.scaling}, dropout={self.dropout}"
 
 
+# Linears whose module reads their weight, always or in evaluation, instead of calling them: what stands around them there is not asked
+_READ_BY_THEIR_MODULE = ((nn.MultiheadAttention, ("out_proj",)), (nn.TransformerEncoderLayer, ("linear1", "linear2")))
+
+
 def adapt_linears(module: nn.Module, count: int, rank: int, *, alpha: Optional[float] = None, dropout: float = 0.0, dtype: Optional[torch.dtype] = None,
                   module_filter_fn: Optional[Callable[[nn.Module, str], bool]] = None) -> nn.Module:
     """Puts an ``AdaptedLinear`` around every linear of ``module`` that passes ``module_filter_fn(linear, fqn)``; no parameter of ``module`` but its adapters asks for
-    gradients any more.  A root-level linear is returned adapted; linears that have adapters already keep those."""
+    gradients any more.  A root-level linear is returned adapted; linears that have adapters already keep those.
+
+    ``nn.MultiheadAttention`` does not call its ``out_proj`` and ``nn.TransformerEncoderLayer`` not always its ``linear1`` and ``linear2``: they take the weights and multiply by themselves.  These
+    linears have no adapters, and a filter that asks for one of them raises."""
+    def wanted(m: nn.Module, fqn: str, parent: Optional[nn.Module] = None, name: str = "") -> bool:
+        if not isinstance(m, (nn.Linear, Float8BlockwiseInferenceLinear)) or not (module_filter_fn is None or module_filter_fn(m, fqn)):
+            return False
+        read = any(isinstance(parent, kind) and name in names for kind, names in _READ_BY_THEIR_MODULE)
+        if read and module_filter_fn is not None:
+            raise ValueError(f"adapt_linears: {type(parent).__name__} reads the weight of {fqn!r} instead of calling it, so that adapters around it would do nothing; module_filter_fn has to leave it out")
+        return not read
+
+    found = []  # (module, name, linear): nothing is changed before all of them are known
+
+    def visit(mod: nn.Module, prefix: str) -> None:
+        for name, child in mod.named_children():
+            fqn = f"{prefix}.{name}" if prefix else name
+            if isinstance(child, AdaptedLinear):
+                continue
+            if wanted(child, fqn, mod, name):
+                found.append((mod, name, child))
+            else:
+                visit(child, fqn)
+
+    root = wanted(module, "")
+    if not root and not isinstance(module, AdaptedLinear):
+        visit(module, "")
     kept = {id(p) for m in module.modules() if isinstance(m, AdaptedLinear) for p in (m.adapter_a, m.adapter_b)}
     for p in module.parameters():
         if id(p) not in kept:
             p.requires_grad_(False)
-    wanted = lambda m, fqn: isinstance(m, (nn.Linear, Float8BlockwiseInferenceLinear)) and (module_filter_fn is None or module_filter_fn(m, fqn))
     around = lambda m: AdaptedLinear(m, count, rank, alpha, dropout, dtype).train(m.training)
-    if wanted(module, ""):
+    if root:
         return around(module)
-
-    def visit(mod: nn.Module, prefix: str) -> None:
-        for name, child in list(mod.named_children()):
-            fqn = f"{prefix}.{name}" if prefix else name
-            if isinstance(child, AdaptedLinear):
-                continue
-            if wanted(child, fqn):
-                setattr(mod, name, around(child))
-            else:
-                visit(child, fqn)
-
-    if not isinstance(module, AdaptedLinear):
-        visit(module, "")
+    for mod, name, linear in found:
+        setattr(mod, name, around(linear))
     return module
 
 

@@ -1,0 +1,54 @@
+"""Adapters and the other swaps in modules that hold their layers in unusual ways.  No GPU needed: without selected rows an adapted linear is its linear, and the layers' forward passes are stood in for."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+
+import float8_experimental_amd as f8
+
+x = torch.randn(2, 5, 16, generator=torch.Generator().manual_seed(0))
+ATTENTION = lambda: nn.MultiheadAttention(16, 2, batch_first=True)
+LAYER = lambda: nn.TransformerEncoderLayer(16, 2, 32, batch_first=True)
+OF_TORCH = {  # module, its arguments, the linears that it always calls
+    "attention": (ATTENTION, (x, x, x), []),
+    "encoder layer": (LAYER, (x,), []),
+    "encoder": (lambda: nn.TransformerEncoder(LAYER(), 2), (x,), []),
+    "decoder layer": (lambda: nn.TransformerDecoderLayer(16, 2, 32, batch_first=True), (x, x), ["linear1", "linear2"]),
+    "both": (lambda: nn.Sequential(LAYER(), nn.Linear(16, 4)), (x,), ["1"]),
+    "adaptive softmax": (lambda: nn.AdaptiveLogSoftmaxWithLoss(16, 30, [5, 10]), (torch.randn(4, 16), torch.tensor([1, 7, 20, 29])), ["head", "tail.0.0", "tail.0.1", "tail.1.0", "tail.1.1"]),
+}
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("training", [False, True])
+@pytest.mark.parametrize("name", list(OF_TORCH))
+def test_modules_that_read_the_weights_of_their_linears(monkeypatch, name, training, grad):
+    make, args, called = OF_TORCH[name]
+    torch.manual_seed(0)
+    plain = make().train(training).requires_grad_(False)  # (as adapting it freezes it: torch chooses its path by that)
+    adapted = f8.adapt_linears(copy.deepcopy(plain), 3, 2)
+    names = {id(m): fqn for fqn, m in adapted.named_modules() if isinstance(m, f8.AdaptedLinear)}
+    assert list(names.values()) == called
+    seen, forward = [], f8.AdaptedLinear.forward
+    monkeypatch.setattr(f8.AdaptedLinear, "forward", lambda self, input: seen.append(names[id(self)]) or forward(self, input))
+    first = lambda out: out[0] if isinstance(out, tuple) else out
+    with torch.set_grad_enabled(grad):
+        torch.manual_seed(1)
+        want = first(plain(*args))
+        torch.manual_seed(1)
+        got = first(adapted(*args))
+    assert torch.equal(got, want) and sorted(seen) == sorted(called)  # none of the adapters is passed by
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("make, fqn", [(ATTENTION, "out_proj"), (LAYER, "linear1"), (LAYER, "linear2"), (LAYER, "self_attn.out_proj"), (lambda: nn.Transformer(16, 2, 1, 1, 32), "encoder.layers.0.linear1")])
+def test_a_filter_that_asks_for_what_is_not_called(make, fqn):
+    model = nn.Sequential(nn.Linear(4, 4), make())
+    for ask in (lambda m, name: True, lambda m, name: name == f"1.{fqn}"):
+        with pytest.raises(ValueError, match="reads the weight"):
+            f8.adapt_linears(model, 3, 2, module_filter_fn=ask)
+        assert type(model[0]) is nn.Linear and all(p.requires_grad for p in model.parameters())  # nothing has been changed
+    f8.adapt_linears(model, 3, 2, module_filter_fn=lambda m, name: name == "0")
+    assert type(model[0]) is f8.AdaptedLinear and sum(isinstance(m, f8.AdaptedLinear) for m in model.modules()) == 1
