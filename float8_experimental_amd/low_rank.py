@@ -152,7 +152,7 @@ _READ_BY_THEIR_MODULE = ((nn.MultiheadAttention, ("out_proj",)), (nn.Transformer
 def adapt_linears(module: nn.Module, count: int, rank: int, *, alpha: Optional[float] = None, dropout: float = 0.0, dtype: Optional[torch.dtype] = None,
                   module_filter_fn: Optional[Callable[[nn.Module, str], bool]] = None) -> nn.Module:
     """Puts an ``AdaptedLinear`` around every linear of ``module`` that passes ``module_filter_fn(linear, fqn)``; no parameter of ``module`` but its adapters asks for
-    gradients any more.  A root-level linear is returned adapted; linears that have adapters already keep those.
+    gradients any more.  A root-level linear is returned adapted; linears that have adapters already keep those, and one that is held under several names or by several modules has one set of them.
 
     ``nn.MultiheadAttention`` does not call its ``out_proj`` and ``nn.TransformerEncoderLayer`` not always its ``linear1`` and ``linear2``: they take the weights and multiply by themselves.  These
     linears have no adapters, and a filter that asks for one of them raises."""
@@ -167,9 +167,9 @@ def adapt_linears(module: nn.Module, count: int, rank: int, *, alpha: Optional[f
     found = []  # (module, name, linear): nothing is changed before all of them are known
 
     def visit(mod: nn.Module, prefix: str) -> None:
-        for name, child in mod.named_children():
+        for name, child in mod._modules.items():  # (named_children() has each module under one of its names)
             fqn = f"{prefix}.{name}" if prefix else name
-            if isinstance(child, AdaptedLinear):
+            if child is None or isinstance(child, AdaptedLinear):
                 continue
             if wanted(child, fqn, mod, name):
                 found.append((mod, name, child))
@@ -186,8 +186,11 @@ def adapt_linears(module: nn.Module, count: int, rank: int, *, alpha: Optional[f
     around = lambda m: AdaptedLinear(m, count, rank, alpha, dropout, dtype).train(m.training)
     if root:
         return around(module)
+    made = {}
     for mod, name, linear in found:
-        setattr(mod, name, around(linear))
+        if linear not in made:
+            made[linear] = around(linear)
+        setattr(mod, name, made[linear])
     return module
 
 

@@ -52,3 +52,38 @@ def test_a_filter_that_asks_for_what_is_not_called(make, fqn):
         assert type(model[0]) is nn.Linear and all(p.requires_grad for p in model.parameters())  # nothing has been changed
     f8.adapt_linears(model, 3, 2, module_filter_fn=lambda m, name: name == "0")
     assert type(model[0]) is f8.AdaptedLinear and sum(isinstance(m, f8.AdaptedLinear) for m in model.modules()) == 1
+
+
+class Held(nn.Module):
+    """One layer of each kind under two names and by two modules, one of them held twice itself."""
+
+    def __init__(self, layer):
+        super().__init__()
+        self.a, self.absent, self.inner = layer, None, nn.Sequential(layer, nn.Sequential(layer))
+        self.b, self.again = layer, self.inner
+
+    def forward(self, x):
+        return self.b(self.again(self.inner(self.a(x))))
+
+    def layers(self):
+        return [self.a, self.b, self.inner[0], self.inner[1][0], self.again[0]]
+
+
+def test_a_linear_under_several_names_has_one_set_of_adapters():
+    linear = nn.Linear(16, 16)
+    model = f8.adapt_linears(Held(linear), 3, 2)
+    first, *others = model.layers()
+    assert type(first) is f8.AdaptedLinear and first.linear is linear and all(m is first for m in others)
+    assert len([p for p in model.parameters() if p.requires_grad]) == 2 and model(x).shape == x.shape
+    again = f8.adapt_linears(model, 3, 4)
+    assert again is model and all(m is first for m in model.layers()) and first.linear is linear
+    two = nn.Sequential(nn.Linear(4, 4), nn.Linear(4, 4))
+    two[1].weight = two[0].weight  # a shared weight is not a shared linear
+    f8.adapt_linears(two, 3, 2)
+    assert two[0] is not two[1] and two[0].linear.weight is two[1].linear.weight and two[0].adapter_a is not two[1].adapter_a
+
+
+def test_names_that_the_filter_leaves_out_stay_as_they_are():
+    linear = nn.Linear(16, 16)
+    model = f8.adapt_linears(Held(linear), 3, 2, module_filter_fn=lambda m, fqn: fqn in ("b", "inner.1.0"))
+    assert model.a is linear and model.inner[0] is linear and type(model.b) is f8.AdaptedLinear and model.inner[1][0] is model.b
