@@ -9,6 +9,7 @@ from . import _custom_ops_model as _compiled_model
 from . import _custom_ops_norm_blockwise as _compiled
 from . import _native
 from .float8_blockwise import BlockwiseActivations
+from .module_swap import swap_modules
 
 _HP_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -65,14 +66,7 @@ class LayerNorm(nn.LayerNorm):
 
 def convert_layer_norms(module: nn.Module) -> nn.Module:
     """Swaps every ``nn.LayerNorm`` of ``module`` for a ``LayerNorm`` that shares its parameters; a root-level one is returned converted."""
-    if type(module) is nn.LayerNorm:
-        return LayerNorm.from_float(module)
-    for name, child in module.named_children():
-        if type(child) is nn.LayerNorm:
-            setattr(module, name, LayerNorm.from_float(child))
-        else:
-            convert_layer_norms(child)
-    return module
+    return swap_modules(module, nn.LayerNorm, LayerNorm.from_float)
 
 
 def _rms_arguments(what: str, x, normalized_shape, weight, eps, residual):
@@ -161,11 +155,4 @@ class RMSNorm(nn.RMSNorm):
 
 def convert_rms_norms(module: nn.Module) -> nn.Module:
     """Swaps every ``nn.RMSNorm`` of ``module`` for an ``RMSNorm`` that shares its weight; a root-level one is returned converted."""
-    if type(module) is nn.RMSNorm:
-        return RMSNorm.from_float(module)
-    for name, child in module.named_children():
-        if type(child) is nn.RMSNorm:
-            setattr(module, name, RMSNorm.from_float(child))
-        else:
-            convert_rms_norms(child)
-    return module
+    return swap_modules(module, nn.RMSNorm, RMSNorm.from_float)

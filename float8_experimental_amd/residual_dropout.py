@@ -6,6 +6,7 @@ import torch.nn as nn
 
 from . import _custom_ops_model as _compiled
 from . import _native
+from .module_swap import swap_modules
 
 _HP_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -63,11 +64,4 @@ class Dropout(nn.Dropout):
 
 def convert_dropouts(module: nn.Module) -> nn.Module:
     """Swaps every ``nn.Dropout`` of ``module`` for a ``Dropout``; a root-level one is returned converted."""
-    if type(module) is nn.Dropout:
-        return Dropout.from_float(module)
-    for name, child in module.named_children():
-        if type(child) is nn.Dropout:
-            setattr(module, name, Dropout.from_float(child))
-        else:
-            convert_dropouts(child)
-    return module
+    return swap_modules(module, nn.Dropout, Dropout.from_float)

@@ -87,3 +87,21 @@ def test_names_that_the_filter_leaves_out_stay_as_they_are():
     linear = nn.Linear(16, 16)
     model = f8.adapt_linears(Held(linear), 3, 2, module_filter_fn=lambda m, fqn: fqn in ("b", "inner.1.0"))
     assert model.a is linear and model.inner[0] is linear and type(model.b) is f8.AdaptedLinear and model.inner[1][0] is model.b
+
+
+@pytest.mark.parametrize("convert, plain, own", [(f8.convert_rms_norms, lambda: nn.RMSNorm(16), f8.RMSNorm), (f8.convert_layer_norms, lambda: nn.LayerNorm(16), f8.LayerNorm),
+                                                 (f8.convert_dropouts, lambda: nn.Dropout(0.25), f8.Dropout)])
+def test_a_layer_under_several_names_is_converted_under_all_of_them(convert, plain, own):
+    model = Held(plain())
+    params = list(model.parameters())
+    assert convert(model) is model
+    first, *others = model.layers()
+    assert type(first) is own and all(m is first for m in others) and model.absent is None
+    assert all(p is q for p, q in zip(model.parameters(), params)) and convert(model) is model and model.a is first
+    assert type(convert(plain())) is own
+
+    class Of(type(plain())):
+        pass
+
+    of = nn.Sequential(Of(0.5) if own is f8.Dropout else Of(16))
+    assert type(convert(of)[0]) is Of  # a subclass may do something else
