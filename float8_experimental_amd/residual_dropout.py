@@ -48,6 +48,11 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: Optional[torch.Tensor] = None
 class Dropout(nn.Dropout):
     """``nn.Dropout`` on this package's kernel; a residual to add to may come with the input."""
 
+    def __init__(self, p: float = 0.5, inplace: bool = False):
+        if inplace:
+            raise NotImplementedError("dropout in place is not implemented")
+        super().__init__(p)
+
     def forward(self, input: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if self.training and self.p > 0.0:
             return dropout(input, self.p, residual=residual)
@@ -55,9 +60,7 @@ class Dropout(nn.Dropout):
 
     @classmethod
     def from_float(cls, mod: nn.Dropout) -> "Dropout":
-        if mod.inplace:
-            raise NotImplementedError("dropout in place is not implemented")
-        new_mod = cls(mod.p)
+        new_mod = cls(mod.p, mod.inplace)
         new_mod.train(mod.training)
         return new_mod
 

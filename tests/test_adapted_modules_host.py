@@ -105,3 +105,13 @@ def test_a_layer_under_several_names_is_converted_under_all_of_them(convert, pla
 
     of = nn.Sequential(Of(0.5) if own is f8.Dropout else Of(16))
     assert type(convert(of)[0]) is Of  # a subclass may do something else
+
+
+def test_dropout_in_place_is_refused():
+    for make in (lambda: f8.Dropout(0.5, inplace=True), lambda: f8.Dropout(0.5, True), lambda: f8.Dropout.from_float(nn.Dropout(0.5, True)), lambda: f8.convert_dropouts(nn.Sequential(nn.Dropout(0.5, True)))):
+        with pytest.raises(NotImplementedError, match="in place"):
+            make()
+    layer = f8.Dropout(0.25, inplace=False)
+    assert layer.p == 0.25 and not layer.inplace and f8.Dropout().p == 0.5 and f8.Dropout(p=0.1).p == 0.1
+    with pytest.raises(ValueError):
+        f8.Dropout(1.5)
