@@ -892,6 +892,15 @@ __global__ __launch_bounds__(256) void adapter_outer_finish_kernel(const OuterSu
     else ((uint16_t*)g.out)[to] = (uint16_t)pack2<F8MI_FP16>(s, 0.f);
 }
 
+// The gradients of a batch without rows.  (Its table holds nothing, so that the kernel above has no chunks to look up.)
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_zeros_kernel(T* __restrict__ first, int64_t first_size, T* __restrict__ second, int64_t second_size) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < first_size + second_size; i += (int64_t)gridDim.x * 256) {
+        if (i < first_size) first[i] = 0;
+        else second[i - first_size] = 0;
+    }
+}
+
 // ---- [batch][rows][cols] -> [batch][cols][rows]
 template <typename T>
 __global__ __launch_bounds__(256) void adapter_transpose_kernel(const T* __restrict__ in, T* __restrict__ out, int rows, int cols, int tiles_c) {
@@ -1099,6 +1108,13 @@ static int launch_outer_finish(const AdapterShape& s, const OuterSums& da, const
     return check_hip(hipGetLastError(), "adapter gradient sum kernel launch");
 }
 
+static int launch_zeros(void* da, int64_t da_size, void* db, int64_t db_size, int out_dtype, hipStream_t stream) {
+    const dim3 grid((unsigned)std::min<int64_t>((da_size + db_size + 255) / 256, (int64_t)cu_count() * 8));
+    if (out_dtype == F8MI_FP32) hipLaunchKernelGGL(adapter_zeros_kernel<uint32_t>, grid, dim3(256), 0, stream, (uint32_t*)da, da_size, (uint32_t*)db, db_size);
+    else hipLaunchKernelGGL(adapter_zeros_kernel<uint16_t>, grid, dim3(256), 0, stream, (uint16_t*)da, da_size, (uint16_t*)db, db_size);
+    return check_hip(hipGetLastError(), "adapter gradient zeros kernel launch");
+}
+
 static int adapters_check(const char* what, const AdapterShape& s) {
     if (s.dtype < 0 || s.dtype > 2) { set_error("%s: unknown dtype code %d", what, s.dtype); return F8MI_ERR_INVALID_ARG; }
     if (s.m < 0 || s.k < 1 || s.n < 1 || s.r < 1 || s.count < 1) { set_error("%s: bad shape m=%lld k=%lld n=%lld r=%lld count=%lld", what, (long long)s.m, (long long)s.k, (long long)s.n, (long long)s.r, (long long)s.count); return F8MI_ERR_INVALID_ARG; }
@@ -1160,8 +1176,9 @@ extern "C" int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const v
     const AdapterShape s{m, k, n, r, count, dtype};
     hipStream_t stream = (hipStream_t)stream_;
     if (int rc = adapters_check("f8mi_adapters_backward", s)) return rc;
-    if (m == 0 || (!dx && !da && !db)) return F8MI_OK;
+    if (!dx && !da && !db) return F8MI_OK;
     if (p_dtype < 0 || p_dtype > 2) { set_error("f8mi_adapters_backward: unknown dtype code %d", p_dtype); return F8MI_ERR_INVALID_ARG; }
+    if (m == 0) return da || db ? launch_zeros(da, da ? count * r * k : 0, db, db ? count * n * r : 0, p_dtype, stream) : F8MI_OK;
     if (!dout || !table || bad_stride(ld_dout, n) || (da && (!x || bad_stride(ldx, k))) || (dx && !a) || ((dx || da) && !b) || (db && !h)) { set_error("f8mi_adapters_backward: null pointer or row stride"); return F8MI_ERR_INVALID_ARG; }
     const AdapterBackwardSpace space(s, dx, da, db);
     if (space.bytes && (!workspace || workspace_bytes < space.bytes || (uintptr_t)workspace % 256 != 0)) { set_error("f8mi_adapters_backward: 256-byte aligned workspace of %lld bytes needed", (long long)space.bytes); return F8MI_ERR_INVALID_ARG; }

@@ -560,7 +560,8 @@ int f8mi_adapter_rows(const void* ids, int id_bytes, int64_t m, int64_t count, v
 int64_t f8mi_adapters_workspace_bytes(int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype);
 int f8mi_adapters(const void* x, int64_t ldx, const void* a, const void* b, const float* scale, float factor, const void* table, int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype,
                   const void* y, int64_t ldy, void* out, float* h, void* workspace, int64_t workspace_bytes, void* stream);
-/* dx (dense, without what comes through y), da, db (p_dtype, whole: zeros for an adapter without rows); each may be NULL.  workspace: 256-byte aligned. */
+/* dx (dense, without what comes through y), da, db (p_dtype, whole: zeros for an adapter without rows, and for all of them where m is 0: then nothing else is read); each may be
+ * NULL.  workspace: 256-byte aligned. */
 int64_t f8mi_adapters_backward_workspace_bytes(int64_t m, int64_t k, int64_t n, int64_t r, int64_t count, int dtype, int need_dx, int need_da, int need_db);
 int f8mi_adapters_backward(const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const void* a, const void* b, const float* scale, float factor, const void* table, const float* h, int64_t m,
                            int64_t k, int64_t n, int64_t r, int64_t count, int dtype, void* dx, void* da, void* db, int p_dtype, void* workspace, int64_t workspace_bytes, void* stream);
