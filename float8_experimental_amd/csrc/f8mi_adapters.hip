@@ -9,8 +9,8 @@
 // as both operands have the same one, so the four lanes that share a row take 64 neighbouring bytes of it, two instructions a line of the cache.
 //
 // h and dh are sums and stay in 32 bits: 16-bit matrix instructions get them as the sum of two 16-bit values (an error of 2^-17 of h, where one alone
-// would be off by as much as the rounding of the result), fp16 ones after a power of two for each row, so that nothing overflows or falls among the
-// subnormals.
+// would be off by as much as the rounding of the result), fp16 ones after a power of two for each row, so that nothing overflows, and of the row's largest no more
+// than 2^-39 is lost among the subnormals.
 #include <algorithm>
 
 #include "f8mi_adapters.h"
@@ -363,16 +363,17 @@ __device__ __forceinline__ void stage_h(const AdapterArgs& g, const AdapterTile&
     }
     __syncthreads();
     factor = 1.f;
-    if constexpr (DT == F8MI_FP16) {  // a power of two, 2^(e - 127), that brings the row's largest to [1, 2)
-        auto exponent = [&](int row) __attribute__((always_inline)) { return (uint32_t)min(max((int)(row_most[row] >> 23), 1), 253); };
+    if constexpr (DT == F8MI_FP16) {  // a power of two, 2^(141 - e), that brings the row's largest to [2^14, 2^15): the low parts of values down to 2^-23 of it have their bits (brought
+        // to [1, 2), those of 2^-9 had lost some, and where B takes no part of the large ones, that was the result); 2^39 at most, of 256 of the rank, in the sums
+        auto exponent = [&](int row) __attribute__((always_inline)) { return (uint32_t)min(max((int)(row_most[row] >> 23), 15), 254); };
         for (int item = t; item < ROWS * quads; item += THREADS) {
             const int row = item / quads;
             const float4 q = *(const float4*)(sums + item * 4);
-            const float f = __uint_as_float((254u - exponent(row)) << 23);
+            const float f = __uint_as_float((268u - exponent(row)) << 23);
             const float v[4] = {q.x * f, q.y * f, q.z * f, q.w * f};
             keep(row, (item - row * quads) * 4, v);
         }
-        factor = __uint_as_float(exponent(my_row) << 23);
+        factor = __uint_as_float((exponent(my_row) - 14u) << 23);
         __syncthreads();
     }
 }
