@@ -8,7 +8,8 @@
 //
 // HBM-bound, as layer norm (f8mi_layer_norm.hip), and built the same way: a row stays in the registers of T lanes between its first read and its
 // last use, one barrier a row (there is one sum, where layer norm has two), the next row on its way meanwhile; a workgroup takes every (number of workgroups)-th row, so that the weight is read
-// once and, backward, a lane sums the columns it owns over its rows in registers; a second launch adds the workgroups' sums in a fixed order.
+// once and, backward, a lane sums the columns it owns over its rows in registers; a second launch adds the workgroups' sums in a fixed order.  The widest rows backward, three pieces a lane of 16-bit values
+// and five of fp32, keep those sums in LDS and spill 20 to 112 bytes a lane all the same (1024 lanes leave each 128 registers), addresses mostly.
 // Measured, out of HBM (a large copy: 5.1 - 5.4 TB/s): 8192 x 4096 bf16 with a residual and an fp32 weight forward 45 us (6.0 TB/s), backward 45 (5.9) and 4 for the sums;
 // 8192 x 8192 bf16 with a residual into e4m3 78 us (6.0 TB/s); 4099 x 4097 fp32 forward 26 us (5.1 TB/s), backward 39 (5.2); 2048 x 20000 bf16 with a residual, both passes, 131 us
 // (5.0 TB/s); 16 rows of 8192 into e4m3 5.5 us and one of 4096 2.5 us, latency.  16-bit rows of an odd number of values begin at odd multiples of two bytes: 8192 x 4097

@@ -53,8 +53,8 @@ def low_rank_adapters(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter
     (no gradient).  ``adapters``: an ``AdapterRows`` of this batch, or the numbers themselves, which are then sorted in this call.
 
     x in bfloat16, float16 or float32; a and b may have another of these types, they are rounded to x's for the products and their gradients have their own, rounded once; a row's
-    ``a[e] @ x_i`` is kept in 32 bits, to 2^-16 of itself in the second product of 16-bit types (float16: or to 2^-39 of the row's largest).  Sums are fp32, in a fixed order.  Under autocast x and y take the
-    autocast type first."""
+    ``a[e] @ x_i`` is kept in 32 bits, to 2^-16 of itself in the second product of 16-bit types (float16: or to 2^-39 of the row's largest).  Sums are fp32, in a fixed order; an
+    infinity in 16-bit x, a, b or the gradient of the result may come out as NaN.  Under autocast x and y take the autocast type first."""
     if torch.is_autocast_enabled():
         dtype = torch.get_autocast_dtype("cuda")
         x, y = x.to(dtype), None if y is None else y.to(dtype)
