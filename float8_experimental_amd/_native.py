@@ -1171,6 +1171,7 @@ def adapters(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, table: torch.Ten
     out = torch.empty((m, n), dtype=x.dtype, device=x.device)
     h = torch.empty((m, -(-rank // 16) * 16), dtype=torch.float32, device=x.device) if need_h else None
     _check_device(x.device)
+    table.record_stream(torch.cuda.current_stream(x.device))  # (the next batch's table takes its place, on the stream that it was made on)
     need = lib().f8mi_adapters_workspace_bytes(m, k, n, rank, count, _DT[x.dtype])
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
     _check(lib().f8mi_adapters(xs.data_ptr(), ld, a.data_ptr(), b.data_ptr(), _ptr(scale), factor, table.data_ptr(), m, k, n, rank, count, _DT[x.dtype], _ptr(ys), ld_y, out.data_ptr(), _ptr(h),

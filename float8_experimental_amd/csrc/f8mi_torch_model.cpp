@@ -5,6 +5,8 @@
 // Every function returns None, without having queued or allocated anything, for what it does not take (subclasses, other devices, types or shapes) and while
 // somebody has to see operators (modes, traces): the caller then says what is wrong, or goes through the registered operators.  Workspaces are temporaries of
 // torch's caching allocator, which hands their memory out again in stream order.
+#include <c10/hip/HIPCachingAllocator.h>
+
 #include "f8mi_torch_util.h"
 
 namespace {
@@ -144,6 +146,9 @@ struct Adapters : torch::autograd::Function<Adapters> {
     static at::Tensor compute(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const at::Tensor& y, const at::Tensor& table, const at::Tensor& scale, double factor, at::Tensor* h) {
         const c10::DeviceGuard guard(x.device());
         const Below below;
+        // A batch's table belongs to the stream that it was made on, and the next batch's takes its place (select_adapters): the allocator has to know that another stream still reads it.  (Nothing
+        // where it is the same stream.)
+        c10::hip::HIPCachingAllocator::recordStream(table.storage().data_ptr(), c10::hip::getCurrentHIPStream(x.get_device()));
         const int64_t count = a.size(0), rank = a.size(1), k = a.size(2), n = b.size(1);
         const Rows xr(x, k);
         std::optional<Rows> yr;

@@ -24,7 +24,7 @@ MAX_RANK, MAX_COUNT, MAX_ROWS = 256, 32768, 1 << 24  # F8MI_ADAPTER_MAX_*
 
 class AdapterRows:
     """The rows of a batch by adapter: ``adapters`` has one whole number for each row (``x.numel() / k`` of them, in their order), that of its adapter among ``count``; any other
-    number, -1 for instance, means none.  Made once for a batch and used by all its layers; it keeps what the numbers were then.
+    number, -1 for instance, means none.  Made once for a batch and used by all its layers, on any stream that waits for the one it is made on; it keeps what the numbers were then.
 
     A captured graph reads the table that it was captured with: it has to outlive the graph, or is made inside the capture, from numbers that are written between replays."""
 
