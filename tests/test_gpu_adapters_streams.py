@@ -74,3 +74,27 @@ def test_batches_one_after_another_on_another_stream(f8):
                 got.append(layer(x))
         torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_a_captured_graph_reads_a_table_from_outside(f8):
+    """Made on another stream than the capturing one, read at each replay, and let go once the graph is."""
+    torch.manual_seed(1)
+    layer = f8.AdaptedLinear(nn.Linear(64, 128, device="cuda", dtype=BF16), 3, 4).eval()
+    x, ids = torch.randn(9, 64, device="cuda", dtype=BF16), torch.arange(9, device="cuda") % 4 - 1
+    with torch.no_grad():
+        layer.adapter_b.normal_()
+        f8.select_adapters(layer, ids)
+        layer(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer(x)
+        for i in range(3):
+            x.copy_(torch.randn(9, 64, generator=torch.Generator().manual_seed(i)).to(BF16))
+            want = layer(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        del graph, out
+        f8.select_adapters(layer, ids[:5])
+        assert layer(x[:5]).isfinite().all()
